@@ -74,6 +74,10 @@ SIGNATURES = {
     "g4_ple_mix": (_int, [_vp, _vp, _vp, _int, _int, _int, _vp]),
     "g4_embed": (_int, [_vp, _int, _int, _vp, _int, _c.c_float, _vp]),
     "g4_argmax": (_int, [_vp, _int, _vp]),
+    "g4_attention_tree": (_int, [_vp, _vp, _vp, _int, _int, _int, _int, _vp, _int, _int, _vp]),
+    "g4_bf16_head_rows": (_int, [_vp, _int, _vp, _int, _int, _vp, _sz, _c.c_float, _c.c_float]),
+    "g4_sample": (_int, [_vp, _sz, _int, _int, _vp, _vp, _vp, _vp]),
+    "g4_cache_rows": (_int, [_vp, _vp, _vp, _int, _vp, _int, _int, _int]),
     "g4_w4_load_dev": (_int, [_vp, _vp, _int, _int, _int, _c.POINTER(_vp)]),
     "g4_w4_load_opts": (_int, [_vp, _vp, _int, _int, _int, _int, _c.POINTER(_vp)]),
     "g4_ple_upload_shard_dev": (_int, [_vp, _int, _vp, _sz]),
@@ -123,6 +127,11 @@ class GemmaConfig(_c.Structure):
                 ("full", _int * GEMMA_MAX_LAYERS), ("kv_source", _int * GEMMA_MAX_LAYERS),
                 ("rope_base", _c.c_float * GEMMA_MAX_LAYERS),
                 ("rope_prop", _c.c_float * GEMMA_MAX_LAYERS)]
+
+
+class SampleParams(_c.Structure):
+    _fields_ = [("temperature", _c.c_float), ("top_k", _int), ("top_p", _c.c_float),
+                ("min_p", _c.c_float)]
 
 
 class G4Error(RuntimeError):
@@ -463,6 +472,46 @@ def embed(E, vocab, width, ids, n, s, y):
 
 def argmax(x, n, out):
     check(lib().g4_argmax(_f(x), n, _f(out)))
+
+
+def attention_tree(q, k, v, nodes, heads, hd, prefix, parents, sliding, window, y):
+    """g4_attention_tree: drafted tokens over a cache, parents int32 [nodes] on the device."""
+    check(lib().g4_attention_tree(_f(q), _f(k), _f(v), nodes, heads, hd, prefix, _f(parents),
+                                  1 if sliding else 0, window, _f(y)))
+
+
+def bf16_head_rows(x, n, E, rows, in_dim, out, out_stride=None, scale=1.0, softcap=30.0):
+    """g4_bf16_head_rows: the tied head for n hidden states."""
+    check(lib().g4_bf16_head_rows(_f(x), n, _f(E), rows, in_dim, _f(out),
+                                  rows if out_stride is None else out_stride, scale, softcap))
+
+
+def sample(logits, rows, vocab, u, tokens, probs=None, stride=None, temperature=1.0, top_k=0,
+           top_p=1.0, min_p=0.0):
+    """g4_sample: one token per row of logits, from the random numbers u."""
+    p = SampleParams(temperature, top_k, top_p, min_p)
+    check(lib().g4_sample(_f(logits), vocab if stride is None else stride, rows, vocab,
+                          _c.byref(p), _f(u), _f(tokens), _f(probs)))
+
+
+class CachePlanes:
+    """The planes of g4_cache_rows: dst and src (buffers or device pointers; the same ones to
+    keep rows in place) and the FP32 values per row of each."""
+
+    def __init__(self, dst, src, widths):
+        n = len(widths)
+        if len(dst) != n or len(src) != n:
+            raise ValueError("one dst, src and width per plane")
+        self.planes = n
+        self._keep = (dst, src)
+        self._dst = (_vp * n)(*[_f(p) for p in dst])
+        self._src = (_vp * n)(*[_f(p) for p in src])
+        self._widths = (_int * n)(*widths)
+
+    def rows(self, rows, n, dst_row, src_rows):
+        """dst[p][dst_row + i] = src[p][rows[i]], rows int32 [n] on the device."""
+        check(lib().g4_cache_rows(self._dst, self._src, self._widths, self.planes, _f(rows), n,
+                                  dst_row, src_rows))
 
 
 def fill_random(buf, count, kind, seed, sigma=1.0):

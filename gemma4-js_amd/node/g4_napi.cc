@@ -995,6 +995,116 @@ napi_value F_argmax(napi_env env, napi_callback_info info) {
   return undefined(env);
 }
 
+// attentionTree(q, k, v, nodes, heads, hd, prefix, parents, sliding, window, y)
+napi_value F_attentionTree(napi_env env, napi_callback_info info) {
+  napi_value a[11], self;
+  if (!get_args(env, info, 11, a, &self)) return nullptr;
+  void *q, *k, *vv, *par, *y;
+  int64_t v[6];
+  static const int idx[6] = {3, 4, 5, 6, 8, 9};
+  static const char *const names[6] = {"nodes", "heads", "hd", "prefix", "sliding", "window"};
+  if (!dev(env, a[0], "q", &q) || !dev(env, a[1], "k", &k) || !dev(env, a[2], "v", &vv) ||
+      !ints(env, a, idx, v, 6, names) || !dev(env, a[7], "parents", &par) ||
+      !dev(env, a[10], "y", &y))
+    return nullptr;
+  G4_CALL(env, g4_attention_tree((const float *)q, (const float *)k, (const float *)vv, (int)v[0],
+                                 (int)v[1], (int)v[2], (int)v[3], (const int32_t *)par, (int)v[4],
+                                 (int)v[5], (float *)y));
+  return undefined(env);
+}
+
+// bf16HeadRows(x, n, E, rows, inDim, out, outStride, scale, softcap, outByteOffset = 0)
+napi_value F_bf16HeadRows(napi_env env, napi_callback_info info) {
+  napi_value a[10], self;
+  if (!get_args(env, info, 10, a, &self)) return nullptr;
+  void *x, *E, *out;
+  int64_t n, rows, k, stride;
+  double scale, softcap;
+  if (!dev(env, a[0], "x", &x) || !to_int(env, a[1], &n, "n") || !dev(env, a[2], "E", &E) ||
+      !to_int(env, a[3], &rows, "rows") || !to_int(env, a[4], &k, "inDim") ||
+      !buf_at(env, a[5], a[9], "out", &out) || !to_i64(env, a[6], &stride, "outStride") ||
+      !to_f64(env, a[7], &scale, "scale") || !to_f64(env, a[8], &softcap, "softcap"))
+    return nullptr;
+  if (stride < 0) {
+    napi_throw_range_error(env, nullptr, "outStride must be >= 0");
+    return nullptr;
+  }
+  G4_CALL(env, g4_bf16_head_rows((const float *)x, (int)n, E, (int)rows, (int)k, (float *)out,
+                                 (size_t)stride, (float)scale, (float)softcap));
+  return undefined(env);
+}
+
+// sample(logits, stride, rows, vocab, temperature, topK, topP, minP, u, tokens, probs = null)
+napi_value F_sample(napi_env env, napi_callback_info info) {
+  napi_value a[11], self;
+  if (!get_args(env, info, 11, a, &self)) return nullptr;
+  void *x, *u, *tok, *pr = nullptr;
+  int64_t stride, rows, vocab, top_k;
+  double temp, top_p, min_p;
+  napi_valuetype t;
+  if (!dev(env, a[0], "logits", &x) || !to_i64(env, a[1], &stride, "stride") ||
+      !to_int(env, a[2], &rows, "rows") || !to_int(env, a[3], &vocab, "vocab") ||
+      !to_f64(env, a[4], &temp, "temperature") || !to_int(env, a[5], &top_k, "topK") ||
+      !to_f64(env, a[6], &top_p, "topP") || !to_f64(env, a[7], &min_p, "minP") ||
+      !dev(env, a[8], "u", &u) || !dev(env, a[9], "tokens", &tok))
+    return nullptr;
+  napi_typeof(env, a[10], &t);
+  if (t != napi_undefined && t != napi_null && !dev(env, a[10], "probs", &pr)) return nullptr;
+  if (stride < 0) {
+    napi_throw_range_error(env, nullptr, "stride must be >= 0");
+    return nullptr;
+  }
+  const g4_sample_params p = {(float)temp, (int)top_k, (float)top_p, (float)min_p};
+  G4_CALL(env, g4_sample((const float *)x, (size_t)stride, (int)rows, (int)vocab, &p,
+                         (const float *)u, (int32_t *)tok, (float *)pr));
+  return undefined(env);
+}
+
+// cacheRows(dst[], src[], widths[], rows, n, dstRow, srcRows): one DeviceBuffer per plane
+napi_value F_cacheRows(napi_env env, napi_callback_info info) {
+  napi_value a[7], self;
+  if (!get_args(env, info, 7, a, &self)) return nullptr;
+  uint32_t n[3] = {0, 0, 0};
+  for (int i = 0; i < 3; ++i) {
+    bool is = false;
+    napi_is_array(env, a[i], &is);
+    if (!is) {
+      napi_throw_type_error(env, nullptr, "cacheRows: dst, src and widths are arrays");
+      return nullptr;
+    }
+    NAPI_CALL(env, napi_get_array_length(env, a[i], &n[i]));
+  }
+  if (n[0] != n[1] || n[0] != n[2] || n[0] < 1 || n[0] > G4_CACHE_MAX_PLANES) {
+    napi_throw_range_error(env, nullptr, "cacheRows: one dst, src and width per plane, at most 128");
+    return nullptr;
+  }
+  float *dst[G4_CACHE_MAX_PLANES];
+  const float *src[G4_CACHE_MAX_PLANES];
+  int widths[G4_CACHE_MAX_PLANES];
+  for (uint32_t i = 0; i < n[0]; ++i) {
+    napi_value e;
+    void *p;
+    int64_t w;
+    NAPI_CALL(env, napi_get_element(env, a[0], i, &e));
+    if (!dev(env, e, "dst", &p)) return nullptr;
+    dst[i] = static_cast<float *>(p);
+    NAPI_CALL(env, napi_get_element(env, a[1], i, &e));
+    if (!dev(env, e, "src", &p)) return nullptr;
+    src[i] = static_cast<const float *>(p);
+    NAPI_CALL(env, napi_get_element(env, a[2], i, &e));
+    if (!to_int(env, e, &w, "width")) return nullptr;
+    widths[i] = (int)w;
+  }
+  void *rows;
+  int64_t v[3];
+  static const int idx[3] = {4, 5, 6};
+  static const char *const names[3] = {"n", "dstRow", "srcRows"};
+  if (!dev(env, a[3], "rows", &rows) || !ints(env, a, idx, v, 3, names)) return nullptr;
+  G4_CALL(env, g4_cache_rows(dst, src, widths, (int)n[0], (const int32_t *)rows, (int)v[0],
+                             (int)v[1], (int)v[2]));
+  return undefined(env);
+}
+
 // ---- GemmaEngine (g4_gemma_*) ---------------------------------------------------
 // The native decoder engine behind Gemma4WebGPU's load/forward/logits/greedy
 // surface (gemma4-webgpu.js:139-481), plus decode(steps) on a recorded step.
@@ -1482,7 +1592,10 @@ napi_value Init(napi_env env, napi_value exports) {
       METHOD("timeMs", F_timeMs), METHOD("rms", F_rms), METHOD("addScale", F_addScale),
       METHOD("scale", F_scale), METHOD("geluMul", F_geluMul), METHOD("geluPle", F_geluPle),
       METHOD("normRope", F_normRope), METHOD("attention", F_attention),
-      METHOD("pleMix", F_pleMix), METHOD("argmax", F_argmax), METHOD("e2bConfig", F_e2bConfig), METHOD("fillRandom", F_fillRandom)};
+      METHOD("pleMix", F_pleMix), METHOD("argmax", F_argmax),
+      METHOD("attentionTree", F_attentionTree), METHOD("bf16HeadRows", F_bf16HeadRows),
+      METHOD("sample", F_sample), METHOD("cacheRows", F_cacheRows),
+      METHOD("e2bConfig", F_e2bConfig), METHOD("fillRandom", F_fillRandom)};
   NAPI_CALL(env, napi_define_properties(env, exports, sizeof fns / sizeof fns[0], fns));
   napi_value v;
   napi_create_int32(env, G4_F32, &v);

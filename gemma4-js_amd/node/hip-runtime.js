@@ -305,6 +305,32 @@ class GPUOps {
     if (weightChunk.size < rows * inDim * 2) throw new Error('headChunk: weight chunk too small');
     native.bf16Head(x, weightChunk, rows, inDim, out, 1.0, 30.0, 0, outOffset * 4);
   }
+  // ---- drafted tokens and picks by probability (no reference counterpart) ----
+  // attention() of a tree of drafted tokens appended at rows prefix .. of the caches;
+  // parents: int32 DeviceBuffer, -1 or an earlier node's index per node
+  attentionTree(encoder, q, kcache, vcache, nodes, heads, hd, prefix, parents, sliding, window, garbage = null) {
+    const out = this.emptyF32(nodes * heads * hd, 'attn-tree-out');
+    native.attentionTree(q, kcache, vcache, nodes, heads, hd, prefix, parents, sliding ? 1 : 0, window, out);
+    return out;
+  }
+  // headChunk() for n hidden states: out[j * outStride + outOffset + r]
+  headRows(encoder, x, n, weightChunk, out, outOffset, outStride, rows, garbage = null, inDim = 1536) {
+    if (weightChunk.size < rows * inDim * 2) throw new Error('headRows: weight chunk too small');
+    native.bf16HeadRows(x, n, weightChunk, rows, inDim, out, outStride, 1.0, 30.0, outOffset * 4);
+  }
+  // one token per row of logits from the random numbers u (FP32 DeviceBuffer, in [0, 1));
+  // returns {tokens (int32), probs (FP32)} as DeviceBuffers
+  sample(encoder, logits, rows, vocab, u, { temperature = 1, topK = 0, topP = 1, minP = 0 } = {}, garbage = null) {
+    const tokens = this.emptyF32(rows, 'sample-tokens'), probs = this.emptyF32(rows, 'sample-probs');
+    native.sample(logits, vocab, rows, vocab, temperature, topK, topP, minP, u, tokens, probs);
+    return { tokens, probs };
+  }
+  // rows of every plane {dst, src, width}: dst[dstRow + i] = src[rows[i]], i < n, all read
+  // before any is written (dst === src keeps accepted rows in place)
+  cacheRows(encoder, planes, rows, n, dstRow, srcRows) {
+    native.cacheRows(planes.map((p) => p.dst), planes.map((p) => p.src), planes.map((p) => p.width),
+      rows, n, dstRow, srcRows);
+  }
   dispose() {}
 }
 

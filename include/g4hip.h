@@ -357,6 +357,80 @@ int g4_embed(const void *E, int vocab, int width, const int32_t *ids_dev,
  * index of the largest finite x[i], or -1 if none is finite (topK throws). */
 int g4_argmax(const float *x, int n, int32_t *out_dev);
 
+/* ---- drafted tokens and picks by probability -------------------------------
+ * No counterparts in the reference, which feeds one greedy token at a time.  A
+ * step that checks several drafted tokens at once appends their k/v rows to the
+ * caches, runs their attention as a tree, reads the tied head once for all of
+ * them, picks a token per row and keeps the cache rows of the accepted path:
+ *   g4_norm_rope of the nodes of one depth as one row of nodes * heads heads,
+ *   g4_attention_tree, g4_bf16_head_rows, g4_sample, g4_cache_rows.
+ * Arguments are checked before anything else, so a refusal needs no device.
+ * All four can be recorded; inside an encoder g4_attention_tree, g4_sample and a
+ * g4_cache_rows that works in place need one earlier call of those sizes. */
+
+/* Attention of a tree of drafted tokens over a cache: g4_attention with each
+ * node seeing the prefix, itself and its ancestors.
+ *   q [nodes, heads, head_dim]; k, v [prefix + nodes, head_dim], node j's rows
+ *   at prefix + j (one KV head shared by all query heads); y as q.
+ *   parents: DEVICE int32 [nodes], -1 (the node follows the prefix) or the index
+ *   of an earlier node.  Node i sits at position prefix + (number of its
+ *   ancestors); with `sliding` it sees only what lies at positions > its own -
+ *   window.
+ * A parent outside [-1, i) gives NaN rows for node i and every node below it.
+ * k/v rows that no node sees have no influence, whatever they hold.
+ * heads <= 8; head_dim 64, 128, 256 or 512; nodes <= 256. */
+int g4_attention_tree(const float *q, const float *k, const float *v, int nodes,
+                      int heads, int head_dim, int prefix, const int32_t *parents,
+                      int sliding, int window, float *y);
+
+/* g4_bf16_head for n hidden states, the table read once for (up to 64 of) them:
+ *   out[j * out_stride + r] = softcap * tanh((scale * sum_k x[j, k] * E[r, k]) / softcap)
+ * x: device FP32 [n, in_dim]; E: device BF16 [rows, in_dim]; out_stride >= rows
+ * (floats; a chunk of the vocabulary writes into a wider logits row).  in_dim a
+ * positive multiple of 8, <= 4096; E 16-byte aligned; softcap <= 0 disables the
+ * cap.  n = 1 gives g4_bf16_head's bits. */
+int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int in_dim,
+                      float *out, size_t out_stride, float scale, float softcap);
+
+/* One token per row of logits, by probability.
+ *   logits: device FP32, row j at logits + j * stride (stride >= vocab)
+ *   u:      device FP32 [rows], uniform random numbers in [0, 1)
+ *   tokens: device int32 [rows]; probs: device FP32 [rows] or NULL
+ * Only finite logits take part.  Probabilities are softmax(logits / temperature);
+ * the tokens in order of their logits, equal ones by index, are cut
+ *   top_k  to the first top_k (0: not at all),
+ *   top_p  to those before which less than top_p of the (top-k) mass lies
+ *          (1: not at all; the first token always stays),
+ *   min_p  to those of at least min_p of the largest probability (0: not at all),
+ * and the row's token is the first one, by index, up to which more than u of the
+ * kept mass lies (the last kept one for u >= 1; u < 0 or NaN counts as 0).  Its
+ * probability among the kept tokens goes to probs.  temperature 0 picks
+ * g4_argmax's token, with probability 1.  A row without a finite logit gets token
+ * -1 and probability 0.  Probabilities are summed in 64-bit fixed point (2^-44 of
+ * the largest at 262144 tokens), so the sums have no order. */
+typedef struct {
+  float temperature; /* >= 0 */
+  int top_k;         /* >= 0 */
+  float top_p;       /* in (0, 1] */
+  float min_p;       /* in [0, 1] */
+} g4_sample_params;
+int g4_sample(const float *logits, size_t stride, int rows, int vocab,
+              const g4_sample_params *params, const float *u, int32_t *tokens,
+              float *probs);
+
+/* Rows of a cache's planes (k and v of every layer): for each plane p
+ *   dst[p][dst_row + i] = src[p][rows[i]],  i < n
+ * as if every row were read before any is written, so with dst[p] == src[p] the
+ * accepted rows move together in place; with other planes it copies (forks) a
+ * cache or picks rows from it.  Plane p: FP32 rows of widths[p] values, src_rows
+ * of them in src[p], at least dst_row + n in dst[p].  rows: DEVICE int32 [n]; an
+ * entry outside [0, src_rows) gives a NaN row.  Memory of different planes must
+ * not overlap.  1 <= planes <= G4_CACHE_MAX_PLANES; dst, src and widths are HOST
+ * arrays, read during the call. */
+#define G4_CACHE_MAX_PLANES 128
+int g4_cache_rows(float *const *dst, const float *const *src, const int *widths,
+                  int planes, const int32_t *rows, int n, int dst_row, int src_rows);
+
 /* ---- synthetic data (random-init models) ----------------------------------
  * No reference counterpart: the benchmarks run random-init weights of the
  * checkpoint's shapes, generated on the device.  Fills `count` elements of

@@ -1,0 +1,98 @@
+"""g4_bf16_head_rows against x . E^T and the cap in 64 bits.
+
+Tolerance: the products are exact to 2^-23 and summed in FP32; a sum of K of them in any
+order is off by a few times 2^-24 sqrt(K) of their absolute sum's mean step: 2^-24 *
+(8 + sqrt(K)) * sum |x E| bounds what is seen by far.  The cap's slope is at most 1, its
+tanh off by a few ulps: 4 * 2^-23 of the cap's output."""
+import numpy as np
+import pytest
+
+import synthetic as syn
+
+pytestmark = pytest.mark.gpu
+
+
+def case(rng, n, rows, k):
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    x[0] *= 30
+    E = syn.bf16_rne((rng.standard_normal((rows, k)) * 0.05).astype(np.float32))
+    return x, E
+
+
+def run(g4, x, E, stride=None, scale=1.0, softcap=30.0):
+    n, k = x.shape
+    rows = E.shape[0]
+    stride = rows if stride is None else stride
+    out = g4.Buffer.from_array(np.full((n, stride), 7.0, np.float32))
+    g4.bf16_head_rows(g4.Buffer.from_array(x), n, g4.Buffer.from_array(E), rows, k, out, stride,
+                      scale, softcap)
+    return out.download(np.float32).reshape(n, stride)
+
+
+def check(got, x, E, scale=1.0, softcap=30.0):
+    e = syn.bf16_to_f32(E).astype(np.float64)
+    x64 = x.astype(np.float64)
+    z = scale * (x64 @ e.T)
+    want = softcap * np.tanh(z / softcap) if softcap > 0 else z
+    off = 2.0 ** -24 * (8 + np.sqrt(x.shape[1])) * abs(scale) * (np.abs(x64) @ np.abs(e).T)
+    assert (np.abs(got - want) <= off + 4 * 2.0 ** -23 * np.abs(want) + 1e-37).all()
+
+
+@pytest.mark.parametrize("n,rows,k", [
+    (1, 100, 1536), (2, 1, 8), (2, 257, 1536), (3, 4096, 1536), (5, 1000, 64), (8, 333, 40),
+    (15, 515, 1528), (16, 64, 256), (17, 129, 1536), (31, 700, 2048), (33, 255, 520),
+    (48, 1025, 1536), (63, 130, 4096), (64, 4096, 1536), (65, 300, 1536), (130, 77, 104)])
+def test_shapes(g4, n, rows, k):
+    print("head rows", n, rows, k, flush=True)
+    x, E = case(np.random.default_rng([n, rows, k]), n, rows, k)
+    check(run(g4, x, E), x, E)
+
+
+@pytest.mark.parametrize("n", [2, 20, 70])
+def test_scale_without_cap_and_stride(g4, n):
+    x, E = case(np.random.default_rng(n), n, 301, 512)
+    got = run(g4, x, E, stride=333, scale=-0.37, softcap=0.0)
+    check(got[:, :301], x, E, scale=-0.37, softcap=0.0)
+    assert (got[:, 301:] == 7.0).all()  # the rest of a row stays
+
+
+def test_one_state_has_the_single_head_s_bits(g4):
+    x, E = case(np.random.default_rng(4), 1, 1000, 1536)
+    out, xb, eb = g4.Buffer(4000), g4.Buffer.from_array(x), g4.Buffer.from_array(E)
+    g4.bf16_head(xb.ptr, eb.ptr, 1000, 1536, out.ptr)
+    np.testing.assert_array_equal(run(g4, x, E)[0], out.download(np.float32))
+
+
+@pytest.mark.parametrize("n", [4, 64])
+def test_a_state_s_logits_do_not_depend_on_the_others(g4, n):
+    x, E = case(np.random.default_rng(n), n, 500, 1536)
+    a = run(g4, x, E)
+    y = x.copy()
+    y[1:] = np.nan
+    y[2] = np.inf
+    np.testing.assert_array_equal(run(g4, y, E)[0], a[0])
+    b = run(g4, y, E)
+    assert np.isnan(b[1]).all() and not np.isnan(b[0]).any()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_sizes_of_the_states(g4, size):
+    x, E = case(np.random.default_rng(8), 6, 200, 1536)
+    x = (x * np.float32(size)).astype(np.float32)
+    check(run(g4, x, E, scale=1.0, softcap=0.0), x, E, softcap=0.0)
+
+
+def test_a_largest_finite_state(g4):
+    x, E = case(np.random.default_rng(9), 3, 64, 256)
+    x[1] = 0.0
+    x[1, 7] = 3.4e38  # rounds to infinity in BF16
+    E[:, 7] = syn.bf16_rne(np.full(64, 1e-30, np.float32))
+    check(run(g4, x, E, softcap=0.0), x, E, softcap=0.0)
+
+
+def test_refuses_short_buffers(g4):
+    x, e, o = g4.Buffer(4 * 64 * 4), g4.Buffer(10 * 64 * 2), g4.Buffer(4 * 10 * 4)
+    for args in ((x, 5, e, 10, 64, o), (x, 4, e, 11, 64, o), (x, 4, e, 10, 64, o, 11),
+                 (x, 4, None, 10, 64, o)):
+        with pytest.raises(g4.G4Error):
+            g4.bf16_head_rows(*args)
