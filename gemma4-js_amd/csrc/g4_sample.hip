@@ -5,13 +5,22 @@
 //   top-k  the first k
 //   top-p  those with less than top_p * mass(top-k) before them
 //   min-p  those with p >= min_p
-// so the kept set is all tokens above one logit and the first `ties` (by index)
-// of those that equal it.  The token is the first one, by index, up to which more
-// than u * (kept mass) lies.
+// The token is the first one, by index, up to which more than u * (kept mass) lies.
 //
-// Numerics.  d, e^d and the borders are computed in binary64 and masses are summed
-// as integers, round(p * 2^s), 2^s * vocab < 2^62: a token's border may lie next to
-// u, and integer sums do not depend on their order.
+// Numerics.  A token's border may lie next to u, so borders are binary64 and masses are
+// integers: round(p * 2^k), 2^k * vocab < 2^62, whose sums do not depend on their order.
+// e^d is e^(-b/16) (a table) times e^((f-1)/16) (a polynomial, exact to 2^-53), b and f
+// from x * 16 / temperature = whole part and fraction; below e^-31 a mass counts as 0
+// (2^-44, a unit of the sums at 262144 tokens).
+//
+// Two launches over slices of the rows; each one's last block of a row goes on alone:
+//   sample_plan_kernel  per slice the largest logit and, by whole part of x * 16 / T,
+//                       count and mass; the row's last block finds the bins in which the
+//                       cuts lie (bins above them are kept, those below dropped)
+//   sample_pick_kernel  the kept mass of every slice, and a list of the tokens in those
+//                       bins; the row's last block finds the cuts among them, the slice
+//                       and the token
+// A row of one slice takes both halves in one launch (sample_row_kernel).
 #include <math.h>
 
 #include "g4_internal.h"
@@ -19,176 +28,659 @@
 namespace g4 {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int NT = 512;       // threads per block
+constexpr int kWaves = NT / 64;
+constexpr int kBins = NT;     // one thread each; the last one holds the rest
+constexpr int kRest = kBins - 1;
+constexpr double kPerUnit = 16.0;  // bins per unit of d
+constexpr int kPer = 16;           // listed tokens per thread
+constexpr int kList = kPer * NT;
+constexpr int kMaxRows = 256;      // rows per launch
+constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxSlices = 2 * NT;
+constexpr int kOneSlice = 8192;    // longest row of one slice
+// a bin's packed sum: count << 50 | mass in units of 2^-38 of the bin's upper edge
+constexpr int kCountShift = 50;
+constexpr double kBinUnit = 274877906944.0;
+typedef unsigned long long u64;
+
+// What the first launch leaves for the second.
+struct Plan {
+  double id;        // whole part of max * s
+  double before_k;  // mass above top-k's bin
+  double total;     // mass of all bins
+  float top;        // largest logit
+  int any;          // 0: no finite logit
+  int sure;         // bins below this one are kept (but for min-p)
+  int lo, hi;       // bins in which top-p's cut may lie (lo > hi: no such cut)
+  int kb;           // the bin of top-k's cut, or -1
+  uint32_t k_left;  // tokens of it that top-k keeps
+  uint32_t n;       // listed tokens
+};
 
 struct SampleArgs {
   const float *x;
   size_t stride;
-  int vocab, top_k;
-  double inv_t, top_p, log_min;
-  double unit;  // 2^s
+  int vocab, top_k, slices, per;
+  double inv_t, s, top_p, log_min, unit;
   const float *u;
   int *tokens;
   float *probs;
+  Plan *plan;
+  u64 *hist;        // [rows][slices][kBins]
+  uint32_t *maxes;  // [rows][slices] keys
+  u64 *list;        // [rows][kList]
+  u64 *mass;        // [rows][slices]
+  uint32_t *count;  // [2][kMaxRows] blocks that are done, 0 between launches
 };
 
 // Order-preserving key of a finite logit (zeros alike); 0 for any other.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (!isfinite(x)) return 0;
   const uint32_t b = __float_as_uint(x + 0.f);
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  const uint32_t k = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  return (b & 0x7f800000u) == 0x7f800000u ? 0u : k;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ uint64_t mass_of(double d, double unit) {
-  return (uint64_t)(exp(d) * unit + 0.5);
+// e^((f - 1/2) / 16), f in [0, 1): |z| <= 1/32, z^8 / 8! < 2^-55
+__device__ __forceinline__ double exp_part(double f) {
+  const double z = (f - 0.5) * (1.0 / kPerUnit);
+  double r = fma(z, 1.0 / 5040, 1.0 / 720);
+  r = fma(r, z, 1.0 / 120);
+  r = fma(r, z, 1.0 / 24);
+  r = fma(r, z, 1.0 / 6);
+  r = fma(r, z, 0.5);
+  r = fma(r, z, 1.0);
+  return fma(r, z, 1.0);
+}
+constexpr double kHalfBin = 0.96923323447634408;  // e^(-1/32)
+
+// Nearest integer of v in [0, 2^51)
+__device__ __forceinline__ u64 to_units(double v) {
+  return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull;
 }
 
-// One block per row.
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
-  __shared__ uint32_t cnt[256];
-  __shared__ unsigned long long mass[256];
-  __shared__ uint32_t s_key, s_n;
-  __shared__ unsigned long long s_mass;
-  __shared__ unsigned long long part[kThreads];
-  const int t = threadIdx.x;
-  const float *x = a.x + (size_t)blockIdx.x * a.stride;
-  if (t == 0) s_key = 0;
+// Accesses that other XCDs' L2s see without a fence.
+template <typename T>
+__device__ __forceinline__ void put(T *p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T get(const T *p) {
+  return __hip_atomic_load(const_cast<T *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+struct Shared {
+  u64 bins[kBins];  // packed sums of a slice, then the digits' weights
+  uint32_t cnt[256];
+  double tab[kBins];  // unit * e^(-b/16) * e^(-1/32)
+  u64 mass[kMaxSlices];
+  u64 wave[kWaves], pick, lo, hi;
+  double waved[kWaves];
+  double vd[4];
+  uint32_t v[8];
+  Plan plan;
+};
+
+// Inclusive sum over the block's threads; *total: all of them.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T *wave, T *total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T up = __shfl_up(v, o, 64);
+    if (lane >= o) v += up;
+  }
+  __syncthreads();  // wave is free
+  if (lane == 63) wave[w] = v;
   __syncthreads();
+  T before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) before += wave[i];
+    all += wave[i];
+  }
+  *total = all;
+  return before + v;
+}
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v, Shared &sm) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  if ((threadIdx.x & 63) == 0) sm.v[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) v = max(v, sm.v[i]);
+  return v;
+}
+
+// Whether this block is the last one of its row to get here (all of its coherent
+// stores done before).
+__device__ __forceinline__ bool last_block(uint32_t *count, int slices, Shared &sm) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t n = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sm.v[0] = n + 1 == (uint32_t)slices;
+    if (n + 1 == (uint32_t)slices) *count = 0;
+  }
+  __syncthreads();
+  const bool last = sm.v[0] != 0;
+  __syncthreads();
+  return last;
+}
+
+// The slice's logits in thread order, their keys, and the largest key.
+template <int E>
+__device__ __forceinline__ uint32_t load_slice(const SampleArgs &a, const float *x, int i0, int n,
+                                               uint32_t (&key)[E], Shared &sm) {
   uint32_t best = 0;
-  for (int i = t; i < a.vocab; i += kThreads) best = max(best, key_of(x[i]));
-  atomicMax(&s_key, best);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = threadIdx.x + NT * e;
+    key[e] = i < n ? key_of(x[i0 + i]) : 0;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) best = max(best, key[e]);
+  return block_max(best, sm);
+}
+
+// Count and mass of the slice's logits by bins below the largest one's.
+template <int E>
+__device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (&key)[E],
+                                           uint32_t best, Shared &sm) {
+  sm.bins[threadIdx.x] = 0;
   __syncthreads();
-  best = s_key;
-  if (best == 0) {
-    if (t == 0) {
-      a.tokens[blockIdx.x] = -1;
-      if (a.probs) a.probs[blockIdx.x] = 0.f;
-    }
-    return;
+  const double id = floor((double)logit_of(best) * a.s);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (key[e] == 0) continue;
+    const double y = (double)logit_of(key[e]) * a.s, fl = floor(y), db = id - fl;
+    if (db < kRest)
+      atomicAdd(&sm.bins[(int)db],
+                (1ull << kCountShift) + to_units(exp_part(y - fl) * (kBinUnit * kHalfBin)));
   }
-  const double top = logit_of(best);
-  auto d_of = [&](uint32_t key) { return ((double)logit_of(key) - top) * a.inv_t; };
-  // the cut: keys above `cut`, and the first `ties` that equal it
-  uint32_t cut = 1, ties = 0xffffffffu;
-  // One digit after the other: the key at which `want` tokens (or `want` mass) are
-  // reached from the top, and what is left of `want` there.
-  auto select = [&](bool by_mass, unsigned long long want, uint32_t lim, uint32_t lim_ties) {
-    uint32_t prefix = 0;
-    unsigned long long left = want, w_tie = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (t < 256) cnt[t] = 0, mass[t] = 0;
-      __syncthreads();
-      for (int i = t; i < a.vocab; i += kThreads) {
-        const uint32_t k = key_of(x[i]);
-        if (k == 0 || k < lim || (k ^ prefix) >> shift >> 8) continue;
-        const uint32_t bin = k >> shift & 255;
-        atomicAdd(&cnt[bin], 1u);
-        if (by_mass && k > lim) atomicAdd(&mass[bin], (unsigned long long)mass_of(d_of(k), a.unit));
-      }
-      __syncthreads();
-      if (t == 0) {
-        if (by_mass && lim > 1 && !((lim ^ prefix) >> shift >> 8)) {  // the ties that top-k kept
-          const uint64_t n = cnt[lim >> shift & 255] ? lim_ties : 0;
-          mass[lim >> shift & 255] += n * mass_of(d_of(lim), a.unit);
-        }
-        int b = 255;
-        unsigned long long l = left;
-        for (; b > 0; --b) {
-          const unsigned long long m = by_mass ? mass[b] : cnt[b];
-          if (m >= l) break;
-          l -= m;
-        }
-        s_n = b;
-        s_mass = l;
-      }
-      __syncthreads();
-      prefix |= s_n << shift;
-      left = s_mass;
-    }
-    cut = prefix;
-    if (by_mass) {
-      w_tie = mass_of(d_of(cut), a.unit);
-      const unsigned long long n = w_tie ? (left + w_tie - 1) / w_tie : 0;
-      ties = n < 0xffffffffull ? (uint32_t)n : 0xffffffffu;
-      if (cut == lim && lim_ties < ties) ties = lim_ties;
-    } else {
-      ties = (uint32_t)left;
-    }
-    __syncthreads();
-  };
-  auto block_sum = [&](unsigned long long v) {  // exclusive sum before this thread; total in s_mass
-    part[t] = v;
-    __syncthreads();
-    for (int o = 1; o < kThreads; o <<= 1) {
-      const unsigned long long w = t >= o ? part[t - o] : 0;
-      __syncthreads();
-      part[t] += w;
-      __syncthreads();
-    }
-    if (t == 0) s_mass = part[kThreads - 1];
-    const unsigned long long before = part[t] - v;
-    __syncthreads();
-    return before;
-  };
-  // each thread's run of consecutive tokens
-  const int per = (a.vocab + kThreads - 1) / kThreads;
-  const int i0 = min(t * per, a.vocab), i1 = min(i0 + per, a.vocab);
-  unsigned long long n_all = 0;
-  for (int i = i0; i < i1; ++i) n_all += key_of(x[i]) != 0;
-  block_sum(n_all);
-  const unsigned long long finite = s_mass;
-  if (a.top_k > 0 && (unsigned long long)a.top_k < finite) select(false, a.top_k, 1, 0);
-  auto kept_mass = [&]() {
-    unsigned long long eq = 0;
-    for (int i = i0; i < i1; ++i) eq += key_of(x[i]) == cut;
-    uint32_t rank = (uint32_t)block_sum(eq);
-    unsigned long long m = 0;
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t k = key_of(x[i]);
-      if (k == 0 || k < cut || (k == cut && rank++ >= ties)) continue;
-      const double d = d_of(k);
-      if (d >= a.log_min) m += mass_of(d, a.unit);
-    }
-    return m;
-  };
+  __syncthreads();
+}
+
+// The row's plan from the sums of its bins (thread t: bin t), in sm.plan.
+__device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32_t n, u64 bin_mass,
+                                          Shared &sm) {
+  const int b = threadIdx.x;
+  const double edge = exp(-(double)b / kPerUnit);
+  const double m = b < kRest ? (double)bin_mass * edge * (a.unit / kBinUnit) : 0.0;
+  double total;
+  u64 finite;
+  const double upto = block_scan(m, sm.waved, &total), before = upto - m;
+  const u64 n_upto = block_scan((u64)(b < kRest ? n : 0), sm.wave, &finite), n_before = n_upto - n;
+  Plan &p = sm.plan;
+  if (b == 0) {
+    p.id = floor((double)top * a.s);
+    p.top = top;
+    p.any = 1;
+    p.kb = -1;
+    p.k_left = 0;
+    p.lo = 1;
+    p.hi = 0;
+    p.sure = kBins;
+    p.before_k = 0;
+    p.total = total;
+    p.n = 0;
+    sm.vd[0] = sm.vd[1] = total;  // mass of top-k's tokens: at least, at most
+  }
+  __syncthreads();
+  const u64 k = a.top_k;
+  if (k > 0 && b < kRest && n_before < k && k <= n_upto) {
+    p.kb = b;
+    p.k_left = (uint32_t)(k - n_before);
+    p.before_k = before;
+    sm.vd[0] = before;
+    sm.vd[1] = upto;
+    p.sure = b;
+  }
+  __syncthreads();
   if (a.top_p < 1.0) {
-    const double log_min = a.log_min;
-    a.log_min = -INFINITY;
-    block_sum(kept_mass());
-    const unsigned long long want = (unsigned long long)ceil(a.top_p * (double)s_mass);
-    select(true, want, cut, ties);
-    a.log_min = log_min;
+    // the bins' sums are exact to 2^-38: a little room on both sides
+    const double lo = a.top_p * sm.vd[0] * (1 - 1e-10), hi = a.top_p * sm.vd[1] * (1 + 1e-10);
+    const int last = p.kb >= 0 ? p.kb : kRest - 1;
+    if (b == 0) p.lo = p.hi = last;
+    __syncthreads();
+    if (b < last && before < lo && lo <= upto) p.lo = b;
+    if (b < last && before < hi && hi <= upto) p.hi = b;
+    // (before the first bin: any positive mass wanted lies in it or below)
+    __syncthreads();
+    if (b == 0) p.sure = p.lo;
+    __syncthreads();
   }
-  const unsigned long long m = kept_mass();
-  const unsigned long long before = block_sum(m), total = s_mass;
-  const float u = a.u[blockIdx.x];
-  unsigned long long want = 0;  // the token is the first with a running mass above this
-  if (u >= 1.f) {
+  // min-p alone decides where everything in the cuts' bins is too small for it: there
+  // (max - x) * s > sure - 1
+  if (b == 0 && -a.log_min * kPerUnit + 0.01 <= p.sure - 1) {
+    p.kb = -1;
+    p.lo = 1;
+    p.hi = 0;
+    p.sure = kBins;
+  }
+  __syncthreads();
+}
+
+// A logit's place in the plan.
+struct Place {
+  int b;
+  double part, x;
+  __device__ Place(const SampleArgs &a, const Plan &p, uint32_t key) {
+    x = (double)logit_of(key);
+    const double y = x * a.s, fl = floor(y), db = p.id - fl;
+    b = db < kRest ? (int)db : kRest;
+    part = y - fl;
+  }
+  __device__ bool listed(const Plan &p) const { return (b >= p.lo && b <= p.hi) || b == p.kb; }
+  __device__ bool likely(const SampleArgs &a, const Plan &p) const {
+    return (x - (double)p.top) * a.inv_t >= a.log_min;
+  }
+  __device__ double mass(const Shared &sm) const { return b < kRest ? sm.tab[b] * exp_part(part) : 0.0; }
+};
+
+// A token in the order of the cuts: larger is earlier.
+__device__ __forceinline__ u64 rank_of(uint32_t key, int i) {
+  return (u64)key << 32 | (0xffffffffu - (uint32_t)i);
+}
+
+// Of the ranks that each() visits, the one at which the `want`-th unit of weight from the
+// top lies (want >= 1; the last one if there is less).
+template <typename Each, typename Weight>
+__device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, Shared &sm) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  if (t == 0) sm.lo = ~0ull, sm.hi = 0;
+  __syncthreads();
+  u64 lo = ~0ull, hi = 0;
+  each([&](u64 r) {
+    lo = r < lo ? r : lo;
+    hi = r > hi ? r : hi;
+  });
+  if (hi) {
+    atomicMin(&sm.lo, lo);
+    atomicMax(&sm.hi, hi);
+  }
+  __syncthreads();
+  lo = sm.lo;
+  hi = sm.hi;
+  if (lo >= hi) return hi;
+  int rem = 64 - __clzll(lo ^ hi);
+  u64 prefix = rem < 64 ? hi >> rem << rem : 0;
+  while (rem > 0) {
+    const int w = rem < 8 ? rem : 8, above = rem;
+    rem -= w;
+    __syncthreads();
+    if (t < 256) sm.bins[t] = 0, sm.cnt[t] = 0;
+    __syncthreads();
+    each([&](u64 r) {
+      if (above < 64 && (r ^ prefix) >> above) return;
+      const int d = (int)(r >> rem) & ((1 << w) - 1);
+      atomicAdd(&sm.bins[d], weight(r));
+      atomicAdd(&sm.cnt[d], 1u);
+    });
+    __syncthreads();
+    const u64 own = t < 256 ? sm.bins[255 - t] : 0;
+    const uint32_t n = t < 256 ? sm.cnt[255 - t] : 0;
+    u64 total;
+    const u64 upto = block_scan(own, sm.wave, &total);
+    if (want > total) want = total;
+    if (t == 0) sm.v[1] = 0, sm.v[2] = 0;
+    __syncthreads();
+    if (upto - own < want && want <= upto) {
+      sm.v[1] = 255 - t;
+      sm.v[2] = n;
+      sm.pick = upto - own;
+    }
+    __syncthreads();
+    prefix |= (u64)sm.v[1] << rem;
+    if (want > 0) want -= sm.pick;
+    const bool one = sm.v[2] == 1;
+    if (one && rem > 0) {  // a single token is left: itself
+      __syncthreads();
+      each([&](u64 r) {
+        if (r >> rem == prefix >> rem) sm.pick = r;
+      });
+      __syncthreads();
+      return sm.pick;
+    }
+  }
+  return prefix;
+}
+
+// The end of a row, for one block: the cuts among the listed tokens, the slice that holds
+// the picked mass, the token.  LIST: the tokens of the cuts' bins are in a.list (if they
+// fit), else they are found in the row again.  sm.plan and sm.tab are set; sm.mass holds
+// the slices' sure mass.
+template <bool LIST>
+__device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm) {
+  const int t = threadIdx.x;
+  const Plan &p = sm.plan;
+  auto bin_of = [&](u64 r) { return Place(a, p, (uint32_t)(r >> 32)).b; };
+  auto mass_of = [&](u64 r) { return to_units(Place(a, p, (uint32_t)(r >> 32)).mass(sm)); };
+  u64 cut = 0;
+  if (p.kb >= 0 || p.lo <= p.hi) {
+    const bool fits = LIST && p.n <= kList;
+    u64 mine[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine[i] = 0;
+    if (fits) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (NT * i < (int)p.n) {
+          const u64 r = get(a.list + (size_t)row * kList + min(NT * i + t, (int)p.n - 1));
+          mine[i] = NT * i + t < (int)p.n ? r : 0;
+        }
+    }
+    auto each_listed = [&](auto &&f) {
+      if (fits) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (mine[i]) f(mine[i]);
+      } else {
+        for (int i = t; i < a.vocab; i += NT) {
+          const uint32_t k = key_of(x[i]);
+          if (k && Place(a, p, k).listed(p)) f(rank_of(k, i));
+        }
+      }
+    };
+    auto sum = [&](u64 v) {
+      u64 total;
+      block_scan(v, sm.wave, &total);
+      return total;
+    };
+    double all = p.total;
+    u64 k_cut = 0;
+    if (p.kb >= 0) {
+      k_cut = select([&](auto &&f) { each_listed([&](u64 r) { if (bin_of(r) == p.kb) f(r); }); },
+                     [](u64) { return 1ull; }, p.k_left, sm);
+      if (p.lo <= p.hi) {
+        u64 m = 0;
+        each_listed([&](u64 r) { if (bin_of(r) == p.kb && r >= k_cut) m += mass_of(r); });
+        all = p.before_k + (double)sum(m);
+      }
+      cut = k_cut;
+    }
+    if (p.lo <= p.hi) {
+      // (where min-p drops any token above these bins, it drops all that lie in them, and
+      // it does not matter that the slices' mass lacks what top-p counts)
+      u64 above = 0;
+      for (int i = t; i < a.slices; i += NT) above += sm.mass[i];
+      above = sum(above);
+      const double want = ceil(a.top_p * all);
+      const u64 w = want > (double)above ? (u64)want - above : 1;
+      cut = select([&](auto &&f) {
+        each_listed([&](u64 r) {
+          const int b = bin_of(r);
+          if (b >= p.lo && b <= p.hi && r >= k_cut) f(r);
+        });
+      }, mass_of, w, sm);
+    }
+    __syncthreads();
+    each_listed([&](u64 r) {
+      if (r >= cut && Place(a, p, (uint32_t)(r >> 32)).likely(a, p))
+        atomicAdd(&sm.mass[(0xffffffffu - (uint32_t)r) / (uint32_t)a.per], mass_of(r));
+    });
+  }
+  if (t == 0) sm.v[0] = 0, sm.pick = 0;
+  __syncthreads();
+  // the slice
+  const u64 m0 = 2 * t < a.slices ? sm.mass[2 * t] : 0, m1 = 2 * t + 1 < a.slices ? sm.mass[2 * t + 1] : 0;
+  u64 total;
+  const u64 upto = block_scan(m0 + m1, sm.wave, &total);
+  const float u = a.u[row];
+  u64 want = 0;  // the token is the first with a running mass above this
+  if (u >= 1.f)
     want = total - 1;
-  } else if (u > 0.f) {
-    want = __umul64hi((unsigned long long)((double)u * 18446744073709551616.0), total);
+  else if (u > 0.f)
+    want = __umul64hi((u64)((double)u * 18446744073709551616.0), total);
+  const u64 before = upto - m0 - m1;
+  if (before <= want && want < upto) {
+    const bool second = want >= before + m0;
+    sm.v[0] = 2 * t + second;
+    sm.pick = want - before - (second ? m0 : 0);
   }
-  if (want < before || want >= before + m) return;
-  unsigned long long run = before;
-  uint32_t rank = 0;
-  if (ties != 0xffffffffu)
-    for (int i = 0; i < i0; ++i) rank += key_of(x[i]) == cut;
-  for (int i = i0; i < i1; ++i) {
+  __syncthreads();
+  // and in it, a run of consecutive tokens per thread
+  const int s0 = sm.v[0] * a.per, s1 = min(s0 + a.per, a.vocab);
+  want = sm.pick;
+  const int run = (s1 - s0 + NT - 1) / NT;
+  const int i0 = min(s0 + t * run, s1), i1 = min(i0 + run, s1);
+  auto kept = [&](int i, double *m) {
     const uint32_t k = key_of(x[i]);
-    if (k == 0 || k < cut || (k == cut && rank++ >= ties)) continue;
-    const double d = d_of(k);
-    if (d < a.log_min) continue;
-    run += mass_of(d, a.unit);
-    if (run > want) {
-      a.tokens[blockIdx.x] = i;
-      if (a.probs) a.probs[blockIdx.x] = (float)(exp(d) * a.unit / (double)total);
+    if (!k) return false;
+    const Place at(a, p, k);
+    if (at.b >= p.sure && !(at.listed(p) && rank_of(k, i) >= cut)) return false;
+    *m = at.mass(sm);
+    return at.likely(a, p);
+  };
+  u64 mine = 0, all_in;
+  for (int i = i0; i < i1; ++i) {
+    double m;
+    if (kept(i, &m)) mine += to_units(m);
+  }
+  u64 at = block_scan(mine, sm.wave, &all_in) - mine;
+  if (want < at || want >= at + mine) return;
+  for (int i = i0; i < i1; ++i) {
+    double m;
+    if (!kept(i, &m)) continue;
+    at += to_units(m);
+    if (at > want) {
+      a.tokens[row] = i;
+      if (a.probs) a.probs[row] = (float)(m / (double)total);
       return;
     }
   }
+}
+
+__device__ __forceinline__ void none_finite(const SampleArgs &a, int row) {
+  if (threadIdx.x == 0) {
+    a.tokens[row] = -1;
+    if (a.probs) a.probs[row] = 0.f;
+  }
+}
+
+__device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
+  sm.tab[threadIdx.x] = exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin);
+}
+
+template <int E>
+__global__ __launch_bounds__(NT) void sample_plan_kernel(SampleArgs a) {
+  __shared__ Shared sm;
+  const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+  const float *x = a.x + (size_t)row * a.stride;
+  const bool cuts = a.top_k > 0 || a.top_p < 1.0;
+  uint32_t key[E];
+  const int i0 = slice * a.per;
+  uint32_t best = load_slice<E>(a, x, i0, min(a.per, a.vocab - i0), key, sm);
+  uint32_t *maxes = a.maxes + (size_t)row * a.slices;
+  u64 *hist = a.hist + (size_t)row * a.slices * kBins;
+  if (cuts && best) {
+    slice_bins<E>(a, key, best, sm);
+    put(hist + (size_t)slice * kBins + t, sm.bins[t]);
+  }
+  if (t == 0) put(maxes + slice, best);
+  if (!last_block(a.count + row, a.slices, sm)) return;
+  best = 0;
+  for (int i = t; i < a.slices; i += NT) {
+    const uint32_t k = get(maxes + i);
+    reinterpret_cast<uint32_t *>(sm.mass)[i] = k;
+    best = max(best, k);
+  }
+  best = block_max(best, sm);
+  Plan *out = a.plan + row;
+  if (best == 0) {
+    none_finite(a, row);
+    if (t == 0) out->any = 0;
+    return;
+  }
+  const float top = logit_of(best);
+  const double id = floor((double)top * a.s);
+  uint32_t n = 0;
+  u64 m = 0;
+  if (cuts) {
+    // a batch of loads at a time; bins that a slice does not have re-read its bin t
+    constexpr int U = 16;
+    for (int i0 = 0; i0 < a.slices; i0 += U) {
+      u64 v[U];
+      bool has[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = min(i0 + j, a.slices - 1);
+        const uint32_t k = reinterpret_cast<const uint32_t *>(sm.mass)[i];
+        const double shift = k ? id - floor((double)logit_of(k) * a.s) : kBins;
+        const int b = t - (int)(shift < kBins ? shift : kBins);
+        has[j] = b >= 0 && i0 + j < a.slices;
+        v[j] = get(hist + (size_t)i * kBins + (b >= 0 ? b : t));
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (has[j]) {
+          n += (uint32_t)(v[j] >> kCountShift);
+          m += v[j] & ((1ull << kCountShift) - 1);
+        }
+    }
+  }
+  make_plan(a, top, n, m, sm);
+  if (t == 0) *out = sm.plan;
+}
+
+template <int E>
+__global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
+  __shared__ Shared sm;
+  const int t = threadIdx.x, lane = t & 63, slice = blockIdx.x, row = blockIdx.y;
+  const float *x = a.x + (size_t)row * a.stride;
+  Plan *plan = a.plan + row;
+  const int i0 = slice * a.per, n = min(a.per, a.vocab - i0);
+  uint32_t key[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = t + NT * e;
+    key[e] = i < n ? key_of(x[i0 + i]) : 0;
+  }
+  make_table(a, sm);
+  if (t == 0) sm.plan = *plan;
+  __syncthreads();
+  const Plan &p = sm.plan;
+  if (!p.any) return;
+  u64 m = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    bool list = false;
+    if (key[e]) {
+      const Place at(a, p, key[e]);
+      if (at.b < p.sure) {
+        if (at.likely(a, p)) m += to_units(at.mass(sm));
+      } else {
+        list = at.listed(p);
+      }
+    }
+    const u64 who = __ballot(list);
+    if (who) {
+      uint32_t base = 0;
+      if (lane == __ffsll((long long)who) - 1) base = atomicAdd(&plan->n, (uint32_t)__popcll(who));
+      base = __shfl((int)base, __ffsll((long long)who) - 1, 64);
+      const uint32_t pos = base + __popcll(who & ((1ull << lane) - 1));
+      if (list && pos < kList)
+        put(a.list + (size_t)row * kList + pos, rank_of(key[e], i0 + t + NT * e));
+    }
+  }
+  u64 total;
+  block_scan(m, sm.wave, &total);
+  u64 *mass = a.mass + (size_t)row * a.slices;
+  if (t == 0) put(mass + slice, total);
+  if (!last_block(a.count + kMaxRows + row, a.slices, sm)) return;
+  for (int i = t; i < a.slices; i += NT) sm.mass[i] = get(mass + i);
+  if (t == 0) sm.plan.n = get(&plan->n);
+  __syncthreads();
+  finish_row<true>(a, x, row, sm);
+}
+
+// Both halves for rows of one slice.
+template <int E>
+__global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
+  __shared__ Shared sm;
+  const int t = threadIdx.x, row = blockIdx.x;
+  const float *x = a.x + (size_t)row * a.stride;
+  uint32_t key[E];
+  const uint32_t best = load_slice<E>(a, x, 0, a.vocab, key, sm);
+  if (best == 0) {
+    none_finite(a, row);
+    return;
+  }
+  make_table(a, sm);
+  slice_bins<E>(a, key, best, sm);
+  make_plan(a, logit_of(best), (uint32_t)(sm.bins[t] >> kCountShift),
+            sm.bins[t] & ((1ull << kCountShift) - 1), sm);
+  const Plan &p = sm.plan;
+  u64 m = 0, total;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (key[e]) {
+      const Place at(a, p, key[e]);
+      if (at.b < p.sure && at.likely(a, p)) m += to_units(at.mass(sm));
+    }
+  block_scan(m, sm.wave, &total);
+  if (t == 0) sm.mass[0] = total;
+  __syncthreads();
+  finish_row<false>(a, x, row, sm);
+}
+
+Workspace g_sample_ws, g_sample_count;
+
+int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+// Rows of several slices, at most kMaxRows of them.
+int launch_slices(SampleArgs a, int rows) {
+  // 4096 logits to a slice, for one row's latency; longer ones where the rows fill the GPU
+  const int e = cdiv(a.vocab, 8 * NT) > kMaxSlices || (long)rows * cdiv(a.vocab, 8 * NT) > 2048 ? 32 : 8;
+  a.per = e * NT;
+  a.slices = cdiv(a.vocab, a.per);
+  const size_t n = (size_t)rows * a.slices;
+  const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
+  const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 8;
+  void *mem = nullptr, *count = nullptr;
+  int rc = g_sample_count.get(2 * kMaxRows * 4, &count, "g4_sample");  // zeros when new
+  if (!rc) rc = g_sample_ws.get(bytes, &mem, "g4_sample");
+  if (rc) return rc;
+  uint8_t *at = static_cast<uint8_t *>(mem);
+  a.plan = reinterpret_cast<Plan *>(at);
+  a.maxes = reinterpret_cast<uint32_t *>(at + plan);
+  a.mass = reinterpret_cast<u64 *>(at + plan + max);
+  a.list = a.mass + n;
+  a.hist = a.list + (size_t)rows * kList;
+  a.count = static_cast<uint32_t *>(count);
+  const dim3 grid(a.slices, rows);
+  hipLaunchKernelGGL(e == 8 ? sample_plan_kernel<8> : sample_plan_kernel<32>, grid, dim3(NT), 0,
+                     stream(), a);
+  G4_LAUNCH_CHECK("sample_plan_kernel");
+  hipLaunchKernelGGL(e == 8 ? sample_pick_kernel<8> : sample_pick_kernel<32>, grid, dim3(NT), 0,
+                     stream(), a);
+  G4_LAUNCH_CHECK("sample_pick_kernel");
+  return G4_OK;
+}
+
+int launch_sample(SampleArgs a, int rows) {
+  if (a.vocab <= kOneSlice) {
+    a.slices = 1;
+    a.per = kOneSlice;
+    hipLaunchKernelGGL(a.vocab <= 4 * NT ? sample_row_kernel<4> : sample_row_kernel<kOneSlice / NT>,
+                       dim3(rows), dim3(NT), 0, stream(), a);
+    G4_LAUNCH_CHECK("sample_row_kernel");
+    return G4_OK;
+  }
+  for (int r = 0; r < rows; r += kMaxRows) {
+    SampleArgs b = a;
+    b.x += (size_t)r * a.stride;
+    b.u += r;
+    b.tokens += r;
+    if (b.probs) b.probs += r;
+    if (int rc = launch_slices(b, rows - r < kMaxRows ? rows - r : kMaxRows)) return rc;
+  }
+  return G4_OK;
 }
 
 }  // namespace
@@ -198,8 +690,9 @@ using namespace g4;
 
 G4_API int g4_sample(const float *logits, size_t stride, int rows, int vocab,
                      const g4_sample_params *params, const float *u, int32_t *tokens, float *probs) {
-  if (rows < 0 || vocab <= 0 || stride < (size_t)vocab)
-    return fail(G4_E_ARG, "g4_sample: rows %d, vocab %d, stride %zu", rows, vocab, stride);
+  if (rows < 0 || vocab <= 0 || vocab > kMaxVocab || stride < (size_t)vocab)
+    return fail(G4_E_ARG, "g4_sample: rows %d, vocab %d (1..%d), stride %zu", rows, vocab, kMaxVocab,
+                stride);
   if (!params) return fail(G4_E_ARG, "g4_sample: null params");
   const g4_sample_params &p = *params;
   if (!(p.temperature >= 0.f) || !isfinite(p.temperature) || p.top_k < 0 || !(p.top_p > 0.f) ||
@@ -220,17 +713,18 @@ G4_API int g4_sample(const float *logits, size_t stride, int rows, int vocab,
   a.stride = stride;
   a.vocab = vocab;
   // temperature 0: the first of the largest alone
-  a.top_k = p.temperature > 0.f ? p.top_k : 1;
-  a.inv_t = p.temperature > 0.f ? 1.0 / (double)p.temperature : 0.0;
-  a.top_p = p.top_p;
-  a.log_min = log((double)p.min_p);
+  const bool greedy = p.temperature == 0.f;
+  a.top_k = greedy ? 1 : p.top_k;
+  a.inv_t = greedy ? 1.0 : 1.0 / (double)p.temperature;
+  a.s = kPerUnit * a.inv_t;
+  a.top_p = greedy ? 1.0 : (double)p.top_p;
+  a.log_min = greedy ? -INFINITY : log((double)p.min_p);
   int bits = 0;
-  while (bits < 31 && (1u << bits) < (unsigned)vocab) ++bits;
-  a.unit = ldexp(1.0, 62 - bits < 52 ? 62 - bits : 52);
+  while ((1 << bits) < vocab) ++bits;
+  a.unit = ldexp(1.0, bits > 12 ? 62 - bits : 50);
   a.u = u;
   a.tokens = tokens;
   a.probs = probs;
-  hipLaunchKernelGGL(sample_row_kernel, dim3(rows), dim3(kThreads), 0, stream(), a);
-  G4_LAUNCH_CHECK("sample_row_kernel");
-  return ok();
+  rc = launch_sample(a, rows);
+  return rc ? rc : ok();
 }
