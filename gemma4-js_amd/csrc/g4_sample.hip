@@ -7,14 +7,14 @@
 //   min-p  those with p >= min_p
 // The token is the first one, by index, up to which more than u * (kept mass) lies.
 //
-// Numerics.  A token's border may lie next to u, so borders are binary64 and masses are
+// Numerics.  A token's border may lie next to u, so d is binary64 and masses are
 // integers: round(p * 2^k), 2^k * vocab < 2^62, whose sums do not depend on their order.
-// e^d is e^(-b/16) (a table) times e^((f-1)/16) (a polynomial, exact to 2^-53), b and f
-// from x * 16 / temperature = whole part and fraction; below e^-31 a mass counts as 0
+// e^d is e^(-b/8) (a table) times e^((f-1)/8) (a polynomial, exact to 2^-53), b and f
+// from x * 8 / temperature = whole part and fraction; below e^-31 a mass counts as 0
 // (2^-44, a unit of the sums at 262144 tokens).
 //
 // Two launches over slices of the rows; each one's last block of a row goes on alone:
-//   sample_plan_kernel  per slice the largest logit and, by whole part of x * 16 / T,
+//   sample_plan_kernel  per slice the largest logit and, by whole part of x * 8 / T,
 //                       count and mass; the row's last block finds the bins in which the
 //                       cuts lie (bins above them are kept, those below dropped)
 //   sample_pick_kernel  the kept mass of every slice, and a list of the tokens in those
@@ -23,6 +23,8 @@
 // A row of one slice takes both halves in one launch (sample_row_kernel).
 #include <math.h>
 
+#include <type_traits>
+
 #include "g4_internal.h"
 
 namespace g4 {
@@ -30,25 +32,22 @@ namespace {
 
 constexpr int NT = 512;       // threads per block
 constexpr int kWaves = NT / 64;
-constexpr int kBins = NT;     // one thread each; the last one holds the rest
+constexpr int kBins = 256;    // the last one holds the rest
 constexpr int kRest = kBins - 1;
-constexpr double kPerUnit = 16.0;  // bins per unit of d
-constexpr int kPer = 16;           // listed tokens per thread
-constexpr int kList = kPer * NT;
+constexpr double kPerUnit = 8.0;   // bins per unit of d
+constexpr int kList = 16384;       // listed tokens of a row
+constexpr int kFew = 128;          // tokens that are compared with each other
 constexpr int kMaxRows = 256;      // rows per launch
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxSlices = 2 * NT;
 constexpr int kOneSlice = 8192;    // longest row of one slice
-// a bin's packed sum: count << 50 | mass in units of 2^-38 of the bin's upper edge
-constexpr int kCountShift = 50;
-constexpr double kBinUnit = 274877906944.0;
 typedef unsigned long long u64;
 
 // What the first launch leaves for the second.
 struct Plan {
   double id;        // whole part of max * s
-  double before_k;  // mass above top-k's bin
-  double total;     // mass of all bins
+  u64 before_k;     // mass above top-k's bin
+  u64 total;        // mass of all bins
   float top;        // largest logit
   int any;          // 0: no finite logit
   int sure;         // bins below this one are kept (but for min-p)
@@ -62,12 +61,14 @@ struct SampleArgs {
   const float *x;
   size_t stride;
   int vocab, top_k, slices, per;
-  double inv_t, s, top_p, log_min, unit;
+  u64 top_p64;  // top_p * 2^64, 0: no such cut
+  double inv_t, s, log_min, unit;
   const float *u;
   int *tokens;
   float *probs;
   Plan *plan;
-  u64 *hist;        // [rows][slices][kBins]
+  u64 *hist;        // [rows][slices][kBins] masses
+  uint32_t *counts; // and counts
   uint32_t *maxes;  // [rows][slices] keys
   u64 *list;        // [rows][kList]
   u64 *mass;        // [rows][slices]
@@ -84,10 +85,11 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// e^((f - 1/2) / 16), f in [0, 1): |z| <= 1/32, z^8 / 8! < 2^-55
+// e^((f - 1/2) / 8), f in [0, 1): |z| <= 1/16, z^9 / 9! < 2^-54
 __device__ __forceinline__ double exp_part(double f) {
   const double z = (f - 0.5) * (1.0 / kPerUnit);
-  double r = fma(z, 1.0 / 5040, 1.0 / 720);
+  double r = fma(z, 1.0 / 40320, 1.0 / 5040);
+  r = fma(r, z, 1.0 / 720);
   r = fma(r, z, 1.0 / 120);
   r = fma(r, z, 1.0 / 24);
   r = fma(r, z, 1.0 / 6);
@@ -95,7 +97,7 @@ __device__ __forceinline__ double exp_part(double f) {
   r = fma(r, z, 1.0);
   return fma(r, z, 1.0);
 }
-constexpr double kHalfBin = 0.96923323447634408;  // e^(-1/32)
+constexpr double kHalfBin = 0.93941306281347579;  // e^(-1/16)
 
 // Nearest integer of v in [0, 2^51)
 __device__ __forceinline__ u64 to_units(double v) {
@@ -113,26 +115,35 @@ __device__ __forceinline__ T get(const T *p) {
 }
 
 struct Shared {
-  u64 bins[kBins];  // packed sums of a slice, then the digits' weights
-  uint32_t cnt[256];
-  double tab[kBins];  // unit * e^(-b/16) * e^(-1/32)
+  u64 bins[2][kBins];  // masses of a slice's bins by wave parity; the digits' weights
+  uint32_t cnt[2][kBins];
+  double tab[kBins];   // unit * e^(-b/8) * e^(-1/16)
   u64 mass[kMaxSlices];
+  u64 few[kFew], weight[kFew];
   u64 wave[kWaves], pick, lo, hi;
-  double waved[kWaves];
-  double vd[4];
-  uint32_t v[8];
+  uint32_t v[8], n;
   Plan plan;
 };
+
+// v of an earlier lane (0 where there is none), as DPP moves of its halves
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_before(T v) {
+  const u64 b = __builtin_bit_cast(u64, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+}
 
 // Inclusive sum over the block's threads; *total: all of them.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T *wave, T *total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T up = __shfl_up(v, o, 64);
-    if (lane >= o) v += up;
-  }
+  v += lane_before<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8 in rows of 16 lanes
+  v += lane_before<0x112, 0xf>(v);
+  v += lane_before<0x114, 0xf>(v);
+  v += lane_before<0x118, 0xf>(v);
+  v += lane_before<0x142, 0xa>(v);  // row_bcast:15 to rows 1 and 3
+  v += lane_before<0x143, 0xc>(v);  // row_bcast:31 to rows 2 and 3
   __syncthreads();  // wave is free
   if (lane == 63) wave[w] = v;
   __syncthreads();
@@ -187,34 +198,37 @@ __device__ __forceinline__ uint32_t load_slice(const SampleArgs &a, const float 
   return block_max(best, sm);
 }
 
-// Count and mass of the slice's logits by bins below the largest one's.
+// Count and mass of the slice's logits by bins below the largest one's (as far as the
+// cuts ask for them), each in two parts.  A mass is in units of 1 / a.unit of its bin's
+// upper edge.
 template <int E>
 __device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (&key)[E],
                                            uint32_t best, Shared &sm) {
-  sm.bins[threadIdx.x] = 0;
+  sm.bins[0][threadIdx.x] = 0;  // both parts
+  sm.cnt[0][threadIdx.x] = 0;
   __syncthreads();
-  const double id = floor((double)logit_of(best) * a.s);
+  const double id = floor((double)logit_of(best) * a.s), unit = a.unit * kHalfBin;
+  const int part = threadIdx.x >> 6 & 1;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (key[e] == 0) continue;
     const double y = (double)logit_of(key[e]) * a.s, fl = floor(y), db = id - fl;
-    if (db < kRest)
-      atomicAdd(&sm.bins[(int)db],
-                (1ull << kCountShift) + to_units(exp_part(y - fl) * (kBinUnit * kHalfBin)));
+    if (db < kRest) {
+      if (a.top_p64) atomicAdd(&sm.bins[part][(int)db], to_units(exp_part(y - fl) * unit));
+      if (a.top_k) atomicAdd(&sm.cnt[part][(int)db], 1u);
+    }
   }
   __syncthreads();
 }
 
-// The row's plan from the sums of its bins (thread t: bin t), in sm.plan.
+// The row's plan from the sums of its bins (thread t < kBins: bin t; the others 0), in
+// sm.plan.
 __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32_t n, u64 bin_mass,
                                           Shared &sm) {
   const int b = threadIdx.x;
-  const double edge = exp(-(double)b / kPerUnit);
-  const double m = b < kRest ? (double)bin_mass * edge * (a.unit / kBinUnit) : 0.0;
-  double total;
-  u64 finite;
-  const double upto = block_scan(m, sm.waved, &total), before = upto - m;
-  const u64 n_upto = block_scan((u64)(b < kRest ? n : 0), sm.wave, &finite), n_before = n_upto - n;
+  // (bin 0 as it is: equal logits alone have borders at round shares of their mass)
+  const u64 m = b == 0 ? bin_mass : b < kRest ? (u64)((double)bin_mass * exp(-(double)b / kPerUnit)) : 0;
+  u64 total, finite;
   Plan &p = sm.plan;
   if (b == 0) {
     p.id = floor((double)top * a.s);
@@ -226,32 +240,37 @@ __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32
     p.hi = 0;
     p.sure = kBins;
     p.before_k = 0;
-    p.total = total;
     p.n = 0;
-    sm.vd[0] = sm.vd[1] = total;  // mass of top-k's tokens: at least, at most
+  }
+  const u64 upto = block_scan(m, sm.wave, &total), before = upto - m;
+  const u64 own = b < kRest ? n : 0, n_upto = block_scan(own, sm.wave, &finite), n_before = n_upto - own;
+  const u64 k = a.top_k;
+  if (b == 0) {
+    p.total = total;
+    sm.lo = sm.hi = total;  // mass of top-k's tokens: at least, at most
   }
   __syncthreads();
-  const u64 k = a.top_k;
-  if (k > 0 && b < kRest && n_before < k && k <= n_upto) {
+  if (b < kRest && n_before < k && k <= n_upto) {
     p.kb = b;
     p.k_left = (uint32_t)(k - n_before);
     p.before_k = before;
-    sm.vd[0] = before;
-    sm.vd[1] = upto;
+    sm.lo = before;
+    sm.hi = upto;
     p.sure = b;
   }
   __syncthreads();
-  if (a.top_p < 1.0) {
-    // the bins' sums are exact to 2^-38: a little room on both sides
-    const double lo = a.top_p * sm.vd[0] * (1 - 1e-10), hi = a.top_p * sm.vd[1] * (1 + 1e-10);
+  if (a.top_p64) {
+    // a bin's sum is off by what its tokens' masses are rounded by
+    const u64 room = (total >> 30) + a.vocab;
+    u64 lo = __umul64hi(a.top_p64, sm.lo);
+    const u64 hi = __umul64hi(a.top_p64, sm.hi) + room;
+    lo = lo > room ? lo - room : 0;
     const int last = p.kb >= 0 ? p.kb : kRest - 1;
-    if (b == 0) p.lo = p.hi = last;
     __syncthreads();
-    if (b < last && before < lo && lo <= upto) p.lo = b;
+    if (b == 0) p.lo = p.sure = lo ? last : 0, p.hi = last;
+    __syncthreads();
+    if (b < last && before < lo && lo <= upto) p.lo = p.sure = b;
     if (b < last && before < hi && hi <= upto) p.hi = b;
-    // (before the first bin: any positive mass wanted lies in it or below)
-    __syncthreads();
-    if (b == 0) p.sure = p.lo;
     __syncthreads();
   }
   // min-p alone decides where everything in the cuts' bins is too small for it: there
@@ -288,67 +307,92 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, int i) {
 }
 
 // Of the ranks that each() visits, the one at which the `want`-th unit of weight from the
-// top lies (want >= 1; the last one if there is less).
+// top lies (want >= 1; the last one if there is less).  A digit of 8 bits after the other
+// until kFew are left (`few`: there are no more), which are then compared pairwise.
 template <typename Each, typename Weight>
-__device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, Shared &sm) {
+__device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, bool few, Shared &sm) {
   const int t = threadIdx.x;
+  int rem = 64;
+  u64 prefix = 0;
   __syncthreads();
-  if (t == 0) sm.lo = ~0ull, sm.hi = 0;
+  if (t == 0) sm.lo = ~0ull, sm.hi = 0, sm.n = 0;
   __syncthreads();
-  u64 lo = ~0ull, hi = 0;
-  each([&](u64 r) {
-    lo = r < lo ? r : lo;
-    hi = r > hi ? r : hi;
-  });
-  if (hi) {
-    atomicMin(&sm.lo, lo);
-    atomicMax(&sm.hi, hi);
-  }
-  __syncthreads();
-  lo = sm.lo;
-  hi = sm.hi;
-  if (lo >= hi) return hi;
-  int rem = 64 - __clzll(lo ^ hi);
-  u64 prefix = rem < 64 ? hi >> rem << rem : 0;
-  while (rem > 0) {
-    const int w = rem < 8 ? rem : 8, above = rem;
-    rem -= w;
-    __syncthreads();
-    if (t < 256) sm.bins[t] = 0, sm.cnt[t] = 0;
-    __syncthreads();
+  if (!few) {
+    u64 lo = ~0ull, hi = 0;
+    uint32_t n = 0;
     each([&](u64 r) {
-      if (above < 64 && (r ^ prefix) >> above) return;
-      const int d = (int)(r >> rem) & ((1 << w) - 1);
-      atomicAdd(&sm.bins[d], weight(r));
-      atomicAdd(&sm.cnt[d], 1u);
+      lo = r < lo ? r : lo;
+      hi = r > hi ? r : hi;
+      ++n;
     });
-    __syncthreads();
-    const u64 own = t < 256 ? sm.bins[255 - t] : 0;
-    const uint32_t n = t < 256 ? sm.cnt[255 - t] : 0;
-    u64 total;
-    const u64 upto = block_scan(own, sm.wave, &total);
-    if (want > total) want = total;
-    if (t == 0) sm.v[1] = 0, sm.v[2] = 0;
-    __syncthreads();
-    if (upto - own < want && want <= upto) {
-      sm.v[1] = 255 - t;
-      sm.v[2] = n;
-      sm.pick = upto - own;
+    if (n) {
+      atomicMin(&sm.lo, lo);
+      atomicMax(&sm.hi, hi);
+      atomicAdd(&sm.n, n);
     }
     __syncthreads();
-    prefix |= (u64)sm.v[1] << rem;
-    if (want > 0) want -= sm.pick;
-    const bool one = sm.v[2] == 1;
-    if (one && rem > 0) {  // a single token is left: itself
+    lo = sm.lo;
+    hi = sm.hi;
+    n = sm.n;
+    if (lo >= hi) return hi;
+    rem = 64 - __clzll(lo ^ hi);
+    prefix = rem < 64 ? hi >> rem << rem : 0;
+    while (rem > 0 && n > kFew) {
+      const int w = rem < 8 ? rem : 8, above = rem;
+      rem -= w;
+      __syncthreads();
+      if (t < 256) sm.bins[0][t] = 0, sm.cnt[0][t] = 0;
+      if (t == 0) sm.v[1] = 0, sm.v[2] = 0, sm.pick = 0;
       __syncthreads();
       each([&](u64 r) {
-        if (r >> rem == prefix >> rem) sm.pick = r;
+        if (above < 64 && (r ^ prefix) >> above) return;
+        const int d = (int)(r >> rem) & ((1 << w) - 1);
+        atomicAdd(&sm.bins[0][d], weight(r));
+        atomicAdd(&sm.cnt[0][d], 1u);
       });
       __syncthreads();
-      return sm.pick;
+      const u64 own = t < 256 ? sm.bins[0][255 - t] : 0;
+      u64 total;
+      const u64 upto = block_scan(own, sm.wave, &total);
+      if (want > total) want = total;
+      if (upto - own < want && want <= upto) {
+        sm.v[1] = 255 - t;
+        sm.v[2] = sm.cnt[0][255 - t];
+        sm.pick = upto - own;
+      }
+      __syncthreads();
+      prefix |= (u64)sm.v[1] << rem;
+      n = sm.v[2];
+      want -= sm.pick;
     }
+    if (rem == 0) return prefix;
+    if (t == 0) sm.n = 0;
+    __syncthreads();
   }
-  return prefix;
+  if (t == 0) sm.pick = 0;
+  each([&](u64 r) {
+    if (rem < 64 && (r ^ prefix) >> rem) return;
+    const uint32_t at = atomicAdd(&sm.n, 1u);
+    sm.few[at] = r;
+    sm.weight[at] = weight(r);
+  });
+  __syncthreads();
+  const int n = sm.n;
+  if (t < n) {
+    const u64 r = sm.few[t], own = sm.weight[t];
+    u64 before = 0, total = 0;
+    for (int i = 0; i < n; ++i) {
+      const u64 w = sm.weight[i];
+      total += w;
+      if (sm.few[i] > r) before += w;
+    }
+    if (want > total) want = total;
+    if (before < want && want <= before + own) sm.pick = r;
+  }
+  __syncthreads();
+  const u64 got = sm.pick;
+  __syncthreads();
+  return got;
 }
 
 // The end of a row, for one block: the cuts among the listed tokens, the slice that holds
@@ -363,23 +407,12 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   auto mass_of = [&](u64 r) { return to_units(Place(a, p, (uint32_t)(r >> 32)).mass(sm)); };
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
-    const bool fits = LIST && p.n <= kList;
-    u64 mine[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) mine[i] = 0;
-    if (fits) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (NT * i < (int)p.n) {
-          const u64 r = get(a.list + (size_t)row * kList + min(NT * i + t, (int)p.n - 1));
-          mine[i] = NT * i + t < (int)p.n ? r : 0;
-        }
-    }
+    const bool fits = LIST && p.n <= kList, few = LIST && p.n <= kFew;
+    const u64 first = fits && t < (int)p.n ? get(a.list + (size_t)row * kList + t) : 0;
     auto each_listed = [&](auto &&f) {
       if (fits) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (mine[i]) f(mine[i]);
+        if (first) f(first);
+        for (int i = t + NT; i < (int)p.n; i += NT) f(get(a.list + (size_t)row * kList + i));
       } else {
         for (int i = t; i < a.vocab; i += NT) {
           const uint32_t k = key_of(x[i]);
@@ -392,15 +425,15 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       block_scan(v, sm.wave, &total);
       return total;
     };
-    double all = p.total;
+    u64 all = p.total;
     u64 k_cut = 0;
     if (p.kb >= 0) {
       k_cut = select([&](auto &&f) { each_listed([&](u64 r) { if (bin_of(r) == p.kb) f(r); }); },
-                     [](u64) { return 1ull; }, p.k_left, sm);
+                     [](u64) { return 1ull; }, p.k_left, few, sm);
       if (p.lo <= p.hi) {
         u64 m = 0;
         each_listed([&](u64 r) { if (bin_of(r) == p.kb && r >= k_cut) m += mass_of(r); });
-        all = p.before_k + (double)sum(m);
+        all = p.before_k + sum(m);
       }
       cut = k_cut;
     }
@@ -410,21 +443,21 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       u64 above = 0;
       for (int i = t; i < a.slices; i += NT) above += sm.mass[i];
       above = sum(above);
-      const double want = ceil(a.top_p * all);
-      const u64 w = want > (double)above ? (u64)want - above : 1;
+      const u64 want = __umul64hi(a.top_p64, all) + (a.top_p64 * all != 0);  // rounded up
+      const u64 w = want > above ? want - above : 1;
       cut = select([&](auto &&f) {
         each_listed([&](u64 r) {
           const int b = bin_of(r);
           if (b >= p.lo && b <= p.hi && r >= k_cut) f(r);
         });
-      }, mass_of, w, sm);
+      }, mass_of, w, few, sm);
     }
-    __syncthreads();
     each_listed([&](u64 r) {
       if (r >= cut && Place(a, p, (uint32_t)(r >> 32)).likely(a, p))
         atomicAdd(&sm.mass[(0xffffffffu - (uint32_t)r) / (uint32_t)a.per], mass_of(r));
     });
   }
+  __syncthreads();
   if (t == 0) sm.v[0] = 0, sm.pick = 0;
   __syncthreads();
   // the slice
@@ -484,7 +517,8 @@ __device__ __forceinline__ void none_finite(const SampleArgs &a, int row) {
 }
 
 __device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
-  sm.tab[threadIdx.x] = exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin);
+  if (threadIdx.x < kBins)
+    sm.tab[threadIdx.x] = exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin);
 }
 
 template <int E>
@@ -492,15 +526,19 @@ __global__ __launch_bounds__(NT) void sample_plan_kernel(SampleArgs a) {
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
-  const bool cuts = a.top_k > 0 || a.top_p < 1.0;
+  const bool cuts = a.top_k || a.top_p64;
   uint32_t key[E];
   const int i0 = slice * a.per;
   uint32_t best = load_slice<E>(a, x, i0, min(a.per, a.vocab - i0), key, sm);
   uint32_t *maxes = a.maxes + (size_t)row * a.slices;
   u64 *hist = a.hist + (size_t)row * a.slices * kBins;
+  uint32_t *counts = a.counts + (size_t)row * a.slices * kBins;
   if (cuts && best) {
     slice_bins<E>(a, key, best, sm);
-    put(hist + (size_t)slice * kBins + t, sm.bins[t]);
+    if (t < kBins) {
+      if (a.top_p64) put(hist + (size_t)slice * kBins + t, sm.bins[0][t] + sm.bins[1][t]);
+      if (a.top_k) put(counts + (size_t)slice * kBins + t, sm.cnt[0][t] + sm.cnt[1][t]);
+    }
   }
   if (t == 0) put(maxes + slice, best);
   if (!last_block(a.count + row, a.slices, sm)) return;
@@ -519,30 +557,42 @@ __global__ __launch_bounds__(NT) void sample_plan_kernel(SampleArgs a) {
   }
   const float top = logit_of(best);
   const double id = floor((double)top * a.s);
+  auto shift_of = [&](uint32_t k) {  // bins from the row's largest logit to the slice's
+    const double d = k ? id - floor((double)logit_of(k) * a.s) : kBins;
+    return d < kBins ? d : (double)kBins;
+  };
   uint32_t n = 0;
   u64 m = 0;
   if (cuts) {
-    // a batch of loads at a time; bins that a slice does not have re-read its bin t
-    constexpr int U = 16;
-    for (int i0 = 0; i0 < a.slices; i0 += U) {
-      u64 v[U];
-      bool has[U];
+    // threads t and t + kBins take every other slice's bin t, a batch of loads at a time;
+    // bins that a slice does not have re-read its bin t
+    constexpr int U = 32;
+    const int bin = t & (kBins - 1);
+    auto add = [&](const auto *from, auto &to) {
+      for (int i0 = t / kBins; i0 < a.slices; i0 += 2 * U) {
+        std::remove_reference_t<decltype(to)> v[U];
+        bool has[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = min(i0 + j, a.slices - 1);
-        const uint32_t k = reinterpret_cast<const uint32_t *>(sm.mass)[i];
-        const double shift = k ? id - floor((double)logit_of(k) * a.s) : kBins;
-        const int b = t - (int)(shift < kBins ? shift : kBins);
-        has[j] = b >= 0 && i0 + j < a.slices;
-        v[j] = get(hist + (size_t)i * kBins + (b >= 0 ? b : t));
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (has[j]) {
-          n += (uint32_t)(v[j] >> kCountShift);
-          m += v[j] & ((1ull << kCountShift) - 1);
+        for (int j = 0; j < U; ++j) {
+          const int i = min(i0 + 2 * j, a.slices - 1);
+          const int b = bin - (int)shift_of(reinterpret_cast<const uint32_t *>(sm.mass)[i]);
+          has[j] = b >= 0 && i0 + 2 * j < a.slices;
+          v[j] = get(from + (size_t)i * kBins + (b >= 0 ? b : bin));
         }
-    }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if (has[j]) to += v[j];
+      }
+    };
+    if (a.top_p64) add(hist, m);
+    if (a.top_k) add(counts, n);
+    __syncthreads();
+    if (t >= kBins) sm.bins[0][bin] = m, sm.cnt[0][bin] = n;
+    __syncthreads();
+    if (t < kBins)
+      m += sm.bins[0][t], n += sm.cnt[0][t];
+    else
+      m = n = 0;
   }
   make_plan(a, top, n, m, sm);
   if (t == 0) *out = sm.plan;
@@ -551,7 +601,7 @@ __global__ __launch_bounds__(NT) void sample_plan_kernel(SampleArgs a) {
 template <int E>
 __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   __shared__ Shared sm;
-  const int t = threadIdx.x, lane = t & 63, slice = blockIdx.x, row = blockIdx.y;
+  const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
   Plan *plan = a.plan + row;
   const int i0 = slice * a.per, n = min(a.per, a.vocab - i0);
@@ -567,29 +617,31 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   const Plan &p = sm.plan;
   if (!p.any) return;
   u64 m = 0;
+  uint32_t listed = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    bool list = false;
-    if (key[e]) {
-      const Place at(a, p, key[e]);
-      if (at.b < p.sure) {
-        if (at.likely(a, p)) m += to_units(at.mass(sm));
-      } else {
-        list = at.listed(p);
-      }
-    }
-    const u64 who = __ballot(list);
-    if (who) {
-      uint32_t base = 0;
-      if (lane == __ffsll((long long)who) - 1) base = atomicAdd(&plan->n, (uint32_t)__popcll(who));
-      base = __shfl((int)base, __ffsll((long long)who) - 1, 64);
-      const uint32_t pos = base + __popcll(who & ((1ull << lane) - 1));
-      if (list && pos < kList)
-        put(a.list + (size_t)row * kList + pos, rank_of(key[e], i0 + t + NT * e));
+    if (key[e] == 0) continue;
+    const Place at(a, p, key[e]);
+    if (at.b < p.sure) {
+      if (at.likely(a, p)) m += to_units(at.mass(sm));
+    } else if (at.listed(p)) {
+      listed |= 1u << e;
     }
   }
-  u64 total;
+  u64 total, found;
   block_scan(m, sm.wave, &total);
+  const u64 own = __popc(listed), upto = block_scan(own, sm.wave, &found);
+  if (found) {
+    if (t == 0) sm.n = atomicAdd(&plan->n, (uint32_t)found);
+    __syncthreads();
+    uint32_t pos = sm.n + (uint32_t)(upto - own);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (listed >> e & 1) {
+        if (pos < kList) put(a.list + (size_t)row * kList + pos, rank_of(key[e], i0 + t + NT * e));
+        ++pos;
+      }
+  }
   u64 *mass = a.mass + (size_t)row * a.slices;
   if (t == 0) put(mass + slice, total);
   if (!last_block(a.count + kMaxRows + row, a.slices, sm)) return;
@@ -613,8 +665,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   }
   make_table(a, sm);
   slice_bins<E>(a, key, best, sm);
-  make_plan(a, logit_of(best), (uint32_t)(sm.bins[t] >> kCountShift),
-            sm.bins[t] & ((1ull << kCountShift) - 1), sm);
+  make_plan(a, logit_of(best), t < kBins ? sm.cnt[0][t] + sm.cnt[1][t] : 0,
+            t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0, sm);
   const Plan &p = sm.plan;
   u64 m = 0, total;
 #pragma unroll
@@ -641,7 +693,7 @@ int launch_slices(SampleArgs a, int rows) {
   a.slices = cdiv(a.vocab, a.per);
   const size_t n = (size_t)rows * a.slices;
   const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
-  const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 8;
+  const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 12;
   void *mem = nullptr, *count = nullptr;
   int rc = g_sample_count.get(2 * kMaxRows * 4, &count, "g4_sample");  // zeros when new
   if (!rc) rc = g_sample_ws.get(bytes, &mem, "g4_sample");
@@ -652,6 +704,7 @@ int launch_slices(SampleArgs a, int rows) {
   a.mass = reinterpret_cast<u64 *>(at + plan + max);
   a.list = a.mass + n;
   a.hist = a.list + (size_t)rows * kList;
+  a.counts = reinterpret_cast<uint32_t *>(a.hist + n * kBins);
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
   hipLaunchKernelGGL(e == 8 ? sample_plan_kernel<8> : sample_plan_kernel<32>, grid, dim3(NT), 0,
@@ -714,10 +767,13 @@ G4_API int g4_sample(const float *logits, size_t stride, int rows, int vocab,
   a.vocab = vocab;
   // temperature 0: the first of the largest alone
   const bool greedy = p.temperature == 0.f;
-  a.top_k = greedy ? 1 : p.top_k;
+  a.top_k = greedy ? 1 : p.top_k < vocab ? p.top_k : 0;
   a.inv_t = greedy ? 1.0 : 1.0 / (double)p.temperature;
   a.s = kPerUnit * a.inv_t;
-  a.top_p = greedy ? 1.0 : (double)p.top_p;
+  if (!greedy && p.top_p < 1.f) {
+    a.top_p64 = (u64)ldexp((double)p.top_p, 64);
+    if (a.top_p64 == 0) a.top_p64 = 1;
+  }
   a.log_min = greedy ? -INFINITY : log((double)p.min_p);
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
