@@ -13,14 +13,15 @@
 // from x * 8 / temperature = whole part and fraction; below e^-31 a mass counts as 0
 // (2^-44, a unit of the sums at 262144 tokens).
 //
-// Two launches over slices of the rows; each one's last block of a row goes on alone:
+// Two launches over slices of 4096 logits; each one's last block of a row goes on alone:
 //   sample_plan_kernel  per slice the largest logit and, by whole part of x * 8 / T,
 //                       count and mass; the row's last block finds the bins in which the
 //                       cuts lie (bins above them are kept, those below dropped)
 //   sample_pick_kernel  the kept mass of every slice, and a list of the tokens in those
 //                       bins; the row's last block finds the cuts among them, the slice
 //                       and the token
-// A row of one slice takes both halves in one launch (sample_row_kernel).
+// With the temperature alone the first launch ends the row, and a row of one slice takes
+// it all in one launch (sample_row_kernel).
 #include <math.h>
 
 #include <type_traits>
@@ -36,10 +37,13 @@ constexpr int kBins = 256;    // the last one holds the rest
 constexpr int kRest = kBins - 1;
 constexpr double kPerUnit = 8.0;   // bins per unit of d
 constexpr int kList = 16384;       // listed tokens of a row
+constexpr int kNear = 4096;        // of these in LDS
 constexpr int kFew = 128;          // tokens that are compared with each other
 constexpr int kMaxRows = 256;      // rows per launch
-constexpr int kMaxVocab = 1 << 24;
+constexpr int kE = 8;              // logits of a slice per thread
+constexpr int kSlice = kE * NT;
 constexpr int kMaxSlices = 2 * NT;
+constexpr int kMaxVocab = kMaxSlices * kSlice;
 constexpr int kOneSlice = 8192;    // longest row of one slice
 typedef unsigned long long u64;
 
@@ -50,11 +54,13 @@ struct Plan {
   u64 total;        // mass of all bins
   float top;        // largest logit
   int any;          // 0: no finite logit
-  int sure;         // bins below this one are kept (but for min-p)
+  int sure;         // bins below this one are kept,
+  int part;         // and from there to below this one what min-p leaves
   int lo, hi;       // bins in which top-p's cut may lie (lo > hi: no such cut)
   int kb;           // the bin of top-k's cut, or -1
   uint32_t k_left;  // tokens of it that top-k keeps
   uint32_t n;       // listed tokens
+  float x0[2], x1[2];  // logits that may lie in bins sure .. hi, and in kb
 };
 
 struct SampleArgs {
@@ -102,6 +108,12 @@ constexpr double kHalfBin = 0.93941306281347579;  // e^(-1/16)
 // Nearest integer of v in [0, 2^51)
 __device__ __forceinline__ u64 to_units(double v) {
   return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull;
+}
+
+// A sum of masses below the upper edge of bin 0, given below that of bin b.  (Bin 0 as it
+// is: equal logits alone have borders at round shares of their mass.)
+__device__ __forceinline__ u64 from_bin(u64 mass, int b) {
+  return b == 0 ? mass : b < kRest ? (u64)((double)mass * exp(-(double)b / kPerUnit) + 0.5) : 0;
 }
 
 // Accesses that other XCDs' L2s see without a fence.
@@ -198,9 +210,8 @@ __device__ __forceinline__ uint32_t load_slice(const SampleArgs &a, const float 
   return block_max(best, sm);
 }
 
-// Count and mass of the slice's logits by bins below the largest one's (as far as the
-// cuts ask for them), each in two parts.  A mass is in units of 1 / a.unit of its bin's
-// upper edge.
+// Count (for top-k) and mass of the slice's logits by bins below the largest one's, each
+// in two parts.  A mass is in units of 1 / a.unit of its bin's upper edge.
 template <int E>
 __device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (&key)[E],
                                            uint32_t best, Shared &sm) {
@@ -214,7 +225,7 @@ __device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (
     if (key[e] == 0) continue;
     const double y = (double)logit_of(key[e]) * a.s, fl = floor(y), db = id - fl;
     if (db < kRest) {
-      if (a.top_p64) atomicAdd(&sm.bins[part][(int)db], to_units(exp_part(y - fl) * unit));
+      atomicAdd(&sm.bins[part][(int)db], to_units(exp_part(y - fl) * unit));
       if (a.top_k) atomicAdd(&sm.cnt[part][(int)db], 1u);
     }
   }
@@ -226,9 +237,8 @@ __device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (
 __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32_t n, u64 bin_mass,
                                           Shared &sm) {
   const int b = threadIdx.x;
-  // (bin 0 as it is: equal logits alone have borders at round shares of their mass)
-  const u64 m = b == 0 ? bin_mass : b < kRest ? (u64)((double)bin_mass * exp(-(double)b / kPerUnit)) : 0;
-  u64 total, finite;
+  const u64 m = from_bin(bin_mass, b);
+  u64 total, finite = 0;
   Plan &p = sm.plan;
   if (b == 0) {
     p.id = floor((double)top * a.s);
@@ -243,20 +253,21 @@ __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32
     p.n = 0;
   }
   const u64 upto = block_scan(m, sm.wave, &total), before = upto - m;
-  const u64 own = b < kRest ? n : 0, n_upto = block_scan(own, sm.wave, &finite), n_before = n_upto - own;
-  const u64 k = a.top_k;
   if (b == 0) {
     p.total = total;
     sm.lo = sm.hi = total;  // mass of top-k's tokens: at least, at most
   }
-  __syncthreads();
-  if (b < kRest && n_before < k && k <= n_upto) {
-    p.kb = b;
-    p.k_left = (uint32_t)(k - n_before);
-    p.before_k = before;
-    sm.lo = before;
-    sm.hi = upto;
-    p.sure = b;
+  if (a.top_k) {
+    const u64 own = b < kRest ? n : 0, k = a.top_k;
+    const u64 n_upto = block_scan(own, sm.wave, &finite), n_before = n_upto - own;
+    if (b < kRest && n_before < k && k <= n_upto) {
+      p.kb = b;
+      p.k_left = (uint32_t)(k - n_before);
+      p.before_k = before;
+      sm.lo = before;
+      sm.hi = upto;
+      p.sure = b;
+    }
   }
   __syncthreads();
   if (a.top_p64) {
@@ -273,13 +284,30 @@ __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32
     if (b < last && before < hi && hi <= upto) p.hi = b;
     __syncthreads();
   }
-  // min-p alone decides where everything in the cuts' bins is too small for it: there
-  // (max - x) * s > sure - 1
-  if (b == 0 && -a.log_min * kPerUnit + 0.01 <= p.sure - 1) {
-    p.kb = -1;
-    p.lo = 1;
-    p.hi = 0;
-    p.sure = kBins;
+  if (b == 0) {
+    // bin b holds (max - x) * s in (b - 1, b + 1), min-p keeps what is <= d
+    const double d = -a.log_min * kPerUnit;
+    int sure = p.sure;
+    if (d + 0.01 <= sure - 1) {  // the other cuts lie below
+      p.kb = -1;
+      p.lo = 1;
+      p.hi = 0;
+      sure = kBins;
+    }
+    const int cut = sure;
+    if (d - 1.01 < cut) sure = d > 1.01 ? (int)(d - 1.01) : 0;
+    const int end = d + 1.01 < kRest ? (int)(d + 1.01) + 1 : kRest;
+    p.sure = sure;
+    p.part = end < cut ? end : cut;
+    // (room for the roundings of x * s)
+    auto range = [&](int i, int first, int past) {
+      const double u = (p.id - (past - 1)) / a.s, v = (p.id - first + 1) / a.s;
+      p.x0[i] = first < past ? (float)(u - fabs(u) * 1e-6) : INFINITY;
+      p.x1[i] = first < past ? (float)(v + fabs(v) * 1e-6) : -INFINITY;
+    };
+    const bool listed = p.lo <= p.hi;
+    range(0, sure < p.part || !listed ? sure : p.lo, listed ? p.hi + 1 : p.part);
+    range(1, p.kb, p.kb >= 0 ? p.kb + 1 : p.kb);
   }
   __syncthreads();
 }
@@ -294,6 +322,8 @@ struct Place {
     b = db < kRest ? (int)db : kRest;
     part = y - fl;
   }
+  // (bins below p.sure are kept as they are)
+  __device__ bool partial(const Plan &p) const { return b >= p.sure && b < p.part; }
   __device__ bool listed(const Plan &p) const { return (b >= p.lo && b <= p.hi) || b == p.kb; }
   __device__ bool likely(const SampleArgs &a, const Plan &p) const {
     return (x - (double)p.top) * a.inv_t >= a.log_min;
@@ -398,7 +428,7 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, bo
 // The end of a row, for one block: the cuts among the listed tokens, the slice that holds
 // the picked mass, the token.  LIST: the tokens of the cuts' bins are in a.list (if they
 // fit), else they are found in the row again.  sm.plan and sm.tab are set; sm.mass holds
-// the slices' sure mass.
+// the slices' mass outside those bins.
 template <bool LIST>
 __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm) {
   const int t = threadIdx.x;
@@ -408,12 +438,24 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
     const bool fits = LIST && p.n <= kList, few = LIST && p.n <= kFew;
-    const u64 first = fits && t < (int)p.n ? get(a.list + (size_t)row * kList + t) : 0;
+    // the first of them in LDS, loaded together
+    __shared__ u64 listed[LIST ? kNear : 1];
+    const u64 *list = a.list + (size_t)row * kList;
+    const int n = fits ? p.n : 0;
+    if (LIST) {
+      constexpr int R = kNear / NT;
+      u64 r[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) r[i] = n ? get(list + min(NT * i + t, n - 1)) : 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) listed[NT * i + t] = r[i];
+    }
     auto each_listed = [&](auto &&f) {
-      if (fits) {
-        if (first) f(first);
-        for (int i = t + NT; i < (int)p.n; i += NT) f(get(a.list + (size_t)row * kList + i));
+      if (fits) {  // (each thread reads what it wrote)
+#pragma unroll 1
+        for (int i = t; i < n; i += NT) f(i < kNear ? listed[i] : get(list + i));
       } else {
+#pragma unroll 1
         for (int i = t; i < a.vocab; i += NT) {
           const uint32_t k = key_of(x[i]);
           if (k && Place(a, p, k).listed(p)) f(rank_of(k, i));
@@ -486,9 +528,9 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     const uint32_t k = key_of(x[i]);
     if (!k) return false;
     const Place at(a, p, k);
-    if (at.b >= p.sure && !(at.listed(p) && rank_of(k, i) >= cut)) return false;
     *m = at.mass(sm);
-    return at.likely(a, p);
+    return at.b < p.sure ||
+           ((at.partial(p) || (at.listed(p) && rank_of(k, i) >= cut)) && at.likely(a, p));
   };
   u64 mine = 0, all_in;
   for (int i = i0; i < i1; ++i) {
@@ -496,6 +538,8 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     if (kept(i, &m)) mine += to_units(m);
   }
   u64 at = block_scan(mine, sm.wave, &all_in) - mine;
+  // (the slice's mass was summed by bins, and rounded otherwise)
+  if (want >= all_in) want = all_in - 1;
   if (want < at || want >= at + mine) return;
   for (int i = i0; i < i1; ++i) {
     double m;
@@ -521,96 +565,116 @@ __device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
     sm.tab[threadIdx.x] = exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin);
 }
 
-template <int E>
-__global__ __launch_bounds__(NT) void sample_plan_kernel(SampleArgs a) {
+// ALONE: nothing is cut, and the row ends here.
+template <bool ALONE>
+__global__ __launch_bounds__(NT, 6) void sample_plan_kernel(SampleArgs a) {
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
-  const bool cuts = a.top_k || a.top_p64;
-  uint32_t key[E];
-  const int i0 = slice * a.per;
-  uint32_t best = load_slice<E>(a, x, i0, min(a.per, a.vocab - i0), key, sm);
+  uint32_t key[kE];
+  const int i0 = slice * kSlice;
+  uint32_t best = load_slice<kE>(a, x, i0, min(kSlice, a.vocab - i0), key, sm);
   uint32_t *maxes = a.maxes + (size_t)row * a.slices;
+  u64 *mass = a.mass + (size_t)row * a.slices;
   u64 *hist = a.hist + (size_t)row * a.slices * kBins;
   uint32_t *counts = a.counts + (size_t)row * a.slices * kBins;
-  if (cuts && best) {
-    slice_bins<E>(a, key, best, sm);
-    if (t < kBins) {
-      if (a.top_p64) put(hist + (size_t)slice * kBins + t, sm.bins[0][t] + sm.bins[1][t]);
+  if (best) {
+    slice_bins<kE>(a, key, best, sm);
+    const u64 m = t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0;
+    if (ALONE) {
+      u64 total;
+      block_scan(from_bin(m, t), sm.wave, &total);
+      if (t == 0) put(mass + slice, total);
+    } else if (t < kBins) {
+      put(hist + (size_t)slice * kBins + t, m);
       if (a.top_k) put(counts + (size_t)slice * kBins + t, sm.cnt[0][t] + sm.cnt[1][t]);
     }
   }
   if (t == 0) put(maxes + slice, best);
   if (!last_block(a.count + row, a.slices, sm)) return;
+  uint32_t *shift = reinterpret_cast<uint32_t *>(sm.mass);
   best = 0;
   for (int i = t; i < a.slices; i += NT) {
-    const uint32_t k = get(maxes + i);
-    reinterpret_cast<uint32_t *>(sm.mass)[i] = k;
-    best = max(best, k);
+    shift[i] = get(maxes + i);
+    best = max(best, shift[i]);
   }
   best = block_max(best, sm);
-  Plan *out = a.plan + row;
   if (best == 0) {
     none_finite(a, row);
-    if (t == 0) out->any = 0;
+    if (t == 0) a.plan[row].any = 0;
     return;
   }
   const float top = logit_of(best);
   const double id = floor((double)top * a.s);
-  auto shift_of = [&](uint32_t k) {  // bins from the row's largest logit to the slice's
+  // bins from the row's largest logit to a slice's, at most kBins
+  auto shift_of = [&](uint32_t k) {
     const double d = k ? id - floor((double)logit_of(k) * a.s) : kBins;
-    return d < kBins ? d : (double)kBins;
+    return d < kBins ? (int)d : kBins;
   };
   uint32_t n = 0;
   u64 m = 0;
-  if (cuts) {
-    // threads t and t + kBins take every other slice's bin t, a batch of loads at a time;
-    // bins that a slice does not have re-read its bin t
-    constexpr int U = 32;
-    const int bin = t & (kBins - 1);
-    auto add = [&](const auto *from, auto &to) {
-      for (int i0 = t / kBins; i0 < a.slices; i0 += 2 * U) {
-        std::remove_reference_t<decltype(to)> v[U];
-        bool has[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int i = min(i0 + 2 * j, a.slices - 1);
-          const int b = bin - (int)shift_of(reinterpret_cast<const uint32_t *>(sm.mass)[i]);
-          has[j] = b >= 0 && i0 + 2 * j < a.slices;
-          v[j] = get(from + (size_t)i * kBins + (b >= 0 ? b : bin));
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-          if (has[j]) to += v[j];
-      }
-    };
-    if (a.top_p64) add(hist, m);
-    if (a.top_k) add(counts, n);
+  if (ALONE) {
+    make_table(a, sm);
+    u64 own[2];
+    for (int j = 0; j < 2; ++j) {
+      const int i = t + NT * j;
+      const uint32_t k = i < a.slices ? shift[i] : 0;
+      own[j] = k ? from_bin(get(mass + i), shift_of(k)) : 0;
+    }
     __syncthreads();
-    if (t >= kBins) sm.bins[0][bin] = m, sm.cnt[0][bin] = n;
-    __syncthreads();
-    if (t < kBins)
-      m += sm.bins[0][t], n += sm.cnt[0][t];
-    else
-      m = n = 0;
+    for (int j = 0; j < 2; ++j) sm.mass[t + NT * j] = own[j];
+    make_plan(a, top, 0, 0, sm);
+    finish_row<false>(a, x, row, sm);
+    return;
   }
+  for (int i = t; i < a.slices; i += NT) shift[i] = shift_of(shift[i]);
+  __syncthreads();
+  // threads t and t + kBins take every other slice's bin t, a batch of loads at a time;
+  // bins that a slice does not have re-read its bin t
+  constexpr int U = 16;
+  const int bin = t & (kBins - 1);
+  for (int i0 = t / kBins; i0 < a.slices; i0 += 2 * U) {
+    u64 v[U];
+    uint32_t c[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = min(i0 + 2 * j, a.slices - 1), b = bin - (int)shift[i];
+      const size_t at = (size_t)i * kBins + (b >= 0 ? b : bin);
+      v[j] = get(hist + at);
+      c[j] = a.top_k ? get(counts + at) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (i0 + 2 * j < a.slices && bin >= (int)shift[min(i0 + 2 * j, a.slices - 1)]) {
+        m += v[j];
+        n += c[j];
+      }
+  }
+  __syncthreads();
+  if (t >= kBins) sm.bins[0][bin] = m, sm.cnt[0][bin] = n;
+  __syncthreads();
+  if (t < kBins)
+    m += sm.bins[0][t], n += sm.cnt[0][t];
+  else
+    m = n = 0;
   make_plan(a, top, n, m, sm);
-  if (t == 0) *out = sm.plan;
+  if (t == 0) a.plan[row] = sm.plan;
 }
 
-template <int E>
-__global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
+__global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
   Plan *plan = a.plan + row;
-  const int i0 = slice * a.per, n = min(a.per, a.vocab - i0);
-  uint32_t key[E];
+  const int i0 = slice * kSlice, n = min(kSlice, a.vocab - i0);
+  uint32_t key[kE];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
+  for (int e = 0; e < kE; ++e) {
     const int i = t + NT * e;
     key[e] = i < n ? key_of(x[i0 + i]) : 0;
   }
+  const uint32_t best = a.maxes[(size_t)row * a.slices + slice];
+  const u64 bin = a.hist[((size_t)row * a.slices + slice) * kBins + (t & (kBins - 1))];
   make_table(a, sm);
   if (t == 0) sm.plan = *plan;
   __syncthreads();
@@ -618,11 +682,17 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   if (!p.any) return;
   u64 m = 0;
   uint32_t listed = 0;
+  if (best && t < kBins) {
+    const double d = p.id - floor((double)logit_of(best) * a.s) + t;
+    if (d < p.sure) m = from_bin(bin, (int)d);
+  }
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (key[e] == 0) continue;
+  for (int e = 0; e < kE; ++e) {
+    const float v = logit_of(key[e]);
+    const bool near = (v >= p.x0[0] && v <= p.x1[0]) || (v >= p.x0[1] && v <= p.x1[1]);
+    if (key[e] == 0 || !near) continue;
     const Place at(a, p, key[e]);
-    if (at.b < p.sure) {
+    if (at.partial(p)) {
       if (at.likely(a, p)) m += to_units(at.mass(sm));
     } else if (at.listed(p)) {
       listed |= 1u << e;
@@ -636,7 +706,7 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
     __syncthreads();
     uint32_t pos = sm.n + (uint32_t)(upto - own);
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int e = 0; e < kE; ++e)
       if (listed >> e & 1) {
         if (pos < kList) put(a.list + (size_t)row * kList + pos, rank_of(key[e], i0 + t + NT * e));
         ++pos;
@@ -668,13 +738,15 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   make_plan(a, logit_of(best), t < kBins ? sm.cnt[0][t] + sm.cnt[1][t] : 0,
             t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0, sm);
   const Plan &p = sm.plan;
-  u64 m = 0, total;
+  u64 m = t < p.sure && t < kBins ? from_bin(sm.bins[0][t] + sm.bins[1][t], t) : 0, total;
+  if (p.sure < p.part) {
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (key[e]) {
-      const Place at(a, p, key[e]);
-      if (at.b < p.sure && at.likely(a, p)) m += to_units(at.mass(sm));
-    }
+    for (int e = 0; e < E; ++e)
+      if (key[e]) {
+        const Place at(a, p, key[e]);
+        if (at.partial(p) && at.likely(a, p)) m += to_units(at.mass(sm));
+      }
+  }
   block_scan(m, sm.wave, &total);
   if (t == 0) sm.mass[0] = total;
   __syncthreads();
@@ -687,10 +759,8 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // Rows of several slices, at most kMaxRows of them.
 int launch_slices(SampleArgs a, int rows) {
-  // 4096 logits to a slice, for one row's latency; longer ones where the rows fill the GPU
-  const int e = cdiv(a.vocab, 8 * NT) > kMaxSlices || (long)rows * cdiv(a.vocab, 8 * NT) > 2048 ? 32 : 8;
-  a.per = e * NT;
-  a.slices = cdiv(a.vocab, a.per);
+  a.per = kSlice;
+  a.slices = cdiv(a.vocab, kSlice);
   const size_t n = (size_t)rows * a.slices;
   const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
   const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 12;
@@ -707,11 +777,12 @@ int launch_slices(SampleArgs a, int rows) {
   a.counts = reinterpret_cast<uint32_t *>(a.hist + n * kBins);
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
-  hipLaunchKernelGGL(e == 8 ? sample_plan_kernel<8> : sample_plan_kernel<32>, grid, dim3(NT), 0,
+  const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
+  hipLaunchKernelGGL(alone ? sample_plan_kernel<true> : sample_plan_kernel<false>, grid, dim3(NT), 0,
                      stream(), a);
   G4_LAUNCH_CHECK("sample_plan_kernel");
-  hipLaunchKernelGGL(e == 8 ? sample_pick_kernel<8> : sample_pick_kernel<32>, grid, dim3(NT), 0,
-                     stream(), a);
+  if (alone) return G4_OK;
+  hipLaunchKernelGGL(sample_pick_kernel, grid, dim3(NT), 0, stream(), a);
   G4_LAUNCH_CHECK("sample_pick_kernel");
   return G4_OK;
 }

@@ -393,7 +393,7 @@ int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int in_dim
                       float *out, size_t out_stride, float scale, float softcap);
 
 /* One token per row of logits, by probability.
- *   logits: device FP32, row j at logits + j * stride (stride >= vocab; vocab <= 2^24)
+ *   logits: device FP32, row j at logits + j * stride (stride >= vocab; vocab <= 2^22)
  *   u:      device FP32 [rows], uniform random numbers in [0, 1)
  *   tokens: device int32 [rows]; probs: device FP32 [rows] or NULL
  * Only finite logits take part.  Probabilities are softmax(logits / temperature);

@@ -38,7 +38,7 @@ def test_head_rows(n, E, rows, k, stride):
     (-1, 10, 10, 1, 0, 1, 0), (1, 0, 10, 1, 0, 1, 0), (1, 10, 9, 1, 0, 1, 0),
     (1, 10, 10, -0.5, 0, 1, 0), (1, 10, 10, INF, 0, 1, 0), (1, 10, 10, NAN, 0, 1, 0),
     (1, 10, 10, 1, -1, 1, 0), (1, 10, 10, 1, 0, 0, 0), (1, 10, 10, 1, 0, 1.5, 0),
-    (1, (1 << 24) + 1, 1 << 25, 1, 0, 1, 0), (1, 10, 10, 1, 0, NAN, 0), (1, 10, 10, 1, 0, 1, -0.1), (1, 10, 10, 1, 0, 1, 1.1),
+    (1, (1 << 22) + 1, 1 << 25, 1, 0, 1, 0), (1, 10, 10, 1, 0, NAN, 0), (1, 10, 10, 1, 0, 1, -0.1), (1, 10, 10, 1, 0, 1, 1.1),
     (1, 10, 10, 1, 0, 1, NAN)])
 def test_sample(rows, vocab, stride, t, k, p, m):
     params = g4hip.SampleParams(t, k, p, m)
