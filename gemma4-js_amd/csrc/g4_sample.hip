@@ -13,7 +13,7 @@
 // from x * 8 / temperature = whole part and fraction; below e^-31 a mass counts as 0
 // (2^-44, a unit of the sums at 262144 tokens).
 //
-// Two launches over slices of 4096 logits; each one's last block of a row goes on alone:
+// Two launches over slices of a row; each one's last block of a row goes on alone:
 //   sample_plan_kernel  per slice the largest logit and, by whole part of x * 8 / T,
 //                       count and mass; the row's last block finds the bins in which the
 //                       cuts lie (bins above them are kept, those below dropped)
@@ -40,10 +40,9 @@ constexpr int kList = 16384;       // listed tokens of a row
 constexpr int kNear = 4096;        // of these in LDS
 constexpr int kFew = 128;          // tokens that are compared with each other
 constexpr int kMaxRows = 256;      // rows per launch
-constexpr int kE = 8;              // logits of a slice per thread
-constexpr int kSlice = kE * NT;
+constexpr int kIndexBits = 22;
+constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxSlices = 2 * NT;
-constexpr int kMaxVocab = kMaxSlices * kSlice;
 constexpr int kOneSlice = 8192;    // longest row of one slice
 typedef unsigned long long u64;
 
@@ -146,16 +145,23 @@ __device__ __forceinline__ T lane_before(T v) {
   return __builtin_bit_cast(T, (u64)hi << 32 | lo);
 }
 
-// Inclusive sum over the block's threads; *total: all of them.
+// Inclusive sum over the wave's lanes.
 template <typename T>
-__device__ __forceinline__ T block_scan(T v, T *wave, T *total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__device__ __forceinline__ T wave_scan(T v) {
   v += lane_before<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8 in rows of 16 lanes
   v += lane_before<0x112, 0xf>(v);
   v += lane_before<0x114, 0xf>(v);
   v += lane_before<0x118, 0xf>(v);
   v += lane_before<0x142, 0xa>(v);  // row_bcast:15 to rows 1 and 3
   v += lane_before<0x143, 0xc>(v);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+
+// Inclusive sum over the block's threads; *total: all of them.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T *wave, T *total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  v = wave_scan(v);
   __syncthreads();  // wave is free
   if (lane == 63) wave[w] = v;
   __syncthreads();
@@ -333,50 +339,37 @@ struct Place {
 
 // A token in the order of the cuts: larger is earlier.
 __device__ __forceinline__ u64 rank_of(uint32_t key, int i) {
-  return (u64)key << 32 | (0xffffffffu - (uint32_t)i);
+  return (u64)key << kIndexBits | (uint32_t)(kMaxVocab - 1 - i);
+}
+__device__ __forceinline__ uint32_t rank_key(u64 r) { return (uint32_t)(r >> kIndexBits); }
+__device__ __forceinline__ int rank_index(u64 r) {
+  return kMaxVocab - 1 - (int)((uint32_t)r & (kMaxVocab - 1));
 }
 
-// Of the ranks that each() visits, the one at which the `want`-th unit of weight from the
-// top lies (want >= 1; the last one if there is less).  A digit of 8 bits after the other
-// until kFew are left (`few`: there are no more), which are then compared pairwise.
+// Of the ranks that each() visits, all in [lo, hi], the one at which the `want`-th unit of
+// weight from the top lies (want >= 1; the last one if there is less).  A digit of 8 bits
+// after the other until kFew are left (`few`: there are no more), which are then compared
+// pairwise.
 template <typename Each, typename Weight>
-__device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, bool few, Shared &sm) {
+__device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 lo, u64 hi, u64 want,
+                                      bool few, Shared &sm) {
   const int t = threadIdx.x;
-  int rem = 64;
-  u64 prefix = 0;
-  __syncthreads();
-  if (t == 0) sm.lo = ~0ull, sm.hi = 0, sm.n = 0;
-  __syncthreads();
+  int rem = 64;     // bits of r - lo below the digits taken
+  u64 prefix = 0;   // and those digits
   if (!few) {
-    u64 lo = ~0ull, hi = 0;
-    uint32_t n = 0;
-    each([&](u64 r) {
-      lo = r < lo ? r : lo;
-      hi = r > hi ? r : hi;
-      ++n;
-    });
-    if (n) {
-      atomicMin(&sm.lo, lo);
-      atomicMax(&sm.hi, hi);
-      atomicAdd(&sm.n, n);
-    }
-    __syncthreads();
-    lo = sm.lo;
-    hi = sm.hi;
-    n = sm.n;
-    if (lo >= hi) return hi;
-    rem = 64 - __clzll(lo ^ hi);
-    prefix = rem < 64 ? hi >> rem << rem : 0;
+    rem = 64 - __clzll((hi - lo) | 1);
+    uint32_t n = kFew + 1;
     while (rem > 0 && n > kFew) {
-      const int w = rem < 8 ? rem : 8, above = rem;
+      const int w = rem < 8 ? rem : 8;
       rem -= w;
       __syncthreads();
       if (t < 256) sm.bins[0][t] = 0, sm.cnt[0][t] = 0;
       if (t == 0) sm.v[1] = 0, sm.v[2] = 0, sm.pick = 0;
       __syncthreads();
       each([&](u64 r) {
-        if (above < 64 && (r ^ prefix) >> above) return;
-        const int d = (int)(r >> rem) & ((1 << w) - 1);
+        const u64 c = (r - lo) >> rem;
+        if (c >> w != prefix) return;
+        const int d = (int)c & ((1 << w) - 1);
         atomicAdd(&sm.bins[0][d], weight(r));
         atomicAdd(&sm.cnt[0][d], 1u);
       });
@@ -391,17 +384,21 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, bo
         sm.pick = upto - own;
       }
       __syncthreads();
-      prefix |= (u64)sm.v[1] << rem;
+      prefix = prefix << w | sm.v[1];
       n = sm.v[2];
       want -= sm.pick;
     }
-    if (rem == 0) return prefix;
-    if (t == 0) sm.n = 0;
-    __syncthreads();
+    if (rem == 0) {
+      __syncthreads();
+      return lo + prefix;
+    }
   }
+  __syncthreads();
+  if (t == 0) sm.n = 0;
+  __syncthreads();
   if (t == 0) sm.pick = 0;
   each([&](u64 r) {
-    if (rem < 64 && (r ^ prefix) >> rem) return;
+    if (rem < 64 && (r - lo) >> rem != prefix) return;
     const uint32_t at = atomicAdd(&sm.n, 1u);
     sm.few[at] = r;
     sm.weight[at] = weight(r);
@@ -430,16 +427,16 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 want, bo
 // fit), else they are found in the row again.  sm.plan and sm.tab are set; sm.mass holds
 // the slices' mass outside those bins.
 template <bool LIST>
-__device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm) {
+__device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm,
+                                           u64 *listed) {
   const int t = threadIdx.x;
   const Plan &p = sm.plan;
-  auto bin_of = [&](u64 r) { return Place(a, p, (uint32_t)(r >> 32)).b; };
-  auto mass_of = [&](u64 r) { return to_units(Place(a, p, (uint32_t)(r >> 32)).mass(sm)); };
+  auto bin_of = [&](u64 r) { return Place(a, p, rank_key(r)).b; };
+  auto mass_of = [&](u64 r) { return to_units(Place(a, p, rank_key(r)).mass(sm)); };
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
     const bool fits = LIST && p.n <= kList, few = LIST && p.n <= kFew;
     // the first of them in LDS, loaded together
-    __shared__ u64 listed[LIST ? kNear : 1];
     const u64 *list = a.list + (size_t)row * kList;
     const int n = fits ? p.n : 0;
     if (LIST) {
@@ -447,6 +444,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       u64 r[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) r[i] = n ? get(list + min(NT * i + t, n - 1)) : 0;
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < R; ++i) listed[NT * i + t] = r[i];
     }
@@ -467,19 +465,25 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       block_scan(v, sm.wave, &total);
       return total;
     };
-    u64 all = p.total;
-    u64 k_cut = 0;
-    if (p.kb >= 0) {
-      k_cut = select([&](auto &&f) { each_listed([&](u64 r) { if (bin_of(r) == p.kb) f(r); }); },
-                     [](u64) { return 1ull; }, p.k_left, few, sm);
-      if (p.lo <= p.hi) {
+    // a listed token is in top-k's bin, or in one where top-p may cut, or both
+    const bool k_cuts = p.kb >= 0, p_cuts = p.lo <= p.hi, both = k_cuts && p_cuts;
+    auto in_k = [&](u64 r) { return !both || bin_of(r) == p.kb; };
+    auto in_p = [&](u64 r) { return !both || bin_of(r) <= p.hi; };
+    const uint32_t top = key_of(p.top);
+    auto low = [&](int i) { return rank_of(max(key_of(p.x0[i]), 1u), kMaxVocab - 1); };
+    auto high = [&](int i) { return rank_of(p.x1[i] < p.top ? key_of(p.x1[i]) : top, 0); };
+    u64 all = p.total, k_cut = 0;
+    if (k_cuts) {
+      k_cut = select([&](auto &&f) { each_listed([&](u64 r) { if (in_k(r)) f(r); }); },
+                     [](u64) { return 1ull; }, low(1), high(1), p.k_left, few, sm);
+      if (both) {
         u64 m = 0;
-        each_listed([&](u64 r) { if (bin_of(r) == p.kb && r >= k_cut) m += mass_of(r); });
+        each_listed([&](u64 r) { if (in_k(r) && r >= k_cut) m += mass_of(r); });
         all = p.before_k + sum(m);
       }
       cut = k_cut;
     }
-    if (p.lo <= p.hi) {
+    if (p_cuts) {
       // (where min-p drops any token above these bins, it drops all that lie in them, and
       // it does not matter that the slices' mass lacks what top-p counts)
       u64 above = 0;
@@ -487,16 +491,12 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       above = sum(above);
       const u64 want = __umul64hi(a.top_p64, all) + (a.top_p64 * all != 0);  // rounded up
       const u64 w = want > above ? want - above : 1;
-      cut = select([&](auto &&f) {
-        each_listed([&](u64 r) {
-          const int b = bin_of(r);
-          if (b >= p.lo && b <= p.hi && r >= k_cut) f(r);
-        });
-      }, mass_of, w, few, sm);
+      cut = select([&](auto &&f) { each_listed([&](u64 r) { if (r >= k_cut && in_p(r)) f(r); }); },
+                   mass_of, low(0), high(0), w, few, sm);
     }
     each_listed([&](u64 r) {
-      if (r >= cut && Place(a, p, (uint32_t)(r >> 32)).likely(a, p))
-        atomicAdd(&sm.mass[(0xffffffffu - (uint32_t)r) / (uint32_t)a.per], mass_of(r));
+      if (r >= cut && Place(a, p, rank_key(r)).likely(a, p))
+        atomicAdd(&sm.mass[(uint32_t)rank_index(r) / (uint32_t)a.per], mass_of(r));
     });
   }
   __syncthreads();
@@ -519,11 +519,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     sm.pick = want - before - (second ? m0 : 0);
   }
   __syncthreads();
-  // and in it, a run of consecutive tokens per thread
-  const int s0 = sm.v[0] * a.per, s1 = min(s0 + a.per, a.vocab);
-  want = sm.pick;
-  const int run = (s1 - s0 + NT - 1) / NT;
-  const int i0 = min(s0 + t * run, s1), i1 = min(i0 + run, s1);
+  // and in it: the wave's part of consecutive tokens, of that again, and its 64s in turn
   auto kept = [&](int i, double *m) {
     const uint32_t k = key_of(x[i]);
     if (!k) return false;
@@ -532,24 +528,56 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     return at.b < p.sure ||
            ((at.partial(p) || (at.listed(p) && rank_of(k, i) >= cut)) && at.likely(a, p));
   };
-  u64 mine = 0, all_in;
-  for (int i = i0; i < i1; ++i) {
+  const int lane = t & 63, w = t >> 6;
+  int i0 = sm.v[0] * a.per, i1 = min(i0 + a.per, a.vocab);
+  want = sm.pick;
+  // A slice's mass was summed by bins and rounded otherwise: beyond its tokens' masses it
+  // is the last one's, and tokens of less than half a unit count 1 where there are no others.
+  u64 least = 0;
+  auto units = [&](int i) {
     double m;
-    if (kept(i, &m)) mine += to_units(m);
-  }
-  u64 at = block_scan(mine, sm.wave, &all_in) - mine;
-  // (the slice's mass was summed by bins, and rounded otherwise)
-  if (want >= all_in) want = all_in - 1;
-  if (want < at || want >= at + mine) return;
-  for (int i = i0; i < i1; ++i) {
-    double m;
-    if (!kept(i, &m)) continue;
-    at += to_units(m);
-    if (at > want) {
-      a.tokens[row] = i;
-      if (a.probs) a.probs[row] = (float)(m / (double)total);
-      return;
+    if (!kept(i, &m)) return (u64)0;
+    const u64 v = to_units(m);
+    return v > least ? v : least;
+  };
+  while (i1 - i0 > 64) {
+    const int part = ((i1 - i0 + kWaves - 1) / kWaves + 63) & ~63;
+    const int j0 = i0 + w * part, j1 = min(j0 + part, i1);
+    u64 own = 0, in;
+    for (int j = j0 + lane; j < j1; j += 64) own += units(j);
+    block_scan(own, sm.wave, &in);
+    if (in == 0) {
+      if (least) return;
+      least = 1;
+      continue;
     }
+    if (want >= in) want = in - 1;
+    u64 first = 0;
+    for (int i = 0; i < w; ++i) first += sm.wave[i];
+    if (lane == 0 && first <= want && want < first + sm.wave[w]) {
+      sm.v[0] = w;
+      sm.pick = want - first;
+    }
+    __syncthreads();
+    i0 += (int)sm.v[0] * part;
+    i1 = min(i0 + part, i1);
+    want = sm.pick;
+  }
+  if (w > 0) return;
+  const int i = i0 + lane;
+  u64 own = i < i1 ? units(i) : 0, upto_i = wave_scan(own), in = __shfl(upto_i, 63, 64);
+  if (in == 0) {
+    least = 1;
+    own = i < i1 ? units(i) : 0;
+    upto_i = wave_scan(own);
+    in = __shfl(upto_i, 63, 64);
+  }
+  if (want >= in) want = in - 1;
+  if (upto_i - own <= want && want < upto_i) {
+    double m;
+    kept(i, &m);
+    a.tokens[row] = i;
+    if (a.probs) a.probs[row] = (float)(m / (double)total);
   }
 }
 
@@ -566,20 +594,20 @@ __device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
 }
 
 // ALONE: nothing is cut, and the row ends here.
-template <bool ALONE>
-__global__ __launch_bounds__(NT, 6) void sample_plan_kernel(SampleArgs a) {
+template <int E, bool ALONE>
+__global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kernel(SampleArgs a) {
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
-  uint32_t key[kE];
-  const int i0 = slice * kSlice;
-  uint32_t best = load_slice<kE>(a, x, i0, min(kSlice, a.vocab - i0), key, sm);
+  uint32_t key[E];
+  const int i0 = slice * (E * NT);
+  uint32_t best = load_slice<E>(a, x, i0, min((E * NT), a.vocab - i0), key, sm);
   uint32_t *maxes = a.maxes + (size_t)row * a.slices;
   u64 *mass = a.mass + (size_t)row * a.slices;
   u64 *hist = a.hist + (size_t)row * a.slices * kBins;
   uint32_t *counts = a.counts + (size_t)row * a.slices * kBins;
   if (best) {
-    slice_bins<kE>(a, key, best, sm);
+    slice_bins<E>(a, key, best, sm);
     const u64 m = t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0;
     if (ALONE) {
       u64 total;
@@ -624,14 +652,14 @@ __global__ __launch_bounds__(NT, 6) void sample_plan_kernel(SampleArgs a) {
     __syncthreads();
     for (int j = 0; j < 2; ++j) sm.mass[t + NT * j] = own[j];
     make_plan(a, top, 0, 0, sm);
-    finish_row<false>(a, x, row, sm);
+    finish_row<false>(a, x, row, sm, nullptr);
     return;
   }
   for (int i = t; i < a.slices; i += NT) shift[i] = shift_of(shift[i]);
   __syncthreads();
   // threads t and t + kBins take every other slice's bin t, a batch of loads at a time;
   // bins that a slice does not have re-read its bin t
-  constexpr int U = 16;
+  constexpr int U = E > 8 ? 8 : 16;
   const int bin = t & (kBins - 1);
   for (int i0 = t / kBins; i0 < a.slices; i0 += 2 * U) {
     u64 v[U];
@@ -661,56 +689,73 @@ __global__ __launch_bounds__(NT, 6) void sample_plan_kernel(SampleArgs a) {
   if (t == 0) a.plan[row] = sm.plan;
 }
 
+template <int E>
 __global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
   __shared__ Shared sm;
+  __shared__ u64 near[kNear];
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
   Plan *plan = a.plan + row;
-  const int i0 = slice * kSlice, n = min(kSlice, a.vocab - i0);
-  uint32_t key[kE];
+  constexpr int C = 8;  // logits per thread at a time
+  const int i0 = slice * (E * NT), n = min(E * NT, a.vocab - i0);
+  float v[C];
+  auto load = [&](int c) {
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    const int i = t + NT * e;
-    key[e] = i < n ? key_of(x[i0 + i]) : 0;
-  }
+    for (int e = 0; e < C; ++e) {
+      const int i = t + NT * (c * C + e);
+      v[e] = i < n ? x[i0 + i] : NAN;
+    }
+  };
+  load(0);
   const uint32_t best = a.maxes[(size_t)row * a.slices + slice];
   const u64 bin = a.hist[((size_t)row * a.slices + slice) * kBins + (t & (kBins - 1))];
   make_table(a, sm);
-  if (t == 0) sm.plan = *plan;
+  if (t == 0) sm.plan = *plan, sm.n = 0;
   __syncthreads();
   const Plan &p = sm.plan;
   if (!p.any) return;
   u64 m = 0;
-  uint32_t listed = 0;
   if (best && t < kBins) {
     const double d = p.id - floor((double)logit_of(best) * a.s) + t;
     if (d < p.sure) m = from_bin(bin, (int)d);
   }
+  const float x0 = p.x0[0], x1 = p.x1[0], k0 = p.x0[1], k1 = p.x1[1];
+  for (int c = 0;;) {
+    uint32_t near_by = 0;
+    float u[C];
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    const float v = logit_of(key[e]);
-    const bool near = (v >= p.x0[0] && v <= p.x1[0]) || (v >= p.x0[1] && v <= p.x1[1]);
-    if (key[e] == 0 || !near) continue;
-    const Place at(a, p, key[e]);
-    if (at.partial(p)) {
-      if (at.likely(a, p)) m += to_units(at.mass(sm));
-    } else if (at.listed(p)) {
-      listed |= 1u << e;
+    for (int e = 0; e < C; ++e) {
+      u[e] = v[e];
+      if ((u[e] >= x0 && u[e] <= x1) || (u[e] >= k0 && u[e] <= k1)) near_by |= 1u << e;
     }
-  }
-  u64 total, found;
-  block_scan(m, sm.wave, &total);
-  const u64 own = __popc(listed), upto = block_scan(own, sm.wave, &found);
-  if (found) {
-    if (t == 0) sm.n = atomicAdd(&plan->n, (uint32_t)found);
-    __syncthreads();
-    uint32_t pos = sm.n + (uint32_t)(upto - own);
+    const bool more = ++c < E / C;
+    if (more) load(c);
 #pragma unroll
-    for (int e = 0; e < kE; ++e)
-      if (listed >> e & 1) {
-        if (pos < kList) put(a.list + (size_t)row * kList + pos, rank_of(key[e], i0 + t + NT * e));
-        ++pos;
+    for (int e = 0; e < C; ++e) {
+      if (!(near_by >> e & 1)) continue;
+      const uint32_t key = key_of(u[e]);
+      if (!key) continue;
+      const Place at(a, p, key);
+      if (at.partial(p)) {
+        if (at.likely(a, p)) m += to_units(at.mass(sm));
+      } else if (at.listed(p)) {
+        const uint32_t pos = atomicAdd(&sm.n, 1u);
+        if (pos < kNear) near[pos] = rank_of(key, i0 + t + NT * ((c - 1) * C + e));
       }
+    }
+    if (!more) break;
+  }
+  u64 total;
+  block_scan(m, sm.wave, &total);
+  const uint32_t found = sm.n;
+  if (found) {
+    __syncthreads();
+    // more than fit: the row is read again at its end
+    if (t == 0) sm.n = atomicAdd(&plan->n, found <= kNear ? found : kList + 1u);
+    __syncthreads();
+    const uint32_t base = sm.n;
+    for (uint32_t i = t; i < found && i < kNear && base < kList && base + i < kList; i += NT)
+      put(a.list + (size_t)row * kList + base + i, near[i]);
   }
   u64 *mass = a.mass + (size_t)row * a.slices;
   if (t == 0) put(mass + slice, total);
@@ -718,7 +763,7 @@ __global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
   for (int i = t; i < a.slices; i += NT) sm.mass[i] = get(mass + i);
   if (t == 0) sm.plan.n = get(&plan->n);
   __syncthreads();
-  finish_row<true>(a, x, row, sm);
+  finish_row<true>(a, x, row, sm, near);
 }
 
 // Both halves for rows of one slice.
@@ -750,7 +795,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   block_scan(m, sm.wave, &total);
   if (t == 0) sm.mass[0] = total;
   __syncthreads();
-  finish_row<false>(a, x, row, sm);
+  finish_row<false>(a, x, row, sm, nullptr);
 }
 
 Workspace g_sample_ws, g_sample_count;
@@ -759,8 +804,10 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // Rows of several slices, at most kMaxRows of them.
 int launch_slices(SampleArgs a, int rows) {
-  a.per = kSlice;
-  a.slices = cdiv(a.vocab, kSlice);
+  // 4096 logits to a slice, for one row's latency; longer ones where they fill the GPU
+  const int e = (long)rows * cdiv(a.vocab, 32 * NT) >= 512 || a.vocab > kMaxSlices * 8 * NT ? 32 : 8;
+  a.per = e * NT;
+  a.slices = cdiv(a.vocab, a.per);
   const size_t n = (size_t)rows * a.slices;
   const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
   const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 12;
@@ -778,11 +825,13 @@ int launch_slices(SampleArgs a, int rows) {
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
   const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
-  hipLaunchKernelGGL(alone ? sample_plan_kernel<true> : sample_plan_kernel<false>, grid, dim3(NT), 0,
-                     stream(), a);
+  void (*plan_kernel)(SampleArgs) = e == 8 ? (alone ? sample_plan_kernel<8, true> : sample_plan_kernel<8, false>)
+                                           : (alone ? sample_plan_kernel<32, true> : sample_plan_kernel<32, false>);
+  hipLaunchKernelGGL(plan_kernel, grid, dim3(NT), 0, stream(), a);
   G4_LAUNCH_CHECK("sample_plan_kernel");
   if (alone) return G4_OK;
-  hipLaunchKernelGGL(sample_pick_kernel, grid, dim3(NT), 0, stream(), a);
+  hipLaunchKernelGGL(e == 8 ? sample_pick_kernel<8> : sample_pick_kernel<32>, grid, dim3(NT), 0,
+                     stream(), a);
   G4_LAUNCH_CHECK("sample_pick_kernel");
   return G4_OK;
 }
