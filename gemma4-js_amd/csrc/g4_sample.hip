@@ -28,6 +28,10 @@
 
 #include "g4_internal.h"
 
+// A logit's bin and its place in the bin come from one rounded product, wherever they are
+// computed: products are fused into sums only where fma() says so.
+#pragma clang fp contract(off)
+
 namespace g4 {
 namespace {
 
@@ -334,7 +338,7 @@ struct Place {
   __device__ bool likely(const SampleArgs &a, const Plan &p) const {
     return (x - (double)p.top) * a.inv_t >= a.log_min;
   }
-  __device__ double mass(const Shared &sm) const { return b < kRest ? sm.tab[b] * exp_part(part) : 0.0; }
+  __device__ double mass(const Shared &sm) const { return sm.tab[b] * exp_part(part); }
 };
 
 // A token in the order of the cuts: larger is earlier.
@@ -439,14 +443,15 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     // the first of them in LDS, loaded together
     const u64 *list = a.list + (size_t)row * kList;
     const int n = fits ? p.n : 0;
-    if (LIST) {
-      constexpr int R = kNear / NT;
-      u64 r[R];
+    if (LIST) {  // (the caller has loaded the first NT)
+      constexpr int R = kNear / NT - 1;
+      if (n > NT) {
+        u64 r[R];
 #pragma unroll
-      for (int i = 0; i < R; ++i) r[i] = n ? get(list + min(NT * i + t, n - 1)) : 0;
-      __syncthreads();
+        for (int i = 0; i < R; ++i) r[i] = get(list + min(NT * (i + 1) + t, n - 1));
 #pragma unroll
-      for (int i = 0; i < R; ++i) listed[NT * i + t] = r[i];
+        for (int i = 0; i < R; ++i) listed[NT * (i + 1) + t] = r[i];
+      }
     }
     auto each_listed = [&](auto &&f) {
       if (fits) {  // (each thread reads what it wrote)
@@ -520,13 +525,12 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   }
   __syncthreads();
   // and in it: the wave's part of consecutive tokens, of that again, and its 64s in turn
-  auto kept = [&](int i, double *m) {
-    const uint32_t k = key_of(x[i]);
-    if (!k) return false;
-    const Place at(a, p, k);
+  auto kept = [&](float v, int i, double *m) {
+    const uint32_t k = key_of(v);
+    const Place at(a, p, k ? k : 1u);
     *m = at.mass(sm);
-    return at.b < p.sure ||
-           ((at.partial(p) || (at.listed(p) && rank_of(k, i) >= cut)) && at.likely(a, p));
+    const int cuts = at.partial(p) | ((int)at.listed(p) & (rank_of(k, i) >= cut));
+    return ((k != 0) & ((int)(at.b < p.sure) | (cuts & (int)at.likely(a, p)))) != 0;  // no branches
   };
   const int lane = t & 63, w = t >> 6;
   int i0 = sm.v[0] * a.per, i1 = min(i0 + a.per, a.vocab);
@@ -534,17 +538,24 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   // A slice's mass was summed by bins and rounded otherwise: beyond its tokens' masses it
   // is the last one's, and tokens of less than half a unit count 1 where there are no others.
   u64 least = 0;
-  auto units = [&](int i) {
+  auto units = [&](float x_i, int i) {
     double m;
-    if (!kept(i, &m)) return (u64)0;
+    const bool is = kept(x_i, i, &m);
     const u64 v = to_units(m);
-    return v > least ? v : least;
+    return !is ? (u64)0 : v > least ? v : least;
   };
   while (i1 - i0 > 64) {
     const int part = ((i1 - i0 + kWaves - 1) / kWaves + 63) & ~63;
     const int j0 = i0 + w * part, j1 = min(j0 + part, i1);
     u64 own = 0, in;
-    for (int j = j0 + lane; j < j1; j += 64) own += units(j);
+    constexpr int U = 4;  // loads and chains of binary64 arithmetic together
+    for (int j = j0 + lane; j < j1; j += 64 * U) {
+      float y[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) y[k] = x[min(j + 64 * k, j1 - 1)];
+#pragma unroll
+      for (int k = 0; k < U; ++k) own += units(j + 64 * k < j1 ? y[k] : NAN, j + 64 * k);
+    }
     block_scan(own, sm.wave, &in);
     if (in == 0) {
       if (least) return;
@@ -565,17 +576,18 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   }
   if (w > 0) return;
   const int i = i0 + lane;
-  u64 own = i < i1 ? units(i) : 0, upto_i = wave_scan(own), in = __shfl(upto_i, 63, 64);
+  const float x_i = x[min(i, i1 - 1)];
+  u64 own = i < i1 ? units(x_i, i) : 0, upto_i = wave_scan(own), in = __shfl(upto_i, 63, 64);
   if (in == 0) {
     least = 1;
-    own = i < i1 ? units(i) : 0;
+    own = i < i1 ? units(x_i, i) : 0;
     upto_i = wave_scan(own);
     in = __shfl(upto_i, 63, 64);
   }
   if (want >= in) want = in - 1;
   if (upto_i - own <= want && want < upto_i) {
     double m;
-    kept(i, &m);
+    kept(x_i, i, &m);
     a.tokens[row] = i;
     if (a.probs) a.probs[row] = (float)(m / (double)total);
   }
@@ -590,7 +602,8 @@ __device__ __forceinline__ void none_finite(const SampleArgs &a, int row) {
 
 __device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
   if (threadIdx.x < kBins)
-    sm.tab[threadIdx.x] = exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin);
+    sm.tab[threadIdx.x] =
+        threadIdx.x < kRest ? exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin) : 0.0;
 }
 
 // ALONE: nothing is cut, and the row ends here.
@@ -760,8 +773,10 @@ __global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
   u64 *mass = a.mass + (size_t)row * a.slices;
   if (t == 0) put(mass + slice, total);
   if (!last_block(a.count + kMaxRows + row, a.slices, sm)) return;
+  const u64 first = get(a.list + (size_t)row * kList + t);
   for (int i = t; i < a.slices; i += NT) sm.mass[i] = get(mass + i);
   if (t == 0) sm.plan.n = get(&plan->n);
+  near[t] = first;
   __syncthreads();
   finish_row<true>(a, x, row, sm, near);
 }
