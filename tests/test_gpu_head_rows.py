@@ -41,7 +41,10 @@ def check(got, x, E, scale=1.0, softcap=30.0):
 @pytest.mark.parametrize("n,rows,k", [
     (1, 100, 1536), (2, 1, 8), (2, 257, 1536), (3, 4096, 1536), (5, 1000, 64), (8, 333, 40),
     (15, 515, 1528), (16, 64, 256), (17, 129, 1536), (31, 700, 2048), (33, 255, 520),
-    (48, 1025, 1536), (63, 130, 4096), (64, 4096, 1536), (65, 300, 1536), (130, 77, 104)])
+    (48, 1025, 1536), (63, 130, 4096), (64, 4096, 1536), (65, 300, 1536), (130, 77, 104),
+    # many rows: the table's tiles, one and several per block
+    (5, 50001, 1536), (16, 66001, 72), (20, 25003, 1528), (40, 17002, 520), (64, 13001, 1536),
+    (64, 150007, 64), (130, 13003, 104)])
 def test_shapes(g4, n, rows, k):
     print("head rows", n, rows, k, flush=True)
     x, E = case(np.random.default_rng([n, rows, k]), n, rows, k)
@@ -49,11 +52,12 @@ def test_shapes(g4, n, rows, k):
 
 
 @pytest.mark.parametrize("n", [2, 20, 70])
-def test_scale_without_cap_and_stride(g4, n):
-    x, E = case(np.random.default_rng(n), n, 301, 512)
-    got = run(g4, x, E, stride=333, scale=-0.37, softcap=0.0)
-    check(got[:, :301], x, E, scale=-0.37, softcap=0.0)
-    assert (got[:, 301:] == 7.0).all()  # the rest of a row stays
+@pytest.mark.parametrize("rows,stride", [(301, 333), (50001, 50020)])
+def test_scale_without_cap_and_stride(g4, n, rows, stride):
+    x, E = case(np.random.default_rng(n), n, rows, 128)
+    got = run(g4, x, E, stride=stride, scale=-0.37, softcap=0.0)
+    check(got[:, :rows], x, E, scale=-0.37, softcap=0.0)
+    assert (got[:, rows:] == 7.0).all()  # the rest of a row stays
 
 
 def test_one_state_has_the_single_head_s_bits(g4):
@@ -63,9 +67,9 @@ def test_one_state_has_the_single_head_s_bits(g4):
     np.testing.assert_array_equal(run(g4, x, E)[0], out.download(np.float32))
 
 
-@pytest.mark.parametrize("n", [4, 64])
-def test_a_state_s_logits_do_not_depend_on_the_others(g4, n):
-    x, E = case(np.random.default_rng(n), n, 500, 1536)
+@pytest.mark.parametrize("n,rows", [(4, 500), (64, 500), (4, 50000), (64, 13000)])
+def test_a_state_s_logits_do_not_depend_on_the_others(g4, n, rows):
+    x, E = case(np.random.default_rng(n), n, rows, 256)
     a = run(g4, x, E)
     y = x.copy()
     y[1:] = np.nan
@@ -75,9 +79,10 @@ def test_a_state_s_logits_do_not_depend_on_the_others(g4, n):
     assert np.isnan(b[1]).all() and not np.isnan(b[0]).any()
 
 
+@pytest.mark.parametrize("rows", [200, 50003])
 @pytest.mark.parametrize("size", [1e-30, 1e30])
-def test_sizes_of_the_states(g4, size):
-    x, E = case(np.random.default_rng(8), 6, 200, 1536)
+def test_sizes_of_the_states(g4, size, rows):
+    x, E = case(np.random.default_rng(8), 6, rows, 264)
     x = (x * np.float32(size)).astype(np.float32)
     check(run(g4, x, E, scale=1.0, softcap=0.0), x, E, softcap=0.0)
 
