@@ -8,91 +8,445 @@
 namespace g4 {
 namespace {
 
-constexpr int kMaxNodes = 256;
+constexpr int kMaxNodes = 256, kNodeWords = kMaxNodes / 32;
+constexpr int kTile = 16;  // keys per tile
+constexpr int kMaxSplits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
 
 struct TreeArgs {
   const float *q, *k, *v;
   float *y;
   const int *parents;
   int nodes, heads, prefix, window;  // window 0: none
+  int first;    // first prefix key of the first tile
+  int ptiles;   // tiles of the prefix; those of the tree follow
+  int tiles, tps, splits;
+  float *part;  // [splits][rows][hd] unnormalised outputs
+  float2 *ml;   // [splits][rows] (max, sum)
 };
 
-// One block per (node, head); its waves take turns over the keys, lane l holding dims
-// DPL l .. of q, k, v and the output, with a running maximum and sum each.
-template <int DPL>
-__global__ __launch_bounds__(256) void attn_tree_kernel(TreeArgs a) {
-  constexpr int HD = 64 * DPL;
-  __shared__ uint32_t sees[kMaxNodes / 32];
-  __shared__ int s_depth;
-  __shared__ float sm[4], sl[4], so[4][HD];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int node = blockIdx.x / a.heads;
-  if (t < kMaxNodes / 32) sees[t] = 0;
-  __syncthreads();
-  if (t == 0) {
-    int depth = 0;
-    for (int i = node;;) {
-      sees[i >> 5] |= 1u << (i & 31);
-      const int p = a.parents[i];
-      if (p < -1 || p >= i) depth = -1;
-      if (p < 0 || p >= i) break;
-      ++depth;
-      i = p;
+// Ancestors of the nodes as bits (themselves among them) and their number.
+struct Tree {
+  uint32_t sees[kMaxNodes][kNodeWords];
+  int up[kMaxNodes];         // -1: none left
+  short depth[kMaxNodes];    // -1: some parent on the way is not an earlier node
+};
+
+// Every node at once, the distance to the ancestor `up` doubling in each round.
+template <int NTH>
+__device__ __forceinline__ void make_tree(const TreeArgs &a, Tree &tr) {
+  const int t = threadIdx.x;
+  static_assert(NTH >= 256, "a thread per node");
+  const bool mine = t < a.nodes;
+  uint32_t s[kNodeWords];
+  int up = -1, depth = 0;
+#pragma unroll
+  for (int w = 0; w < kNodeWords; ++w) s[w] = 0;
+  if (mine) {
+    up = a.parents[t];
+    if (up < -1 || up >= t) up = -1, depth = -1;
+    if (up >= 0) depth = 1;
+#pragma unroll
+    for (int w = 0; w < kNodeWords; ++w) s[w] = t >> 5 == w ? 1u << (t & 31) : 0u;
+  }
+  bool more = true;
+  while (more) {
+    if (mine) {
+#pragma unroll
+      for (int w = 0; w < kNodeWords; ++w) tr.sees[t][w] = s[w];
+      tr.up[t] = up;
+      tr.depth[t] = (short)depth;
     }
-    s_depth = depth;
-  }
-  __syncthreads();
-  const int depth = s_depth;
-  float *y = a.y + (size_t)blockIdx.x * HD;
-  if (depth < 0) {
-    for (int i = t; i < HD; i += 256) y[i] = __int_as_float(0x7fc00000);
-    return;
-  }
-  float q[DPL], o[DPL], m = -INFINITY, l = 0.f;
+    more = __syncthreads_or(up >= 0);
+    if (up >= 0) {
 #pragma unroll
-  for (int j = 0; j < DPL; ++j) {
-    q[j] = a.q[(size_t)blockIdx.x * HD + DPL * lane + j];
-    o[j] = 0.f;
+      for (int w = 0; w < kNodeWords; ++w) s[w] |= tr.sees[up][w];
+      const int d = tr.depth[up];
+      depth = d < 0 || depth < 0 ? -1 : depth + d;
+      up = tr.up[up];
+    }
+    __syncthreads();
   }
-  auto key = [&](size_t at) {
-    const float *k = a.k + at * HD + DPL * lane, *v = a.v + at * HD + DPL * lane;
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < DPL; ++j) s = fmaf(q[j], k[j], s);
-    s = wave_sum(s);
-    const float mn = fmaxf(m, s);
-    const float c = expf(m - mn), p = expf(s - mn);
-    l = fmaf(l, c, p);
-#pragma unroll
-    for (int j = 0; j < DPL; ++j) o[j] = fmaf(p, v[j], o[j] * c);
-    m = mn;
+}
+
+// max over the lanes c, c + 16, c + 32, c + 48
+__device__ __forceinline__ float group_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int HD>
+constexpr int kDimWaves = HD >= 256 ? 4 : HD / 64;
+
+// A block owns 16 RT rows of [nodes * heads, hd] and a run of key tiles, which its KG key
+// groups take in turn; the DQ waves of a group share the head dim.  On the FP32 matrix
+// cores (v_mfma_f32_16x16x4f32), lane (c, g) of a wave working for row c throughout:
+//   S^T = K . Q^T     a wave's dims; the group's waves add theirs through LDS, in wave order,
+//                     so that they hold the same scores: keys 4 g .. + 3 per lane
+//   softmax           running maximum and sum per row
+//   O^T += V^T . P^T  the lane's probabilities are its operand as they are (step i takes keys
+//                     4 g + i); output tile 4 q + e holds dims 64 q + 4 c + e, so V and O
+//                     move as 16-byte vectors
+// The next tile's K is loaded once the scores are formed, its V once the outputs are.
+template <int HD, int RT, int KG>
+__global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(TreeArgs a) {
+  constexpr int DQ = kDimWaves<HD>, DW = HD / DQ, NJ = DW / 16, NQ = DW / 64;
+  constexpr int NTH = 64 * DQ * KG, R = 16 * RT;
+  struct Loop {
+    Tree tree;
+    f32x4 sx[2][KG][DQ][RT][64];  // the waves' scores, two buffers
   };
-  // positions above `low` are seen
-  const int low = a.window > 0 ? a.prefix + depth - a.window : -1;
-  for (int i = (low >= 0 ? low + 1 : 0) + w; i < a.prefix; i += 4) key(i);
-  if (w == 0) {
-    int at = depth;
-    for (int i = node; i >= 0; --i)
-      if (sees[i >> 5] >> (i & 31) & 1)
-        if (a.prefix + at-- > low) key((size_t)a.prefix + i);
+  union Smem {
+    Loop loop;
+    float o[R][HD + 4];
+  };
+  __shared__ Smem sm;
+  __shared__ float2 wml[KG][R];
+  const int t = threadIdx.x, lane = t & 63, w = (t >> 6) % DQ, kg = (t >> 6) / DQ;
+  const int c = lane & 15, g = lane >> 4;
+  const int nrows = a.nodes * a.heads, d0 = w * DW;
+  int split = blockIdx.y, R0 = blockIdx.x * R;
+  if (a.splits % 8 == 0) {
+    // the row blocks of a split go to one XCD (blocks are dealt to the 8 in turn), whose L2
+    // then holds the split's k and v for all of them
+    const int b = blockIdx.y * gridDim.x + blockIdx.x, n = b / 8;
+    split = n / (int)gridDim.x * 8 + b % 8;
+    R0 = n % (int)gridDim.x * R;
   }
-  if (lane == 0) sm[w] = m, sl[w] = l;
+  const int t0 = split * a.tps, t1 = min(t0 + a.tps, a.tiles);
+  // (rows past the last: the last one again, not stored)
+  int row[RT], node[RT];
 #pragma unroll
-  for (int j = 0; j < DPL; ++j) so[w][DPL * lane + j] = o[j];
+  for (int r = 0; r < RT; ++r) {
+    row[r] = min(R0 + 16 * r + c, nrows - 1);
+    node[r] = row[r] / a.heads;
+  }
+  const int last = a.prefix + a.nodes - 1;  // last cache row
+  const bool has_tree = t1 > a.ptiles;
+  auto key0_of = [&](int tile) {
+    return tile < a.ptiles ? a.first + tile * kTile : a.prefix + (tile - a.ptiles) * kTile;
+  };
+  auto end_of = [&](int tile) { return tile < a.ptiles ? a.prefix - 1 : last; };
+  float4 kr[NJ], vr[4][NQ];
+  auto load_k = [&](int tile) {
+    tile = min(tile, t1 - 1);
+    const float *p = a.k + (size_t)min(key0_of(tile) + c, end_of(tile)) * HD + d0 + 4 * g;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const float4 *>(p + 16 * j);
+  };
+  auto load_v = [&](int tile) {
+    tile = min(tile, t1 - 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float *p = a.v + (size_t)min(key0_of(tile) + 4 * g + i, end_of(tile)) * HD + d0 + 4 * c;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) vr[i][q] = *reinterpret_cast<const float4 *>(p + 64 * q);
+    }
+  };
+  load_k(t0 + kg);
+  load_v(t0 + kg);
+  float4 qr[RT][NJ];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      qr[r][j] = *reinterpret_cast<const float4 *>(a.q + (size_t)row[r] * HD + d0 + 16 * j + 4 * g);
+  if (has_tree || a.window > 0) make_tree<NTH>(a, sm.loop.tree);
+  // keys at positions > low are in the row's window
+  int low[RT], high = -1;
+  bool bad[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int depth = has_tree || a.window > 0 ? sm.loop.tree.depth[node[r]] : 0;
+    bad[r] = depth < 0;
+    low[r] = a.window > 0 ? a.prefix + depth - a.window : -1;
+    high = max(high, low[r]);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) high = max(high, __shfl_xor(high, o, 64));
+
+  float m[RT], l[RT];  // l: this lane's keys only
+  f32x4 o[RT][4 * NQ];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = kNoScore;
+    l[r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4 * NQ; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  const int steps = (t1 - t0 + KG - 1) / KG;
+  for (int it = 0; it < steps; ++it) {
+    const int tile = t0 + kg + it * KG;
+    const bool mine = tile < t1;
+    const int key0 = key0_of(min(tile, t1 - 1));
+    f32x4 s[RT];
+    {
+      f32x4 sa[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) sa[r][0] = sa[r][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const float kk[4] = {kr[j].x, kr[j].y, kr[j].z, kr[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float qq[4] = {qr[r][j].x, qr[r][j].y, qr[r][j].z, qr[r][j].w};
+            sa[r][i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[i], qq[i], sa[r][i & 1], 0, 0, 0);
+          }
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r] = sa[r][0] + sa[r][1];
+    }
+    load_k(tile + KG);
+    if (DQ > 1) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) sm.loop.sx[it & 1][kg][w][r][lane] = s[r];
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        s[r] = sm.loop.sx[it & 1][kg][0][r][lane];
+#pragma unroll
+        for (int d = 1; d < DQ; ++d) s[r] += sm.loop.sx[it & 1][kg][d][r][lane];
+      }
+    }
+    // whether every row sees every key of the tile
+    const bool inner = mine && tile < a.ptiles && key0 > high && key0 + kTile <= a.prefix;
+    uint32_t seen[RT];  // bit i: row c sees key 4 g + i
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      seen[r] = 15u;
+      if (!inner) {
+        uint32_t bits = 0;
+        if (tile >= a.ptiles) {
+          const int j0 = key0 - a.prefix;  // of 16 within 32 nodes
+          bits = mine ? sm.loop.tree.sees[node[r]][j0 >> 5] >> (j0 & 16) >> (4 * g) & 15u : 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = min(j0 + 4 * g + i, a.nodes - 1);
+            if (a.prefix + sm.loop.tree.depth[j] <= low[r]) bits &= ~(1u << i);
+          }
+        } else if (mine) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 4 * g + i;
+            if (key < a.prefix && key > low[r]) bits |= 1u << i;
+          }
+        }
+        seen[r] = bits;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(bits >> i & 1)) s[r][i] = -INFINITY;
+      }
+    }
+    float p[RT][4];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float tm = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
+      // (fmaxf drops a NaN score, whose p is NaN.)
+      const float mn = fmaxf(m[r], group_max(tm));
+      const float corr = __builtin_amdgcn_exp2f((m[r] - mn) * kLog2e);
+      m[r] = mn;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[r][i] = __builtin_amdgcn_exp2f((s[r][i] - mn) * kLog2e);
+      l[r] = fmaf(l[r], corr, (p[r][0] + p[r][1]) + (p[r][2] + p[r][3]));
+      if (__any(corr != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < 4 * NQ; ++n) o[r][n] *= corr;
+      }
+    }
+    // a weight of 0 times a value that is not finite would reach rows that do not see the key
+    bool odd = false;
+    if (!inner) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const float4 x = vr[i][q];
+          odd = odd || !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w));
+        }
+      odd = __any(odd);
+    }
+    if (!odd) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const float vv[4] = {vr[i][q].x, vr[i][q].y, vr[i][q].z, vr[i][q].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+              o[r][4 * q + e] =
+                  __builtin_amdgcn_mfma_f32_16x16x4f32(vv[e], p[r][i], o[r][4 * q + e], 0, 0, 0);
+        }
+    } else if (mine) {  // keys that the row sees, one by one
+      for (int kk = 0; kk < kTile; ++kk)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int from = 16 * (kk >> 2) + c, i = kk & 3;
+          const float pi = i == 0 ? p[r][0] : i == 1 ? p[r][1] : i == 2 ? p[r][2] : p[r][3];
+          const float pk = __shfl(pi, from, 64);
+          const uint32_t see = (uint32_t)__shfl((int)seen[r], from, 64) >> i & 1u;
+          if (!see) continue;
+          // lane (c, g): tile n, register v holds dim 64 q + 4 (4 g + v) + e
+          const float *vp = a.v + (size_t)min(key0 + kk, end_of(tile)) * HD + d0 + 16 * g;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const float4 x = *reinterpret_cast<const float4 *>(vp + 64 * q + 4 * v);
+              o[r][4 * q][v] = fmaf(pk, x.x, o[r][4 * q][v]);
+              o[r][4 * q + 1][v] = fmaf(pk, x.y, o[r][4 * q + 1][v]);
+              o[r][4 * q + 2][v] = fmaf(pk, x.z, o[r][4 * q + 2][v]);
+              o[r][4 * q + 3][v] = fmaf(pk, x.w, o[r][4 * q + 3][v]);
+              __builtin_amdgcn_sched_barrier(0);  // few registers: this is rare
+            }
+        }
+    }
+    load_v(tile + KG);
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor(l[r], 16, 64);
+    l[r] += __shfl_xor(l[r], 32, 64);
+    if (bad[r]) l[r] = __int_as_float(0x7fc00000);
+    if (w == 0 && g == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
+  }
   __syncthreads();
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float f[4], L = 0.f;
+  // the key groups, added in order
+  float M[RT], L[RT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = sl[i] != 0.f ? expf(sm[i] - M) : 0.f;
-    L += f[i] * sl[i];
-  }
-  for (int i = t; i < HD; i += 256) {
-    float s = 0.f;
+  for (int r = 0; r < RT; ++r) {
+    M[r] = kNoScore;
+    L[r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s += f[j] != 0.f ? f[j] * so[j][i] : 0.f;
-    y[i] = s / L;
+    for (int k = 0; k < KG; ++k) M[r] = fmaxf(M[r], wml[k][16 * r + c].x);
+#pragma unroll
+    for (int k = 0; k < KG; ++k)
+      L[r] = fmaf(wml[k][16 * r + c].y, __builtin_amdgcn_exp2f((wml[k][16 * r + c].x - M[r]) * kLog2e), L[r]);
+    const float f = __builtin_amdgcn_exp2f((m[r] - M[r]) * kLog2e);
+    if (KG > 1)
+#pragma unroll
+      for (int n = 0; n < 4 * NQ; ++n) o[r][n] *= f;
   }
+  for (int k = KG - 1; k >= 1; --k) {
+    if (kg == k)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            float4 *dst = reinterpret_cast<float4 *>(&sm.o[16 * r + c][d0 + 64 * q + 16 * g + 4 * v]);
+            *dst = make_float4(o[r][4 * q][v], o[r][4 * q + 1][v], o[r][4 * q + 2][v], o[r][4 * q + 3][v]);
+          }
+    __syncthreads();
+    if (kg == 0)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float4 x = *reinterpret_cast<const float4 *>(&sm.o[16 * r + c][d0 + 64 * q + 16 * g + 4 * v]);
+            o[r][4 * q][v] += x.x;
+            o[r][4 * q + 1][v] += x.y;
+            o[r][4 * q + 2][v] += x.z;
+            o[r][4 * q + 3][v] += x.w;
+          }
+    __syncthreads();
+  }
+  if (kg > 0) return;
+  const bool whole = a.splits == 1;
+  float *out = whole ? a.y : a.part + (size_t)split * nrows * HD;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    if (R0 + 16 * r + c >= nrows) continue;
+    if (!whole && w == 0 && g == 0) a.ml[(size_t)split * nrows + row[r]] = make_float2(M[r], L[r]);
+    float *p = out + (size_t)row[r] * HD + d0 + 16 * g;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float4 x = make_float4(o[r][4 * q][v], o[r][4 * q + 1][v], o[r][4 * q + 2][v], o[r][4 * q + 3][v]);
+        if (whole) x = make_float4(x.x / L[r], x.y / L[r], x.z / L[r], x.w / L[r]);
+        *reinterpret_cast<float4 *>(p + 64 * q + 4 * v) = x;
+      }
+  }
+}
+
+// Adds the key splits of a row in order: y = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
+// A block is one row, a thread one 16-byte unit of it (hd / 4 threads, at least a wave).
+template <int HD>
+__global__ __launch_bounds__(HD >= 256 ? HD / 4 : 64) void attn_tree_merge_kernel(TreeArgs a) {
+  const int t = threadIdx.x, lane = t & 63, row = blockIdx.x, nrows = a.nodes * a.heads;
+  __shared__ float wt[kMaxSplits];
+  __shared__ float sum;
+  if (t < 64) {  // a lane per split
+    const float2 ml = a.ml[(size_t)min(lane, a.splits - 1) * nrows + row];
+    float M = ml.x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float e = lane < a.splits ? __builtin_amdgcn_exp2f((ml.x - M) * kLog2e) : 0.f;
+    wt[lane] = e;
+    const float L = wave_sum(lane < a.splits ? e * ml.y : 0.f);
+    if (lane == 0) sum = L;
+  }
+  __syncthreads();
+  if (t >= HD / 4) return;
+  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + t;
+  const size_t step = (size_t)nrows * HD / 4;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 8;
+  for (int s0 = 0; s0 < a.splits; s0 += U) {
+    f32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = p[min(s0 + u, a.splits - 1) * step];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u < a.splits) y += wt[s0 + u] * x[u];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] /= sum;
+  reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[t] = y;
+}
+
+int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+Workspace g_tree_ws;
+
+template <int HD, int RT, int KG>
+int launch_tree(TreeArgs a) {
+  const int rows = a.nodes * a.heads, blocks = cdiv(rows, 16 * RT);
+  // a block per CU; two where each then has many tiles (two blocks' latencies overlap, and
+  // the splits' outputs are few beside the tiles)
+  const int one = cu_count() / blocks, two = 2 * cu_count() / blocks;
+  int splits = one < 1 ? 1 : one;
+  if (cdiv(a.tiles, splits) > 8) splits = two < 1 ? 1 : two;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  if (splits > 8 && a.tiles > 8 * splits) splits = splits / 8 * 8;
+  a.tps = cdiv(a.tiles, splits);
+  if (a.tps < KG) a.tps = KG;
+  a.splits = cdiv(a.tiles, a.tps);
+  if (a.splits > 1) {
+    void *mem = nullptr;
+    const size_t part = (size_t)a.splits * rows * HD;
+    if (int rc = g_tree_ws.get((part + (size_t)a.splits * rows * 2) * 4, &mem, "g4_attention_tree"))
+      return rc;
+    a.part = static_cast<float *>(mem);
+    a.ml = reinterpret_cast<float2 *>(a.part + part);
+  }
+  hipLaunchKernelGGL((attn_tree_kernel<HD, RT, KG>), dim3(blocks, a.splits),
+                     dim3(64 * kDimWaves<HD> * KG), 0, stream(), a);
+  G4_LAUNCH_CHECK("attn_tree_kernel");
+  if (a.splits == 1) return G4_OK;
+  hipLaunchKernelGGL(attn_tree_merge_kernel<HD>, dim3(rows), dim3(HD >= 256 ? HD / 4 : 64), 0, stream(), a);
+  G4_LAUNCH_CHECK("attn_tree_merge_kernel");
+  return G4_OK;
 }
 
 }  // namespace
@@ -104,13 +458,17 @@ G4_API int g4_attention_tree(const float *q, const float *k, const float *v, int
                              int head_dim, int prefix, const int32_t *parents, int sliding,
                              int window, float *y) {
   if (nodes < 0 || nodes > kMaxNodes || heads <= 0 || heads > 8 || prefix < 0 ||
-      prefix > 0x7fffffff - kMaxNodes ||
+      prefix > 0x7fffffff - 2 * kMaxNodes ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) ||
       (sliding && window <= 0))
     return fail(G4_E_ARG,
                 "g4_attention_tree: nodes %d (<= %d), heads %d (<= 8), head_dim %d (64, 128, 256 or "
                 "512), prefix %d, window %d",
                 nodes, kMaxNodes, heads, head_dim, prefix, window);
+  const void *ptrs[] = {q, k, v, y};
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15)
+      return fail(G4_E_ARG, "g4_attention_tree: q, k, v and y must be 16-byte aligned");
   G4_CHECK_INIT();
   if (nodes == 0) return ok();
   const size_t qn = (size_t)nodes * heads * head_dim * 4;
@@ -121,14 +479,25 @@ G4_API int g4_attention_tree(const float *q, const float *k, const float *v, int
   if (!rc) rc = check_device_range(parents, (size_t)nodes * 4, "g4_attention_tree parents");
   if (!rc) rc = check_device_range(y, qn, "g4_attention_tree y");
   if (rc) return rc;
-  TreeArgs a{q, k, v, y, parents, nodes, heads, prefix, sliding ? window : 0};
-  const dim3 grid(nodes * heads);
-  switch (head_dim / 64) {
-    case 1: hipLaunchKernelGGL(attn_tree_kernel<1>, grid, dim3(256), 0, stream(), a); break;
-    case 2: hipLaunchKernelGGL(attn_tree_kernel<2>, grid, dim3(256), 0, stream(), a); break;
-    case 4: hipLaunchKernelGGL(attn_tree_kernel<4>, grid, dim3(256), 0, stream(), a); break;
-    default: hipLaunchKernelGGL(attn_tree_kernel<8>, grid, dim3(256), 0, stream(), a); break;
+  TreeArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.y = y;
+  a.parents = parents;
+  a.nodes = nodes;
+  a.heads = heads;
+  a.prefix = prefix;
+  a.window = sliding ? window : 0;
+  // a root sees the most of the prefix: positions > prefix - window
+  a.first = a.window > 0 && prefix >= a.window ? prefix - a.window + 1 : 0;
+  a.ptiles = a.first < prefix ? cdiv(prefix - a.first, kTile) : 0;
+  a.tiles = a.ptiles + cdiv(nodes, kTile);
+  switch (head_dim) {
+    case 64: rc = launch_tree<64, 2, 4>(a); break;
+    case 128: rc = launch_tree<128, 2, 2>(a); break;
+    case 256: rc = launch_tree<256, 1, 1>(a); break;
+    default: rc = launch_tree<512, 1, 1>(a); break;
   }
-  G4_LAUNCH_CHECK("attn_tree_kernel");
-  return ok();
+  return rc ? rc : ok();
 }
