@@ -401,7 +401,7 @@ __global__ __launch_bounds__(HD >= 256 ? HD / 4 : 64) void attn_tree_merge_kerne
   const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + t;
   const size_t step = (size_t)nrows * HD / 4;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 8;
+  constexpr int U = 16;
   for (int s0 = 0; s0 < a.splits; s0 += U) {
     f32x4 x[U];
 #pragma unroll

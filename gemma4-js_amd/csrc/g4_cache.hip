@@ -13,17 +13,85 @@ struct Planes {
   int width[kMaxPlanes];
 };
 
-// One block per (row, plane): dst row dst_row + i = src row rows[i], or NaN for an
-// entry outside [0, src_rows).  rows == nullptr: row i itself.
-__global__ __launch_bounds__(256) void cache_rows_kernel(Planes p, const int *__restrict__ rows,
-                                                         int dst_row, int src_rows) {
-  const int i = blockIdx.x, plane = blockIdx.y;
+constexpr int kChunk = 64;    // 16-byte units (WIDE; else floats) of a row that a wave moves at once
+constexpr int kCopyRows = 8;  // chunks per wave of a copy, their loads together
+constexpr int kPlaceRows = 64;  // rows that move in place in one launch
+
+template <bool WIDE>
+struct Unit {
+  typedef f32x4 type;
+  static constexpr int floats = 4;
+};
+template <>
+struct Unit<false> {
+  typedef float type;
+  static constexpr int floats = 1;
+};
+
+// Unit `at` of source row rows[i] (row i itself without rows), or NaN for an entry outside
+// [0, src_rows).
+template <bool WIDE>
+__device__ __forceinline__ typename Unit<WIDE>::type row_unit(const float *src, int units, const int *rows,
+                                                              int i, int src_rows, int at) {
+  typedef typename Unit<WIDE>::type T;
   const int r = rows ? rows[i] : i;
   const bool ok = r >= 0 && r < src_rows;
-  const int width = p.width[plane];
-  const float *s = p.src[plane] + (size_t)(ok ? r : 0) * width;
-  float *d = p.dst[plane] + ((size_t)dst_row + i) * width;
-  for (int c = threadIdx.x; c < width; c += 256) d[c] = ok ? s[c] : __int_as_float(0x7fc00000);
+  const T v = __builtin_nontemporal_load(reinterpret_cast<const T *>(src) + (size_t)(ok ? r : 0) * units + at);
+  return ok ? v : (T)(0.f) + __int_as_float(0x7fc00000);
+}
+
+// dst row dst_row + i = src row rows[i]; blockIdx.y is the plane, a wave takes kCopyRows
+// chunks one after the other.  Bound by memory: 4000 rows of 30 planes (147 MB read, as
+// much written) 52 us, 5.7 TB/s; through the caches 59, with a block per row and 4 bytes
+// per lane 94.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void cache_copy_kernel(Planes p, const int *__restrict__ rows, int n,
+                                                         int dst_row, int src_rows) {
+  typedef typename Unit<WIDE>::type T;
+  const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int plane = blockIdx.y, units = p.width[plane] / Unit<WIDE>::floats;
+  const int chunks = (units + kChunk - 1) / kChunk;
+  const float *src = p.src[plane];
+  T *dst = reinterpret_cast<T *>(p.dst[plane]) + (size_t)dst_row * units;
+  const long first = (long)wave * kCopyRows, all = (long)n * chunks;
+  if (first >= all) return;
+  T v[kCopyRows];
+#pragma unroll
+  for (int u = 0; u < kCopyRows; ++u) {
+    const long k = first + u < all ? first + u : all - 1;
+    const int i = (int)(k / chunks), at = (int)(k - (long)i * chunks) * kChunk + lane;
+    v[u] = row_unit<WIDE>(src, units, rows, i, src_rows, at < units ? at : units - 1);
+  }
+#pragma unroll
+  for (int u = 0; u < kCopyRows; ++u) {
+    const long k = first + u;
+    const int i = (int)(k / chunks), at = (int)(k - (long)i * chunks) * kChunk + lane;
+    if (k < all && at < units) __builtin_nontemporal_store(v[u], dst + (size_t)i * units + at);
+  }
+}
+
+// The same in place for up to kPlaceRows rows: a block owns 64 units of every row of a
+// plane and reads them all before it writes any.  Bound by the launch: 5 rows of 30 planes
+// 5.7 us per call, 9.3 through scratch in two launches.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void cache_place_kernel(Planes p, const int *__restrict__ rows, int n,
+                                                          int dst_row, int src_rows) {
+  typedef typename Unit<WIDE>::type T;
+  constexpr int U = kPlaceRows / 4;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int plane = blockIdx.y, units = p.width[plane] / Unit<WIDE>::floats;
+  const int at = blockIdx.x * kChunk + lane;
+  if (blockIdx.x * kChunk >= units) return;  // whole blocks
+  T v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (w + 4 * u < n)
+      v[u] = row_unit<WIDE>(p.src[plane], units, rows, w + 4 * u, src_rows, at < units ? at : units - 1);
+  __syncthreads();
+  T *dst = reinterpret_cast<T *>(p.dst[plane]) + (size_t)dst_row * units;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (w + 4 * u < n && at < units) dst[(size_t)(w + 4 * u) * units + at] = v[u];
 }
 
 Workspace g_cache_ws;
@@ -47,7 +115,8 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
   int rc = check_device_range(rows, (size_t)n * 4, "g4_cache_rows rows");
   Planes out{}, in{};
   size_t staged = 0;
-  bool place = false;
+  bool place = false, wide = true;
+  int widest = 0;
   for (int p = 0; p < planes && !rc; ++p) {
     const size_t w = (size_t)widths[p];
     rc = check_device_range(dst[p], ((size_t)dst_row + n) * w * 4, "g4_cache_rows dst");
@@ -59,26 +128,44 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
     const uintptr_t s0 = reinterpret_cast<uintptr_t>(src[p]);
     place = place || (d0 < s0 + src_rows * w * 4 && s0 < d0 + n * w * 4);
     staged += n * w;
+    if (widths[p] > widest) widest = widths[p];
+    wide = wide && widths[p] % 4 == 0 &&
+           ((reinterpret_cast<uintptr_t>(dst[p]) | reinterpret_cast<uintptr_t>(src[p])) & 15) == 0;
   }
   if (rc) return rc;
-  const dim3 grid(n, planes);
-  if (!place) {
+  if (place && n <= kPlaceRows) {
     for (int p = 0; p < planes; ++p) in.dst[p] = out.dst[p];
-    hipLaunchKernelGGL(cache_rows_kernel, grid, dim3(256), 0, stream(), in, rows, dst_row, src_rows);
-    G4_LAUNCH_CHECK("cache_rows_kernel");
+    const int units = wide ? widest / 4 : widest;
+    hipLaunchKernelGGL(wide ? cache_place_kernel<true> : cache_place_kernel<false>,
+                       dim3((units + kChunk - 1) / kChunk, planes), dim3(256), 0, stream(), in, rows, n,
+                       dst_row, src_rows);
+    G4_LAUNCH_CHECK("cache_place_kernel");
     return ok();
   }
+  auto copy = [&](const Planes &pl, const int32_t *from, int to, int limit) {
+    const long units = wide ? widest / 4 : widest, chunks = (units + kChunk - 1) / kChunk;
+    const long blocks = (n * chunks + 4 * kCopyRows - 1) / (4 * kCopyRows);
+    if (blocks > 0x7fffffffl / 2) return fail(G4_E_ARG, "g4_cache_rows: %d rows of %d values", n, widest);
+    hipLaunchKernelGGL(wide ? cache_copy_kernel<true> : cache_copy_kernel<false>,
+                       dim3((unsigned)blocks, planes), dim3(256), 0, stream(), pl, from, n, to, limit);
+    G4_LAUNCH_CHECK("cache_copy_kernel");
+    return G4_OK;
+  };
+  if (!place) {
+    for (int p = 0; p < planes; ++p) in.dst[p] = out.dst[p];
+    rc = copy(in, rows, dst_row, src_rows);
+    return rc ? rc : ok();
+  }
+  // more rows in place: all of them to scratch, then to where they go
   void *mem = nullptr;
   if ((rc = g_cache_ws.get(staged * 4, &mem, "g4_cache_rows"))) return rc;
-  float *at = static_cast<float *>(mem);
+  float *to = static_cast<float *>(mem);
   for (int p = 0; p < planes; ++p) {
-    in.dst[p] = at;
-    out.src[p] = at;
-    at += (size_t)n * widths[p];
+    in.dst[p] = to;
+    out.src[p] = to;
+    to += (size_t)n * widths[p];
   }
-  hipLaunchKernelGGL(cache_rows_kernel, grid, dim3(256), 0, stream(), in, rows, 0, src_rows);
-  G4_LAUNCH_CHECK("cache_rows_kernel");
-  hipLaunchKernelGGL(cache_rows_kernel, grid, dim3(256), 0, stream(), out, nullptr, dst_row, n);
-  G4_LAUNCH_CHECK("cache_rows_kernel");
-  return ok();
+  rc = copy(in, rows, 0, src_rows);
+  if (!rc) rc = copy(out, nullptr, dst_row, n);
+  return rc ? rc : ok();
 }

@@ -378,7 +378,8 @@ int g4_argmax(const float *x, int n, int32_t *out_dev);
  *   window.
  * A parent outside [-1, i) gives NaN rows for node i and every node below it.
  * k/v rows that no node sees have no influence, whatever they hold.
- * heads <= 8; head_dim 64, 128, 256 or 512; nodes <= 256. */
+ * heads <= 8; head_dim 64, 128, 256 or 512; nodes <= 256; q, k, v and y 16-byte
+ * aligned. */
 int g4_attention_tree(const float *q, const float *k, const float *v, int nodes,
                       int heads, int head_dim, int prefix, const int32_t *parents,
                       int sliding, int window, float *y);
