@@ -14,7 +14,7 @@ struct Planes {
 };
 
 constexpr int kChunk = 64;    // 16-byte units (WIDE; else floats) of a row that a wave moves at once
-constexpr int kCopyRows = 8;  // chunks per wave of a copy, their loads together
+constexpr int kCopyRows = 4;  // chunks per wave of a copy, their loads together
 constexpr int kPlaceRows = 64;  // rows that move in place in one launch
 
 template <bool WIDE>
@@ -42,8 +42,8 @@ __device__ __forceinline__ typename Unit<WIDE>::type row_unit(const float *src, 
 
 // dst row dst_row + i = src row rows[i]; blockIdx.y is the plane, a wave takes kCopyRows
 // chunks one after the other.  Bound by memory: 4000 rows of 30 planes (147 MB read, as
-// much written) 52 us, 5.7 TB/s; through the caches 59, with a block per row and 4 bytes
-// per lane 94.
+// much written) 48 us, 6.2 TB/s; 8 chunks per wave 52, these through the caches 59, a block
+// per row with 4 bytes per lane 94.
 template <bool WIDE>
 __global__ __launch_bounds__(256) void cache_copy_kernel(Planes p, const int *__restrict__ rows, int n,
                                                          int dst_row, int src_rows) {
