@@ -22,6 +22,7 @@ struct TreeArgs {
   int first;    // first prefix key of the first tile
   int ptiles;   // tiles of the prefix; those of the tree follow
   int tiles, tps, splits;
+  bool one_l2;  // the row blocks of a split go to one XCD
   float *part;  // [splits][rows][hd] unnormalised outputs
   float2 *ml;   // [splits][rows] (max, sum)
 };
@@ -81,9 +82,9 @@ __device__ __forceinline__ float group_max(float v) {
 template <int HD>
 constexpr int kDimWaves = HD >= 256 ? 4 : HD / 64;
 
-// A block owns 16 RT rows of [nodes * heads, hd] and a run of key tiles, which its KG key
-// groups take in turn; the DQ waves of a group share the head dim.  On the FP32 matrix
-// cores (v_mfma_f32_16x16x4f32), lane (c, g) of a wave working for row c throughout:
+// A block owns 16 rows of [nodes * heads, hd] and a run of key tiles, which its KG key groups
+// take in turn; the DQ waves of a group share the head dim.  On the FP32 matrix cores
+// (v_mfma_f32_16x16x4f32), lane (c, g) of a wave working for row c throughout:
 //   S^T = K . Q^T     a wave's dims; the group's waves add theirs through LDS, in wave order,
 //                     so that they hold the same scores: keys 4 g .. + 3 per lane
 //   softmax           running maximum and sum per row
@@ -91,13 +92,23 @@ constexpr int kDimWaves = HD >= 256 ? 4 : HD / 64;
 //                     4 g + i); output tile 4 q + e holds dims 64 q + 4 c + e, so V and O
 //                     move as 16-byte vectors
 // The next tile's K is loaded once the scores are formed, its V once the outputs are.
-template <int HD, int RT, int KG>
+//
+// Over long caches the FP32 products bound it: 64 nodes x 8 heads of 512 over 16000 keys, 16.8
+// GFLOP, take 150 us (112 TFLOP/s) with two blocks per CU.  What a wave does between its products
+// is what is left: rows of V that are not finite, dealt with in a branch of its own beside the
+// products, cost 32 register moves per tile (182 us, without 171); 64-bit addresses per lane
+// instead of a scalar base 15 us more.  32 rows per block (half the loads of K and V) take 209 us,
+// two such groups of 16 in step 217, the scores of the next tile formed ahead of the softmax 210.
+// Short caches wait for their loads: 4 nodes over 203 keys 8.9 us, two launches.
+// Head dims of 64 and 128: 4 and 2 key groups; twice as many take 9.8 us instead of 8.6 for 4
+// nodes over 200 keys of dim 64, 38 instead of 33 for 64 nodes over 16000.
+template <int HD, int KG>
 __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(TreeArgs a) {
   constexpr int DQ = kDimWaves<HD>, DW = HD / DQ, NJ = DW / 16, NQ = DW / 64;
-  constexpr int NTH = 64 * DQ * KG, R = 16 * RT;
+  constexpr int NTH = 64 * DQ * KG, R = 16;
   struct Loop {
     Tree tree;
-    f32x4 sx[2][KG][DQ][RT][64];  // the waves' scores, two buffers
+    f32x4 sx[2][KG][DQ][64];  // the waves' scores, two buffers
   };
   union Smem {
     Loop loop;
@@ -105,25 +116,20 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
   };
   __shared__ Smem sm;
   __shared__ float2 wml[KG][R];
-  const int t = threadIdx.x, lane = t & 63, w = (t >> 6) % DQ, kg = (t >> 6) / DQ;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int w = wave % DQ, kg = wave / DQ;
   const int c = lane & 15, g = lane >> 4;
   const int nrows = a.nodes * a.heads, d0 = w * DW;
   int split = blockIdx.y, R0 = blockIdx.x * R;
-  if (a.splits % 8 == 0) {
-    // the row blocks of a split go to one XCD (blocks are dealt to the 8 in turn), whose L2
-    // then holds the split's k and v for all of them
+  if (a.one_l2) {  // blocks are dealt to the 8 XCDs in turn; there are multiples of 8 splits
     const int b = blockIdx.y * gridDim.x + blockIdx.x, n = b / 8;
     split = n / (int)gridDim.x * 8 + b % 8;
     R0 = n % (int)gridDim.x * R;
+    if (split >= a.splits) return;
   }
   const int t0 = split * a.tps, t1 = min(t0 + a.tps, a.tiles);
   // (rows past the last: the last one again, not stored)
-  int row[RT], node[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    row[r] = min(R0 + 16 * r + c, nrows - 1);
-    node[r] = row[r] / a.heads;
-  }
+  const int row = min(R0 + c, nrows - 1), node = row / a.heads;
   const int last = a.prefix + a.nodes - 1;  // last cache row
   const bool has_tree = t1 > a.ptiles;
   auto key0_of = [&](int tile) {
@@ -131,133 +137,115 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
   };
   auto end_of = [&](int tile) { return tile < a.ptiles ? a.prefix - 1 : last; };
   float4 kr[NJ], vr[4][NQ];
+  // (the tile's first key is the same for the wave: a scalar base, 32-bit offsets within the tile)
   auto load_k = [&](int tile) {
     tile = min(tile, t1 - 1);
-    const float *p = a.k + (size_t)min(key0_of(tile) + c, end_of(tile)) * HD + d0 + 4 * g;
+    const int k0 = key0_of(tile);
+    const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + d0);
+    const uint32_t at = (uint32_t)(min(c, end_of(tile) - k0) * HD + 4 * g) * 4;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const float4 *>(p + 16 * j);
+    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const float4 *>(p + at + 64 * j);
   };
   auto load_v = [&](int tile) {
     tile = min(tile, t1 - 1);
+    const int k0 = key0_of(tile);
+    const char *p = reinterpret_cast<const char *>(a.v + (size_t)k0 * HD + d0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float *p = a.v + (size_t)min(key0_of(tile) + 4 * g + i, end_of(tile)) * HD + d0 + 4 * c;
+      const uint32_t at = (uint32_t)(min(4 * g + i, end_of(tile) - k0) * HD + 4 * c) * 4;
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) vr[i][q] = *reinterpret_cast<const float4 *>(p + 64 * q);
+      for (int q = 0; q < NQ; ++q) vr[i][q] = *reinterpret_cast<const float4 *>(p + at + 256 * q);
     }
   };
   load_k(t0 + kg);
   load_v(t0 + kg);
-  float4 qr[RT][NJ];
+  float4 qr[NJ];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      qr[r][j] = *reinterpret_cast<const float4 *>(a.q + (size_t)row[r] * HD + d0 + 16 * j + 4 * g);
+  for (int j = 0; j < NJ; ++j)
+    qr[j] = *reinterpret_cast<const float4 *>(a.q + (size_t)row * HD + d0 + 16 * j + 4 * g);
   if (has_tree || a.window > 0) make_tree<NTH>(a, sm.loop.tree);
   // keys at positions > low are in the row's window
-  int low[RT], high = -1;
-  bool bad[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int depth = has_tree || a.window > 0 ? sm.loop.tree.depth[node[r]] : 0;
-    bad[r] = depth < 0;
-    low[r] = a.window > 0 ? a.prefix + depth - a.window : -1;
-    high = max(high, low[r]);
-  }
+  const int depth = has_tree || a.window > 0 ? sm.loop.tree.depth[node] : 0;
+  const bool bad = depth < 0;
+  const int low = a.window > 0 ? a.prefix + depth - a.window : -1;
+  int high = low;  // the highest of the 16 rows
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) high = max(high, __shfl_xor(high, o, 64));
+  high = __builtin_amdgcn_readfirstlane(high);
 
-  float m[RT], l[RT];  // l: this lane's keys only
-  f32x4 o[RT][4 * NQ];
+  float m = kNoScore, l = 0.f;  // l: this lane's keys only
+  f32x4 o[4 * NQ];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m[r] = kNoScore;
-    l[r] = 0.f;
-#pragma unroll
-    for (int n = 0; n < 4 * NQ; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int n = 0; n < 4 * NQ; ++n) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  // Everything loaded so far has to be there: a wait in the loop counts the loads behind the one
+  // it is for, and would count by the loop's entry, q among them, in every turn.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const int steps = (t1 - t0 + KG - 1) / KG;
   for (int it = 0; it < steps; ++it) {
     const int tile = t0 + kg + it * KG;
     const bool mine = tile < t1;
     const int key0 = key0_of(min(tile, t1 - 1));
-    f32x4 s[RT];
+    f32x4 s;
     {
-      f32x4 sa[RT][2];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) sa[r][0] = sa[r][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      f32x4 sa[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const float kk[4] = {kr[j].x, kr[j].y, kr[j].z, kr[j].w};
+        const float qq[4] = {qr[j].x, qr[j].y, qr[j].z, qr[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const float qq[4] = {qr[r][j].x, qr[r][j].y, qr[r][j].z, qr[r][j].w};
-            sa[r][i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[i], qq[i], sa[r][i & 1], 0, 0, 0);
-          }
+          sa[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[i], qq[i], sa[i & 1], 0, 0, 0);
       }
-#pragma unroll
-      for (int r = 0; r < RT; ++r) s[r] = sa[r][0] + sa[r][1];
+      s = sa[0] + sa[1];
     }
     load_k(tile + KG);
+    __builtin_amdgcn_s_setprio(1);  // before the other blocks' products (3% at head dim 256)
     if (DQ > 1) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r) sm.loop.sx[it & 1][kg][w][r][lane] = s[r];
+      sm.loop.sx[it & 1][kg][w][lane] = s;
       __syncthreads();
+      s = sm.loop.sx[it & 1][kg][0][lane];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        s[r] = sm.loop.sx[it & 1][kg][0][r][lane];
-#pragma unroll
-        for (int d = 1; d < DQ; ++d) s[r] += sm.loop.sx[it & 1][kg][d][r][lane];
-      }
+      for (int d = 1; d < DQ; ++d) s += sm.loop.sx[it & 1][kg][d][lane];
     }
     // whether every row sees every key of the tile
     const bool inner = mine && tile < a.ptiles && key0 > high && key0 + kTile <= a.prefix;
-    uint32_t seen[RT];  // bit i: row c sees key 4 g + i
+    uint32_t seen = 15u;  // bit i: row c sees key 4 g + i
+    if (!inner) {
+      uint32_t bits = 0;
+      if (tile >= a.ptiles) {
+        const int j0 = key0 - a.prefix;  // of 16 within 32 nodes
+        bits = mine ? sm.loop.tree.sees[node][j0 >> 5] >> (j0 & 16) >> (4 * g) & 15u : 0u;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      seen[r] = 15u;
-      if (!inner) {
-        uint32_t bits = 0;
-        if (tile >= a.ptiles) {
-          const int j0 = key0 - a.prefix;  // of 16 within 32 nodes
-          bits = mine ? sm.loop.tree.sees[node[r]][j0 >> 5] >> (j0 & 16) >> (4 * g) & 15u : 0u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = min(j0 + 4 * g + i, a.nodes - 1);
-            if (a.prefix + sm.loop.tree.depth[j] <= low[r]) bits &= ~(1u << i);
-          }
-        } else if (mine) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 4 * g + i;
-            if (key < a.prefix && key > low[r]) bits |= 1u << i;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int j = min(j0 + 4 * g + i, a.nodes - 1);
+          if (a.prefix + sm.loop.tree.depth[j] <= low) bits &= ~(1u << i);
         }
-        seen[r] = bits;
+      } else if (mine) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(bits >> i & 1)) s[r][i] = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 4 * g + i;
+          if (key < a.prefix && key > low) bits |= 1u << i;
+        }
       }
+      seen = bits;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(bits >> i & 1)) s[i] = -INFINITY;
     }
-    float p[RT][4];
+    float p[4];
+    const float tm = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    // (fmaxf drops a NaN score, whose p is NaN.)
+    const float mn = fmaxf(m, group_max(tm));
+    const float corr = __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+    m = mn;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const float tm = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
-      // (fmaxf drops a NaN score, whose p is NaN.)
-      const float mn = fmaxf(m[r], group_max(tm));
-      const float corr = __builtin_amdgcn_exp2f((m[r] - mn) * kLog2e);
-      m[r] = mn;
+    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f((s[i] - mn) * kLog2e);
+    l = fmaf(l, corr, (p[0] + p[1]) + (p[2] + p[3]));
+    if (__any(corr != 1.f)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[r][i] = __builtin_amdgcn_exp2f((s[r][i] - mn) * kLog2e);
-      l[r] = fmaf(l[r], corr, (p[r][0] + p[r][1]) + (p[r][2] + p[r][3]));
-      if (__any(corr != 1.f)) {
-#pragma unroll
-        for (int n = 0; n < 4 * NQ; ++n) o[r][n] *= corr;
-      }
+      for (int n = 0; n < 4 * NQ; ++n) o[n] *= corr;
     }
+    __builtin_amdgcn_s_setprio(0);
     // a weight of 0 times a value that is not finite would reach rows that do not see the key
     bool odd = false;
     if (!inner) {
@@ -270,28 +258,13 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
         }
       odd = __any(odd);
     }
-    if (!odd) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          const float vv[4] = {vr[i][q].x, vr[i][q].y, vr[i][q].z, vr[i][q].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-              o[r][4 * q + e] =
-                  __builtin_amdgcn_mfma_f32_16x16x4f32(vv[e], p[r][i], o[r][4 * q + e], 0, 0, 0);
-        }
-    } else if (mine) {  // keys that the row sees, one by one
-      for (int kk = 0; kk < kTile; ++kk)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int from = 16 * (kk >> 2) + c, i = kk & 3;
-          const float pi = i == 0 ? p[r][0] : i == 1 ? p[r][1] : i == 2 ? p[r][2] : p[r][3];
-          const float pk = __shfl(pi, from, 64);
-          const uint32_t see = (uint32_t)__shfl((int)seen[r], from, 64) >> i & 1u;
-          if (!see) continue;
+    if (odd) {  // keys that the row sees, one by one; then nothing is left of the tile
+      for (int kk = 0; mine && kk < kTile; ++kk) {
+        const int from = 16 * (kk >> 2) + c, i = kk & 3;
+        const float pi = i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3];
+        const float pk = __shfl(pi, from, 64);
+        const uint32_t see = (uint32_t)__shfl((int)seen, from, 64) >> i & 1u;
+        if (see) {
           // lane (c, g): tile n, register v holds dim 64 q + 4 (4 g + v) + e
           const float *vp = a.v + (size_t)min(key0 + kk, end_of(tile)) * HD + d0 + 16 * g;
 #pragma unroll
@@ -299,84 +272,83 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               const float4 x = *reinterpret_cast<const float4 *>(vp + 64 * q + 4 * v);
-              o[r][4 * q][v] = fmaf(pk, x.x, o[r][4 * q][v]);
-              o[r][4 * q + 1][v] = fmaf(pk, x.y, o[r][4 * q + 1][v]);
-              o[r][4 * q + 2][v] = fmaf(pk, x.z, o[r][4 * q + 2][v]);
-              o[r][4 * q + 3][v] = fmaf(pk, x.w, o[r][4 * q + 3][v]);
+              o[4 * q][v] = fmaf(pk, x.x, o[4 * q][v]);
+              o[4 * q + 1][v] = fmaf(pk, x.y, o[4 * q + 1][v]);
+              o[4 * q + 2][v] = fmaf(pk, x.z, o[4 * q + 2][v]);
+              o[4 * q + 3][v] = fmaf(pk, x.w, o[4 * q + 3][v]);
               __builtin_amdgcn_sched_barrier(0);  // few registers: this is rare
             }
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) vr[i][q] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float vv[4] = {vr[i][q].x, vr[i][q].y, vr[i][q].z, vr[i][q].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[4 * q + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[e], p[i], o[4 * q + e], 0, 0, 0);
+      }
     load_v(tile + KG);
   }
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] += __shfl_xor(l[r], 16, 64);
-    l[r] += __shfl_xor(l[r], 32, 64);
-    if (bad[r]) l[r] = __int_as_float(0x7fc00000);
-    if (w == 0 && g == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
-  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (bad) l = __int_as_float(0x7fc00000);
+  if (w == 0 && g == 0) wml[kg][c] = make_float2(m, l);
   __syncthreads();
   // the key groups, added in order
-  float M[RT], L[RT];
+  float M = kNoScore, L = 0.f;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    M[r] = kNoScore;
-    L[r] = 0.f;
+  for (int k = 0; k < KG; ++k) M = fmaxf(M, wml[k][c].x);
 #pragma unroll
-    for (int k = 0; k < KG; ++k) M[r] = fmaxf(M[r], wml[k][16 * r + c].x);
+  for (int k = 0; k < KG; ++k)
+    L = fmaf(wml[k][c].y, __builtin_amdgcn_exp2f((wml[k][c].x - M) * kLog2e), L);
+  const float f = __builtin_amdgcn_exp2f((m - M) * kLog2e);
+  if (KG > 1)
 #pragma unroll
-    for (int k = 0; k < KG; ++k)
-      L[r] = fmaf(wml[k][16 * r + c].y, __builtin_amdgcn_exp2f((wml[k][16 * r + c].x - M[r]) * kLog2e), L[r]);
-    const float f = __builtin_amdgcn_exp2f((m[r] - M[r]) * kLog2e);
-    if (KG > 1)
-#pragma unroll
-      for (int n = 0; n < 4 * NQ; ++n) o[r][n] *= f;
-  }
+    for (int n = 0; n < 4 * NQ; ++n) o[n] *= f;
   for (int k = KG - 1; k >= 1; --k) {
     if (kg == k)
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            float4 *dst = reinterpret_cast<float4 *>(&sm.o[16 * r + c][d0 + 64 * q + 16 * g + 4 * v]);
-            *dst = make_float4(o[r][4 * q][v], o[r][4 * q + 1][v], o[r][4 * q + 2][v], o[r][4 * q + 3][v]);
-          }
+        for (int v = 0; v < 4; ++v) {
+          float4 *dst = reinterpret_cast<float4 *>(&sm.o[c][d0 + 64 * q + 16 * g + 4 * v]);
+          *dst = make_float4(o[4 * q][v], o[4 * q + 1][v], o[4 * q + 2][v], o[4 * q + 3][v]);
+        }
     __syncthreads();
     if (kg == 0)
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float4 x = *reinterpret_cast<const float4 *>(&sm.o[16 * r + c][d0 + 64 * q + 16 * g + 4 * v]);
-            o[r][4 * q][v] += x.x;
-            o[r][4 * q + 1][v] += x.y;
-            o[r][4 * q + 2][v] += x.z;
-            o[r][4 * q + 3][v] += x.w;
-          }
+        for (int v = 0; v < 4; ++v) {
+          const float4 x = *reinterpret_cast<const float4 *>(&sm.o[c][d0 + 64 * q + 16 * g + 4 * v]);
+          o[4 * q][v] += x.x;
+          o[4 * q + 1][v] += x.y;
+          o[4 * q + 2][v] += x.z;
+          o[4 * q + 3][v] += x.w;
+        }
     __syncthreads();
   }
   if (kg > 0) return;
   const bool whole = a.splits == 1;
   float *out = whole ? a.y : a.part + (size_t)split * nrows * HD;
+  if (R0 + c >= nrows) return;
+  if (!whole && w == 0 && g == 0) a.ml[(size_t)split * nrows + row] = make_float2(M, L);
+  float *p = out + (size_t)row * HD + d0 + 16 * g;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if (R0 + 16 * r + c >= nrows) continue;
-    if (!whole && w == 0 && g == 0) a.ml[(size_t)split * nrows + row[r]] = make_float2(M[r], L[r]);
-    float *p = out + (size_t)row[r] * HD + d0 + 16 * g;
+  for (int q = 0; q < NQ; ++q)
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        float4 x = make_float4(o[r][4 * q][v], o[r][4 * q + 1][v], o[r][4 * q + 2][v], o[r][4 * q + 3][v]);
-        if (whole) x = make_float4(x.x / L[r], x.y / L[r], x.z / L[r], x.w / L[r]);
-        *reinterpret_cast<float4 *>(p + 64 * q + 4 * v) = x;
-      }
-  }
+    for (int v = 0; v < 4; ++v) {
+      float4 x = make_float4(o[4 * q][v], o[4 * q + 1][v], o[4 * q + 2][v], o[4 * q + 3][v]);
+      if (whole) x = make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
+      *reinterpret_cast<float4 *>(p + 64 * q + 4 * v) = x;
+    }
 }
 
 // Adds the key splits of a row in order: y = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
@@ -419,16 +391,23 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 Workspace g_tree_ws;
 
-template <int HD, int RT, int KG>
+template <int HD, int KG>
 int launch_tree(TreeArgs a) {
-  const int rows = a.nodes * a.heads, blocks = cdiv(rows, 16 * RT);
-  // a block per CU; two where each then has many tiles (two blocks' latencies overlap, and
-  // the splits' outputs are few beside the tiles)
+  const int rows = a.nodes * a.heads, blocks = cdiv(rows, 16);
+  // A block per CU; two, whose waits overlap, where each then has many tiles and the splits'
+  // outputs are little beside them.  16 nodes of 8 heads of 512 over 1900 keys (4 tiles per
+  // block): 21 us, with two blocks 25.5; 64 nodes of 256 over 1500 (13 tiles): 19.9, with two
+  // 23.8; 64 nodes of 512 over 16000 (126 tiles): 175, with two 155.
   const int one = cu_count() / blocks, two = 2 * cu_count() / blocks;
   int splits = one < 1 ? 1 : one;
-  if (cdiv(a.tiles, splits) > 8) splits = two < 1 ? 1 : two;
+  if (cdiv(a.tiles, splits) > 16) splits = two < 1 ? 1 : two;
   if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits > 8 && a.tiles > 8 * splits) splits = splits / 8 * 8;
+  // With few row blocks the tiles are done sooner than 8 L2s can all be filled with the same k
+  // and v, so each gets splits of its own: 16 nodes of 8 heads of 512 (8 blocks) over 16000 keys
+  // 56 us, else 84; over 1900 20.0, else 21.0.  With more, their loads of the same lines at the
+  // same time cost more: 32 nodes (16 blocks) over 2000 keys 25.4, else 23.1; 20 nodes over 16000
+  // 92, else 86.
+  a.one_l2 = blocks <= 8 && splits > 8;
   a.tps = cdiv(a.tiles, splits);
   if (a.tps < KG) a.tps = KG;
   a.splits = cdiv(a.tiles, a.tps);
@@ -440,7 +419,7 @@ int launch_tree(TreeArgs a) {
     a.part = static_cast<float *>(mem);
     a.ml = reinterpret_cast<float2 *>(a.part + part);
   }
-  hipLaunchKernelGGL((attn_tree_kernel<HD, RT, KG>), dim3(blocks, a.splits),
+  hipLaunchKernelGGL((attn_tree_kernel<HD, KG>), dim3(blocks, a.one_l2 ? cdiv(a.splits, 8) * 8 : a.splits),
                      dim3(64 * kDimWaves<HD> * KG), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_tree_kernel");
   if (a.splits == 1) return G4_OK;
@@ -494,10 +473,10 @@ G4_API int g4_attention_tree(const float *q, const float *k, const float *v, int
   a.ptiles = a.first < prefix ? cdiv(prefix - a.first, kTile) : 0;
   a.tiles = a.ptiles + cdiv(nodes, kTile);
   switch (head_dim) {
-    case 64: rc = launch_tree<64, 2, 4>(a); break;
-    case 128: rc = launch_tree<128, 2, 2>(a); break;
-    case 256: rc = launch_tree<256, 1, 1>(a); break;
-    default: rc = launch_tree<512, 1, 1>(a); break;
+    case 64: rc = launch_tree<64, 4>(a); break;
+    case 128: rc = launch_tree<128, 2>(a); break;
+    case 256: rc = launch_tree<256, 1>(a); break;
+    default: rc = launch_tree<512, 1>(a); break;
   }
   return rc ? rc : ok();
 }
