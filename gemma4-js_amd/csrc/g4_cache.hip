@@ -87,6 +87,7 @@ __global__ __launch_bounds__(256) void cache_place_kernel(Planes p, const int *_
   for (int u = 0; u < U; ++u)
     if (w + 4 * u < n)
       v[u] = row_unit<WIDE>(p.src[plane], units, rows, w + 4 * u, src_rows, at < units ? at : units - 1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the barrier waits for LDS only)
   __syncthreads();
   T *dst = reinterpret_cast<T *>(p.dst[plane]) + (size_t)dst_row * units;
 #pragma unroll
@@ -115,7 +116,7 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
   int rc = check_device_range(rows, (size_t)n * 4, "g4_cache_rows rows");
   Planes out{}, in{};
   size_t staged = 0;
-  bool place = false, wide = true;
+  bool place = false, shifted = false, wide = true;
   int widest = 0;
   for (int p = 0; p < planes && !rc; ++p) {
     const size_t w = (size_t)widths[p];
@@ -126,14 +127,18 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
     out.width[p] = in.width[p] = widths[p];
     const uintptr_t d0 = reinterpret_cast<uintptr_t>(dst[p] + (size_t)dst_row * w);
     const uintptr_t s0 = reinterpret_cast<uintptr_t>(src[p]);
-    place = place || (d0 < s0 + src_rows * w * 4 && s0 < d0 + n * w * 4);
+    if (d0 < s0 + src_rows * w * 4 && s0 < d0 + n * w * 4) {
+      place = true;
+      // a column's block would write what another one's reads
+      shifted = shifted || (d0 > s0 ? d0 - s0 : s0 - d0) % (w * 4) != 0;
+    }
     staged += n * w;
     if (widths[p] > widest) widest = widths[p];
     wide = wide && widths[p] % 4 == 0 &&
            ((reinterpret_cast<uintptr_t>(dst[p]) | reinterpret_cast<uintptr_t>(src[p])) & 15) == 0;
   }
   if (rc) return rc;
-  if (place && n <= kPlaceRows) {
+  if (place && !shifted && n <= kPlaceRows) {
     for (int p = 0; p < planes; ++p) in.dst[p] = out.dst[p];
     const int units = wide ? widest / 4 : widest;
     hipLaunchKernelGGL(wide ? cache_place_kernel<true> : cache_place_kernel<false>,

@@ -365,8 +365,9 @@ int g4_argmax(const float *x, int n, int32_t *out_dev);
  *   g4_norm_rope of the nodes of one depth as one row of nodes * heads heads,
  *   g4_attention_tree, g4_bf16_head_rows, g4_sample, g4_cache_rows.
  * Arguments are checked before anything else, so a refusal needs no device.
- * All four can be recorded; inside an encoder g4_attention_tree, g4_sample and a
- * g4_cache_rows that works in place need one earlier call of those sizes. */
+ * All four can be recorded; they hold scratch (g4_cache_rows only where more than
+ * 64 rows move in place), so inside an encoder they need one earlier call of those
+ * sizes. */
 
 /* Attention of a tree of drafted tokens over a cache: g4_attention with each
  * node seeing the prefix, itself and its ancestors.
@@ -388,8 +389,11 @@ int g4_attention_tree(const float *q, const float *k, const float *v, int nodes,
  *   out[j * out_stride + r] = softcap * tanh((scale * sum_k x[j, k] * E[r, k]) / softcap)
  * x: device FP32 [n, in_dim]; E: device BF16 [rows, in_dim]; out_stride >= rows
  * (floats; a chunk of the vocabulary writes into a wider logits row).  in_dim a
- * positive multiple of 8, <= 4096; E 16-byte aligned; softcap <= 0 disables the
- * cap.  n = 1 gives g4_bf16_head's bits. */
+ * positive multiple of 8, <= 4096; n <= 65536; rows <= 2^30; E 16-byte aligned;
+ * softcap <= 0 disables the cap.  n = 1 gives g4_bf16_head's bits.  For n > 1 the
+ * states enter as sums of three BF16 values: what lies below 2^-126 of a state is
+ * lost, and a state or a row of E that is not finite gives logits that are NaN
+ * where FP32 products would leave an infinity. */
 int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int in_dim,
                       float *out, size_t out_stride, float scale, float softcap);
 
@@ -421,8 +425,8 @@ int g4_sample(const float *logits, size_t stride, int rows, int vocab,
 
 /* Rows of a cache's planes (k and v of every layer): for each plane p
  *   dst[p][dst_row + i] = src[p][rows[i]],  i < n
- * as if every row were read before any is written, so with dst[p] == src[p] the
- * accepted rows move together in place; with other planes it copies (forks) a
+ * as if every row were read before any is written, so with dst[p] == src[p] (or
+ * any other overlap of the two) the accepted rows move together in place; with other planes it copies (forks) a
  * cache or picks rows from it.  Plane p: FP32 rows of widths[p] values, src_rows
  * of them in src[p], at least dst_row + n in dst[p].  rows: DEVICE int32 [n]; an
  * entry outside [0, src_rows) gives a NaN row.  Memory of different planes must

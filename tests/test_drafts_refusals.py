@@ -28,7 +28,8 @@ def test_attention_tree(nodes, heads, hd, prefix, sliding, window):
 
 @pytest.mark.parametrize("n,E,rows,k,stride", [
     (-1, 16, 8, 64, 8), (2, 16, -1, 64, 8), (2, 16, 8, 0, 8), (2, 16, 8, 12, 8), (2, 16, 8, 4104, 8),
-    (2, 16, 8, 64, 7), (2, 8, 8, 64, 8)])
+    (2, 16, 8, 64, 7), (2, 8, 8, 64, 8), (65537, 16, 8, 64, 8),
+    (2, 16, (1 << 30) + 1, 64, 1 << 31)])
 def test_head_rows(n, E, rows, k, stride):
     refused(g4hip.lib().g4_bf16_head_rows(16, n, E, rows, k, 16, stride, 1.0, 30.0),
             "g4_bf16_head_rows")

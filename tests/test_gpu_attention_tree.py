@@ -173,3 +173,24 @@ def test_refuses_short_buffers(g4):
                  (kv, kv, kv, 2, 8, 256, 10, None, False, 0, x)):
         with pytest.raises(g4.G4Error):
             g4.attention_tree(*args)
+
+
+@pytest.mark.parametrize("nodes,prefix", [(16, 9000), (7, 16383), (20, 9000)])
+def test_key_splits_by_the_row_blocks(g4, nodes, prefix):
+    # 8, 4 and 10 blocks of 16 rows, whose key splits are no multiples of 8
+    check(g4, np.random.default_rng([nodes, prefix]), nodes, 8, 256, prefix, "random", 0)
+
+
+def test_a_cache_past_32_bits(g4):
+    # a window at the end of 4.3 million rows of 512: offsets past 2^31 values
+    hd, prefix, nodes, window, near = 512, 4300000, 6, 300, 400
+    rng = np.random.default_rng(43)
+    q, k, v = inputs(rng, nodes, 4, hd, near)
+    parents = tree(rng, nodes, "random")
+    kb, vb = (g4.Buffer((prefix + nodes) * hd * 4) for _ in range(2))
+    kb.upload(k, (prefix - near) * hd * 4)
+    vb.upload(v, (prefix - near) * hd * 4)
+    qb, pb, y = g4.Buffer.from_array(q), g4.Buffer.from_array(parents), g4.Buffer(q.nbytes)
+    g4.attention_tree(qb, kb, vb, nodes, 4, hd, prefix, pb, True, window, y)
+    want = ref.attention_tree(q, k, v, near, parents.tolist(), window)
+    assert np.abs(y.download(np.float32).reshape(q.shape) - want).max() <= 2e-5 * np.abs(v).max()

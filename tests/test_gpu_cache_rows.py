@@ -99,3 +99,32 @@ def test_refuses_rows_outside_the_planes(g4):
         assert e.value.code == g4.G4_E_RANGE
     with pytest.raises(g4.G4Error):
         g4.CachePlanes(b, b, [16, 16]).rows(idx(g4, [0]), 2, 0, 10)
+
+
+@pytest.mark.parametrize("shift", [4, 1, 8, 64, 260, 512])
+@pytest.mark.parametrize("n", [7, 64, 100])
+def test_planes_that_overlap_at_any_shift(g4, shift, n):
+    # dst begins `shift` values behind src: whole rows of 256 or not
+    rng = np.random.default_rng([shift, n])
+    w, cap, at = 256, 200, 30
+    a = rng.standard_normal(cap * w + shift).astype(np.float32)
+    rows = rng.integers(0, cap, n)
+    for d, s in ((shift, 0), (0, shift)):
+        b = g4.Buffer.from_array(a)
+        g4.CachePlanes([b.at(4 * d)], [b.at(4 * s)], [w]).rows(idx(g4, rows), n, at, cap)
+        want = a.copy()
+        want[d + at * w:d + (at + n) * w] = a[s:s + cap * w].reshape(cap, w)[rows].ravel()
+        np.testing.assert_array_equal(b.download(np.float32), want)
+
+
+def test_a_cache_past_32_bits(g4):
+    w, cap = 512, 2 ** 22 + 500  # the last rows lie past 2^31 values
+    rng = np.random.default_rng(7)
+    b, near = g4.Buffer(cap * w * 4), rng.standard_normal((300, w)).astype(np.float32)
+    for n in (40, 200):
+        b.upload(near, (cap - 300) * w * 4)
+        rows = np.sort(rng.choice(300, n, False))
+        g4.CachePlanes([b], [b], [w]).rows(idx(g4, cap - 300 + rows), n, cap - 300, cap)
+        got = b.download(np.float32, 300 * w, (cap - 300) * w * 4).reshape(300, w)
+        np.testing.assert_array_equal(got[:n], near[rows])
+        np.testing.assert_array_equal(got[n:], near[n:])

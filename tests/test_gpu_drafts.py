@@ -4,6 +4,7 @@ import json
 import os
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -186,6 +187,44 @@ def test_two_recordings_and_eager_calls_share_scratch(g4):
         for s, w in zip((a, b), want):
             for got, x in zip(s.results(), w):
                 np.testing.assert_array_equal(got, x)
+
+
+def test_a_recording_without_an_earlier_call_is_refused():
+    # in a process of its own, where nothing has made scratch
+    code = """
+import sys
+sys.path.insert(0, %r)
+import numpy as np
+import g4hip as g4
+g4.init(0)
+nodes, hd, prefix, vocab, k = 8, 256, 4000, 70000, 64
+q, y, kv = g4.Buffer(nodes * 8 * hd * 4), g4.Buffer(nodes * 8 * hd * 4), g4.Buffer((prefix + nodes) * hd * 4)
+parents = g4.Buffer.from_array(np.arange(-1, nodes - 1, dtype=np.int32))
+x, E, z = g4.Buffer(nodes * k * 4), g4.Buffer(vocab * k * 2), g4.Buffer(nodes * vocab * 4)
+u, tok, pr = g4.Buffer(4 * nodes), g4.Buffer(4 * nodes), g4.Buffer(4 * nodes)
+path = g4.Buffer.from_array(np.arange(100, 200, dtype=np.int32))
+calls = [lambda: g4.attention_tree(q, kv, kv, nodes, 8, hd, prefix, parents, False, 0, y),
+         lambda: g4.bf16_head_rows(x, nodes, E, vocab, k, z, vocab, 1.0, 30.0),
+         lambda: g4.sample(z, nodes, vocab, u, tok, pr, vocab, top_k=4),
+         lambda: g4.CachePlanes([kv], [kv], [hd]).rows(path, 100, 90, prefix)]
+for call in calls:
+    with g4.Encoder() as enc:
+        try:
+            call()
+            raise SystemExit("recorded")
+        except g4.G4Error as e:
+            assert e.code == g4.G4_E_STATE, e
+for call in calls:
+    call()
+with g4.Encoder() as enc:
+    for call in calls:
+        call()
+enc.cmdbuf.submit()
+g4.sync()
+""" % os.path.join(ROOT, "gemma4-js_amd")
+    p = subprocess.run([sys.executable, "-c", code], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                       text=True, timeout=100)
+    assert p.returncode == 0, p.stdout[-2000:]
 
 
 def test_calls_are_repeatable(g4):

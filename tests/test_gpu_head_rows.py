@@ -101,3 +101,15 @@ def test_refuses_short_buffers(g4):
                  (x, 4, None, 10, 64, o)):
         with pytest.raises(g4.G4Error):
             g4.bf16_head_rows(*args)
+
+
+def test_a_table_past_32_bits(g4):
+    # 2.3e9 values, the last 40 rows checked
+    rows, k, n = 1100003, 2048, 3
+    E = g4.Buffer(rows * k * 2)
+    g4.fill_random(E, rows * k, g4.RAND_BF16_NORMAL, 11, 0.05)
+    x = np.random.default_rng(8).standard_normal((n, k)).astype(np.float32)
+    out = g4.Buffer(n * rows * 4)
+    g4.bf16_head_rows(g4.Buffer.from_array(x), n, E, rows, k, out, rows, 1.0, 30.0)
+    got = out.download(np.float32).reshape(n, rows)[:, -40:]
+    check(got, x, E.download(np.uint16, 40 * k, (rows - 40) * k * 2).reshape(40, k))

@@ -60,6 +60,47 @@ def test_many_rows(g4, rows, vocab):
         check(g4, x, rng.random(rows), **cuts)
 
 
+@pytest.mark.parametrize("rows,vocab", [(130, 70000), (300, 9000)])
+def test_many_rows_of_several_slices(g4, rows, vocab):
+    # 130 rows: enough for long slices; 300 rows: more than one launch takes
+    rng = np.random.default_rng([rows, vocab])
+    x = logits(rng, rows, vocab, spread=1.5)
+    x[1] = 0.5  # more equal logits than a list holds
+    x[2] = rng.integers(-3, 2, vocab)
+    x[3] = rng.integers(-9, 2, vocab)
+    x[rows - 1, ::3] = -np.inf
+    x[rows - 2] = np.nan
+    for cuts in [dict(), dict(temperature=0.7), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.02),
+                 dict(top_k=vocab // 5), dict(temperature=1.3, top_k=vocab // 4, top_p=0.8, min_p=0.001)]:
+        check(g4, x, rng.random(rows), **cuts)
+
+
+def test_the_largest_vocabulary(g4):
+    vocab = 1 << 22
+    rng = np.random.default_rng(22)
+    x = logits(rng, 2, vocab)
+    x[1] = rng.integers(-2, 3, vocab)
+    for cuts in [dict(), dict(temperature=0.8, top_k=100, top_p=0.95), dict(top_k=vocab // 3),
+                 dict(top_p=0.9), dict(min_p=0.02)]:
+        check(g4, x, rng.random(2), **cuts)
+
+
+def test_rows_far_apart(g4):
+    # the second row starts past 2^31 values
+    vocab, stride = 10001, 2 ** 31 + 12
+    rng = np.random.default_rng(23)
+    x, u = logits(rng, 2, vocab), rng.random(2).astype(np.float32)
+    b = g4.Buffer((stride + vocab) * 4)
+    for r in range(2):
+        b.upload(x[r], r * stride * 4)
+    bu, tok, pr = g4.Buffer.from_array(u), g4.Buffer(8), g4.Buffer(8)
+    for cuts in (dict(), dict(top_k=50, top_p=0.9)):
+        g4.sample(b, 2, vocab, bu, tok, pr, stride, **cuts)
+        want = [ref.sample(x[r], u[r], **cuts) for r in range(2)]
+        assert tok.download(np.int32).tolist() == [w[0] for w in want]
+        np.testing.assert_allclose(pr.download(np.float32), [w[1] for w in want], rtol=1e-6)
+
+
 @pytest.mark.parametrize("vocab", [257, 20000, 150000])
 def test_ties_go_to_the_lowest_index(g4, vocab):
     # logits of few values: every cut falls among equal ones
