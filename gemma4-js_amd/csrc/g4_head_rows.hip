@@ -14,6 +14,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxTiles = 4;  // 16-state tiles of a block
 constexpr int kSteps = 2;     // steps of 32 k per stage
+constexpr int kMaxStates = 65536, kMaxRows = 1 << 30;
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
@@ -304,7 +305,9 @@ using namespace g4;
 
 G4_API int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int in_dim, float *out,
                              size_t out_stride, float scale, float softcap) {
-  if (n < 0 || rows < 0) return fail(G4_E_ARG, "g4_bf16_head_rows: n %d, rows %d", n, rows);
+  if (n < 0 || n > kMaxStates || rows < 0 || rows > kMaxRows)
+    return fail(G4_E_ARG, "g4_bf16_head_rows: n %d (<= %d), rows %d (<= %d)", n, kMaxStates, rows,
+                kMaxRows);
   if (in_dim <= 0 || in_dim % 8 != 0 || in_dim > 4096)
     return fail(G4_E_ARG, "g4_bf16_head_rows: in_dim %d must be a positive multiple of 8 <= 4096",
                 in_dim);

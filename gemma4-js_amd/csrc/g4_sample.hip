@@ -192,7 +192,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, Shared &sm) {
 // Whether this block is the last one of its row to get here (all of its coherent
 // stores done before).
 __device__ __forceinline__ bool last_block(uint32_t *count, int slices, Shared &sm) {
-  __builtin_amdgcn_s_waitcnt(0);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint32_t n = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -820,7 +820,7 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 // Rows of several slices, at most kMaxRows of them.
 int launch_slices(SampleArgs a, int rows) {
   // 4096 logits to a slice, for one row's latency; longer ones where they fill the GPU
-  const int e = (long)rows * cdiv(a.vocab, 32 * NT) >= 512 || a.vocab > kMaxSlices * 8 * NT ? 32 : 8;
+  const int e = (long)rows * cdiv(a.vocab, 32 * NT) >= 512 ? 32 : 8;
   a.per = e * NT;
   a.slices = cdiv(a.vocab, a.per);
   const size_t n = (size_t)rows * a.slices;
