@@ -13,15 +13,14 @@
 // from x * 8 / temperature = whole part and fraction; below e^-31 a mass counts as 0
 // (2^-44, a unit of the sums at 262144 tokens).
 //
-// Two launches over slices of a row; each one's last block of a row goes on alone:
-//   sample_plan_kernel  per slice the largest logit and, by whole part of x * 8 / T,
-//                       count and mass; the row's last block finds the bins in which the
-//                       cuts lie (bins above them are kept, those below dropped)
-//   sample_pick_kernel  the kept mass of every slice, and a list of the tokens in those
-//                       bins; the row's last block finds the cuts among them, the slice
-//                       and the token
-// With the temperature alone the first launch ends the row, and a row of one slice takes
-// it all in one launch (sample_row_kernel).
+// Three launches, the first two over slices of the rows:
+//   sample_plan_kernel    per slice the largest logit and, by whole part of x * 8 / T, count
+//                         and mass; a row's last block finds the bins in which the cuts lie
+//                         (bins above them are kept, those below dropped)
+//   sample_pick_kernel    the kept mass of every slice, and a list of the tokens in those bins
+//   sample_finish_kernel  per row the cuts among them, the slice and the token
+// With the temperature alone there is nothing to pick, and a row of one slice takes it all in
+// one launch (sample_row_kernel).
 #include <math.h>
 
 #include <type_traits>
@@ -81,7 +80,7 @@ struct SampleArgs {
   uint32_t *maxes;  // [rows][slices] keys
   u64 *list;        // [rows][kList]
   u64 *mass;        // [rows][slices]
-  uint32_t *count;  // [2][kMaxRows] blocks that are done, 0 between launches
+  uint32_t *count;  // [kMaxRows] blocks that are done, 0 between launches
 };
 
 // Order-preserving key of a finite logit (zeros alike); 0 for any other.
@@ -130,8 +129,8 @@ __device__ __forceinline__ T get(const T *p) {
 }
 
 struct Shared {
-  u64 bins[2][kBins];  // masses of a slice's bins by wave parity; the digits' weights
-  uint32_t cnt[2][kBins];
+  u64 bins[kBins];     // masses of a slice's bins; the digits' weights
+  uint32_t cnt[kBins];
   double tab[kBins];   // unit * e^(-b/8) * e^(-1/16)
   u64 mass[kMaxSlices];
   u64 few[kFew], weight[kFew];
@@ -220,23 +219,21 @@ __device__ __forceinline__ uint32_t load_slice(const SampleArgs &a, const float 
   return block_max(best, sm);
 }
 
-// Count (for top-k) and mass of the slice's logits by bins below the largest one's, each
-// in two parts.  A mass is in units of 1 / a.unit of its bin's upper edge.
+// Count (for top-k) and mass of the slice's logits by bins below the largest one's.  A mass
+// is in units of 1 / a.unit of its bin's upper edge.
 template <int E>
 __device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (&key)[E],
                                            uint32_t best, Shared &sm) {
-  sm.bins[0][threadIdx.x] = 0;  // both parts
-  sm.cnt[0][threadIdx.x] = 0;
+  if (threadIdx.x < kBins) sm.bins[threadIdx.x] = 0, sm.cnt[threadIdx.x] = 0;
   __syncthreads();
   const double id = floor((double)logit_of(best) * a.s), unit = a.unit * kHalfBin;
-  const int part = threadIdx.x >> 6 & 1;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (key[e] == 0) continue;
     const double y = (double)logit_of(key[e]) * a.s, fl = floor(y), db = id - fl;
     if (db < kRest) {
-      atomicAdd(&sm.bins[part][(int)db], to_units(exp_part(y - fl) * unit));
-      if (a.top_k) atomicAdd(&sm.cnt[part][(int)db], 1u);
+      atomicAdd(&sm.bins[(int)db], to_units(exp_part(y - fl) * unit));
+      if (a.top_k) atomicAdd(&sm.cnt[(int)db], 1u);
     }
   }
   __syncthreads();
@@ -338,7 +335,7 @@ struct Place {
   __device__ bool likely(const SampleArgs &a, const Plan &p) const {
     return (x - (double)p.top) * a.inv_t >= a.log_min;
   }
-  __device__ double mass(const Shared &sm) const { return sm.tab[b] * exp_part(part); }
+  __device__ double mass(const double *tab) const { return tab[b] * exp_part(part); }
 };
 
 // A token in the order of the cuts: larger is earlier.
@@ -367,24 +364,24 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 lo, u64 
       const int w = rem < 8 ? rem : 8;
       rem -= w;
       __syncthreads();
-      if (t < 256) sm.bins[0][t] = 0, sm.cnt[0][t] = 0;
+      if (t < 256) sm.bins[t] = 0, sm.cnt[t] = 0;
       if (t == 0) sm.v[1] = 0, sm.v[2] = 0, sm.pick = 0;
       __syncthreads();
       each([&](u64 r) {
         const u64 c = (r - lo) >> rem;
         if (c >> w != prefix) return;
         const int d = (int)c & ((1 << w) - 1);
-        atomicAdd(&sm.bins[0][d], weight(r));
-        atomicAdd(&sm.cnt[0][d], 1u);
+        atomicAdd(&sm.bins[d], weight(r));
+        atomicAdd(&sm.cnt[d], 1u);
       });
       __syncthreads();
-      const u64 own = t < 256 ? sm.bins[0][255 - t] : 0;
+      const u64 own = t < 256 ? sm.bins[255 - t] : 0;
       u64 total;
       const u64 upto = block_scan(own, sm.wave, &total);
       if (want > total) want = total;
       if (upto - own < want && want <= upto) {
         sm.v[1] = 255 - t;
-        sm.v[2] = sm.cnt[0][255 - t];
+        sm.v[2] = sm.cnt[255 - t];
         sm.pick = upto - own;
       }
       __syncthreads();
@@ -428,15 +425,16 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 lo, u64 
 
 // The end of a row, for one block: the cuts among the listed tokens, the slice that holds
 // the picked mass, the token.  LIST: the tokens of the cuts' bins are in a.list (if they
-// fit), else they are found in the row again.  sm.plan and sm.tab are set; sm.mass holds
+// fit), else they are found in the row again.  E: tokens of a slice
+// per thread.  sm.plan and sm.tab are set; sm.mass holds
 // the slices' mass outside those bins.
-template <bool LIST>
+template <int E, bool LIST>
 __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm,
                                            u64 *listed) {
   const int t = threadIdx.x;
   const Plan &p = sm.plan;
   auto bin_of = [&](u64 r) { return Place(a, p, rank_key(r)).b; };
-  auto mass_of = [&](u64 r) { return to_units(Place(a, p, rank_key(r)).mass(sm)); };
+  auto mass_of = [&](u64 r) { return to_units(Place(a, p, rank_key(r)).mass(sm.tab)); };
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
     const bool fits = LIST && p.n <= kList, few = LIST && p.n <= kFew;
@@ -448,7 +446,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
       if (n > NT) {
         u64 r[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) r[i] = get(list + min(NT * (i + 1) + t, n - 1));
+        for (int i = 0; i < R; ++i) r[i] = list[min(NT * (i + 1) + t, n - 1)];
 #pragma unroll
         for (int i = 0; i < R; ++i) listed[NT * (i + 1) + t] = r[i];
       }
@@ -456,7 +454,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     auto each_listed = [&](auto &&f) {
       if (fits) {  // (each thread reads what it wrote)
 #pragma unroll 1
-        for (int i = t; i < n; i += NT) f(i < kNear ? listed[i] : get(list + i));
+        for (int i = t; i < n; i += NT) f(i < kNear ? listed[i] : list[i]);
       } else {
 #pragma unroll 1
         for (int i = t; i < a.vocab; i += NT) {
@@ -524,16 +522,16 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     sm.pick = want - before - (second ? m0 : 0);
   }
   __syncthreads();
-  // and in it: the wave's part of consecutive tokens, of that again, and its 64s in turn
+  // and in it the wave's part of consecutive tokens, and of that the thread's
   auto kept = [&](float v, int i, double *m) {
     const uint32_t k = key_of(v);
     const Place at(a, p, k ? k : 1u);
-    *m = at.mass(sm);
+    *m = at.mass(sm.tab);
     const int cuts = at.partial(p) | ((int)at.listed(p) & (rank_of(k, i) >= cut));
     return ((k != 0) & ((int)(at.b < p.sure) | (cuts & (int)at.likely(a, p)))) != 0;  // no branches
   };
   const int lane = t & 63, w = t >> 6;
-  int i0 = sm.v[0] * a.per, i1 = min(i0 + a.per, a.vocab);
+  const int i0 = sm.v[0] * a.per, i1 = min(i0 + a.per, a.vocab);
   want = sm.pick;
   // A slice's mass was summed by bins and rounded otherwise: beyond its tokens' masses it
   // is the last one's, and tokens of less than half a unit count 1 where there are no others.
@@ -544,52 +542,52 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     const u64 v = to_units(m);
     return !is ? (u64)0 : v > least ? v : least;
   };
-  while (i1 - i0 > 64) {
-    const int part = ((i1 - i0 + kWaves - 1) / kWaves + 63) & ~63;
-    const int j0 = i0 + w * part, j1 = min(j0 + part, i1);
-    u64 own = 0, in;
-    constexpr int U = 4;  // loads and chains of binary64 arithmetic together
-    for (int j = j0 + lane; j < j1; j += 64 * U) {
-      float y[U];
+  constexpr int Q = E > 8 ? E / 8 : 1;  // tokens of a thread
+  u64 in = 0;
+  for (int turn = 0; turn < 2; ++turn) {
+    const int j = i0 + w * (64 * E) + lane;
+    float y[E];
+    u64 own = 0;
 #pragma unroll
-      for (int k = 0; k < U; ++k) y[k] = x[min(j + 64 * k, j1 - 1)];
+    for (int k = 0; k < E; ++k) y[k] = x[min(j + 64 * k, i1 - 1)];
 #pragma unroll
-      for (int k = 0; k < U; ++k) own += units(j + 64 * k < j1 ? y[k] : NAN, j + 64 * k);
-    }
+    for (int k = 0; k < E; ++k) own += units(j + 64 * k < i1 ? y[k] : NAN, j + 64 * k);
     block_scan(own, sm.wave, &in);
-    if (in == 0) {
-      if (least) return;
-      least = 1;
-      continue;
-    }
-    if (want >= in) want = in - 1;
-    u64 first = 0;
-    for (int i = 0; i < w; ++i) first += sm.wave[i];
-    if (lane == 0 && first <= want && want < first + sm.wave[w]) {
-      sm.v[0] = w;
-      sm.pick = want - first;
-    }
-    __syncthreads();
-    i0 += (int)sm.v[0] * part;
-    i1 = min(i0 + part, i1);
-    want = sm.pick;
-  }
-  if (w > 0) return;
-  const int i = i0 + lane;
-  const float x_i = x[min(i, i1 - 1)];
-  u64 own = i < i1 ? units(x_i, i) : 0, upto_i = wave_scan(own), in = __shfl(upto_i, 63, 64);
-  if (in == 0) {
+    if (in) break;
     least = 1;
-    own = i < i1 ? units(x_i, i) : 0;
-    upto_i = wave_scan(own);
-    in = __shfl(upto_i, 63, 64);
   }
+  if (in == 0) return;
   if (want >= in) want = in - 1;
-  if (upto_i - own <= want && want < upto_i) {
-    double m;
-    kept(x_i, i, &m);
-    a.tokens[row] = i;
-    if (a.probs) a.probs[row] = (float)(m / (double)total);
+  u64 first = 0;
+  for (int i = 0; i < w; ++i) first += sm.wave[i];
+  if (lane == 0 && first <= want && want < first + sm.wave[w]) {
+    sm.v[0] = w;
+    sm.pick = want - first;
+  }
+  __syncthreads();
+  const int j0 = i0 + (int)sm.v[0] * (64 * E), j1 = min(j0 + 64 * E, i1), j = j0 + Q * t;
+  want = sm.pick;
+  float y[Q];
+  u64 v[Q], own = 0;
+#pragma unroll
+  for (int k = 0; k < Q; ++k) y[k] = x[min(j + k, j1 - 1)];
+#pragma unroll
+  for (int k = 0; k < Q; ++k) {
+    v[k] = units(j + k < j1 ? y[k] : NAN, j + k);
+    own += v[k];
+  }
+  u64 left = want - (block_scan(own, sm.wave, &in) - own);
+  if (left >= own) return;  // (also where what lies before is more than want)
+#pragma unroll
+  for (int k = 0; k < Q; ++k) {
+    if (left < v[k]) {
+      double m;
+      kept(y[k], j + k, &m);
+      a.tokens[row] = j + k;
+      if (a.probs) a.probs[row] = (float)(m / (double)total);
+      return;
+    }
+    left -= v[k];
   }
 }
 
@@ -600,15 +598,21 @@ __device__ __forceinline__ void none_finite(const SampleArgs &a, int row) {
   }
 }
 
-__device__ __forceinline__ void make_table(const SampleArgs &a, Shared &sm) {
+__device__ __forceinline__ void make_table(const SampleArgs &a, double *tab) {
   if (threadIdx.x < kBins)
-    sm.tab[threadIdx.x] =
+    tab[threadIdx.x] =
         threadIdx.x < kRest ? exp(-(double)threadIdx.x / kPerUnit) * (a.unit * kHalfBin) : 0.0;
 }
 
-// ALONE: nothing is cut, and the row ends here.
+// From the row's largest logit, of whole part id, to a slice's: bins, at most kBins.
+__device__ __forceinline__ int shift_of(const SampleArgs &a, double id, uint32_t key) {
+  const double d = key ? id - floor((double)logit_of(key) * a.s) : kBins;
+  return d < kBins ? (int)d : kBins;
+}
+
+// ALONE: nothing is cut.
 template <int E, bool ALONE>
-__global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kernel(SampleArgs a) {
+__global__ __launch_bounds__(NT, E > 8 ? 8 : 6) void sample_plan_kernel(SampleArgs a) {
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
@@ -616,20 +620,22 @@ __global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kerne
   const int i0 = slice * (E * NT);
   uint32_t best = load_slice<E>(a, x, i0, min((E * NT), a.vocab - i0), key, sm);
   uint32_t *maxes = a.maxes + (size_t)row * a.slices;
-  u64 *mass = a.mass + (size_t)row * a.slices;
   u64 *hist = a.hist + (size_t)row * a.slices * kBins;
   uint32_t *counts = a.counts + (size_t)row * a.slices * kBins;
   if (best) {
     slice_bins<E>(a, key, best, sm);
-    const u64 m = t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0;
     if (ALONE) {
       u64 total;
-      block_scan(from_bin(m, t), sm.wave, &total);
-      if (t == 0) put(mass + slice, total);
+      block_scan(t < kBins ? from_bin(sm.bins[t], t) : 0, sm.wave, &total);
+      if (t == 0) a.mass[(size_t)row * a.slices + slice] = total;
     } else if (t < kBins) {
-      put(hist + (size_t)slice * kBins + t, m);
-      if (a.top_k) put(counts + (size_t)slice * kBins + t, sm.cnt[0][t] + sm.cnt[1][t]);
+      put(hist + (size_t)slice * kBins + t, sm.bins[t]);
+      if (a.top_k) put(counts + (size_t)slice * kBins + t, sm.cnt[t]);
     }
+  }
+  if (ALONE) {
+    if (t == 0) maxes[slice] = best;
+    return;
   }
   if (t == 0) put(maxes + slice, best);
   if (!last_block(a.count + row, a.slices, sm)) return;
@@ -641,34 +647,14 @@ __global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kerne
   }
   best = block_max(best, sm);
   if (best == 0) {
-    none_finite(a, row);
     if (t == 0) a.plan[row].any = 0;
     return;
   }
   const float top = logit_of(best);
   const double id = floor((double)top * a.s);
-  // bins from the row's largest logit to a slice's, at most kBins
-  auto shift_of = [&](uint32_t k) {
-    const double d = k ? id - floor((double)logit_of(k) * a.s) : kBins;
-    return d < kBins ? (int)d : kBins;
-  };
   uint32_t n = 0;
   u64 m = 0;
-  if (ALONE) {
-    make_table(a, sm);
-    u64 own[2];
-    for (int j = 0; j < 2; ++j) {
-      const int i = t + NT * j;
-      const uint32_t k = i < a.slices ? shift[i] : 0;
-      own[j] = k ? from_bin(get(mass + i), shift_of(k)) : 0;
-    }
-    __syncthreads();
-    for (int j = 0; j < 2; ++j) sm.mass[t + NT * j] = own[j];
-    make_plan(a, top, 0, 0, sm);
-    finish_row<false>(a, x, row, sm, nullptr);
-    return;
-  }
-  for (int i = t; i < a.slices; i += NT) shift[i] = shift_of(shift[i]);
+  for (int i = t; i < a.slices; i += NT) shift[i] = shift_of(a, id, shift[i]);
   __syncthreads();
   // threads t and t + kBins take every other slice's bin t, a batch of loads at a time;
   // bins that a slice does not have re-read its bin t
@@ -692,10 +678,10 @@ __global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kerne
       }
   }
   __syncthreads();
-  if (t >= kBins) sm.bins[0][bin] = m, sm.cnt[0][bin] = n;
+  if (t >= kBins) sm.bins[bin] = m, sm.cnt[bin] = n;
   __syncthreads();
   if (t < kBins)
-    m += sm.bins[0][t], n += sm.cnt[0][t];
+    m += sm.bins[t], n += sm.cnt[t];
   else
     m = n = 0;
   make_plan(a, top, n, m, sm);
@@ -703,9 +689,11 @@ __global__ __launch_bounds__(NT, E > 8 && !ALONE ? 8 : 6) void sample_plan_kerne
 }
 
 template <int E>
-__global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
-  __shared__ Shared sm;
-  __shared__ u64 near[kNear];
+__global__ __launch_bounds__(NT, 8) void sample_pick_kernel(SampleArgs a) {
+  __shared__ double tab[kBins];
+  __shared__ u64 near[kNear], wave[kWaves];
+  __shared__ Plan p;
+  __shared__ uint32_t found, base;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
   Plan *plan = a.plan + row;
@@ -722,10 +710,9 @@ __global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
   load(0);
   const uint32_t best = a.maxes[(size_t)row * a.slices + slice];
   const u64 bin = a.hist[((size_t)row * a.slices + slice) * kBins + (t & (kBins - 1))];
-  make_table(a, sm);
-  if (t == 0) sm.plan = *plan, sm.n = 0;
+  make_table(a, tab);
+  if (t == 0) p = *plan, found = 0;
   __syncthreads();
-  const Plan &p = sm.plan;
   if (!p.any) return;
   u64 m = 0;
   if (best && t < kBins) {
@@ -750,35 +737,67 @@ __global__ __launch_bounds__(NT, 6) void sample_pick_kernel(SampleArgs a) {
       if (!key) continue;
       const Place at(a, p, key);
       if (at.partial(p)) {
-        if (at.likely(a, p)) m += to_units(at.mass(sm));
+        if (at.likely(a, p)) m += to_units(at.mass(tab));
       } else if (at.listed(p)) {
-        const uint32_t pos = atomicAdd(&sm.n, 1u);
+        const uint32_t pos = atomicAdd(&found, 1u);
         if (pos < kNear) near[pos] = rank_of(key, i0 + t + NT * ((c - 1) * C + e));
       }
     }
     if (!more) break;
   }
   u64 total;
-  block_scan(m, sm.wave, &total);
-  const uint32_t found = sm.n;
-  if (found) {
-    __syncthreads();
+  block_scan(m, wave, &total);
+  if (t == 0) {
+    a.mass[(size_t)row * a.slices + slice] = total;
     // more than fit: the row is read again at its end
-    if (t == 0) sm.n = atomicAdd(&plan->n, found <= kNear ? found : kList + 1u);
-    __syncthreads();
-    const uint32_t base = sm.n;
-    for (uint32_t i = t; i < found && i < kNear && base < kList && base + i < kList; i += NT)
-      put(a.list + (size_t)row * kList + base + i, near[i]);
+    if (found) base = atomicAdd(&plan->n, found <= kNear ? found : kList + 1u);
   }
-  u64 *mass = a.mass + (size_t)row * a.slices;
-  if (t == 0) put(mass + slice, total);
-  if (!last_block(a.count + kMaxRows + row, a.slices, sm)) return;
-  const u64 first = get(a.list + (size_t)row * kList + t);
-  for (int i = t; i < a.slices; i += NT) sm.mass[i] = get(mass + i);
-  if (t == 0) sm.plan.n = get(&plan->n);
-  near[t] = first;
   __syncthreads();
-  finish_row<true>(a, x, row, sm, near);
+  if (found <= kNear && base < kList)
+    for (uint32_t i = t; i < found && base + i < kList; i += NT)
+      a.list[(size_t)row * kList + base + i] = near[i];
+}
+
+// A block per row.
+template <int E, bool ALONE>
+__global__ __launch_bounds__(NT, 2) void sample_finish_kernel(SampleArgs a) {
+  __shared__ Shared sm;
+  __shared__ u64 near[ALONE ? 1 : kNear];
+  const int t = threadIdx.x, row = blockIdx.x;
+  const float *x = a.x + (size_t)row * a.stride;
+  const u64 *mass = a.mass + (size_t)row * a.slices;
+  if (ALONE) {
+    const uint32_t *maxes = a.maxes + (size_t)row * a.slices;
+    uint32_t key[2], best = 0;
+    u64 m[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = min(t + NT * j, a.slices - 1);
+      key[j] = maxes[i];
+      m[j] = mass[i];
+      best = max(best, key[j]);
+    }
+    make_table(a, sm.tab);
+    best = block_max(best, sm);
+    if (best == 0) return none_finite(a, row);
+    const float top = logit_of(best);
+    const double id = floor((double)top * a.s);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      sm.mass[t + NT * j] =
+          t + NT * j < a.slices && key[j] ? from_bin(m[j], shift_of(a, id, key[j])) : 0;
+    make_plan(a, top, 0, 0, sm);
+    finish_row<E, false>(a, x, row, sm, nullptr);
+  } else {
+    const u64 first = a.list[(size_t)row * kList + t];
+    for (int i = t; i < a.slices; i += NT) sm.mass[i] = mass[i];
+    if (t == 0) sm.plan = a.plan[row];
+    make_table(a, sm.tab);
+    near[t] = first;
+    __syncthreads();
+    if (!sm.plan.any) return none_finite(a, row);
+    finish_row<E, true>(a, x, row, sm, near);
+  }
 }
 
 // Both halves for rows of one slice.
@@ -793,24 +812,24 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
     none_finite(a, row);
     return;
   }
-  make_table(a, sm);
+  make_table(a, sm.tab);
   slice_bins<E>(a, key, best, sm);
-  make_plan(a, logit_of(best), t < kBins ? sm.cnt[0][t] + sm.cnt[1][t] : 0,
-            t < kBins ? sm.bins[0][t] + sm.bins[1][t] : 0, sm);
+  make_plan(a, logit_of(best), t < kBins ? sm.cnt[t] : 0,
+            t < kBins ? sm.bins[t] : 0, sm);
   const Plan &p = sm.plan;
-  u64 m = t < p.sure && t < kBins ? from_bin(sm.bins[0][t] + sm.bins[1][t], t) : 0, total;
+  u64 m = t < p.sure && t < kBins ? from_bin(sm.bins[t], t) : 0, total;
   if (p.sure < p.part) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (key[e]) {
         const Place at(a, p, key[e]);
-        if (at.partial(p) && at.likely(a, p)) m += to_units(at.mass(sm));
+        if (at.partial(p) && at.likely(a, p)) m += to_units(at.mass(sm.tab));
       }
   }
   block_scan(m, sm.wave, &total);
   if (t == 0) sm.mass[0] = total;
   __syncthreads();
-  finish_row<false>(a, x, row, sm, nullptr);
+  finish_row<E, false>(a, x, row, sm, nullptr);
 }
 
 Workspace g_sample_ws, g_sample_count;
@@ -827,7 +846,7 @@ int launch_slices(SampleArgs a, int rows) {
   const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
   const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 12;
   void *mem = nullptr, *count = nullptr;
-  int rc = g_sample_count.get(2 * kMaxRows * 4, &count, "g4_sample");  // zeros when new
+  int rc = g_sample_count.get(kMaxRows * 4, &count, "g4_sample");  // zeros when new
   if (!rc) rc = g_sample_ws.get(bytes, &mem, "g4_sample");
   if (rc) return rc;
   uint8_t *at = static_cast<uint8_t *>(mem);
@@ -840,14 +859,19 @@ int launch_slices(SampleArgs a, int rows) {
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
   const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
-  void (*plan_kernel)(SampleArgs) = e == 8 ? (alone ? sample_plan_kernel<8, true> : sample_plan_kernel<8, false>)
-                                           : (alone ? sample_plan_kernel<32, true> : sample_plan_kernel<32, false>);
-  hipLaunchKernelGGL(plan_kernel, grid, dim3(NT), 0, stream(), a);
+  hipLaunchKernelGGL(e == 8 ? (alone ? sample_plan_kernel<8, true> : sample_plan_kernel<8, false>)
+                            : (alone ? sample_plan_kernel<32, true> : sample_plan_kernel<32, false>),
+                     grid, dim3(NT), 0, stream(), a);
   G4_LAUNCH_CHECK("sample_plan_kernel");
-  if (alone) return G4_OK;
-  hipLaunchKernelGGL(e == 8 ? sample_pick_kernel<8> : sample_pick_kernel<32>, grid, dim3(NT), 0,
-                     stream(), a);
-  G4_LAUNCH_CHECK("sample_pick_kernel");
+  if (!alone) {
+    hipLaunchKernelGGL(e == 8 ? sample_pick_kernel<8> : sample_pick_kernel<32>, grid, dim3(NT), 0,
+                       stream(), a);
+    G4_LAUNCH_CHECK("sample_pick_kernel");
+  }
+  hipLaunchKernelGGL(e == 8 ? (alone ? sample_finish_kernel<8, true> : sample_finish_kernel<8, false>)
+                            : (alone ? sample_finish_kernel<32, true> : sample_finish_kernel<32, false>),
+                     dim3(rows), dim3(NT), 0, stream(), a);
+  G4_LAUNCH_CHECK("sample_finish_kernel");
   return G4_OK;
 }
 
