@@ -21,6 +21,13 @@
 //   sample_finish_kernel  per row the cuts among them, the slice and the token
 // With the temperature alone there is nothing to pick, and a row of one slice takes it all in
 // one launch (sample_row_kernel).
+//
+// Measured at 262144 logits: one row by top-k and top-p 28 us (the launches 14, 4 and 10),
+// which is the latency of the steps; 64 rows by top-p 78 us (37, 20 and 22).  There the two
+// passes over the 67 MB are bound by memory for some 25 us; the rest is the 64-bit arithmetic of
+// the first pass (16.8 million exponentials), the histograms' join and the rows' ends.
+// With the ends left to the second launch's last blocks, which share its registers and LDS, it
+// took 91 us; in one launch over whole rows, before that, 15600.
 #include <math.h>
 
 #include <type_traits>
@@ -36,17 +43,20 @@ namespace {
 
 constexpr int NT = 512;       // threads per block
 constexpr int kWaves = NT / 64;
-constexpr int kBins = 256;    // the last one holds the rest
+constexpr int kBins = 256;    // 31 units of d: below, 2^-44 of the largest; the last one holds the rest
 constexpr int kRest = kBins - 1;
 constexpr double kPerUnit = 8.0;   // bins per unit of d
 constexpr int kList = 16384;       // listed tokens of a row
 constexpr int kNear = 4096;        // of these in LDS
-constexpr int kFew = 128;          // tokens that are compared with each other
+constexpr int kFew = 128;          // tokens that are compared with each other; 64 rows of 262144 by
+                                   // top-p take 78 us, with 512 of them 82, by top-k as well 69, with
+                                   // 32 of them 71
 constexpr int kMaxRows = 256;      // rows per launch
 constexpr int kIndexBits = 22;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxSlices = 2 * NT;
-constexpr int kOneSlice = 8192;    // longest row of one slice
+constexpr int kOneSlice = 8192;    // longest row of one slice: 22 us for one row of 8192 and 23 for
+                                   // 256; in slices of 4096 24 and 29
 typedef unsigned long long u64;
 
 // What the first launch leaves for the second.
@@ -423,12 +433,14 @@ __device__ __forceinline__ u64 select(Each &&each, Weight &&weight, u64 lo, u64 
   return got;
 }
 
+// Where the listed tokens are: nowhere (what lies in the cuts' bins is found in the row
+// again), in a.list if they fit, in LDS if they fit there.
+enum List { kNoList, kMemory, kLds };
+
 // The end of a row, for one block: the cuts among the listed tokens, the slice that holds
-// the picked mass, the token.  LIST: the tokens of the cuts' bins are in a.list (if they
-// fit), else they are found in the row again.  E: tokens of a slice
-// per thread.  sm.plan and sm.tab are set; sm.mass holds
-// the slices' mass outside those bins.
-template <int E, bool LIST>
+// the picked mass, the token.  E: tokens of a slice per thread.  sm.plan and sm.tab are
+// set; sm.mass holds the slices' mass outside the cuts' bins.
+template <int E, List LIST>
 __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, int row, Shared &sm,
                                            u64 *listed) {
   const int t = threadIdx.x;
@@ -437,11 +449,11 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   auto mass_of = [&](u64 r) { return to_units(Place(a, p, rank_key(r)).mass(sm.tab)); };
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
-    const bool fits = LIST && p.n <= kList, few = LIST && p.n <= kFew;
+    const bool fits = LIST != kNoList && p.n <= kList, few = LIST != kNoList && p.n <= kFew;
     // the first of them in LDS, loaded together
     const u64 *list = a.list + (size_t)row * kList;
     const int n = fits ? p.n : 0;
-    if (LIST) {  // (the caller has loaded the first NT)
+    if (LIST == kMemory) {  // (the caller has loaded the first NT)
       constexpr int R = kNear / NT - 1;
       if (n > NT) {
         u64 r[R];
@@ -454,7 +466,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     auto each_listed = [&](auto &&f) {
       if (fits) {  // (each thread reads what it wrote)
 #pragma unroll 1
-        for (int i = t; i < n; i += NT) f(i < kNear ? listed[i] : list[i]);
+        for (int i = t; i < n; i += NT) f(LIST == kLds || i < kNear ? listed[i] : list[i]);
       } else {
 #pragma unroll 1
         for (int i = t; i < a.vocab; i += NT) {
@@ -787,7 +799,7 @@ __global__ __launch_bounds__(NT, 2) void sample_finish_kernel(SampleArgs a) {
       sm.mass[t + NT * j] =
           t + NT * j < a.slices && key[j] ? from_bin(m[j], shift_of(a, id, key[j])) : 0;
     make_plan(a, top, 0, 0, sm);
-    finish_row<E, false>(a, x, row, sm, nullptr);
+    finish_row<E, kNoList>(a, x, row, sm, nullptr);
   } else {
     const u64 first = a.list[(size_t)row * kList + t];
     for (int i = t; i < a.slices; i += NT) sm.mass[i] = mass[i];
@@ -796,14 +808,15 @@ __global__ __launch_bounds__(NT, 2) void sample_finish_kernel(SampleArgs a) {
     near[t] = first;
     __syncthreads();
     if (!sm.plan.any) return none_finite(a, row);
-    finish_row<E, true>(a, x, row, sm, near);
+    finish_row<E, kMemory>(a, x, row, sm, near);
   }
 }
 
-// Both halves for rows of one slice.
+// All of it for rows of one slice.
 template <int E>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   __shared__ Shared sm;
+  __shared__ u64 near[E * NT < kNear ? E * NT : kNear];
   const int t = threadIdx.x, row = blockIdx.x;
   const float *x = a.x + (size_t)row * a.stride;
   uint32_t key[E];
@@ -816,20 +829,29 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   slice_bins<E>(a, key, best, sm);
   make_plan(a, logit_of(best), t < kBins ? sm.cnt[t] : 0,
             t < kBins ? sm.bins[t] : 0, sm);
-  const Plan &p = sm.plan;
+  Plan &p = sm.plan;
   u64 m = t < p.sure && t < kBins ? from_bin(sm.bins[t], t) : 0, total;
-  if (p.sure < p.part) {
+  if (p.sure < p.part || p.lo <= p.hi || p.kb >= 0) {
+    if (t == 0) sm.n = 0;
+    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (key[e]) {
-        const Place at(a, p, key[e]);
-        if (at.partial(p) && at.likely(a, p)) m += to_units(at.mass(sm.tab));
+    for (int e = 0; e < E; ++e) {
+      if (!key[e]) continue;
+      const Place at(a, p, key[e]);
+      if (at.partial(p)) {
+        if (at.likely(a, p)) m += to_units(at.mass(sm.tab));
+      } else if (at.listed(p)) {
+        const uint32_t pos = atomicAdd(&sm.n, 1u);
+        if (pos < kNear) near[pos] = rank_of(key[e], t + NT * e);
       }
+    }
+    __syncthreads();
+    if (t == 0) p.n = sm.n <= kNear ? sm.n : kList + 1u;  // more than fit: the row is read again
   }
   block_scan(m, sm.wave, &total);
   if (t == 0) sm.mass[0] = total;
   __syncthreads();
-  finish_row<E, false>(a, x, row, sm, nullptr);
+  finish_row<E, kLds>(a, x, row, sm, near);
 }
 
 Workspace g_sample_ws, g_sample_count;
@@ -838,8 +860,12 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // Rows of several slices, at most kMaxRows of them.
 int launch_slices(SampleArgs a, int rows) {
-  // 4096 logits to a slice, for one row's latency; longer ones where they fill the GPU
-  const int e = (long)rows * cdiv(a.vocab, 32 * NT) >= 512 ? 32 : 8;
+  const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
+  // 4096 logits to a slice, for few rows' latency; 16384 where these fill the GPU and there are
+  // histograms, a quarter as many then.  us per call at 262144 logits, slices of 4096 / 16384, with
+  // top-p: 8 rows 40 / 56, 16 rows 52 / 57, 32 rows 68 / 63, 64 rows 104 / 78 (of 8192: 86); by
+  // the temperature alone 64 rows 37 / 44
+  const int e = !alone && (long)rows * cdiv(a.vocab, 32 * NT) >= 512 ? 32 : 8;
   a.per = e * NT;
   a.slices = cdiv(a.vocab, a.per);
   const size_t n = (size_t)rows * a.slices;
@@ -858,9 +884,9 @@ int launch_slices(SampleArgs a, int rows) {
   a.counts = reinterpret_cast<uint32_t *>(a.hist + n * kBins);
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
-  const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
-  hipLaunchKernelGGL(e == 8 ? (alone ? sample_plan_kernel<8, true> : sample_plan_kernel<8, false>)
-                            : (alone ? sample_plan_kernel<32, true> : sample_plan_kernel<32, false>),
+  hipLaunchKernelGGL((alone    ? sample_plan_kernel<8, true>
+                      : e == 8 ? sample_plan_kernel<8, false>
+                               : sample_plan_kernel<32, false>),
                      grid, dim3(NT), 0, stream(), a);
   G4_LAUNCH_CHECK("sample_plan_kernel");
   if (!alone) {
@@ -868,8 +894,9 @@ int launch_slices(SampleArgs a, int rows) {
                        stream(), a);
     G4_LAUNCH_CHECK("sample_pick_kernel");
   }
-  hipLaunchKernelGGL(e == 8 ? (alone ? sample_finish_kernel<8, true> : sample_finish_kernel<8, false>)
-                            : (alone ? sample_finish_kernel<32, true> : sample_finish_kernel<32, false>),
+  hipLaunchKernelGGL((alone    ? sample_finish_kernel<8, true>
+                      : e == 8 ? sample_finish_kernel<8, false>
+                               : sample_finish_kernel<32, false>),
                      dim3(rows), dim3(NT), 0, stream(), a);
   G4_LAUNCH_CHECK("sample_finish_kernel");
   return G4_OK;
@@ -879,7 +906,9 @@ int launch_sample(SampleArgs a, int rows) {
   if (a.vocab <= kOneSlice) {
     a.slices = 1;
     a.per = kOneSlice;
-    hipLaunchKernelGGL(a.vocab <= 4 * NT ? sample_row_kernel<4> : sample_row_kernel<kOneSlice / NT>,
+    hipLaunchKernelGGL(a.vocab <= 4 * NT   ? sample_row_kernel<4>
+                       : a.vocab <= 8 * NT ? sample_row_kernel<8>
+                                           : sample_row_kernel<kOneSlice / NT>,
                        dim3(rows), dim3(NT), 0, stream(), a);
     G4_LAUNCH_CHECK("sample_row_kernel");
     return G4_OK;

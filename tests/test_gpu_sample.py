@@ -60,6 +60,19 @@ def test_many_rows(g4, rows, vocab):
         check(g4, x, rng.random(rows), **cuts)
 
 
+@pytest.mark.parametrize("vocab", [1900, 3000, 4096, 8191])
+def test_ties_in_rows_of_one_slice(g4, vocab):
+    # 8191 equal logits are more than the tokens listed near by
+    rng = np.random.default_rng(vocab)
+    x = rng.integers(-8, 4, (4, vocab)).astype(np.float32)
+    x[1] = 1.25
+    x[2] = rng.integers(0, 2, vocab) * 0.125
+    x[3] = logits(rng, 1, vocab, 0.3)[0]
+    for cuts in CUTS + [dict(top_k=vocab // 2), dict(top_k=vocab // 3, top_p=0.77),
+                        dict(top_k=17, top_p=0.5, min_p=0.3)]:
+        check(g4, x, rng.random(4), **cuts)
+
+
 @pytest.mark.parametrize("rows,vocab", [(130, 70000), (300, 9000)])
 def test_many_rows_of_several_slices(g4, rows, vocab):
     # 130 rows: enough for long slices; 300 rows: more than one launch takes
