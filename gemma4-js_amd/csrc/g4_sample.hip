@@ -103,17 +103,19 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// e^((f - 1/2) / 8), f in [0, 1): |z| <= 1/16, z^9 / 9! < 2^-54
+// e^z, z = (f - 1/2) / 8, f in [0, 1): the Taylor sum to z^8, its last term spread over the even
+// ones below by the Chebyshev polynomial T8 on |z| <= h = 1/16, 128 y^8 ~ 256 y^6 - 160 y^4 +
+// 32 y^2 - 1 for y = z / h: off by h^8 / (128 * 8!) and z^9 / 9!, 2^-53.4
 __device__ __forceinline__ double exp_part(double f) {
-  const double z = (f - 0.5) * (1.0 / kPerUnit);
-  double r = fma(z, 1.0 / 40320, 1.0 / 5040);
-  r = fma(r, z, 1.0 / 720);
+  constexpr double h2 = 1.0 / 256, last = 1.0 / 40320;
+  const double z = fma(f, 1.0 / kPerUnit, -0.5 / kPerUnit);
+  double r = fma(z, 1.0 / 5040, 1.0 / 720 + 2 * h2 * last);
   r = fma(r, z, 1.0 / 120);
-  r = fma(r, z, 1.0 / 24);
+  r = fma(r, z, 1.0 / 24 - 1.25 * h2 * h2 * last);
   r = fma(r, z, 1.0 / 6);
-  r = fma(r, z, 0.5);
+  r = fma(r, z, 0.5 + 0.25 * h2 * h2 * h2 * last);
   r = fma(r, z, 1.0);
-  return fma(r, z, 1.0);
+  return fma(r, z, 1.0 - h2 * h2 * h2 * h2 * last / 128);
 }
 constexpr double kHalfBin = 0.93941306281347579;  // e^(-1/16)
 
@@ -214,34 +216,36 @@ __device__ __forceinline__ bool last_block(uint32_t *count, int slices, Shared &
   return last;
 }
 
-// The slice's logits in thread order, their keys, and the largest key.
+// The slice's logits in thread order, -inf for what is not finite, and the largest one's key.
 template <int E>
 __device__ __forceinline__ uint32_t load_slice(const SampleArgs &a, const float *x, int i0, int n,
-                                               uint32_t (&key)[E], Shared &sm) {
-  uint32_t best = 0;
+                                               float (&v)[E], Shared &sm) {
+  float best = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int i = threadIdx.x + NT * e;
-    key[e] = i < n ? key_of(x[i0 + i]) : 0;
+    v[e] = i < n ? x[i0 + i] : -INFINITY;
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) best = max(best, key[e]);
-  return block_max(best, sm);
+  for (int e = 0; e < E; ++e) {
+    v[e] = fabsf(v[e]) < INFINITY ? v[e] : -INFINITY;
+    best = fmaxf(best, v[e]);
+  }
+  return block_max(key_of(best), sm);
 }
 
 // Count (for top-k) and mass of the slice's logits by bins below the largest one's.  A mass
 // is in units of 1 / a.unit of its bin's upper edge.
 template <int E>
-__device__ __forceinline__ void slice_bins(const SampleArgs &a, const uint32_t (&key)[E],
+__device__ __forceinline__ void slice_bins(const SampleArgs &a, const float (&v)[E],
                                            uint32_t best, Shared &sm) {
   if (threadIdx.x < kBins) sm.bins[threadIdx.x] = 0, sm.cnt[threadIdx.x] = 0;
   __syncthreads();
   const double id = floor((double)logit_of(best) * a.s), unit = a.unit * kHalfBin;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if (key[e] == 0) continue;
-    const double y = (double)logit_of(key[e]) * a.s, fl = floor(y), db = id - fl;
-    if (db < kRest) {
+    const double y = (double)v[e] * a.s, fl = floor(y), db = id - fl;
+    if (db < kRest) {  // (not for -inf)
       atomicAdd(&sm.bins[(int)db], to_units(exp_part(y - fl) * unit));
       if (a.top_k) atomicAdd(&sm.cnt[(int)db], 1u);
     }
@@ -628,14 +632,14 @@ __global__ __launch_bounds__(NT, E > 8 ? 8 : 6) void sample_plan_kernel(SampleAr
   __shared__ Shared sm;
   const int t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
   const float *x = a.x + (size_t)row * a.stride;
-  uint32_t key[E];
+  float v[E];
   const int i0 = slice * (E * NT);
-  uint32_t best = load_slice<E>(a, x, i0, min((E * NT), a.vocab - i0), key, sm);
+  uint32_t best = load_slice<E>(a, x, i0, min((E * NT), a.vocab - i0), v, sm);
   uint32_t *maxes = a.maxes + (size_t)row * a.slices;
   u64 *hist = a.hist + (size_t)row * a.slices * kBins;
   uint32_t *counts = a.counts + (size_t)row * a.slices * kBins;
   if (best) {
-    slice_bins<E>(a, key, best, sm);
+    slice_bins<E>(a, v, best, sm);
     if (ALONE) {
       u64 total;
       block_scan(t < kBins ? from_bin(sm.bins[t], t) : 0, sm.wave, &total);
@@ -819,14 +823,14 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   __shared__ u64 near[E * NT < kNear ? E * NT : kNear];
   const int t = threadIdx.x, row = blockIdx.x;
   const float *x = a.x + (size_t)row * a.stride;
-  uint32_t key[E];
-  const uint32_t best = load_slice<E>(a, x, 0, a.vocab, key, sm);
+  float v[E];
+  const uint32_t best = load_slice<E>(a, x, 0, a.vocab, v, sm);
   if (best == 0) {
     none_finite(a, row);
     return;
   }
   make_table(a, sm.tab);
-  slice_bins<E>(a, key, best, sm);
+  slice_bins<E>(a, v, best, sm);
   make_plan(a, logit_of(best), t < kBins ? sm.cnt[t] : 0,
             t < kBins ? sm.bins[t] : 0, sm);
   Plan &p = sm.plan;
@@ -836,13 +840,14 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (!key[e]) continue;
-      const Place at(a, p, key[e]);
+      const uint32_t key = key_of(v[e]);
+      if (!key) continue;
+      const Place at(a, p, key);
       if (at.partial(p)) {
         if (at.likely(a, p)) m += to_units(at.mass(sm.tab));
       } else if (at.listed(p)) {
         const uint32_t pos = atomicAdd(&sm.n, 1u);
-        if (pos < kNear) near[pos] = rank_of(key[e], t + NT * e);
+        if (pos < kNear) near[pos] = rank_of(key, t + NT * e);
       }
     }
     __syncthreads();
