@@ -6,6 +6,7 @@ namespace g4 {
 namespace {
 
 constexpr int kMaxPlanes = G4_CACHE_MAX_PLANES;
+constexpr int kMaxWidth = 1 << 24;
 
 struct Planes {
   float *dst[kMaxPlanes];
@@ -110,7 +111,8 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
   if (!dst || !src || !widths) return fail(G4_E_ARG, "g4_cache_rows: null argument");
   if (n > 0 && src_rows == 0) return fail(G4_E_ARG, "g4_cache_rows: %d rows from none", n);
   for (int p = 0; p < planes; ++p)
-    if (widths[p] <= 0) return fail(G4_E_ARG, "g4_cache_rows: plane %d width %d", p, widths[p]);
+    if (widths[p] <= 0 || widths[p] > kMaxWidth)
+      return fail(G4_E_ARG, "g4_cache_rows: plane %d width %d (1..%d)", p, widths[p], kMaxWidth);
   G4_CHECK_INIT();
   if (n == 0) return ok();
   int rc = check_device_range(rows, (size_t)n * 4, "g4_cache_rows rows");

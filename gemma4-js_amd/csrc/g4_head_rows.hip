@@ -311,8 +311,8 @@ G4_API int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int
   if (in_dim <= 0 || in_dim % 8 != 0 || in_dim > 4096)
     return fail(G4_E_ARG, "g4_bf16_head_rows: in_dim %d must be a positive multiple of 8 <= 4096",
                 in_dim);
-  if (out_stride < (size_t)rows)
-    return fail(G4_E_ARG, "g4_bf16_head_rows: out_stride %zu < rows %d", out_stride, rows);
+  if (out_stride < (size_t)rows || out_stride > (size_t(1) << 60) / (n > 0 ? n : 1))
+    return fail(G4_E_ARG, "g4_bf16_head_rows: out_stride %zu for %d rows, n %d", out_stride, rows, n);
   if ((reinterpret_cast<uintptr_t>(E) & 15u) != 0)
     return fail(G4_E_ARG, "g4_bf16_head_rows: E must be 16-byte aligned");
   G4_CHECK_INIT();

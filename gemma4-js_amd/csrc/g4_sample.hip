@@ -935,7 +935,9 @@ using namespace g4;
 
 G4_API int g4_sample(const float *logits, size_t stride, int rows, int vocab,
                      const g4_sample_params *params, const float *u, int32_t *tokens, float *probs) {
-  if (rows < 0 || vocab <= 0 || vocab > kMaxVocab || stride < (size_t)vocab)
+  // (sizes in bytes stay far from 64 bits)
+  if (rows < 0 || vocab <= 0 || vocab > kMaxVocab || stride < (size_t)vocab ||
+      stride > (size_t(1) << 60) / (rows > 0 ? rows : 1))
     return fail(G4_E_ARG, "g4_sample: rows %d, vocab %d (1..%d), stride %zu", rows, vocab, kMaxVocab,
                 stride);
   if (!params) return fail(G4_E_ARG, "g4_sample: null params");

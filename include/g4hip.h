@@ -388,9 +388,9 @@ int g4_attention_tree(const float *q, const float *k, const float *v, int nodes,
 /* g4_bf16_head for n hidden states, the table read once for (up to 64 of) them:
  *   out[j * out_stride + r] = softcap * tanh((scale * sum_k x[j, k] * E[r, k]) / softcap)
  * x: device FP32 [n, in_dim]; E: device BF16 [rows, in_dim]; out_stride >= rows
- * (floats; a chunk of the vocabulary writes into a wider logits row).  in_dim a
- * positive multiple of 8, <= 4096; n <= 65536; rows <= 2^30; E 16-byte aligned;
- * softcap <= 0 disables the cap.  n = 1 gives g4_bf16_head's bits.  For n > 1 the
+ * (floats; a chunk of the vocabulary writes into a wider logits row; n * out_stride
+ * <= 2^60).  in_dim a positive multiple of 8, <= 4096; n <= 65536; rows <= 2^30; E
+ * 16-byte aligned; softcap <= 0 disables the cap.  n = 1 gives g4_bf16_head's bits.  For n > 1 the
  * states enter as sums of three BF16 values: what lies below 2^-126 of a state is
  * lost, and a state or a row of E that is not finite gives logits that are NaN
  * where FP32 products would leave an infinity. */
@@ -398,7 +398,8 @@ int g4_bf16_head_rows(const float *x, int n, const void *E, int rows, int in_dim
                       float *out, size_t out_stride, float scale, float softcap);
 
 /* One token per row of logits, by probability.
- *   logits: device FP32, row j at logits + j * stride (stride >= vocab; vocab <= 2^22)
+ *   logits: device FP32, row j at logits + j * stride (vocab <= 2^22; stride >= vocab,
+ *           rows * stride <= 2^60)
  *   u:      device FP32 [rows], uniform random numbers in [0, 1)
  *   tokens: device int32 [rows]; probs: device FP32 [rows] or NULL
  * Only finite logits take part.  Probabilities are softmax(logits / temperature);
@@ -426,12 +427,12 @@ int g4_sample(const float *logits, size_t stride, int rows, int vocab,
 /* Rows of a cache's planes (k and v of every layer): for each plane p
  *   dst[p][dst_row + i] = src[p][rows[i]],  i < n
  * as if every row were read before any is written, so with dst[p] == src[p] (or
- * any other overlap of the two) the accepted rows move together in place; with other planes it copies (forks) a
- * cache or picks rows from it.  Plane p: FP32 rows of widths[p] values, src_rows
- * of them in src[p], at least dst_row + n in dst[p].  rows: DEVICE int32 [n]; an
- * entry outside [0, src_rows) gives a NaN row.  Memory of different planes must
- * not overlap.  1 <= planes <= G4_CACHE_MAX_PLANES; dst, src and widths are HOST
- * arrays, read during the call. */
+ * any other overlap of the two) the accepted rows move together in place; with
+ * other planes it copies (forks) a cache or picks rows from it.  Plane p: FP32 rows
+ * of widths[p] values, src_rows of them in src[p], at least dst_row + n in dst[p].
+ * rows: DEVICE int32 [n]; an entry outside [0, src_rows) gives a NaN row.  Memory of
+ * different planes must not overlap.  1 <= planes <= G4_CACHE_MAX_PLANES; widths 1
+ * .. 2^24; dst, src and widths are HOST arrays, read during the call. */
 #define G4_CACHE_MAX_PLANES 128
 int g4_cache_rows(float *const *dst, const float *const *src, const int *widths,
                   int planes, const int32_t *rows, int n, int dst_row, int src_rows);

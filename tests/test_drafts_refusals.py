@@ -29,7 +29,7 @@ def test_attention_tree(nodes, heads, hd, prefix, sliding, window):
 @pytest.mark.parametrize("n,E,rows,k,stride", [
     (-1, 16, 8, 64, 8), (2, 16, -1, 64, 8), (2, 16, 8, 0, 8), (2, 16, 8, 12, 8), (2, 16, 8, 4104, 8),
     (2, 16, 8, 64, 7), (2, 8, 8, 64, 8), (65537, 16, 8, 64, 8),
-    (2, 16, (1 << 30) + 1, 64, 1 << 31)])
+    (2, 16, (1 << 30) + 1, 64, 1 << 31), (3, 16, 8, 64, 1 << 61), (2, 16, 8, 64, (1 << 64) - 1)])
 def test_head_rows(n, E, rows, k, stride):
     refused(g4hip.lib().g4_bf16_head_rows(16, n, E, rows, k, 16, stride, 1.0, 30.0),
             "g4_bf16_head_rows")
@@ -40,7 +40,7 @@ def test_head_rows(n, E, rows, k, stride):
     (1, 10, 10, -0.5, 0, 1, 0), (1, 10, 10, INF, 0, 1, 0), (1, 10, 10, NAN, 0, 1, 0),
     (1, 10, 10, 1, -1, 1, 0), (1, 10, 10, 1, 0, 0, 0), (1, 10, 10, 1, 0, 1.5, 0),
     (1, (1 << 22) + 1, 1 << 25, 1, 0, 1, 0), (1, 10, 10, 1, 0, NAN, 0), (1, 10, 10, 1, 0, 1, -0.1), (1, 10, 10, 1, 0, 1, 1.1),
-    (1, 10, 10, 1, 0, 1, NAN)])
+    (1, 10, 10, 1, 0, 1, NAN), (3, 10, 1 << 61, 1, 0, 1, 0), (2, 10, (1 << 64) - 1, 1, 0, 1, 0)])
 def test_sample(rows, vocab, stride, t, k, p, m):
     params = g4hip.SampleParams(t, k, p, m)
     refused(g4hip.lib().g4_sample(8, stride, rows, vocab, ctypes.byref(params), 8, 8, None),
@@ -52,7 +52,8 @@ def test_sample_without_params():
 
 
 @pytest.mark.parametrize("planes,width,n,dst_row,src_rows", [
-    (0, 8, 1, 0, 4), (129, 8, 1, 0, 4), (1, 0, 1, 0, 4), (1, -8, 1, 0, 4), (1, 8, -1, 0, 4),
+    (0, 8, 1, 0, 4), (129, 8, 1, 0, 4), (1, 0, 1, 0, 4), (1, (1 << 24) + 1, 1, 0, 4),
+    (2, 0x7fffffff, 0x7fffffff, 0x7fffffff, 0x7fffffff), (1, -8, 1, 0, 4), (1, 8, -1, 0, 4),
     (1, 8, 1, -1, 4), (1, 8, 1, 0, -1), (1, 8, 1, 0, 0)])
 def test_cache_rows(planes, width, n, dst_row, src_rows):
     p = (ctypes.c_void_p * 129)(*[16] * 129)
