@@ -351,14 +351,27 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
     }
 }
 
-// Adds the key splits of a row in order: y = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
-// A block is one row, a thread one 16-byte unit of it (hd / 4 threads, at least a wave).
+// Adds the key splits of a row: y = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.  A block is
+// one row; thread (g, t) adds splits g, g + 4, .. of 16-byte unit t in order, then the 4 sums
+// are added in order.  Bound by latency, so the first loads leave before the weights are known.
 template <int HD>
-__global__ __launch_bounds__(HD >= 256 ? HD / 4 : 64) void attn_tree_merge_kernel(TreeArgs a) {
-  const int t = threadIdx.x, lane = t & 63, row = blockIdx.x, nrows = a.nodes * a.heads;
+__global__ __launch_bounds__(HD) void attn_tree_merge_kernel(TreeArgs a) {
+  constexpr int G = 4, U = 8;
+  const int t = threadIdx.x % (HD / G), g = threadIdx.x / (HD / G);
+  const int row = blockIdx.x, nrows = a.nodes * a.heads;
   __shared__ float wt[kMaxSplits];
   __shared__ float sum;
-  if (t < 64) {  // a lane per split
+  __shared__ f32x4 sums[G][HD / G];
+  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + t;
+  const size_t step = (size_t)nrows * HD / 4;
+  f32x4 x[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = p[min(s0 + G * u, a.splits - 1) * step];
+  };
+  load(g);
+  if (threadIdx.x < 64) {  // a lane per split
+    const int lane = threadIdx.x;
     const float2 ml = a.ml[(size_t)min(lane, a.splits - 1) * nrows + row];
     float M = ml.x;
 #pragma unroll
@@ -369,19 +382,17 @@ __global__ __launch_bounds__(HD >= 256 ? HD / 4 : 64) void attn_tree_merge_kerne
     if (lane == 0) sum = L;
   }
   __syncthreads();
-  if (t >= HD / 4) return;
-  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + t;
-  const size_t step = (size_t)nrows * HD / 4;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 16;
-  for (int s0 = 0; s0 < a.splits; s0 += U) {
-    f32x4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = p[min(s0 + u, a.splits - 1) * step];
+  for (int s0 = g; s0 < a.splits; s0 += G * U) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (s0 + u < a.splits) y += wt[s0 + u] * x[u];
+      if (s0 + G * u < a.splits) y += wt[s0 + G * u] * x[u];
+    if (s0 + G * U < a.splits) load(s0 + G * U);
   }
+  sums[g][t] = y;
+  __syncthreads();
+  if (g > 0) return;
+  y = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] /= sum;
   reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[t] = y;
@@ -423,7 +434,7 @@ int launch_tree(TreeArgs a) {
                      dim3(64 * kDimWaves<HD> * KG), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_tree_kernel");
   if (a.splits == 1) return G4_OK;
-  hipLaunchKernelGGL(attn_tree_merge_kernel<HD>, dim3(rows), dim3(HD >= 256 ? HD / 4 : 64), 0, stream(), a);
+  hipLaunchKernelGGL(attn_tree_merge_kernel<HD>, dim3(rows), dim3(HD), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_tree_merge_kernel");
   return G4_OK;
 }
