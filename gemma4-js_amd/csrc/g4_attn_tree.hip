@@ -97,11 +97,11 @@ constexpr int kDimWaves = HD >= 256 ? 4 : HD / 64;
 // GFLOP, take 150 us (112 TFLOP/s) with two blocks per CU.  What a wave does between its products
 // is what is left: rows of V that are not finite, dealt with in a branch of its own beside the
 // products, cost 32 register moves per tile (182 us, without 171); 64-bit addresses per lane
-// instead of a scalar base 15 us more.  32 rows per block (half the loads of K and V) take 209 us,
-// two such groups of 16 in step 217, the scores of the next tile formed ahead of the softmax 210.
+// instead of a scalar base 15 us more.  Of 182 to 184, 32 rows per block (half the loads of K and
+// V) took 209, two such groups of 16 in step 217, the next tile's scores ahead of the softmax 210.
 // Short caches wait for their loads: 4 nodes over 203 keys 8.9 us, two launches.
-// Head dims of 64 and 128: 4 and 2 key groups; twice as many take 9.8 us instead of 8.6 for 4
-// nodes over 200 keys of dim 64, 38 instead of 33 for 64 nodes over 16000.
+// Head dims of 64 and 128: 4 and 2 key groups; twice as many take 9.8 us instead of 8.5 for 4
+// nodes over 200 keys of dim 64, 31.4 instead of 28.6 for 64 nodes over 16000.
 template <int HD, int KG>
 __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(TreeArgs a) {
   constexpr int DQ = kDimWaves<HD>, DW = HD / DQ, NJ = DW / 16, NQ = DW / 64;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * kDimWaves<HD> * KG, 2) void attn_tree_kernel(T
       s = sa[0] + sa[1];
     }
     load_k(tile + KG);
-    __builtin_amdgcn_s_setprio(1);  // before the other blocks' products (3% at head dim 256)
+    __builtin_amdgcn_s_setprio(1);  // before the other block's products (2% at head dim 256)
     if (DQ > 1) {
       sm.loop.sx[it & 1][kg][w][lane] = s;
       __syncthreads();
@@ -407,18 +407,22 @@ int launch_tree(TreeArgs a) {
   const int rows = a.nodes * a.heads, blocks = cdiv(rows, 16);
   // A block per CU; two, whose waits overlap, where each then has many tiles and the splits'
   // outputs are little beside them.  16 nodes of 8 heads of 512 over 1900 keys (4 tiles per
-  // block): 21 us, with two blocks 25.5; 64 nodes of 256 over 1500 (13 tiles): 19.9, with two
-  // 23.8; 64 nodes of 512 over 16000 (126 tiles): 175, with two 155.
+  // block): 18.6 us, with two blocks 24.3; 64 nodes of 256 over 1500 (13 tiles): 20.0, with two
+  // 23.9; 64 nodes of 512 over 16000 (126 tiles): 178, with two 159.
   const int one = cu_count() / blocks, two = 2 * cu_count() / blocks;
   int splits = one < 1 ? 1 : one;
   if (cdiv(a.tiles, splits) > 16) splits = two < 1 ? 1 : two;
   if (splits > kMaxSplits) splits = kMaxSplits;
-  // With few row blocks the tiles are done sooner than 8 L2s can all be filled with the same k
-  // and v, so each gets splits of its own: 16 nodes of 8 heads of 512 (8 blocks) over 16000 keys
-  // 56 us, else 84; over 1900 20.0, else 21.0.  With more, their loads of the same lines at the
-  // same time cost more: 32 nodes (16 blocks) over 2000 keys 25.4, else 23.1; 20 nodes over 16000
-  // 92, else 86.
-  a.one_l2 = blocks <= 8 && splits > 8;
+  // Splits of its own for each XCD, whose L2 then is filled with its part of k and v alone: where
+  // few row blocks are done with a tile sooner than all 8 L2s get it, and where k and v pass the 8
+  // L2s (4 MB each); not where that would leave more than an eighth of the blocks out.  us per
+  // call, heads 8 x 512: 16 nodes (8 blocks) over 1900 keys 18.6, else 19.8, over 16000 53, else
+  // 81; 20 nodes over 16000 63, else 83; 32 nodes 88, else 96.  With more blocks over short caches
+  // their loads of the same lines at the same time cost more: 32 nodes over 2000 keys 25, else 22.7;
+  // 48 nodes over 9000 (16 of 21 splits) 93, else 79.
+  const bool past_l2 = (size_t)a.tiles * kTile * HD * 8 > size_t(32) << 20;
+  a.one_l2 = (blocks <= 8 || past_l2) && splits >= 8 && splits % 8 <= splits / 8;
+  if (a.one_l2) splits = splits / 8 * 8;
   a.tps = cdiv(a.tiles, splits);
   if (a.tps < KG) a.tps = KG;
   a.splits = cdiv(a.tiles, a.tps);

@@ -181,6 +181,11 @@ def test_key_splits_by_the_row_blocks(g4, nodes, prefix):
     check(g4, np.random.default_rng([nodes, prefix]), nodes, 8, 256, prefix, "random", 0)
 
 
+@pytest.mark.parametrize("nodes,prefix", [(20, 9000), (13, 8500), (48, 8300)])
+def test_key_splits_of_a_cache_past_the_l2s(g4, nodes, prefix):
+    check(g4, np.random.default_rng([nodes, prefix, 5]), nodes, 8, 512, prefix, "random", 0)
+
+
 def test_a_cache_past_32_bits(g4):
     # a window at the end of 4.3 million rows of 512: offsets past 2^31 values
     hd, prefix, nodes, window, near = 512, 4300000, 6, 300, 400
