@@ -181,12 +181,13 @@ __global__ __launch_bounds__(64 * WV, 2) void head_rows_kernel(HeadArgs a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS outlives its block
 }
 
-// Few rows: a block owns 16 rows and its waves take turns over the stages, which they read
+// Few rows: a block owns 16 rows and its W waves take turns over the stages, which they read
 // straight to registers (states as FP32 rows, split here), the next one under way; the
-// waves' sums meet in LDS.  Bound by the latency of those loads and the launch.
-template <int MT>
-__global__ __launch_bounds__(256, 2) void head_split_kernel(HeadArgs a) {
-  __shared__ f32x4 sums[4][MT][64];
+// waves' sums meet in LDS.  Bound by the latency of those loads and the launch: 17 states, 4096
+// rows of 1536 10.1 us.
+template <int MT, int W>
+__global__ __launch_bounds__(64 * W, 2) void head_split_kernel(HeadArgs a) {
+  __shared__ f32x4 sums[W][MT][64];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, c = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * kMaxTiles, r0 = blockIdx.x * 16;
   const int chunks = a.K / 8;
@@ -215,8 +216,8 @@ __global__ __launch_bounds__(256, 2) void head_split_kernel(HeadArgs a) {
 #pragma unroll
   for (int m = 0; m < MT; ++m) d[m] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int stages = a.steps / kSteps;
-  load(w);
-  for (int st = w; st < stages; st += 4) {
+  load(w < stages ? w : 0);
+  for (int st = w; st < stages; st += W) {
     bf16x8 er[kSteps], xr[kSteps][MT][3];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void head_split_kernel(HeadArgs a) {
           xr[s][m][i] = __builtin_bit_cast(bf16x8, (u32x4){p[i][0], p[i][1], p[i][2], p[i][3]});
       }
     }
-    load(st + 4 < stages ? st + 4 : st);
+    load(st + W < stages ? st + W : st);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -244,7 +245,9 @@ __global__ __launch_bounds__(256, 2) void head_split_kernel(HeadArgs a) {
   for (int m = 0; m < MT; ++m) sums[w][m][lane] = d[m];
   __syncthreads();
   if (w >= MT) return;
-  const f32x4 sum = (sums[0][w][lane] + sums[1][w][lane]) + (sums[2][w][lane] + sums[3][w][lane]);
+  f32x4 sum = sums[0][w][lane];
+#pragma unroll
+  for (int i = 1; i < W; ++i) sum += sums[i][w][lane];
   store_logits(a, sum, 16 * (m0 + w) + c, r0 + 4 * g);
 }
 
@@ -263,7 +266,13 @@ int launch_tiles(const HeadArgs &a, int groups) {
 
 template <int MT>
 int launch_split(const HeadArgs &a, int groups) {
-  hipLaunchKernelGGL(head_split_kernel<MT>, dim3(cdiv(a.rows, 16), groups), dim3(256), 0, stream(), a);
+  // 8 waves where there is no more than a block per CU, for latency; 4 where blocks share a CU.  us
+  // per call, 8 / 4: 17 states 4096 rows 10.1 / 13.7, 64 states 2048 rows 18 / 23, 8192 rows 36 / 31
+  const dim3 grid(cdiv(a.rows, 16), groups);
+  if ((int)(grid.x * grid.y) <= cu_count())
+    hipLaunchKernelGGL((head_split_kernel<MT, 8>), grid, dim3(512), 0, stream(), a);
+  else
+    hipLaunchKernelGGL((head_split_kernel<MT, 4>), grid, dim3(256), 0, stream(), a);
   G4_LAUNCH_CHECK("head_split_kernel");
   return G4_OK;
 }
@@ -272,7 +281,7 @@ int launch_head_rows(HeadArgs a) {
   const int tiles = cdiv(a.n, 16);
   const int groups = cdiv(tiles, kMaxTiles), mt = groups > 1 ? kMaxTiles : tiles;
   a.steps = cdiv(cdiv(a.K, 32), kSteps) * kSteps;
-  // few rows: us per call, split / tiles, at 5 states 4096 rows 8.3 / 28.6, 32768 29 / 34,
+  // few rows: us per call, split / tiles, at 5 states 4096 rows 6.4 / 28.6, 32768 29 / 34,
   // 65536 52 / 43; 20 states 16384 rows 30 / 44, 32768 54 / 45; 40 states 16384 rows 46 / 47;
   // 64 states 8192 rows 31 / 52, 16384 60 / 53
   if (cdiv(a.rows, 16) * mt <= 12 * cu_count()) {
