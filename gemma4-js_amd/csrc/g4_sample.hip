@@ -537,13 +537,19 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     sm.pick = want - before - (second ? m0 : 0);
   }
   __syncthreads();
-  // and in it the wave's part of consecutive tokens, and of that the thread's
+  // and in it the wave's part of consecutive tokens, and of that the thread's.  Kept is what
+  // lies at the cut or before it in the order, in a bin that is not dropped, and min-p leaves.
+  const float cut_x = cut ? logit_of(rank_key(cut)) : -INFINITY;
+  const int cut_i = rank_index(cut);
+  const int last = max(max(p.sure, p.part) - 1, max(p.lo <= p.hi ? p.hi : 0, p.kb));
   auto kept = [&](float v, int i, double *m) {
-    const uint32_t k = key_of(v);
-    const Place at(a, p, k ? k : 1u);
-    *m = at.mass(sm.tab);
-    const int cuts = at.partial(p) | ((int)at.listed(p) & (rank_of(k, i) >= cut));
-    return ((k != 0) & ((int)(at.b < p.sure) | (cuts & (int)at.likely(a, p)))) != 0;  // no branches
+    const bool finite = fabsf(v) < INFINITY;
+    const double y = (double)(finite ? v : p.top) * a.s, fl = floor(y), db = p.id - fl;
+    const int b = db < kRest ? (int)db : kRest;
+    *m = sm.tab[b] * exp_part(y - fl);
+    const int before = (int)(v > cut_x) | ((int)(v == cut_x) & (int)(i <= cut_i));
+    const int likely = ((double)v - (double)p.top) * a.inv_t >= a.log_min;
+    return (before & (int)finite & (int)(b <= last) & likely) != 0;  // no branches
   };
   const int lane = t & 63, w = t >> 6;
   const int i0 = sm.v[0] * a.per, i1 = min(i0 + a.per, a.vocab);
