@@ -22,8 +22,8 @@
 // With the temperature alone there is nothing to pick, and a row of one slice takes it all in
 // one launch (sample_row_kernel).
 //
-// Measured at 262144 logits: one row by top-k and top-p 27 us (the launches 13, 4 and 10),
-// which is the latency of the steps; 64 rows by top-p 71 us (31, 21 and 23).  There the two
+// Measured at 262144 logits: one row by top-k and top-p 26 us (the launches 13, 4 and 9),
+// which is the latency of the steps; 64 rows by top-p 70 us (31, 21 and 21).  There the two
 // passes over the 67 MB are bound by memory for some 25 us; the rest is the 64-bit arithmetic of
 // the first pass (16.8 million exponentials; 8 us more with keys instead of floats in its
 // loops), the histograms' join and the rows' ends.  With the ends left to the second launch's
@@ -49,13 +49,13 @@ constexpr double kPerUnit = 8.0;   // bins per unit of d
 constexpr int kList = 16384;       // listed tokens of a row
 constexpr int kNear = 4096;        // of these in LDS
 constexpr int kFew = 128;          // tokens that are compared with each other: 64 rows of 262144 by
-                                   // top-p 71 us, with 512 of them 75; by top-k as well 63, with 32 64
+                                   // top-p 70 us, with 512 of them 74; by top-k as well 59, with 32 60
 constexpr int kMaxRows = 256;      // rows per launch
 constexpr int kIndexBits = 22;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxSlices = 2 * NT;
-constexpr int kOneSlice = 8192;    // longest row of one slice: 20 us for one row of 8192 and 21 for
-                                   // 256; in slices of 4096 22.5 and 28
+constexpr int kOneSlice = 8192;    // longest row of one slice: 17 us for one row of 8192 and 18 for
+                                   // 256; in slices of 4096 21 and 27
 typedef unsigned long long u64;
 
 // What the first launch leaves for the second.
@@ -873,8 +873,8 @@ int launch_slices(SampleArgs a, int rows) {
   const bool alone = !a.top_k && !a.top_p64 && a.log_min == -INFINITY;
   // 4096 logits to a slice, for few rows' latency; 16384 where these fill the GPU and there are
   // histograms, a quarter as many then.  us per call at 262144 logits, slices of 4096 / 16384, with
-  // top-p: 8 rows 38 / 47, 16 rows 48 / 49, 32 rows 65 / 56, 64 rows 95 / 71 (of 8192: 76); by
-  // the temperature alone 64 rows 30 / 38
+  // top-p: 8 rows 38 / 45, 16 rows 48 / 48, 32 rows 64 / 55, 64 rows 94 / 70 (of 8192: 72); by
+  // the temperature alone 64 rows 29 / 36
   const int e = !alone && (long)rows * cdiv(a.vocab, 32 * NT) >= 512 ? 32 : 8;
   a.per = e * NT;
   a.slices = cdiv(a.vocab, a.per);
