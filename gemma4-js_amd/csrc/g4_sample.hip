@@ -51,6 +51,7 @@ constexpr int kNear = 4096;        // of these in LDS
 constexpr int kFew = 128;          // tokens that are compared with each other: 64 rows of 262144 by
                                    // top-p 70 us, with 512 of them 74; by top-k as well 59, with 32 60
 constexpr int kMaxRows = 256;      // rows per launch
+constexpr int kMaxShortRows = 1 << 22;  // of one slice: a launch has less than 2^32 threads
 constexpr int kIndexBits = 22;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxSlices = 2 * NT;
@@ -912,25 +913,32 @@ int launch_slices(SampleArgs a, int rows) {
   return G4_OK;
 }
 
+// The call without its first r rows.
+SampleArgs from_row(SampleArgs a, int r) {
+  a.x += (size_t)r * a.stride;
+  a.u += r;
+  a.tokens += r;
+  if (a.probs) a.probs += r;
+  return a;
+}
+
 int launch_sample(SampleArgs a, int rows) {
   if (a.vocab <= kOneSlice) {
     a.slices = 1;
     a.per = kOneSlice;
-    hipLaunchKernelGGL(a.vocab <= 4 * NT   ? sample_row_kernel<4>
-                       : a.vocab <= 8 * NT ? sample_row_kernel<8>
-                                           : sample_row_kernel<kOneSlice / NT>,
-                       dim3(rows), dim3(NT), 0, stream(), a);
-    G4_LAUNCH_CHECK("sample_row_kernel");
+    const auto kernel = a.vocab <= 4 * NT   ? sample_row_kernel<4>
+                        : a.vocab <= 8 * NT ? sample_row_kernel<8>
+                                            : sample_row_kernel<kOneSlice / NT>;
+    for (int r = 0; r < rows;) {
+      const int n = min(rows - r, kMaxShortRows);
+      hipLaunchKernelGGL(kernel, dim3(n), dim3(NT), 0, stream(), from_row(a, r));
+      G4_LAUNCH_CHECK("sample_row_kernel");
+      r += n;
+    }
     return G4_OK;
   }
-  for (int r = 0; r < rows; r += kMaxRows) {
-    SampleArgs b = a;
-    b.x += (size_t)r * a.stride;
-    b.u += r;
-    b.tokens += r;
-    if (b.probs) b.probs += r;
-    if (int rc = launch_slices(b, rows - r < kMaxRows ? rows - r : kMaxRows)) return rc;
-  }
+  for (int r = 0; r < rows; r += kMaxRows)
+    if (int rc = launch_slices(from_row(a, r), rows - r < kMaxRows ? rows - r : kMaxRows)) return rc;
   return G4_OK;
 }
 
