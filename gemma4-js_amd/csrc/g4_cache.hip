@@ -17,6 +17,7 @@ struct Planes {
 constexpr int kChunk = 64;    // 16-byte units (WIDE; else floats) of a row that a wave moves at once
 constexpr int kCopyRows = 4;  // chunks per wave of a copy, their loads together
 constexpr int kPlaceRows = 64;  // rows that move in place in one launch
+constexpr long kMaxBlocks = 1 << 23;  // of a launch, which has less than 2^32 threads
 
 template <bool WIDE>
 struct Unit {
@@ -41,19 +42,19 @@ __device__ __forceinline__ typename Unit<WIDE>::type row_unit(const float *src, 
   return ok ? v : (T)(0.f) + __int_as_float(0x7fc00000);
 }
 
-// dst row dst_row + i = src row rows[i]; blockIdx.y is the plane, a wave takes kCopyRows
-// chunks one after the other.  Bound by memory: 4000 rows of 30 planes (147 MB read, as
-// much written) 48 us, 6.2 TB/s; 8 chunks per wave 52, these through the caches 59, a block
-// per row with 4 bytes per lane 94.
+// dst row dst_row + i = src row rows[i] for n rows from row0 on; blockIdx.y is the plane, a wave
+// takes kCopyRows chunks one after the other.  Bound by memory: 4000 rows of 30 planes (147 MB
+// read, as much written) 48 us, 6.2 TB/s; 8 chunks per wave 52, these through the caches 59, a
+// block per row with 4 bytes per lane 94.
 template <bool WIDE>
-__global__ __launch_bounds__(256) void cache_copy_kernel(Planes p, const int *__restrict__ rows, int n,
-                                                         int dst_row, int src_rows) {
+__global__ __launch_bounds__(256) void cache_copy_kernel(Planes p, const int *__restrict__ rows, int row0,
+                                                         int n, int dst_row, int src_rows) {
   typedef typename Unit<WIDE>::type T;
   const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int plane = blockIdx.y, units = p.width[plane] / Unit<WIDE>::floats;
   const int chunks = (units + kChunk - 1) / kChunk;
   const float *src = p.src[plane];
-  T *dst = reinterpret_cast<T *>(p.dst[plane]) + (size_t)dst_row * units;
+  T *dst = reinterpret_cast<T *>(p.dst[plane]) + ((size_t)dst_row + row0) * units;
   const long first = (long)wave * kCopyRows, all = (long)n * chunks;
   if (first >= all) return;
   T v[kCopyRows];
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(Planes p, const int *__
   for (int u = 0; u < kCopyRows; ++u) {
     const long k = first + u < all ? first + u : all - 1;
     const int i = (int)(k / chunks), at = (int)(k - (long)i * chunks) * kChunk + lane;
-    v[u] = row_unit<WIDE>(src, units, rows, i, src_rows, at < units ? at : units - 1);
+    v[u] = row_unit<WIDE>(src, units, rows, row0 + i, src_rows, at < units ? at : units - 1);
   }
 #pragma unroll
   for (int u = 0; u < kCopyRows; ++u) {
@@ -151,11 +152,15 @@ G4_API int g4_cache_rows(float *const *dst, const float *const *src, const int *
   }
   auto copy = [&](const Planes &pl, const int32_t *from, int to, int limit) {
     const long units = wide ? widest / 4 : widest, chunks = (units + kChunk - 1) / kChunk;
-    const long blocks = (n * chunks + 4 * kCopyRows - 1) / (4 * kCopyRows);
-    if (blocks > 0x7fffffffl / 2) return fail(G4_E_ARG, "g4_cache_rows: %d rows of %d values", n, widest);
-    hipLaunchKernelGGL(wide ? cache_copy_kernel<true> : cache_copy_kernel<false>,
-                       dim3((unsigned)blocks, planes), dim3(256), 0, stream(), pl, from, n, to, limit);
-    G4_LAUNCH_CHECK("cache_copy_kernel");
+    const long most = kMaxBlocks * 4 * kCopyRows / chunks;  // rows of a launch
+    for (long row0 = 0; row0 < n; row0 += most) {
+      const long count = n - row0 < most ? n - row0 : most;
+      const long blocks = (count * chunks + 4 * kCopyRows - 1) / (4 * kCopyRows);
+      hipLaunchKernelGGL(wide ? cache_copy_kernel<true> : cache_copy_kernel<false>,
+                         dim3((unsigned)blocks, planes), dim3(256), 0, stream(), pl, from, (int)row0,
+                         (int)count, to, limit);
+      G4_LAUNCH_CHECK("cache_copy_kernel");
+    }
     return G4_OK;
   };
   if (!place) {

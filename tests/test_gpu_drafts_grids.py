@@ -23,3 +23,20 @@ def test_sample_rows_of_more_than_one_grid(g4):
         np.testing.assert_array_equal(tok.download(np.int32), np.array([w[0] for w in want], np.int32)[at])
         # FP32's half step, and 64-bit sums of four exponentials: far below 1e-6
         np.testing.assert_allclose(pr.download(np.float32), np.array([w[1] for w in want])[at], rtol=1e-6)
+
+
+@pytest.mark.parametrize("place", [False, True])
+def test_cache_rows_of_more_than_one_grid(g4, place):
+    # 2^24 blocks of 256 threads are 2^32; a block takes 16 rows of one value
+    n, at, cap = 2 ** 28 + 37, 5, 1009
+    a = np.random.default_rng(2).standard_normal(cap).astype(np.float32)
+    rows = np.arange(n, dtype=np.int32) % cap
+    idx, dst = g4.Buffer.from_array(rows), g4.Buffer((at + n + 3) * 4)
+    src = dst if place else g4.Buffer.from_array(a)
+    if place:  # the source's rows lie where the first ones go
+        dst.upload(a)
+    g4.CachePlanes([dst], [src], [1]).rows(idx, n, at, cap)
+    got = dst.download(np.float32)
+    np.testing.assert_array_equal(got[:at], a[:at] if place else 0)
+    np.testing.assert_array_equal(got[at:at + n], a[rows])
+    assert not got[at + n:].any()
