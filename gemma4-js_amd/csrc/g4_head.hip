@@ -179,12 +179,19 @@ __global__ __launch_bounds__(256) void argmax_final_kernel(const float2 *__restr
   }
 }
 
+// A launch has less than 2^32 threads: 2^28 rows at a time (their argmax partials, which the engine
+// asks for, are of one launch).
 template <int CPL>
 int launch_head(const float *x, const uint16_t *E, int rows, int K, float *out, float scale,
                 float softcap, float2 *partials) {
-  hipLaunchKernelGGL(bf16_head_kernel<CPL>, dim3(head_argmax_blocks(rows)), dim3(256), 0,
-                     stream(), x, E, rows, K, out, scale, softcap, partials);
-  G4_LAUNCH_CHECK("bf16_head_kernel");
+  constexpr int kMost = 1 << 28;
+  if (partials && rows > kMost) return fail(G4_E_ARG, "bf16_head: %d rows (<= %d)", rows, kMost);
+  for (int n; rows > 0; rows -= n, E += (size_t)n * K, out += n) {
+    n = rows < kMost ? rows : kMost;
+    hipLaunchKernelGGL(bf16_head_kernel<CPL>, dim3(head_argmax_blocks(n)), dim3(256), 0,
+                       stream(), x, E, n, K, out, scale, softcap, partials);
+    G4_LAUNCH_CHECK("bf16_head_kernel");
+  }
   return G4_OK;
 }
 

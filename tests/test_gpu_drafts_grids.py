@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import draft_reference as ref
+import synthetic as syn
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,24 @@ def test_cache_rows_of_more_than_one_grid(g4, place):
     np.testing.assert_array_equal(got[:at], a[:at] if place else 0)
     np.testing.assert_array_equal(got[at:at + n], a[rows])
     assert not got[at + n:].any()
+
+
+def test_head_of_one_state_of_more_than_one_grid(g4):
+    # 2^24 blocks of 256 threads are 2^32; a block takes 32 rows of the table
+    rows, k = 2 ** 29 + 45, 8
+    E, out = g4.Buffer(rows * k * 2), g4.Buffer(rows * 4)
+    g4.fill_random(E, rows * k, g4.RAND_BF16_NORMAL, 11, 0.5)
+    x = np.random.default_rng(3).standard_normal((1, k)).astype(np.float32)
+    xb = g4.Buffer.from_array(x)
+    g4.bf16_head_rows(xb, 1, E, rows, k, out, rows, 1.0, 30.0)
+    part = g4.Buffer(4 * 500)
+    for at in (0, 2 ** 28 - 250, rows - 500):  # the last 500 lie around 2^29
+        # the bits of a call of these rows alone, and 30 tanh(x . E / 30): a sum of 8 exact
+        # products' FP32 roundings and tanh's few ulps
+        g4.bf16_head(xb.ptr, E.at(at * k * 2), 500, k, part.ptr)
+        got = out.download(np.float32, 500, at * 4)
+        np.testing.assert_array_equal(got, part.download(np.float32))
+        e = syn.bf16_to_f32(E.download(np.uint16, 500 * k, at * k * 2).reshape(500, k)).astype(np.float64)
+        z = e @ x[0].astype(np.float64)
+        off = 8 * 2.0 ** -24 * (np.abs(e) @ np.abs(x[0]).astype(np.float64)) + 2.0 ** -21 * np.abs(z)
+        assert (np.abs(got - 30 * np.tanh(z / 30)) <= off).all()
