@@ -283,8 +283,10 @@ int launch_head_rows(HeadArgs a) {
   a.steps = cdiv(cdiv(a.K, 32), kSteps) * kSteps;
   // few rows: us per call, split / tiles, at 5 states 4096 rows 6.4 / 28.6, 32768 29 / 34,
   // 65536 52 / 43; 20 states 16384 rows 30 / 44, 32768 54 / 45; 40 states 16384 rows 46 / 47;
-  // 64 states 8192 rows 31 / 52, 16384 60 / 53
-  if (cdiv(a.rows, 16) * mt <= 12 * cu_count()) {
+  // 64 states 8192 rows 31 / 52, 16384 60 / 53.  Every group of 64 states is that work again:
+  // 128 states 4096 rows 31 / 52, 8192 60 / 53; 192 states 4096 rows 49 / 53; 256 states 2048
+  // rows 31 / 54, 4096 58 / 54; 512 states 1000 rows 32 / 56, 8192 223 / 57
+  if ((long)cdiv(a.rows, 16) * mt * groups <= 12 * cu_count()) {
     switch (mt) {
       case 1: return launch_split<1>(a, groups);
       case 2: return launch_split<2>(a, groups);
