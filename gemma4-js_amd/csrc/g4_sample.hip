@@ -46,11 +46,13 @@ constexpr int kWaves = NT / 64;
 constexpr int kBins = 256;    // 31 units of d: below, 2^-44 of the largest; the last one holds the rest
 constexpr int kRest = kBins - 1;
 constexpr double kPerUnit = 8.0;   // bins per unit of d
-constexpr int kList = 16384;       // listed tokens of a row
+constexpr int kShortList = 16384;  // listed tokens of a row, or a quarter of a longer row's: a bin
+                                   // holds 7% of a row of unit spread at temperature 1.5
 constexpr int kNear = 4096;        // of these in LDS
 constexpr int kFew = 128;          // tokens that are compared with each other: 64 rows of 262144 by
                                    // top-p 70 us, with 512 of them 74; by top-k as well 59, with 32 60
-constexpr int kMaxRows = 256;      // rows per launch
+constexpr int kMaxRows = 256;      // rows per launch, fewer where their lists pass
+constexpr size_t kListBytes = 256 << 20;
 constexpr int kMaxShortRows = 1 << 22;  // of one slice: a launch has less than 2^32 threads
 constexpr int kIndexBits = 22;
 constexpr int kMaxVocab = 1 << kIndexBits;
@@ -72,13 +74,14 @@ struct Plan {
   int kb;           // the bin of top-k's cut, or -1
   uint32_t k_left;  // tokens of it that top-k keeps
   uint32_t n;       // listed tokens
+  uint32_t about;   // the same from the bins' masses, at least
   float x0[2], x1[2];  // logits that may lie in bins sure .. hi, and in kb
 };
 
 struct SampleArgs {
   const float *x;
   size_t stride;
-  int vocab, top_k, slices, per;
+  int vocab, top_k, slices, per, list_len;
   u64 top_p64;  // top_p * 2^64, 0: no such cut
   double inv_t, s, log_min, unit;
   const float *u;
@@ -88,7 +91,7 @@ struct SampleArgs {
   u64 *hist;        // [rows][slices][kBins] masses
   uint32_t *counts; // and counts
   uint32_t *maxes;  // [rows][slices] keys
-  u64 *list;        // [rows][kList]
+  u64 *list;        // [rows][list_len]
   u64 *mass;        // [rows][slices]
   uint32_t *count;  // [kMaxRows] blocks that are done, 0 between launches
 };
@@ -271,7 +274,7 @@ __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32
     p.hi = 0;
     p.sure = kBins;
     p.before_k = 0;
-    p.n = 0;
+    p.n = p.about = 0;
   }
   const u64 upto = block_scan(m, sm.wave, &total), before = upto - m;
   if (b == 0) {
@@ -305,6 +308,10 @@ __device__ __forceinline__ void make_plan(const SampleArgs &a, float top, uint32
     if (b < last && before < hi && hi <= upto) p.hi = b;
     __syncthreads();
   }
+  // (a token's mass is more than e^(-1/8) of a unit)
+  if ((b >= p.lo && b <= p.hi) || b == p.kb)
+    atomicAdd(&p.about, (uint32_t)((double)bin_mass / a.unit * 1.134) + 1);
+  __syncthreads();
   if (b == 0) {
     // bin b holds (max - x) * s in (b - 1, b + 1), min-p keeps what is <= d
     const double d = -a.log_min * kPerUnit;
@@ -453,9 +460,9 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
   auto mass_of = [&](u64 r) { return to_units(Place(a, p, rank_key(r)).mass(sm.tab)); };
   u64 cut = 0;
   if (p.kb >= 0 || p.lo <= p.hi) {
-    const bool fits = LIST != kNoList && p.n <= kList, few = LIST != kNoList && p.n <= kFew;
+    const bool fits = LIST != kNoList && p.n <= (uint32_t)a.list_len, few = LIST != kNoList && p.n <= kFew;
     // the first of them in LDS, loaded together
-    const u64 *list = a.list + (size_t)row * kList;
+    const u64 *list = a.list + (size_t)row * a.list_len;
     const int n = fits ? p.n : 0;
     if (LIST == kMemory) {  // (the caller has loaded the first NT)
       constexpr int R = kNear / NT - 1;
@@ -470,7 +477,29 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, const float *x, 
     auto each_listed = [&](auto &&f) {
       if (fits) {  // (each thread reads what it wrote)
 #pragma unroll 1
-        for (int i = t; i < n; i += NT) f(LIST == kLds || i < kNear ? listed[i] : list[i]);
+        for (int i = t; i < min(n, kNear); i += NT) f(listed[i]);
+        if (LIST == kMemory && n > kNear) {  // the rest, the next ones' loads under way
+          constexpr int R = 8;
+          u64 v[R];
+          auto load = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) v[j] = list[min(i + NT * j, n - 1)];
+          };
+          load(kNear + t);
+#pragma unroll 1
+          for (int i = kNear + t; i < n; i += R * NT) {
+            u64 r[R];
+#pragma unroll
+            for (int j = 0; j < R; ++j) r[j] = v[j];
+            if (i + R * NT < n) load(i + R * NT);
+#pragma unroll 1
+            for (int j = i; j < min(i + R * NT, n); j += NT) {
+              f(r[0]);
+#pragma unroll
+              for (int m = 0; m + 1 < R; ++m) r[m] = r[m + 1];
+            }
+          }
+        }
       } else {
 #pragma unroll 1
         for (int i = t; i < a.vocab; i += NT) {
@@ -729,6 +758,7 @@ __global__ __launch_bounds__(NT, 8) void sample_pick_kernel(SampleArgs a) {
       v[e] = i < n ? x[i0 + i] : NAN;
     }
   };
+  u64 *list = a.list + (size_t)row * a.list_len;
   load(0);
   const uint32_t best = a.maxes[(size_t)row * a.slices + slice];
   const u64 bin = a.hist[((size_t)row * a.slices + slice) * kBins + (t & (kBins - 1))];
@@ -742,6 +772,16 @@ __global__ __launch_bounds__(NT, 8) void sample_pick_kernel(SampleArgs a) {
     if (d < p.sure) m = from_bin(bin, (int)d);
   }
   const float x0 = p.x0[0], x1 = p.x1[0], k0 = p.x0[1], k1 = p.x1[1];
+  // From `near` to the list (for the whole block); the row is read again at its end if more than
+  // fit are found.
+  auto put_list = [&] {
+    __syncthreads();
+    const uint32_t n = found;
+    if (t == 0 && n) base = atomicAdd(&plan->n, n <= kNear ? n : a.list_len + 1u);
+    __syncthreads();
+    if (n <= kNear)
+      for (uint32_t i = t; i < n && base + i < (uint32_t)a.list_len; i += NT) list[base + i] = near[i];
+  };
   for (int c = 0;;) {
     uint32_t near_by = 0;
     float u[C];
@@ -766,18 +806,16 @@ __global__ __launch_bounds__(NT, 8) void sample_pick_kernel(SampleArgs a) {
       }
     }
     if (!more) break;
+    if (p.about <= kNear) continue;
+    put_list();  // so that the next ones fit
+    __syncthreads();
+    if (t == 0) found = 0;
+    __syncthreads();
   }
   u64 total;
   block_scan(m, wave, &total);
-  if (t == 0) {
-    a.mass[(size_t)row * a.slices + slice] = total;
-    // more than fit: the row is read again at its end
-    if (found) base = atomicAdd(&plan->n, found <= kNear ? found : kList + 1u);
-  }
-  __syncthreads();
-  if (found <= kNear && base < kList)
-    for (uint32_t i = t; i < found && base + i < kList; i += NT)
-      a.list[(size_t)row * kList + base + i] = near[i];
+  if (t == 0) a.mass[(size_t)row * a.slices + slice] = total;
+  put_list();
 }
 
 // A block per row.
@@ -811,7 +849,7 @@ __global__ __launch_bounds__(NT, 2) void sample_finish_kernel(SampleArgs a) {
     make_plan(a, top, 0, 0, sm);
     finish_row<E, kNoList>(a, x, row, sm, nullptr);
   } else {
-    const u64 first = a.list[(size_t)row * kList + t];
+    const u64 first = a.list[(size_t)row * a.list_len + t];
     for (int i = t; i < a.slices; i += NT) sm.mass[i] = mass[i];
     if (t == 0) sm.plan = a.plan[row];
     make_table(a, sm.tab);
@@ -857,7 +895,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
       }
     }
     __syncthreads();
-    if (t == 0) p.n = sm.n <= kNear ? sm.n : kList + 1u;  // more than fit: the row is read again
+    if (t == 0) p.n = sm.n <= kNear ? sm.n : a.list_len + 1u;  // more than fit: the row is read again
   }
   block_scan(m, sm.wave, &total);
   if (t == 0) sm.mass[0] = total;
@@ -881,7 +919,7 @@ int launch_slices(SampleArgs a, int rows) {
   a.slices = cdiv(a.vocab, a.per);
   const size_t n = (size_t)rows * a.slices;
   const size_t plan = ((size_t)rows * sizeof(Plan) + 15) & ~size_t(15), max = (n * 4 + 15) & ~size_t(15);
-  const size_t bytes = plan + max + n * 8 + (size_t)rows * kList * 8 + n * kBins * 12;
+  const size_t bytes = plan + max + n * 8 + (size_t)rows * a.list_len * 8 + n * kBins * 12;
   void *mem = nullptr, *count = nullptr;
   int rc = g_sample_count.get(kMaxRows * 4, &count, "g4_sample");  // zeros when new
   if (!rc) rc = g_sample_ws.get(bytes, &mem, "g4_sample");
@@ -891,7 +929,7 @@ int launch_slices(SampleArgs a, int rows) {
   a.maxes = reinterpret_cast<uint32_t *>(at + plan);
   a.mass = reinterpret_cast<u64 *>(at + plan + max);
   a.list = a.mass + n;
-  a.hist = a.list + (size_t)rows * kList;
+  a.hist = a.list + (size_t)rows * a.list_len;
   a.counts = reinterpret_cast<uint32_t *>(a.hist + n * kBins);
   a.count = static_cast<uint32_t *>(count);
   const dim3 grid(a.slices, rows);
@@ -926,6 +964,7 @@ int launch_sample(SampleArgs a, int rows) {
   if (a.vocab <= kOneSlice) {
     a.slices = 1;
     a.per = kOneSlice;
+    a.list_len = kNear;
     const auto kernel = a.vocab <= 4 * NT   ? sample_row_kernel<4>
                         : a.vocab <= 8 * NT ? sample_row_kernel<8>
                                             : sample_row_kernel<kOneSlice / NT>;
@@ -937,8 +976,13 @@ int launch_sample(SampleArgs a, int rows) {
     }
     return G4_OK;
   }
-  for (int r = 0; r < rows; r += kMaxRows)
-    if (int rc = launch_slices(from_row(a, r), rows - r < kMaxRows ? rows - r : kMaxRows)) return rc;
+  // Two cuts may lie in three bins.  us per call at 262144 logits of unit spread, temperature 1.5,
+  // with lists of 16384 / 65536: by top-p 0.75 one row 635 / 68, 64 rows 1072 / 118; by top-k
+  // 131072 and top-p 0.9 one row 1340 / 217, 64 rows 2159 / 317.
+  a.list_len = max(kShortList, a.vocab / 4);
+  const int most = min(kMaxRows, (int)(kListBytes / 8 / a.list_len));
+  for (int r = 0; r < rows; r += most)
+    if (int rc = launch_slices(from_row(a, r), min(rows - r, most))) return rc;
   return G4_OK;
 }
 

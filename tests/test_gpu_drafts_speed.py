@@ -35,3 +35,19 @@ def test_head_of_many_groups_of_states(g4, n, rows):
     one, all_ = us(g4, lambda: g4.bf16_head_rows(x, 64, E, rows, k, out),
                    lambda: g4.bf16_head_rows(x, n, E, rows, k, out))
     assert all_ < n // 64 / 2 * one
+
+
+@pytest.mark.parametrize("rows", [1, 64])
+@pytest.mark.parametrize("cuts", [dict(top_p=0.75), dict(top_k=131072), dict(top_k=131072, top_p=0.9)])
+def test_sampling_of_flat_rows(g4, rows, cuts):
+    # at temperature 1.5 the cuts of rows of unit spread lie among some 20000 tokens each, more
+    # than are listed: the row's block reads it again for every step of the search
+    vocab = 262144
+    rng = np.random.default_rng(rows)
+    flat, peaked = (g4.Buffer.from_array((rng.standard_normal((rows, vocab)) * sigma).astype(np.float32))
+                    for sigma in (1.0, 4.0))
+    u = g4.Buffer.from_array(rng.random(rows).astype(np.float32))
+    tok, pr = g4.Buffer(rows * 4), g4.Buffer(rows * 4)
+    one, many = us(g4, lambda: g4.sample(peaked, rows, vocab, u, tok, pr, temperature=1.5, top_p=0.75),
+                   lambda: g4.sample(flat, rows, vocab, u, tok, pr, temperature=1.5, **cuts))
+    assert many < 14 * one
