@@ -94,7 +94,7 @@ constexpr int kDimWaves = HD >= 256 ? 4 : HD / 64;
 // The next tile's K is loaded once the scores are formed, its V once the outputs are.
 //
 // Over long caches the FP32 products bound it: 64 nodes x 8 heads of 512 over 16000 keys, 16.8
-// GFLOP, take 150 us (112 TFLOP/s) with two blocks per CU.  What a wave does between its products
+// GFLOP, take 156 us (107 TFLOP/s) with two blocks per CU.  What a wave does between its products
 // is what is left: rows of V that are not finite, dealt with in a branch of its own beside the
 // products, cost 32 register moves per tile (182 us, without 171); 64-bit addresses per lane
 // instead of a scalar base 15 us more.  Of 182 to 184, 32 rows per block (half the loads of K and
@@ -408,7 +408,7 @@ int launch_tree(TreeArgs a) {
   // A block per CU; two, whose waits overlap, where each then has many tiles and the splits'
   // outputs are little beside them.  16 nodes of 8 heads of 512 over 1900 keys (4 tiles per
   // block): 18.6 us, with two blocks 24.3; 64 nodes of 256 over 1500 (13 tiles): 20.0, with two
-  // 23.9; 64 nodes of 512 over 16000 (126 tiles): 178, with two 159.
+  // 23.9; 64 nodes of 512 over 16000 (126 tiles): 178, with two 157.
   const int one = cu_count() / blocks, two = 2 * cu_count() / blocks;
   int splits = one < 1 ? 1 : one;
   if (cdiv(a.tiles, splits) > 16) splits = two < 1 ? 1 : two;

@@ -22,12 +22,17 @@
 // With the temperature alone there is nothing to pick, and a row of one slice takes it all in
 // one launch (sample_row_kernel).
 //
-// Measured at 262144 logits: one row by top-k and top-p 26 us (the launches 13, 4 and 9),
+// Measured at 262144 logits: one row by top-k and top-p 26 us (the launches 13, 5 and 9),
 // which is the latency of the steps; 64 rows by top-p 70 us (31, 21 and 21).  There the two
 // passes over the 67 MB are bound by memory for some 25 us; the rest is the 64-bit arithmetic of
 // the first pass (16.8 million exponentials; 8 us more with keys instead of floats in its
 // loops), the histograms' join and the rows' ends.  With the ends left to the second launch's
 // last blocks, which share its registers and LDS, 64 rows took 13 us more.
+//
+// A bin of 1/8 holds more of a flat row: of unit spread at temperature 1.5 some 20000 tokens, all
+// listed.  The search's passes over them, by one block, are then most of the time: 67 us for one
+// row by top-p (the last launch 53), 217 by top-k as well, 64 rows 118 and 316.  Flatter rows,
+// which list more than a quarter of their tokens, are read again instead: 985 us at temperature 50.
 #include <math.h>
 
 #include <type_traits>
