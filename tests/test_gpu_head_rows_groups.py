@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 # 16-row blocks times 64-state groups: up to 768 (at 256 CUs) for the first kernel
 @pytest.mark.parametrize("n,rows,k", [
-    (128, 6144, 256), (128, 6145, 256), (193, 3072, 1528), (193, 3088, 1528), (700, 1300, 264),
+    (128, 6144, 256), (128, 6145, 256), (193, 3060, 1528), (193, 3088, 1528), (700, 1300, 264),
     (513, 1000, 1536), (3000, 257, 72), (3000, 255, 72), (12300, 64, 8), (12288, 64, 8), (16000, 3, 40)])
 def test_groups_over_few_rows(g4, n, rows, k):
     print("head rows", n, rows, k, flush=True)
