@@ -1,0 +1,36 @@
+// What the operators of long caches share.
+#pragma once
+
+#include "g4_internal.h"
+
+namespace g4 {
+
+// Shape, alignment and rows at .. at + n - 1 of a cache; nothing of it needs the device.
+int check_kv4(const g4_kv4 *c, int at, int n, const char *who);
+// The memory of its first `rows` rows.
+int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *who);
+
+// Scores of `rows` = query rows * heads, kept for the keys' weights: score[row][key - first], in
+// units of log 2, and (maximum, sum of 2^(score - maximum)) of each row and key split.  Query row
+// i sits at position pos0 + i; a key is seen at positions key .. key + window - 1 (window 0: all
+// from key on).
+struct Scores {
+  float *score;
+  float2 *ml;  // [splits][rows]
+  size_t stride;
+  int rows, heads, splits;
+  int first, end, pos0, window;  // keys first .. end - 1 are seen by some row
+};
+
+// weights[key] = before[key] + sum over the rows of 2^(score - max) / sum, for all keys < keylen;
+// `part` holds weight_part_floats(rows, end - first).
+size_t weight_part_floats(int rows, int keys);
+int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights);
+
+// Arguments that g4_attention_kv4 and g4_attention_weights have in common.
+int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int window,
+                   const float *before, const float *weights, const char *who);
+// Query rows whose scores are kept at once.
+int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window);
+
+}  // namespace g4

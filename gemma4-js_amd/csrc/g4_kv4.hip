@@ -1,0 +1,156 @@
+// k/v rows held in 4 bits: FP32 rows into codes and scales of 32 values each, and back.
+#include "g4_kv4.h"
+
+#include "g4_gemv.h"
+#include "g4_internal.h"
+
+namespace g4 {
+
+int check_kv4(const g4_kv4 *c, int at, int n, const char *who) {
+  if (!c) return fail(G4_E_ARG, "%s: null cache", who);
+  const int hd = c->head_dim;
+  if (c->rows < 0 || (hd != 64 && hd != 128 && hd != 256 && hd != 512))
+    return fail(G4_E_ARG, "%s: cache of %d rows, head_dim %d (64, 128, 256 or 512)", who, c->rows, hd);
+  if (at < 0 || n < 0 || n > c->rows - at)
+    return fail(G4_E_ARG, "%s: rows %d .. + %d of a cache of %d", who, at, n, c->rows);
+  const void *ptrs[] = {c->k, c->v, c->k_scales, c->v_scales};
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15)
+      return fail(G4_E_ARG, "%s: the cache's planes must be 16-byte aligned", who);
+  return G4_OK;
+}
+
+int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *who) {
+  int rc = G4_OK;
+  if (k) rc = check_device_range(c->k, rows * c->head_dim / 2, who);
+  if (k && !rc) rc = check_device_range(c->k_scales, rows * c->head_dim / 16, who);
+  if (v && !rc) rc = check_device_range(c->v, rows * c->head_dim / 2, who);
+  if (v && !rc) rc = check_device_range(c->v_scales, rows * c->head_dim / 16, who);
+  return rc;
+}
+
+namespace {
+
+constexpr long kMaxBlocks = 1 << 23;  // of a launch, which has less than 2^32 threads
+
+struct Rows4 {
+  const float *x[2];
+  float *y[2];
+  uint32_t *codes[2];
+  uint16_t *scales[2];
+  size_t words;  // of a plane's rows
+};
+
+// A lane packs 8 values into a word, 4 lanes share a scale; blockIdx.y is k or v.  The
+// quotients are rounded to FP32 first, which moves none of them onto or across a border between
+// two codes: (code + 1/2) * scale has at most 12 significant bits, so an x next to it is off by an
+// ulp at least, more than half an ulp of the quotient.
+__global__ __launch_bounds__(256) void kv4_append_kernel(Rows4 r, size_t word0) {
+  const size_t w = word0 + (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (w >= r.words) return;  // (words is a multiple of 4: a scale's lanes stay together)
+  const f32x4 *src = reinterpret_cast<const f32x4 *>(r.x[blockIdx.y]) + 2 * w;
+  const f32x4 a = __builtin_nontemporal_load(src), b = __builtin_nontemporal_load(src + 1);
+  uint32_t top = 0;  // as bits, where NaN > infinity > numbers
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = __float_as_uint(a[i]) & 0x7fffffffu, v = __float_as_uint(b[i]) & 0x7fffffffu;
+    top = max(top, max(u, v));
+  }
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));
+  const bool finite = top < 0x7f800000u;
+  uint32_t bits = f32_to_bf16_rne(__uint_as_float(top) / 7.f);
+  if (bits == 0) bits = 0x3f80u;
+  if (!finite) bits = 0x7fc0u;
+  const float s = bf16_to_f32(bits);
+  uint32_t word = 0x88888888u;
+  if (finite) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = rintf((i < 4 ? a[i & 3] : b[i & 3]) / s);
+      word |= (uint32_t)((int)fminf(fmaxf(q, -7.f), 7.f) + 8) << (4 * i);
+    }
+  }
+  r.codes[blockIdx.y][w] = word;
+  if ((w & 3) == 0) r.scales[blockIdx.y][w >> 2] = (uint16_t)bits;
+}
+
+__global__ __launch_bounds__(256) void kv4_read_kernel(Rows4 r, size_t word0) {
+  const size_t w = word0 + (size_t)blockIdx.x * 256 + threadIdx.x;
+  float *y = r.y[blockIdx.y];
+  if (w >= r.words || !y) return;
+  const uint32_t word = r.codes[blockIdx.y][w];
+  const float s = bf16_to_f32(r.scales[blockIdx.y][w >> 2]);
+  float4 o[2];
+  float *f = &o[0].x;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)((int)(word >> (4 * i) & 15u) - 8) * s;
+  st_nt(reinterpret_cast<float4 *>(y) + 2 * w, o[0]);
+  st_nt(reinterpret_cast<float4 *>(y) + 2 * w + 1, o[1]);
+}
+
+Rows4 planes_at(const g4_kv4 *c, int n, int at) {
+  Rows4 r{};
+  const size_t word = (size_t)at * c->head_dim / 8;
+  r.codes[0] = c->k + word;
+  r.codes[1] = c->v + word;
+  r.scales[0] = c->k_scales + word / 4;
+  r.scales[1] = c->v_scales + word / 4;
+  r.words = (size_t)n * c->head_dim / 8;
+  return r;
+}
+
+template <class Kernel>
+int launch_rows(Kernel kernel, const Rows4 &r, const char *name) {
+  for (size_t w0 = 0; w0 < r.words; w0 += (size_t)kMaxBlocks * 256) {
+    const size_t blocks = (r.words - w0 + 255) / 256;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < (size_t)kMaxBlocks ? blocks : kMaxBlocks), 2),
+                       dim3(256), 0, stream(), r, w0);
+    G4_LAUNCH_CHECK(name);
+  }
+  return G4_OK;
+}
+
+bool unaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+}  // namespace
+}  // namespace g4
+
+using namespace g4;
+
+G4_API int g4_kv4_append(const g4_kv4 *c, const float *k, const float *v, int n, int at) {
+  if (int rc = check_kv4(c, at, n, "g4_kv4_append")) return rc;
+  if (unaligned(k) || unaligned(v))
+    return fail(G4_E_ARG, "g4_kv4_append: k and v must be 16-byte aligned");
+  G4_CHECK_INIT();
+  if (n == 0) return ok();
+  const size_t bytes = (size_t)n * c->head_dim * 4;
+  int rc = check_device_range(k, bytes, "g4_kv4_append k");
+  if (!rc) rc = check_device_range(v, bytes, "g4_kv4_append v");
+  if (!rc) rc = check_kv4_memory(c, (size_t)at + n, true, true, "g4_kv4_append cache");
+  if (rc) return rc;
+  Rows4 r = planes_at(c, n, at);
+  r.x[0] = k;
+  r.x[1] = v;
+  rc = launch_rows(kv4_append_kernel, r, "kv4_append_kernel");
+  return rc ? rc : ok();
+}
+
+G4_API int g4_kv4_read(const g4_kv4 *c, int at, int n, float *k, float *v) {
+  if (int rc = check_kv4(c, at, n, "g4_kv4_read")) return rc;
+  if (unaligned(k) || unaligned(v))
+    return fail(G4_E_ARG, "g4_kv4_read: k and v must be 16-byte aligned");
+  G4_CHECK_INIT();
+  if (n == 0 || (!k && !v)) return ok();
+  const size_t bytes = (size_t)n * c->head_dim * 4;
+  int rc = check_kv4_memory(c, (size_t)at + n, k != nullptr, v != nullptr, "g4_kv4_read cache");
+  if (k && !rc) rc = check_device_range(k, bytes, "g4_kv4_read k");
+  if (v && !rc) rc = check_device_range(v, bytes, "g4_kv4_read v");
+  if (rc) return rc;
+  Rows4 r = planes_at(c, n, at);
+  r.y[0] = k;
+  r.y[1] = v;
+  rc = launch_rows(kv4_read_kernel, r, "kv4_read_kernel");
+  return rc ? rc : ok();
+}

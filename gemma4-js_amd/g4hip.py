@@ -78,6 +78,11 @@ SIGNATURES = {
     "g4_bf16_head_rows": (_int, [_vp, _int, _vp, _int, _int, _vp, _sz, _c.c_float, _c.c_float]),
     "g4_sample": (_int, [_vp, _sz, _int, _int, _vp, _vp, _vp, _vp]),
     "g4_cache_rows": (_int, [_vp, _vp, _vp, _int, _vp, _int, _int, _int]),
+    "g4_kv4_append": (_int, [_vp, _vp, _vp, _int, _int]),
+    "g4_kv4_read": (_int, [_vp, _int, _int, _vp, _vp]),
+    "g4_attention_kv4": (_int, [_vp, _vp, _int, _int, _int, _int, _int, _int, _vp, _vp, _vp]),
+    "g4_attention_weights": (_int, [_vp, _vp, _int, _int, _int, _int, _int, _int, _int, _vp, _vp]),
+    "g4_cache_evict": (_int, [_vp, _sz, _int, _int, _int, _int, _int, _vp, _vp]),
     "g4_w4_load_dev": (_int, [_vp, _vp, _int, _int, _int, _c.POINTER(_vp)]),
     "g4_w4_load_opts": (_int, [_vp, _vp, _int, _int, _int, _int, _c.POINTER(_vp)]),
     "g4_ple_upload_shard_dev": (_int, [_vp, _int, _vp, _sz]),
@@ -132,6 +137,11 @@ class GemmaConfig(_c.Structure):
 class SampleParams(_c.Structure):
     _fields_ = [("temperature", _c.c_float), ("top_k", _int), ("top_p", _c.c_float),
                 ("min_p", _c.c_float)]
+
+
+class Kv4(_c.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scales", _vp), ("v_scales", _vp), ("rows", _int),
+                ("head_dim", _int)]
 
 
 class G4Error(RuntimeError):
@@ -512,6 +522,51 @@ class CachePlanes:
         """dst[p][dst_row + i] = src[p][rows[i]], rows int32 [n] on the device."""
         check(lib().g4_cache_rows(self._dst, self._src, self._widths, self.planes, _f(rows), n,
                                   dst_row, src_rows))
+
+
+class Kv4Cache:
+    """One layer's k/v rows in 4 bits (g4_kv4).  buffers: codes and scales of k, codes and scales
+    of v (buffers or device pointers); without them the cache makes its own."""
+
+    def __init__(self, rows, hd, buffers=None):
+        if buffers is None:
+            buffers = [Buffer(rows * hd // (2 if i % 2 == 0 else 16)) for i in range(4)]
+        if len(buffers) != 4:
+            raise ValueError("codes and scales of k and of v")
+        self.rows, self.hd = rows, hd
+        self.k, self.k_scales, self.v, self.v_scales = buffers
+        self._s = Kv4(_f(self.k), _f(self.v), _f(self.k_scales), _f(self.v_scales), rows, hd)
+
+    def append(self, k, v, n, at):
+        """g4_kv4_append: n FP32 rows of k and v to cache rows at .. at + n - 1."""
+        check(lib().g4_kv4_append(_c.byref(self._s), _f(k), _f(v), n, at))
+
+    def read(self, at, n, k, v):
+        """g4_kv4_read: the values of cache rows at .. at + n - 1 (k or v may be None)."""
+        check(lib().g4_kv4_read(_c.byref(self._s), at, n, _f(k), _f(v)))
+
+    def attention(self, q, qrows, heads, keylen, qpos0, sliding, window, y, weights=None,
+                  before=None):
+        """g4_attention_kv4; weights: before (zeros without it) + what each key got."""
+        check(lib().g4_attention_kv4(_f(q), _c.byref(self._s), qrows, heads, keylen, qpos0,
+                                     1 if sliding else 0, window, _f(y), _f(before), _f(weights)))
+
+    def planes(self):
+        """(buffers, widths) of the four planes for CachePlanes, in its 4-byte units."""
+        return ([self.k, self.k_scales, self.v, self.v_scales],
+                [self.hd // 8, self.hd // 64, self.hd // 8, self.hd // 64])
+
+
+def attention_weights(q, k, qrows, heads, hd, keylen, qpos0, sliding, window, weights, before=None):
+    """g4_attention_weights: weights = before (zeros without it) + what each FP32 key got."""
+    check(lib().g4_attention_weights(_f(q), _f(k), qrows, heads, hd, keylen, qpos0,
+                                     1 if sliding else 0, window, _f(before), _f(weights)))
+
+
+def cache_evict(weights, sets, len_, keep, first, recent, rows, kept=None, stride=None):
+    """g4_cache_evict: the rows to keep, int32 [sets, keep], and their weights."""
+    check(lib().g4_cache_evict(_f(weights), len_ if stride is None else stride, sets, len_, keep,
+                               first, recent, _f(rows), _f(kept)))
 
 
 def fill_random(buf, count, kind, seed, sigma=1.0):

@@ -1105,6 +1105,105 @@ napi_value F_cacheRows(napi_env env, napi_callback_info info) {
   return undefined(env);
 }
 
+// ---- long caches ----------------------------------------------------------------
+// A cache of 4 bits is six arguments: k, kScales, v, vScales (DeviceBuffers), rows, hd.
+
+bool kv4_at(napi_env env, const napi_value *a, g4_kv4 *c) {
+  void *k, *ks, *v, *vs;
+  int64_t rows, hd;
+  if (!dev(env, a[0], "cache.k", &k) || !dev(env, a[1], "cache.kScales", &ks) ||
+      !dev(env, a[2], "cache.v", &v) || !dev(env, a[3], "cache.vScales", &vs) ||
+      !to_int(env, a[4], &rows, "cache.rows") || !to_int(env, a[5], &hd, "cache.hd"))
+    return false;
+  *c = g4_kv4{(uint32_t *)k, (uint32_t *)v, (uint16_t *)ks, (uint16_t *)vs, (int)rows, (int)hd};
+  return true;
+}
+
+// kv4Append(cache.., k, v, n, at)
+napi_value F_kv4Append(napi_env env, napi_callback_info info) {
+  napi_value a[10], self;
+  if (!get_args(env, info, 10, a, &self)) return nullptr;
+  g4_kv4 c;
+  void *k, *v;
+  int64_t n, at;
+  if (!kv4_at(env, a, &c) || !dev(env, a[6], "k", &k) || !dev(env, a[7], "v", &v) ||
+      !to_int(env, a[8], &n, "n") || !to_int(env, a[9], &at, "at"))
+    return nullptr;
+  G4_CALL(env, g4_kv4_append(&c, (const float *)k, (const float *)v, (int)n, (int)at));
+  return undefined(env);
+}
+
+// kv4Read(cache.., at, n, k, v)
+napi_value F_kv4Read(napi_env env, napi_callback_info info) {
+  napi_value a[10], self;
+  if (!get_args(env, info, 10, a, &self)) return nullptr;
+  g4_kv4 c;
+  void *k, *v;
+  int64_t at, n;
+  if (!kv4_at(env, a, &c) || !to_int(env, a[6], &at, "at") || !to_int(env, a[7], &n, "n") ||
+      !dev_or_null(env, a[8], "k", &k) || !dev_or_null(env, a[9], "v", &v))
+    return nullptr;
+  G4_CALL(env, g4_kv4_read(&c, (int)at, (int)n, (float *)k, (float *)v));
+  return undefined(env);
+}
+
+// attentionKv4(cache.., q, qrows, heads, keylen, qpos0, sliding, window, y, before, weights)
+napi_value F_attentionKv4(napi_env env, napi_callback_info info) {
+  napi_value a[16], self;
+  if (!get_args(env, info, 16, a, &self)) return nullptr;
+  g4_kv4 c;
+  void *q, *y, *before, *weights;
+  int64_t v[6];
+  static const int idx[6] = {7, 8, 9, 10, 11, 12};
+  static const char *const names[6] = {"qrows", "heads", "keylen", "qpos0", "sliding", "window"};
+  if (!kv4_at(env, a, &c) || !dev(env, a[6], "q", &q) || !ints(env, a, idx, v, 6, names) ||
+      !dev(env, a[13], "y", &y) || !dev_or_null(env, a[14], "before", &before) ||
+      !dev_or_null(env, a[15], "weights", &weights))
+    return nullptr;
+  G4_CALL(env, g4_attention_kv4((const float *)q, &c, (int)v[0], (int)v[1], (int)v[2], (int)v[3],
+                                (int)v[4], (int)v[5], (float *)y, (const float *)before,
+                                (float *)weights));
+  return undefined(env);
+}
+
+// attentionWeights(q, k, qrows, heads, hd, keylen, qpos0, sliding, window, before, weights)
+napi_value F_attentionWeights(napi_env env, napi_callback_info info) {
+  napi_value a[11], self;
+  if (!get_args(env, info, 11, a, &self)) return nullptr;
+  void *q, *k, *before, *weights;
+  int64_t v[7];
+  static const int idx[7] = {2, 3, 4, 5, 6, 7, 8};
+  static const char *const names[7] = {"qrows", "heads", "hd", "keylen", "qpos0", "sliding", "window"};
+  if (!dev(env, a[0], "q", &q) || !dev(env, a[1], "k", &k) || !ints(env, a, idx, v, 7, names) ||
+      !dev_or_null(env, a[9], "before", &before) || !dev(env, a[10], "weights", &weights))
+    return nullptr;
+  G4_CALL(env, g4_attention_weights((const float *)q, (const float *)k, (int)v[0], (int)v[1],
+                                    (int)v[2], (int)v[3], (int)v[4], (int)v[5], (int)v[6],
+                                    (const float *)before, (float *)weights));
+  return undefined(env);
+}
+
+// cacheEvict(weights, stride, sets, len, keep, first, recent, rows, kept = null)
+napi_value F_cacheEvict(napi_env env, napi_callback_info info) {
+  napi_value a[9], self;
+  if (!get_args(env, info, 9, a, &self)) return nullptr;
+  void *w, *rows, *kept;
+  int64_t stride, v[5];
+  static const int idx[5] = {2, 3, 4, 5, 6};
+  static const char *const names[5] = {"sets", "len", "keep", "first", "recent"};
+  if (!dev(env, a[0], "weights", &w) || !to_i64(env, a[1], &stride, "stride") ||
+      !ints(env, a, idx, v, 5, names) || !dev(env, a[7], "rows", &rows) ||
+      !dev_or_null(env, a[8], "kept", &kept))
+    return nullptr;
+  if (stride < 0) {
+    napi_throw_range_error(env, nullptr, "stride must be >= 0");
+    return nullptr;
+  }
+  G4_CALL(env, g4_cache_evict((const float *)w, (size_t)stride, (int)v[0], (int)v[1], (int)v[2],
+                              (int)v[3], (int)v[4], (int32_t *)rows, (float *)kept));
+  return undefined(env);
+}
+
 // ---- GemmaEngine (g4_gemma_*) ---------------------------------------------------
 // The native decoder engine behind Gemma4WebGPU's load/forward/logits/greedy
 // surface (gemma4-webgpu.js:139-481), plus decode(steps) on a recorded step.
@@ -1595,6 +1694,9 @@ napi_value Init(napi_env env, napi_value exports) {
       METHOD("pleMix", F_pleMix), METHOD("argmax", F_argmax),
       METHOD("attentionTree", F_attentionTree), METHOD("bf16HeadRows", F_bf16HeadRows),
       METHOD("sample", F_sample), METHOD("cacheRows", F_cacheRows),
+      METHOD("kv4Append", F_kv4Append), METHOD("kv4Read", F_kv4Read),
+      METHOD("attentionKv4", F_attentionKv4), METHOD("attentionWeights", F_attentionWeights),
+      METHOD("cacheEvict", F_cacheEvict),
       METHOD("e2bConfig", F_e2bConfig), METHOD("fillRandom", F_fillRandom)};
   NAPI_CALL(env, napi_define_properties(env, exports, sizeof fns / sizeof fns[0], fns));
   napi_value v;

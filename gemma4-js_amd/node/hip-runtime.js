@@ -331,6 +331,45 @@ class GPUOps {
     native.cacheRows(planes.map((p) => p.dst), planes.map((p) => p.src), planes.map((p) => p.width),
       rows, n, dstRow, srcRows);
   }
+  // ---- long caches (no reference counterpart) ----
+  // one layer's k/v rows in 4 bits: four DeviceBuffers, which the caller destroys
+  kv4Cache(rows, hd) {
+    const codes = () => this.emptyF32(rows * (hd / 8), 'kv4'), scales = () => this.emptyF32(rows * (hd / 64), 'kv4-scales');
+    return { k: codes(), kScales: scales(), v: codes(), vScales: scales(), rows, hd };
+  }
+  // its planes for cacheRows()
+  kv4Planes({ k, kScales, v, vScales, hd }) {
+    return [[k, hd / 8], [kScales, hd / 64], [v, hd / 8], [vScales, hd / 64]].map(([b, width]) => ({ dst: b, src: b, width }));
+  }
+  // cache rows at .. at + n - 1 = the FP32 rows k and v
+  kv4Append(encoder, cache, k, v, n, at) {
+    native.kv4Append(cache.k, cache.kScales, cache.v, cache.vScales, cache.rows, cache.hd, k, v, n, at);
+  }
+  // their values as FP32 DeviceBuffers {k, v}
+  kv4Read(encoder, cache, at, n) {
+    const k = this.emptyF32(n * cache.hd, 'kv4-k'), v = this.emptyF32(n * cache.hd, 'kv4-v');
+    native.kv4Read(cache.k, cache.kScales, cache.v, cache.vScales, cache.rows, cache.hd, at, n, k, v);
+    return { k, v };
+  }
+  // attention() over the first keylen rows of such a cache; weights (FP32 DeviceBuffer [keylen],
+  // optional): the weight that each key got is added to it
+  attentionKv4(encoder, q, cache, qrows, heads, keylen, qpos0, sliding, window, weights = null, garbage = null) {
+    const out = this.emptyF32(qrows * heads * cache.hd, 'attn-kv4-out');
+    native.attentionKv4(cache.k, cache.kScales, cache.v, cache.vScales, cache.rows, cache.hd, q, qrows, heads, keylen,
+      qpos0, sliding ? 1 : 0, window, out, weights, weights);
+    return out;
+  }
+  // the weight that each FP32 key got in attention() is added to weights
+  attentionWeights(encoder, q, kcache, qrows, heads, hd, keylen, qpos0, sliding, window, weights) {
+    native.attentionWeights(q, kcache, qrows, heads, hd, keylen, qpos0, sliding ? 1 : 0, window, weights, weights);
+  }
+  // the rows to keep of `sets` caches of len rows (int32 DeviceBuffer [sets, keep], ascending): the first,
+  // the last `recent` and the heaviest others; their weights move to the front, zeros behind
+  cacheEvict(encoder, weights, sets, len, keep, first, recent, stride = len) {
+    const rows = this.emptyF32(sets * keep, 'evict-rows');
+    native.cacheEvict(weights, stride, sets, len, keep, first, recent, rows, weights);
+    return rows;
+  }
   dispose() {}
 }
 

@@ -442,6 +442,74 @@ int g4_sample(const float *logits, size_t stride, int rows, int vocab,
 int g4_cache_rows(float *const *dst, const float *const *src, const int *widths,
                   int planes, const int32_t *rows, int n, int dst_row, int src_rows);
 
+/* ---- long caches ------------------------------------------------------------
+ * No counterparts in the reference, whose caches hold every row in FP32.  A long
+ * chat's cache is held in 4 bits (about a seventh of the bytes), or loses the rows
+ * that attention hardly looks at:
+ *   g4_kv4_append the new tokens' k/v rows, g4_attention_kv4 (or g4_attention and
+ *   g4_attention_weights over FP32 rows), now and then g4_cache_evict and
+ *   g4_cache_rows of the rows that it lists, over FP32 planes or over the four planes
+ *   of g4_kv4 (rows of 4-byte units: head_dim / 8 of codes, head_dim / 64 of scales).
+ * Rows keep the RoPE of their own positions; qpos0 counts cache rows.
+ * Arguments are checked before anything else, so a refusal needs no device.  All can
+ * be recorded; those with scratch need one earlier call of those sizes for it. */
+
+/* One layer's k and v rows in 4 bits, in the caller's device memory (no handle: the
+ * struct is read during each call).  Values are (nibble - 8) * scale, as g4_w4_load's:
+ *   k, v               uint32 [rows, head_dim / 8], nibble i of word j is value 8j + i
+ *   k_scales, v_scales BF16 [rows, head_dim / 32], of 32 values each
+ * All four 16-byte aligned.  head_dim 64, 128, 256 or 512. */
+typedef struct {
+  uint32_t *k, *v;
+  uint16_t *k_scales, *v_scales;
+  int rows; /* capacity */
+  int head_dim;
+} g4_kv4;
+
+/* cache rows at .. at + n - 1 = the n FP32 rows k and v [n, head_dim], with the PLE
+ * builder's steps: scale = bf16_rne(max |x| / 7), 1 where that is 0, and codes
+ * rint(x / scale) within 7, halves to even.  32 values of which one is not finite get a
+ * NaN scale: all of them read as NaN.  k and v 16-byte aligned. */
+int g4_kv4_append(const g4_kv4 *cache, const float *k, const float *v, int n, int at);
+
+/* The values of cache rows at .. at + n - 1 as FP32 rows [n, head_dim] (exact); k or v
+ * may be NULL. */
+int g4_kv4_read(const g4_kv4 *cache, int at, int n, float *k, float *v);
+
+/* g4_attention over the first keylen rows of such a cache: q and y [qrows, heads,
+ * head_dim] FP32, query row r at position qpos0 + r sees keys key <= qpos0 + r, with
+ * `sliding` only those with key + window > qpos0 + r; qpos0 + qrows <= keylen.
+ * With `weights` (FP32 [keylen], may be NULL) in addition
+ *   weights[key] = before[key] + the weight of that key, summed over rows and heads,
+ * before NULL counting as zeros; it may be weights itself, but not overlap it otherwise.
+ * Rows that a query row does not see have no influence on it, whatever they hold.
+ * heads <= 8; qrows <= 2^20; keylen <= 2^28; q and y 16-byte aligned.  A q, k or
+ * v that lies more than 2^36 below the largest of its row (of q: of its head) is kept
+ * to that precision. */
+int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int heads, int keylen,
+                     int qpos0, int sliding, int window, float *y, const float *before,
+                     float *weights);
+
+/* Those weights over FP32 keys: k [keylen, head_dim], rows and masks as g4_attention's,
+ * before and weights as above.  head_dim 64, 128, 256 or 512; heads, qrows and keylen
+ * as above; q and k 16-byte aligned. */
+int g4_attention_weights(const float *q, const float *k, int qrows, int heads, int head_dim,
+                         int keylen, int qpos0, int sliding, int window, const float *before,
+                         float *weights);
+
+/* The rows of a cache to keep, for each of `sets` caches of `len` rows: the first `first`
+ * ones, the last `recent` ones, and of those between the heaviest, `keep` in all.
+ *   weights: device FP32, set s at weights + s * stride (stride >= len)
+ *   rows:    device int32 [sets, keep], ascending (g4_cache_rows moves them to the front)
+ *   kept:    FP32 like weights, or NULL: kept[i] = weights[rows[i]] for i < keep, 0 for
+ *            keep <= i < len.  It may be weights itself (then ready for the next calls'
+ *            sums), but not overlap it otherwise.
+ * Of equal weights the lowest indices stay; NaN is below all numbers, -0 equals 0.
+ * 0 <= first, recent; first + recent <= keep <= len <= 2^24; sets <= 256; stride <=
+ * 2^52. */
+int g4_cache_evict(const float *weights, size_t stride, int sets, int len, int keep, int first,
+                   int recent, int32_t *rows, float *kept);
+
 /* ---- synthetic data (random-init models) ----------------------------------
  * No reference counterpart: the benchmarks run random-init weights of the
  * checkpoint's shapes, generated on the device.  Fills `count` elements of
