@@ -1,6 +1,8 @@
 // Attention over a cache held in 4 bits, with the weight that each key got if asked for.
 #include <math.h>
 
+#include <type_traits>
+
 #include "g4_gemv.h"
 #include "g4_internal.h"
 #include "g4_kv4.h"
@@ -8,70 +10,535 @@
 namespace g4 {
 namespace {
 
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
+constexpr int kStep = 32;                   // keys of a wave's step
+constexpr int kWaves = 4;
+constexpr int kMaxSplits = 256;
 
 struct Kv4Args {
   const float *q;
   const uint32_t *k, *v;
   const uint16_t *ks, *vs;
   float *y;
-  Scores s;  // score null: not kept
+  float *part;  // [splits][rows][hd], each split's outputs
+  Scores s;     // score null: not kept
 };
 
-// Values 8 l .. of a row at lane l's share of D of them.
-template <int D>
-__device__ __forceinline__ void values4(const uint32_t *codes, const uint16_t *scales, size_t row, int hd,
-                                        int d0, float (&x)[D]) {
-  const float s = bf16_to_f32(scales[(row * hd + d0) / 32]);
-  const uint32_t w = codes[(row * hd + d0) / 8] >> (4 * (d0 & 7));
-#pragma unroll
-  for (int d = 0; d < D; ++d) x[d] = (float)((int)(w >> (4 * d) & 15u) - 8) * s;
+// Eight values of a cache as FP16, in pairs (0, 4) (1, 5) (2, 6) (3, 7) of the word's nibbles or of
+// two words' halves: a nibble n in the mantissa's upper four bits under the exponent of 16 is
+// 16 + n, and (16 + n) s - 24 s = (n - 8) s is exact in one fused step: s has 8 bits, 24 s 10.
+struct Scale {
+  half2_t s, c;  // s and -24 s
+};
+__device__ __forceinline__ Scale scale_pair(float a, float b) {
+  const half2_t s = __builtin_convertvector((f32x2_t){a, b}, half2_t);
+  return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}};
+}
+template <int T>
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, const Scale &x) {
+  const uint32_t sh = T == 0 ? w << 6 : T == 1 ? w << 2 : T == 2 ? w >> 2 : w >> 6;
+  const half2_t h = __builtin_bit_cast(half2_t, (sh & 0x03c003c0u) | 0x4c004c00u);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(h, x.s, x.c));
 }
 
-// A block per row; a wave takes every fourth key, a lane HD / 64 values of it.
-template <int HD>
-__global__ __launch_bounds__(256) void attn_kv4_kernel(Kv4Args a) {
-  constexpr int D = HD / 64;
-  __shared__ float2 sml[4];
-  __shared__ float so[4][HD];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x, d0 = lane * D;
-  const int pos = a.s.pos0 + row / a.s.heads;
-  const int lo = a.s.window > 0 ? max(a.s.first, pos - a.s.window + 1) : a.s.first;
-  float q[D], o[D] = {};
-#pragma unroll
-  for (int d = 0; d < D; ++d) q[d] = a.q[(size_t)row * HD + d0 + d];
-  float m = kNoScore, l = 0.f;
-  for (int key = lo + w; key <= pos; key += 4) {
-    float kk[D], vv[D], x = 0.f;
-    values4<D>(a.k, a.ks, key, HD, d0, kk);
-    values4<D>(a.v, a.vs, key, HD, d0, vv);
-#pragma unroll
-    for (int d = 0; d < D; ++d) x = fmaf(q[d], kk[d], x);
-    x = wave_sum(x) * kLog2e;
-    if (a.s.score && lane == 0) a.s.score[(size_t)row * a.s.stride + (key - a.s.first)] = x;
-    const float mn = fmaxf(m, x), c = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(x - mn);
-    l = l * c + p;
-#pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = fmaf(p, vv[d], o[d] * c);
-    m = mn;
-  }
-  if (lane == 0) sml[w] = make_float2(m, l);
-#pragma unroll
-  for (int d = 0; d < D; ++d) so[w][d0 + d] = o[d];
-  __syncthreads();
-  float M = kNoScore, L = 0.f, f[4];
-  for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[i].x);
-  for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_exp2f(sml[i].x - M), L += sml[i].y * f[i];
-  for (int d = threadIdx.x; d < HD; d += 256) {
-    float x = 0.f;
-    for (int i = 0; i < 4; ++i) x += so[i][d] * f[i];
-    a.y[(size_t)row * HD + d] = x / L;
-  }
-  if (a.s.ml && threadIdx.x == 0) a.s.ml[row] = make_float2(M, L);
+// max over the lanes c, c + 16, c + 32, c + 48
+__device__ __forceinline__ float group_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// max over aligned teams of 16 lanes
+__device__ __forceinline__ int row_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+  return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+}
+
+// Scales within these bounds (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
+// exponent of their row's largest taken out, which then goes to the score or the weight.
+__device__ __forceinline__ bool plain_scale(uint32_t bits) {
+  return (bits & 0x7fffu) - (uint32_t)((127 - 12) << 7) < (uint32_t)(15 << 7);
+}
+// 2^(8 - e) for -100 <= e <= 127
+__device__ __forceinline__ float pow2_8_minus(int e) { return __int_as_float((135 - e) << 23); }
+__device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7) - 127, -100); }
+
+// A block owns 16 RT rows of [qrows * heads, hd] and a run of 32-key steps, which its waves take
+// in turn, each on its own; lane (c, g) works for row c throughout:
+//   S^T = K . Q^T     keys 4 g .. + 3 of each half per lane; q in LDS as FP16 hi + lo
+//   softmax           running maximum and sum per row
+//   O^T += V^T . P^T  the lane's weights are its operand as they are, FP16 hi + lo; a lane unpacks
+//                     HD / 16 dims of 8 keys
+template <int HD, int RT>
+__global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
+  constexpr int KW = HD / 32;                  // words of a key per lane, and products
+  constexpr int KS = HD >= 128 ? HD / 128 : 1; // scales of a key per lane
+  constexpr int VD = HD / 16;                  // dims per lane, and output tiles
+  constexpr int VW = VD >= 8 ? VD / 8 : 1;     // words of them (64: half a word)
+  constexpr int R = 16 * RT, OS = HD + 4;
+  union Smem {
+    u32x4 q[2][RT][KW][64];
+    float o[kWaves][16][OS];
+  };
+  __shared__ Smem sm;
+  __shared__ int xq[R];
+  __shared__ float2 wml[kWaves][R];
+  const Scores &S = a.s;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int R0 = blockIdx.x * R, split = blockIdx.y;
+  // the rows' positions, and the keys that some of them see
+  const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
+  int lo = S.first;
+  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+  const int hi = pb + 1, steps = (hi - lo + kStep - 1) / kStep;
+  const int per = (steps + S.splits - 1) / S.splits;
+  const int t0 = split * per, t1 = min(t0 + per, steps);
+
+  uint32_t kr[2][KW], ksr[2][KS], vr[8][VW], vsr[8];
+  auto load_k = [&](int step) {
+    const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2);
+    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16);
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      const uint32_t r = (uint32_t)min(16 * T + c, last);
+      if constexpr (HD >= 128) {
+#pragma unroll
+        for (int J = 0; J < KS; ++J) {
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(p + r * (HD / 2) + (4 * J + g) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kr[T][4 * J + i] = x[i];
+          ksr[T][J] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + (4 * J + g) * 2);
+        }
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p + r * (HD / 2) + g * 8);
+        kr[T][0] = x.x;
+        kr[T][1] = x.y;
+        ksr[T][0] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + (g >> 1) * 2);
+      }
+    }
+  };
+  auto load_v = [&](int step) {
+    const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2);
+    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
+      const char *pr = p + r * (HD / 2) + c * (HD / 32);
+      if constexpr (HD == 512) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(pr);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[j][i] = x[i];
+      } else if constexpr (HD == 256) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(pr);
+        vr[j][0] = x.x;
+        vr[j][1] = x.y;
+      } else if constexpr (HD == 128) {
+        vr[j][0] = *reinterpret_cast<const uint32_t *>(pr);
+      } else {
+        vr[j][0] = *reinterpret_cast<const uint16_t *>(pr);
+      }
+      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + c * HD / 512 * 2);
+    }
+  };
+  load_k(t0 + w);
+  load_v(t0 + w);
+
+  // q: a thread takes 8 values of a row, whose largest gets the exponent 13
+  {
+    constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    const int wd = t % TW;
+    for (int r = t / TW; r < R; r += PASS) {
+      const int row = min(R0 + r, S.rows - 1);
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 8 * wd);
+      const f32x4 x0 = p[0], x1 = p[1];
+      int top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
+#pragma unroll
+      for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      if (wd == 0) xq[r] = e - 21;  // (8 of the scales)
+      u32x4 hi4, lo4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2_t x = {ldexpf(x0[i], 13 - e), ldexpf(x1[i], 13 - e)};
+        const half2_t h = __builtin_convertvector(x, half2_t);
+        const half2_t l = __builtin_convertvector(x - __builtin_convertvector(h, f32x2_t), half2_t);
+        hi4[i] = __builtin_bit_cast(uint32_t, h);
+        lo4[i] = __builtin_bit_cast(uint32_t, l);
+      }
+      const int n = HD >= 128 ? (wd >> 4) * 4 + (wd & 3) : wd & 1;
+      const int at = HD >= 128 ? (wd >> 2) & 3 : wd >> 1;
+      sm.q[0][r >> 4][n][(r & 15) + 16 * at] = hi4;
+      sm.q[1][r >> 4][n][(r & 15) + 16 * at] = lo4;
+    }
+  }
+  __syncthreads();
+
+  int pos[RT], xe[RT];
+  float m[RT], l[RT], E[RT];
+  f32x4 o[RT][VD];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    pos[r] = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
+    xe[r] = xq[16 * r + c];
+    m[r] = kNoScore;
+    l[r] = 0.f;
+    E[r] = -1000.f;  // outputs are held times 2^(21 - E)
+#pragma unroll
+    for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  for (int step = t0 + w; step < t1; step += kWaves) {
+    const int key0 = lo + step * kStep;
+    // the keys' exponents, where a scale needs them
+    int ke[2][4] = {};
+    float kmul[2] = {256.f, 256.f};
+    {
+      bool plain = true;
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int J = 0; J < KS; ++J) plain = plain && plain_scale(ksr[T][J]);
+      if (!__all(plain)) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          int top = 0;
+#pragma unroll
+          for (int J = 0; J < KS; ++J) top = max(top, (int)(ksr[T][J] & 0x7fffu));
+          top = max(top, __shfl_xor(top, 16, 64));
+          top = max(top, __shfl_xor(top, 32, 64));
+          const int e = min(scale_exponent(top), 127);
+          kmul[T] = pow2_8_minus(e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ke[T][i] = __shfl(e, 4 * g + i, 64);
+        }
+      }
+    }
+    f32x4 s[RT][2];
+    {
+      f32x4 sh[RT][2], sl[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) sh[r][T] = sl[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int J = 0; J < KS; ++J) {
+        Scale x[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          const float f = bf16_to_f32(ksr[T][J]) * kmul[T];
+          x[T] = scale_pair(f, f);
+        }
+#pragma unroll
+        for (int i = 0; i < KW / KS; ++i) {
+          const int n = J * (KW / KS) + i;
+          half8_t kv[2];
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            const uint32_t wd = kr[T][n];
+            kv[T] = __builtin_bit_cast(
+                half8_t, (u32x4){value_pair<0>(wd, x[T]), value_pair<1>(wd, x[T]), value_pair<2>(wd, x[T]),
+                                 value_pair<3>(wd, x[T])});
+          }
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const half8_t qh = __builtin_bit_cast(half8_t, sm.q[0][r][n][lane]);
+            const half8_t ql = __builtin_bit_cast(half8_t, sm.q[1][r][n][lane]);
+#pragma unroll
+            for (int T = 0; T < 2; ++T) {
+              sh[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], qh, sh[r][T], 0, 0, 0);
+              sl[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], ql, sl[r][T], 0, 0, 0);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) s[r][T] = sh[r][T] + sl[r][T];
+    }
+    load_k(step + kWaves);
+
+    // v's exponents: keys 4 g + i of each half, as the weights are held
+    int ve[8] = {};
+    float vmul[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vmul[j] = 256.f;
+    uint32_t odd = 0;  // keys of which this lane's dims are no numbers
+    bool vplain = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vplain = vplain && plain_scale(vsr[j]);
+    vplain = __all(vplain);
+    if (!vplain) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        int u = vsr[j] & 0x7fff;
+        if (u >= 0x7f80) {
+          odd |= 1u << j;
+          vsr[j] = u = 0;
+        }
+        ve[j] = scale_exponent(row_max(u));
+        vmul[j] = pow2_8_minus(ve[j]);
+      }
+    }
+    // whether every row sees every key of the step
+    const bool inner = key0 + kStep - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
+    half8_t ph[RT], pl[RT];
+    uint32_t seen[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float x[8];
+      seen[r] = 0xffu;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = ldexpf(s[r][j >> 2][j & 3] * kLog2e, xe[r] + ke[j >> 2][j & 3]);
+      if (!inner) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+          if (key > pos[r] || (S.window > 0 && key <= pos[r] - S.window)) {
+            x[j] = -INFINITY;
+            seen[r] &= ~(1u << j);
+          }
+        }
+      }
+      const int row = R0 + 16 * r + c;
+      if (S.score && row < S.rows) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
+          if (at < S.stride)
+            *reinterpret_cast<float4 *>(S.score + (size_t)row * S.stride + at) =
+                make_float4(x[4 * T], x[4 * T + 1], x[4 * T + 2], x[4 * T + 3]);
+        }
+      }
+      float tm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      // (fmaxf drops a NaN score, whose weight is NaN.)
+      const float mn = fmaxf(m[r], group_max(tm));
+      const float corr = __builtin_amdgcn_exp2f(m[r] - mn);
+      float E2 = E[r] + fmaxf(ceilf(m[r] - mn), -1000.f);
+      float bound = 0.f;
+      if (!vplain) {
+        bound = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bound = fmaxf(bound, (float)ve[j] + ceilf(x[j] - mn));
+        bound = group_max(bound);
+      }
+      E2 = fmaxf(fmaxf(E2, bound), -1000.f);
+      float p[8], sum = 0.f;
+      const int up = 13 - (int)E2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(x[j] - mn);
+        sum += p[j];
+      }
+      l[r] = fmaf(l[r], corr, sum);
+      u32x4 h4, l4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x2_t z = {ldexpf(p[2 * j], up + ve[2 * j]), ldexpf(p[2 * j + 1], up + ve[2 * j + 1])};
+        const half2_t h = __builtin_convertvector(z, half2_t);
+        h4[j] = __builtin_bit_cast(uint32_t, h);
+        l4[j] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
+      }
+      ph[r] = __builtin_bit_cast(half8_t, h4);
+      pl[r] = __builtin_bit_cast(half8_t, l4);
+      const float f = ldexpf(corr, (int)(E[r] - E2));
+      m[r] = mn;
+      E[r] = E2;
+      if (__any(f != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < VD; ++n) o[r][n] *= f;
+      }
+    }
+    {
+      Scale x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * vmul[2 * j], bf16_to_f32(vsr[2 * j + 1]) * vmul[2 * j + 1]);
+#pragma unroll
+      for (int i = 0; i < VW; ++i) {
+#pragma unroll
+        for (int h = 0; h < (VD >= 8 ? 2 : 1); ++h) {
+          uint32_t d[4];  // the word's lower or upper four dims of two keys
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            d[j] = __builtin_amdgcn_perm(vr[2 * j + 1][i], vr[2 * j][i], h ? 0x07060302u : 0x05040100u);
+          auto tile = [&](auto T) {
+            constexpr int e = decltype(T)::value;
+            const half8_t vv = __builtin_bit_cast(
+                half8_t, (u32x4){value_pair<e>(d[0], x[0]), value_pair<e>(d[1], x[1]), value_pair<e>(d[2], x[2]),
+                                 value_pair<e>(d[3], x[3])});
+            const int n = 8 * i + 4 * h + e;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
+              o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+            }
+          };
+          tile(std::integral_constant<int, 0>());
+          tile(std::integral_constant<int, 1>());
+          tile(std::integral_constant<int, 2>());
+          tile(std::integral_constant<int, 3>());
+        }
+      }
+    }
+    if (!vplain && __any(odd != 0)) {  // rows that see such a key: NaN in its dims
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        for (int g2 = 0; g2 < 4; ++g2) {
+          const uint32_t sees = __shfl((int)seen[r], 16 * g2 + c, 64);
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (__shfl((int)odd, 16 * g2 + 4 * g + v, 64) & sees) {
+#pragma unroll
+              for (int n = 0; n < VD; ++n) o[r][n][v] = __int_as_float(0x7fc00000);
+            }
+        }
+    }
+    load_v(step + kWaves);
+  }
+
+  // the waves' sums, in order, through LDS
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor(l[r], 16, 64);
+    l[r] += __shfl_xor(l[r], 32, 64);
+    if (g == 0) wml[w][16 * r + c] = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+  const bool whole = S.splits == 1;
+  float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float M = kNoScore, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) M = fmaxf(M, wml[i][16 * r + c].x);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i)
+      L = fmaf(wml[i][16 * r + c].y, __builtin_amdgcn_exp2f(wml[i][16 * r + c].x - M), L);
+    const int row = R0 + 16 * r + c;
+    if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)split * S.rows + row] = make_float2(M, L);
+    // (a split of which the row sees nothing: 0, not 0 / 0)
+    float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
+    if (!whole && L == 0.f) f = 0.f;
+    f = ldexpf(f, (int)E[r] - 21);
+    if (r > 0) __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int n = 0; n < VD; n += 4)
+        *reinterpret_cast<f32x4 *>(&sm.o[w][c][(4 * g + v) * VD + n]) =
+            (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * f;
+    __syncthreads();
+    for (int u = t; u < 16 * HD / 4; u += 64 * kWaves) {
+      const int rr = u / (HD / 4), d = u % (HD / 4) * 4;
+      f32x4 x = *reinterpret_cast<const f32x4 *>(&sm.o[0][rr][d]);
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) x += *reinterpret_cast<const f32x4 *>(&sm.o[i][rr][d]);
+      if (R0 + 16 * r + rr < S.rows)
+        *reinterpret_cast<f32x4 *>(out + (size_t)(R0 + 16 * r + rr) * HD + d) = x;
+    }
+  }
+}
+
+// Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
+// one row's 64 dims; thread (j, u) adds splits j, j + 16, .. of 16-byte unit u in order.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
+  constexpr int U = 16, G = 256 / U;
+  const Scores &S = a.s;
+  const int t = threadIdx.x, u = t % U, j = t / U, row = blockIdx.x;
+  __shared__ float wt[kMaxSplits];
+  __shared__ float wmax[4], wsum[4];
+  __shared__ f32x4 sums[G][U];
+  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + blockIdx.y * U + u;
+  const size_t step = (size_t)S.rows * HD / 4;
+  f32x4 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = p[min(j + G * i, S.splits - 1) * step];
+  const float2 ml = t < S.splits ? S.ml[(size_t)t * S.rows + row] : make_float2(kNoScore, 0.f);
+  float M = ml.x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  if ((t & 63) == 0) wmax[t >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  const float e = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
+  wt[t] = e;
+  const float L = wave_sum(e);
+  if ((t & 63) == 0) wsum[t >> 6] = L;
+  __syncthreads();
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + G * i < S.splits) y += wt[j + G * i] * x[i];
+  for (int s = j + 4 * G; s < S.splits; s += G) y += wt[s] * p[s * step];
+  sums[j][u] = y;
+  __syncthreads();
+  if (j > 0) return;
+  y = sums[0][u];
+#pragma unroll
+  for (int i = 1; i < G; ++i) y += sums[i][u];
+  const float sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] /= sum;
+  reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[blockIdx.y * U + u] = y;
+}
+
+int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 Workspace g_kv4_ws;
+
+// n query rows from row0 on; `before` and `weights` of this call.
+template <int HD, int RT>
+int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
+  Scores &s = a.s;
+  const int blocks = cdiv(s.rows, 16 * RT);
+  const int keys = s.window > 0 ? min(s.end - s.first, s.window + 16 * RT) : s.end - s.first;
+  const int steps = cdiv(keys, kStep);
+  int splits = cu_count() / blocks;
+  if (splits > cdiv(steps, kWaves)) splits = cdiv(steps, kWaves);
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  if (splits < 1) splits = 1;
+  s.splits = splits;
+  const bool ml = weights || splits > 1;
+  const size_t n_part = splits > 1 ? (size_t)splits * s.rows * HD : 0, n_ml = ml ? (size_t)splits * s.rows * 2 : 0;
+  const size_t n_score = weights ? s.rows * s.stride : 0;
+  const size_t n_sum = weights ? weight_part_floats(s.rows, s.end - s.first) : 0;
+  if (n_part + n_ml + n_score + n_sum) {
+    void *mem = nullptr;
+    if (int rc = g_kv4_ws.get((n_part + n_ml + n_score + n_sum) * 4, &mem, "g4_attention_kv4")) return rc;
+    a.part = static_cast<float *>(mem);
+    s.score = weights ? a.part + n_part : nullptr;
+    s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
+  }
+  hipLaunchKernelGGL((attn_kv4_kernel<HD, RT>), dim3(blocks, splits), dim3(64 * kWaves), 0, stream(), a);
+  G4_LAUNCH_CHECK("attn_kv4_kernel");
+  if (splits > 1) {
+    hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 64), dim3(256), 0, stream(), a);
+    G4_LAUNCH_CHECK("attn_kv4_merge_kernel");
+  }
+  if (!weights) return G4_OK;
+  return launch_weights(s, keylen, a.part + n_part + n_score + n_ml, before, weights);
+}
+
+template <int HD>
+int launch_hd(const Kv4Args &a, int keylen, const float *before, float *weights) {
+  return a.s.rows <= 16 ? launch_rows<HD, 1>(a, keylen, before, weights)
+                        : launch_rows<HD, 2>(a, keylen, before, weights);
+}
 
 }  // namespace
 }  // namespace g4
@@ -97,7 +564,7 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
   if (!rc && weights) rc = check_device_range(weights, (size_t)keylen * 4, "g4_attention_kv4 weights");
   if (!rc && before) rc = check_device_range(before, (size_t)keylen * 4, "g4_attention_kv4 before");
   if (rc) return rc;
-  const int win = sliding ? window : 0;
+  const int win = sliding ? (window < keylen ? window : keylen) : 0;
   if (qrows == 0) {
     Scores s{};
     s.heads = 1;
@@ -117,28 +584,18 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
     Scores &s = a.s;
     s.rows = n * heads;
     s.heads = heads;
-    s.splits = 1;
     s.pos0 = qpos0 + r0;
     s.window = win;
     s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
     s.end = s.pos0 + n;
     s.stride = (size_t)((s.end - s.first + 3) & ~3);
-    const size_t scores = weights ? s.rows * s.stride : 0, ml = weights ? (size_t)s.splits * s.rows * 2 : 0;
-    if (weights) {
-      void *mem = nullptr;
-      if ((rc = g_kv4_ws.get((scores + ml + weight_part_floats(s.rows, s.end - s.first)) * 4, &mem, who)))
-        return rc;
-      s.score = static_cast<float *>(mem);
-      s.ml = reinterpret_cast<float2 *>(s.score + scores);
-    }
+    const float *b = r0 ? weights : before;
     switch (head_dim) {
-      case 64: hipLaunchKernelGGL(attn_kv4_kernel<64>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      case 128: hipLaunchKernelGGL(attn_kv4_kernel<128>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      case 256: hipLaunchKernelGGL(attn_kv4_kernel<256>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      default: hipLaunchKernelGGL(attn_kv4_kernel<512>, dim3(s.rows), dim3(256), 0, stream(), a); break;
+      case 64: rc = launch_hd<64>(a, keylen, b, weights); break;
+      case 128: rc = launch_hd<128>(a, keylen, b, weights); break;
+      case 256: rc = launch_hd<256>(a, keylen, b, weights); break;
+      default: rc = launch_hd<512>(a, keylen, b, weights); break;
     }
-    G4_LAUNCH_CHECK("attn_kv4_kernel");
-    if (weights) rc = launch_weights(s, keylen, s.score + scores + ml, r0 ? weights : before, weights);
     if (rc) return rc;
   }
   return ok();

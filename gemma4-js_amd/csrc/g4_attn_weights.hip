@@ -180,7 +180,7 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
   if (!rc && qrows) rc = check_device_range(q, (size_t)qrows * heads * head_dim * 4, "g4_attention_weights q");
   if (!rc) rc = check_device_range(k, (size_t)keylen * head_dim * 4, "g4_attention_weights k");
   if (rc) return rc;
-  const int win = sliding ? window : 0;
+  const int win = sliding ? (window < keylen ? window : keylen) : 0;
   if (qrows == 0) {
     Scores s{};
     s.heads = 1;
