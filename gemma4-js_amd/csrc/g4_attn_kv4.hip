@@ -66,33 +66,46 @@ __device__ __forceinline__ int row_max(int v) {
 __device__ __forceinline__ bool plain_scale(uint32_t bits) {
   return (bits & 0x7fffu) - (uint32_t)((127 - 12) << 7) < (uint32_t)(15 << 7);
 }
+// Signed byte i of a word.
+__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 // 2^(8 - e) for -100 <= e <= 127
 __device__ __forceinline__ float pow2_8_minus(int e) { return __int_as_float((135 - e) << 23); }
 __device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7) - 127, -100); }
 
-// A block owns 16 RT rows of [qrows * heads, hd] and a run of 32-key steps, which its waves take
-// in turn, each on its own; lane (c, g) works for row c throughout:
-//   S^T = K . Q^T     keys 4 g .. + 3 of each half per lane; q in LDS as FP16 hi + lo
+// Dims that a wave works on; the waves of a key group share the head dim.
+template <int HD>
+constexpr int kDims = HD > 256 ? 256 : HD;
+template <int HD>
+constexpr int kGroups = kWaves / (HD / kDims<HD>);  // key groups of a block
+
+// A block owns 16 RT rows of [qrows * heads, hd] and a run of 32-key steps, which its key groups
+// take in turn; lane (c, g) of a wave works for row c throughout:
+//   S^T = K . Q^T     keys 4 g .. + 3 of each half per lane; q in LDS as FP16 hi + lo; a group's
+//                     waves add theirs through LDS, in order, so that they hold the same scores
 //   softmax           running maximum and sum per row
 //   O^T += V^T . P^T  the lane's weights are its operand as they are, FP16 hi + lo; a lane unpacks
-//                     HD / 16 dims of 8 keys
+//                     DW / 16 dims of 8 keys
 template <int HD, int RT>
-__global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
-  constexpr int KW = HD / 32;                  // words of a key per lane, and products
-  constexpr int KS = HD >= 128 ? HD / 128 : 1; // scales of a key per lane
-  constexpr int VD = HD / 16;                  // dims per lane, and output tiles
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
+  constexpr int DW = kDims<HD>, DQ = HD / DW, KG = kGroups<HD>;
+  constexpr int KW = DW / 32;                  // words of a key per lane, and products
+  constexpr int KS = DW >= 128 ? DW / 128 : 1; // scales of a key per lane
+  constexpr int VD = DW / 16;                  // dims per lane, and output tiles
   constexpr int VW = VD >= 8 ? VD / 8 : 1;     // words of them (64: half a word)
   constexpr int R = 16 * RT, OS = HD + 4;
   union Smem {
-    u32x4 q[2][RT][KW][64];
-    float o[kWaves][16][OS];
+    struct {
+      u32x4 q[2][RT][HD / 32][64];
+      f32x4 sx[DQ > 1 ? 2 : 0][KG][DQ][RT][2][64];  // the waves' scores, two buffers
+    } loop;
+    float o[16][OS];
   };
   __shared__ Smem sm;
   __shared__ int xq[R];
-  __shared__ float2 wml[kWaves][R];
+  __shared__ float2 wml[KG][R];
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int c = lane & 15, g = lane >> 4;
+  const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
   // the rows' positions, and the keys that some of them see
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
@@ -105,53 +118,49 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
   uint32_t kr[2][KW], ksr[2][KS], vr[8][VW], vsr[8];
   auto load_k = [&](int step) {
     const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2);
-    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16);
+    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
+    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
       const uint32_t r = (uint32_t)min(16 * T + c, last);
-      if constexpr (HD >= 128) {
+      if constexpr (DW >= 128) {
 #pragma unroll
         for (int J = 0; J < KS; ++J) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(p + r * (HD / 2) + (4 * J + g) * 16);
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (r * (HD / 2) + g * 16) + 64 * J);
 #pragma unroll
           for (int i = 0; i < 4; ++i) kr[T][4 * J + i] = x[i];
-          ksr[T][J] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + (4 * J + g) * 2);
+          ksr[T][J] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + g * 2) + 8 * J);
         }
       } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(p + r * (HD / 2) + g * 8);
+        const uint2 x = *reinterpret_cast<const uint2 *>(p + (r * (HD / 2) + g * 8));
         kr[T][0] = x.x;
         kr[T][1] = x.y;
-        ksr[T][0] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + (g >> 1) * 2);
+        ksr[T][0] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + (g >> 1) * 2));
       }
     }
   };
   auto load_v = [&](int step) {
     const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2);
-    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16);
+    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
+    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
-      const char *pr = p + r * (HD / 2) + c * (HD / 32);
-      if constexpr (HD == 512) {
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(pr);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vr[j][i] = x[i];
-      } else if constexpr (HD == 256) {
+      const char *pr = p + (r * (HD / 2) + c * (DW / 32));
+      if constexpr (DW == 256) {
         const uint2 x = *reinterpret_cast<const uint2 *>(pr);
         vr[j][0] = x.x;
         vr[j][1] = x.y;
-      } else if constexpr (HD == 128) {
+      } else if constexpr (DW == 128) {
         vr[j][0] = *reinterpret_cast<const uint32_t *>(pr);
       } else {
         vr[j][0] = *reinterpret_cast<const uint16_t *>(pr);
       }
-      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + r * (HD / 16) + c * HD / 512 * 2);
+      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
     }
   };
-  load_k(t0 + w);
-  load_v(t0 + w);
+  load_k(t0 + kg);
+  load_v(t0 + kg);
 
   // q: a thread takes 8 values of a row, whose largest gets the exponent 13
   {
@@ -180,8 +189,8 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
       }
       const int n = HD >= 128 ? (wd >> 4) * 4 + (wd & 3) : wd & 1;
       const int at = HD >= 128 ? (wd >> 2) & 3 : wd >> 1;
-      sm.q[0][r >> 4][n][(r & 15) + 16 * at] = hi4;
-      sm.q[1][r >> 4][n][(r & 15) + 16 * at] = lo4;
+      sm.loop.q[0][r >> 4][n][(r & 15) + 16 * at] = hi4;
+      sm.loop.q[1][r >> 4][n][(r & 15) + 16 * at] = lo4;
     }
   }
   __syncthreads();
@@ -199,10 +208,12 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  for (int step = t0 + w; step < t1; step += kWaves) {
-    const int key0 = lo + step * kStep;
+  const int turns = (t1 - t0 + KG - 1) / KG;
+  for (int it = 0; it < turns; ++it) {
+    const int step = t0 + kg + it * KG, key0 = lo + step * kStep;
+    const bool mine = step < t1;
     // the keys' exponents, where a scale needs them
-    int ke[2][4] = {};
+    uint32_t ke[2] = {0, 0};  // a byte each
     float kmul[2] = {256.f, 256.f};
     {
       bool plain = true;
@@ -221,7 +232,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
           const int e = min(scale_exponent(top), 127);
           kmul[T] = pow2_8_minus(e);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ke[T][i] = __shfl(e, 4 * g + i, 64);
+          for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e, 4 * g + i, 64) & 255) << (8 * i);
         }
       }
     }
@@ -253,34 +264,55 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
           }
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
-            const half8_t qh = __builtin_bit_cast(half8_t, sm.q[0][r][n][lane]);
-            const half8_t ql = __builtin_bit_cast(half8_t, sm.q[1][r][n][lane]);
+            const half8_t qh = __builtin_bit_cast(half8_t, sm.loop.q[0][r][dq * KW + n][lane]);
+            const half8_t ql = __builtin_bit_cast(half8_t, sm.loop.q[1][r][dq * KW + n][lane]);
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
               sh[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], qh, sh[r][T], 0, 0, 0);
               sl[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], ql, sl[r][T], 0, 0, 0);
             }
           }
+          if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (else all is unpacked at once, and spilled)
         }
       }
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int T = 0; T < 2; ++T) s[r][T] = sh[r][T] + sl[r][T];
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[r][T][i] = ldexpf((sh[r][T][i] + sl[r][T][i]) * kLog2e, xe[r] + byte_of(ke[T], i));
     }
-    load_k(step + kWaves);
+    load_k(step + KG);
+    if constexpr (DQ > 1) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) sm.loop.sx[it & 1][kg][dq][r][T][lane] = s[r][T];
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          s[r][T] = sm.loop.sx[it & 1][kg][0][r][T][lane];
+#pragma unroll
+          for (int d = 1; d < DQ; ++d) s[r][T] += sm.loop.sx[it & 1][kg][d][r][T][lane];
+        }
+    }
 
     // v's exponents: keys 4 g + i of each half, as the weights are held
-    int ve[8] = {};
-    float vmul[8];
+    uint32_t ve[2] = {0, 0};
+    Scale vx[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vmul[j] = 256.f;
+    for (int j = 0; j < 4; ++j)
+      vx[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * 256.f, bf16_to_f32(vsr[2 * j + 1]) * 256.f);
     uint32_t odd = 0;  // keys of which this lane's dims are no numbers
     bool vplain = true;
 #pragma unroll
     for (int j = 0; j < 8; ++j) vplain = vplain && plain_scale(vsr[j]);
     vplain = __all(vplain);
     if (!vplain) {
+      float f[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         int u = vsr[j] & 0x7fff;
@@ -288,12 +320,15 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
           odd |= 1u << j;
           vsr[j] = u = 0;
         }
-        ve[j] = scale_exponent(row_max(u));
-        vmul[j] = pow2_8_minus(ve[j]);
+        const int e = scale_exponent(row_max(u));
+        ve[j >> 2] |= (uint32_t)(e & 255) << (8 * (j & 3));
+        f[j] = bf16_to_f32(vsr[j]) * pow2_8_minus(e);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vx[j] = scale_pair(f[2 * j], f[2 * j + 1]);
     }
     // whether every row sees every key of the step
-    const bool inner = key0 + kStep - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
+    const bool inner = mine && key0 + kStep - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
     half8_t ph[RT], pl[RT];
     uint32_t seen[RT];
 #pragma unroll
@@ -301,19 +336,19 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
       float x[8];
       seen[r] = 0xffu;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = ldexpf(s[r][j >> 2][j & 3] * kLog2e, xe[r] + ke[j >> 2][j & 3]);
+      for (int j = 0; j < 8; ++j) x[j] = s[r][j >> 2][j & 3];
       if (!inner) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-          if (key > pos[r] || (S.window > 0 && key <= pos[r] - S.window)) {
+          if (!mine || key > pos[r] || (S.window > 0 && key <= pos[r] - S.window)) {
             x[j] = -INFINITY;
             seen[r] &= ~(1u << j);
           }
         }
       }
       const int row = R0 + 16 * r + c;
-      if (S.score && row < S.rows) {
+      if (S.score && mine && dq == 0 && row < S.rows) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
           const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
@@ -331,7 +366,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
       if (!vplain) {
         bound = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) bound = fmaxf(bound, (float)ve[j] + ceilf(x[j] - mn));
+        for (int j = 0; j < 8; ++j) bound = fmaxf(bound, (float)byte_of(ve[j >> 2], j & 3) + ceilf(x[j] - mn));
         bound = group_max(bound);
       }
       E2 = fmaxf(fmaxf(E2, bound), -1000.f);
@@ -346,7 +381,8 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
       u32x4 h4, l4;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x2_t z = {ldexpf(p[2 * j], up + ve[2 * j]), ldexpf(p[2 * j + 1], up + ve[2 * j + 1])};
+        const f32x2_t z = {ldexpf(p[2 * j], up + byte_of(ve[j >> 1], 2 * j & 3)),
+                             ldexpf(p[2 * j + 1], up + byte_of(ve[j >> 1], 2 * j + 1 & 3))};
         const half2_t h = __builtin_convertvector(z, half2_t);
         h4[j] = __builtin_bit_cast(uint32_t, h);
         l4[j] = __builtin_bit_cast(
@@ -363,10 +399,6 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
       }
     }
     {
-      Scale x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * vmul[2 * j], bf16_to_f32(vsr[2 * j + 1]) * vmul[2 * j + 1]);
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
 #pragma unroll
@@ -378,8 +410,8 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
           auto tile = [&](auto T) {
             constexpr int e = decltype(T)::value;
             const half8_t vv = __builtin_bit_cast(
-                half8_t, (u32x4){value_pair<e>(d[0], x[0]), value_pair<e>(d[1], x[1]), value_pair<e>(d[2], x[2]),
-                                 value_pair<e>(d[3], x[3])});
+                half8_t, (u32x4){value_pair<e>(d[0], vx[0]), value_pair<e>(d[1], vx[1]), value_pair<e>(d[2], vx[2]),
+                                 value_pair<e>(d[3], vx[3])});
             const int n = 8 * i + 4 * h + e;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
@@ -391,6 +423,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
           tile(std::integral_constant<int, 1>());
           tile(std::integral_constant<int, 2>());
           tile(std::integral_constant<int, 3>());
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -407,15 +440,15 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
             }
         }
     }
-    load_v(step + kWaves);
+    load_v(step + KG);
   }
 
-  // the waves' sums, in order, through LDS
+  // the key groups' sums, in order, through LDS
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
-    if (g == 0) wml[w][16 * r + c] = make_float2(m[r], l[r]);
+    if (g == 0 && dq == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
   }
   __syncthreads();
   const bool whole = S.splits == 1;
@@ -424,9 +457,9 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
   for (int r = 0; r < RT; ++r) {
     float M = kNoScore, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) M = fmaxf(M, wml[i][16 * r + c].x);
+    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][16 * r + c].x);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i)
+    for (int i = 0; i < KG; ++i)
       L = fmaf(wml[i][16 * r + c].y, __builtin_amdgcn_exp2f(wml[i][16 * r + c].x - M), L);
     const int row = R0 + 16 * r + c;
     if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)split * S.rows + row] = make_float2(M, L);
@@ -434,21 +467,39 @@ __global__ __launch_bounds__(64 * kWaves) void attn_kv4_kernel(Kv4Args a) {
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
     if (!whole && L == 0.f) f = 0.f;
     f = ldexpf(f, (int)E[r] - 21);
-    if (r > 0) __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+    for (int n = 0; n < VD; ++n) o[r][n] *= f;
+    // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
+    float *mine = &sm.o[c][dq * DW + 4 * g * VD];
 #pragma unroll
-      for (int n = 0; n < VD; n += 4)
-        *reinterpret_cast<f32x4 *>(&sm.o[w][c][(4 * g + v) * VD + n]) =
-            (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * f;
-    __syncthreads();
-    for (int u = t; u < 16 * HD / 4; u += 64 * kWaves) {
-      const int rr = u / (HD / 4), d = u % (HD / 4) * 4;
-      f32x4 x = *reinterpret_cast<const f32x4 *>(&sm.o[0][rr][d]);
+    for (int i = KG - 1; i >= 1; --i) {
+      if (kg == i)
 #pragma unroll
-      for (int i = 1; i < kWaves; ++i) x += *reinterpret_cast<const f32x4 *>(&sm.o[i][rr][d]);
-      if (R0 + 16 * r + rr < S.rows)
-        *reinterpret_cast<f32x4 *>(out + (size_t)(R0 + 16 * r + rr) * HD + d) = x;
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int n = 0; n < VD; n += 4)
+            *reinterpret_cast<f32x4 *>(mine + v * VD + n) =
+                (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]};
+      __syncthreads();
+      if (kg == 0)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int n = 0; n < VD; n += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(mine + v * VD + n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][n + e][v] += x[e];
+          }
+      __syncthreads();
+    }
+    if (kg == 0 && row < S.rows) {
+      float *p = out + (size_t)row * HD + dq * DW + 4 * g * VD;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int n = 0; n < VD; n += 4)
+          *reinterpret_cast<f32x4 *>(p + v * VD + n) =
+              (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]};
     }
   }
 }
@@ -508,8 +559,8 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   const int blocks = cdiv(s.rows, 16 * RT);
   const int keys = s.window > 0 ? min(s.end - s.first, s.window + 16 * RT) : s.end - s.first;
   const int steps = cdiv(keys, kStep);
-  int splits = cu_count() / blocks;
-  if (splits > cdiv(steps, kWaves)) splits = cdiv(steps, kWaves);
+  int splits = 2 * cu_count() / blocks;
+  if (splits > cdiv(steps, kGroups<HD>)) splits = cdiv(steps, kGroups<HD>);
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 1) splits = 1;
   s.splits = splits;
