@@ -462,7 +462,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     for (int i = 0; i < KG; ++i)
       L = fmaf(wml[i][16 * r + c].y, __builtin_amdgcn_exp2f(wml[i][16 * r + c].x - M), L);
     const int row = R0 + 16 * r + c;
-    if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)split * S.rows + row] = make_float2(M, L);
+    if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)row * S.splits + split] = make_float2(M, L);
     // (a split of which the row sees nothing: 0, not 0 / 0)
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
     if (!whole && L == 0.f) f = 0.f;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
   f32x4 x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = p[min(j + G * i, S.splits - 1) * step];
-  const float2 ml = t < S.splits ? S.ml[(size_t)t * S.rows + row] : make_float2(kNoScore, 0.f);
+  const float2 ml = t < S.splits ? S.ml[(size_t)row * S.splits + t] : make_float2(kNoScore, 0.f);
   float M = ml.x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));

@@ -37,6 +37,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
 constexpr int kGroup = 64;                  // rows that a block adds up
+constexpr int kMaxSplits = 512;
 
 struct SumArgs {
   Scores s;
@@ -51,26 +52,28 @@ __global__ __launch_bounds__(256) void weights_kernel(SumArgs a) {
   const Scores &s = a.s;
   const int t = threadIdx.x, r0 = blockIdx.y * kGroup;
   const int key = blockIdx.x * 256 + t + (a.part ? s.first : 0);
+  const int n = min(kGroup, s.rows - r0);
   {
-    const int row = min(r0 + t / 4, s.rows - 1);
+    int lanes = 4;  // per row
+    while (lanes < 64 && lanes * 2 * n <= 256) lanes *= 2;
+    const int i = t / lanes;
+    const float2 *ml = s.ml + (size_t)(r0 + min(i, n - 1)) * s.splits;
     float m = kNoScore, l = 0.f;
-    for (int p = t & 3; p < s.splits; p += 4) {
-      const float2 x = s.ml[(size_t)p * s.rows + row];
+    for (int p = t % lanes; p < s.splits; p += lanes) {
+      const float2 x = ml[p];
       const float mn = fmaxf(m, x.x);
       l = l * __builtin_amdgcn_exp2f(m - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
       m = mn;
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
+    for (int o = 1; o < lanes; o <<= 1) {
       const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
       const float x = l * __builtin_amdgcn_exp2f(m - mn), y = l2 * __builtin_amdgcn_exp2f(m2 - mn);
       l = (t & o) ? y + x : x + y;
       m = mn;
     }
-    if ((t & 3) == 0) stat[t / 4] = make_float2(m, 1.f / l);
+    if (t % lanes == 0 && i < n) stat[i] = make_float2(m, 1.f / l);
   }
   __syncthreads();
-  const int n = min(kGroup, s.rows - r0);
   float sum = 0.f;
   if (key >= s.first && key < s.end) {
     const float *p = s.score + (size_t)r0 * s.stride + (key - s.first);
@@ -120,41 +123,260 @@ int launch_weights(const Scores &s, int keylen, float *part, const float *before
 
 namespace {
 
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+
 struct ScoreArgs {
   const float *q, *k;
   Scores s;
 };
 
-// A block per row; a wave takes every fourth key.
-template <int HD>
-__global__ __launch_bounds__(256) void scores_kernel(ScoreArgs a) {
-  constexpr int D = HD / 64;
-  __shared__ float2 sml[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x;
-  const int pos = a.s.pos0 + row / a.s.heads;
-  const int lo = a.s.window > 0 ? max(a.s.first, pos - a.s.window + 1) : a.s.first;
-  float q[D];
+// Eight FP32 values, times `up`, as sums of two FP16 values.
+__device__ __forceinline__ void halves(const f32x4 &a, const f32x4 &b, float up, half8_t &h, half8_t &l) {
+  u32x4 x, y;
 #pragma unroll
-  for (int d = 0; d < D; ++d) q[d] = a.q[(size_t)row * HD + lane * D + d];
-  float m = kNoScore, l = 0.f;
-  for (int key = lo + w; key <= pos; key += 4) {
-    float x = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) x = fmaf(q[d], a.k[(size_t)key * HD + lane * D + d], x);
-    x = wave_sum(x) * kLog2e;
-    if (lane == 0) a.s.score[(size_t)row * a.s.stride + (key - a.s.first)] = x;
-    const float mn = fmaxf(m, x);
-    l = l * __builtin_amdgcn_exp2f(m - mn) + __builtin_amdgcn_exp2f(x - mn);
-    m = mn;
+  for (int i = 0; i < 4; ++i) {
+    const f32x2_t z = {(i < 2 ? a[2 * i] : b[2 * i - 4]) * up, (i < 2 ? a[2 * i + 1] : b[2 * i - 3]) * up};
+    const half2_t u = __builtin_convertvector(z, half2_t);
+    x[i] = __builtin_bit_cast(uint32_t, u);
+    y[i] = __builtin_bit_cast(uint32_t,
+                              __builtin_convertvector(z - __builtin_convertvector(u, f32x2_t), half2_t));
   }
-  if (lane == 0) sml[w] = make_float2(m, l);
+  h = __builtin_bit_cast(half8_t, x);
+  l = __builtin_bit_cast(half8_t, y);
+}
+__device__ __forceinline__ float largest(const f32x4 &a, const f32x4 &b) {
+  float m = fmaxf(fabsf(a[0]), fabsf(a[1]));
+  m = fmaxf(m, fmaxf(fabsf(a[2]), fabsf(a[3])));
+  m = fmaxf(m, fmaxf(fabsf(b[0]), fabsf(b[1])));
+  return fmaxf(m, fmaxf(fabsf(b[2]), fabsf(b[3])));
+}
+// max over the lanes c, c + 16, c + 32, c + 48
+__device__ __forceinline__ float group_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Scores of 16 RT rows and a run of steps of 16 NT keys, which the block's KG key groups take in
+// turn; the DQ waves of a group share the head dim and add their scores through LDS, in order.
+// q and k enter the FP16 matrix cores as two values each (hi hi, hi lo and lo hi; lo lo is below
+// 2^-22 of a product), q with its row's largest at the exponent 13, k times 2^8; a wave in which a
+// key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.
+template <int HD, int DQ, int NT, int RT>
+__global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
+  constexpr int KG = kWaves / DQ, DW = HD / DQ, KN = DW / 32, R = 16 * RT, KEYS = 16 * NT;
+  __shared__ u32x4 sq[2][RT][HD / 32][64];
+  __shared__ f32x4 sx[DQ > 1 ? 2 : 1][KG][DQ][DQ > 1 ? RT : 1][DQ > 1 ? NT : 1][DQ > 1 ? 64 : 1];
+  __shared__ int xq[R];
+  __shared__ float2 wml[KG][R];
+  const Scores &S = a.s;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
+  const int R0 = blockIdx.x * R, split = blockIdx.y;
+  const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
+  int lo = S.first;
+  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
+  const int per = (steps + S.splits - 1) / S.splits;
+  const int t0 = split * per, t1 = min(t0 + per, steps);
+
+  f32x4 kr[2][NT][2];
+  auto load_k = [&](int step, int n, f32x4 (&x)[NT][2]) {
+    const int k0 = lo + min(step, steps - 1) * KEYS, last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + dq * DW);
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 8 * g) * 4;
+      x[T][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
+      x[T][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
+    }
+  };
+  load_k(t0 + kg, 0, kr[0]);
+  {
+    constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    const int wd = t % TW;
+    for (int r = t / TW; r < R; r += PASS) {
+      const int row = min(R0 + r, S.rows - 1);
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 8 * wd);
+      f32x4 x0 = p[0], x1 = p[1];
+      int top = 0;  // as bits, where NaN > infinity > numbers
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
+#pragma unroll
+      for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      if (wd == 0) xq[r] = e - 13;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x0[i] = ldexpf(x0[i], 13 - e), x1[i] = ldexpf(x1[i], 13 - e);
+      half8_t h, l;
+      halves(x0, x1, 1.f, h, l);
+      sq[0][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, h);
+      sq[1][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, l);
+    }
+  }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float M = kNoScore, L = 0.f;
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[i].x);
-    for (int i = 0; i < 4; ++i) L += sml[i].y * __builtin_amdgcn_exp2f(sml[i].x - M);
-    a.s.ml[row] = make_float2(M, L);
+
+  int pos[RT], xe[RT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    pos[r] = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
+    xe[r] = xq[16 * r + c];
+    m[r] = kNoScore;
+    l[r] = 0.f;
   }
+  const int turns = (t1 - t0 + KG - 1) / KG;
+  for (int it = 0; it < turns; ++it) {
+    const int step = t0 + kg + it * KG, key0 = lo + step * KEYS;
+    const bool mine = step < t1;
+    f32x4 s[RT][NT];
+    float up[NT], top[NT];
+#pragma unroll
+    for (int T = 0; T < NT; ++T) up[T] = 256.f;
+    bool again = false;
+    for (int turn = 0; turn < 2; ++turn) {
+#pragma unroll
+      for (int T = 0; T < NT; ++T) top[T] = 0.f;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < NT; ++T) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int n0 = 0; n0 < KN; n0 += 2)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int n = n0 + e;
+        const bool more = n + 1 < KN;
+        load_k(more ? step : step + KG, more ? n + 1 : 0, kr[1 - e]);
+        half8_t kh[NT], kl[NT];
+#pragma unroll
+        for (int T = 0; T < NT; ++T) {
+          top[T] = fmaxf(top[T], largest(kr[e][T][0], kr[e][T][1]));
+          halves(kr[e][T][0], kr[e][T][1], up[T], kh[T], kl[T]);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const half8_t qh = __builtin_bit_cast(half8_t, sq[0][r][dq * KN + n][lane]);
+          const half8_t ql = __builtin_bit_cast(half8_t, sq[1][r][dq * KN + n][lane]);
+#pragma unroll
+          for (int T = 0; T < NT; ++T)
+            s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[T], ql, s[r][T], 0, 0, 0);
+#pragma unroll
+          for (int T = 0; T < NT; ++T)
+            s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[T], qh, s[r][T], 0, 0, 0);
+#pragma unroll
+          for (int T = 0; T < NT; ++T)
+            s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[T], qh, s[r][T], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (turn == 1) break;
+      bool fits = true;
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        top[T] = group_max(top[T]);
+        // (rows without numbers give scores that are none either way)
+        fits = fits && (top[T] == 0.f || (top[T] >= 0x1p-10f && top[T] < 128.f) || !(top[T] < INFINITY));
+      }
+      again = !__all(fits);
+      if (!again) break;
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        const int e = top[T] < INFINITY ? min(max((int)(__float_as_uint(top[T]) >> 23) - 127, -100), 127) : 0;
+        up[T] = __int_as_float((127 + 8 - e) << 23);
+      }
+      load_k(step, 0, kr[0]);
+    }
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      int ke[4] = {-8, -8, -8, -8};
+      if (again)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ke[i] = 127 - (int)(__shfl((int)__float_as_uint(up[T]), 4 * g + i, 64) >> 23);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[r][T][i] = ldexpf(s[r][T][i] * kLog2e, xe[r] + ke[i]);
+    }
+    if constexpr (DQ > 1) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < NT; ++T) sx[it & 1][kg][dq][r][T][lane] = s[r][T];
+      __syncthreads();
+      if (dq > 0) continue;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < NT; ++T)
+#pragma unroll
+          for (int d = 1; d < DQ; ++d) s[r][T] += sx[it & 1][kg][d][r][T][lane];
+    }
+    if (!mine) continue;
+    const bool inner = key0 + KEYS - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      if (!inner) {
+#pragma unroll
+        for (int T = 0; T < NT; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * T + 4 * g + i;
+            if (key > pos[r] || (S.window > 0 && key <= pos[r] - S.window)) s[r][T][i] = -INFINITY;
+          }
+      }
+      const int row = R0 + 16 * r + c;
+      float tm = kNoScore;
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
+        if (row < S.rows && at < S.stride) *reinterpret_cast<f32x4 *>(S.score + (size_t)row * S.stride + at) = s[r][T];
+        tm = fmaxf(tm, fmaxf(fmaxf(s[r][T][0], s[r][T][1]), fmaxf(s[r][T][2], s[r][T][3])));
+      }
+      // (fmaxf drops a NaN score, whose weight is NaN.)
+      const float mn = fmaxf(m[r], group_max(tm));
+      float sum = 0.f;
+#pragma unroll
+      for (int T = 0; T < NT; ++T)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[r][T][i] - mn);
+      l[r] = fmaf(l[r], __builtin_amdgcn_exp2f(m[r] - mn), sum);
+      m[r] = mn;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] += __shfl_xor(l[r], 16, 64);
+    l[r] += __shfl_xor(l[r], 32, 64);
+    if (g == 0 && dq == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+  for (int r = t; r < R; r += 64 * kWaves) {
+    if (R0 + r >= S.rows) break;
+    float M = kNoScore, L = 0.f;
+    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][r].x);
+    for (int i = 0; i < KG; ++i) L = fmaf(wml[i][r].y, __builtin_amdgcn_exp2f(wml[i][r].x - M), L);
+    S.ml[(size_t)(R0 + r) * S.splits + split] = make_float2(M, L);
+  }
+}
+
+// The plan's shape: rows per block, keys per step, key groups.
+struct ScorePlan {
+  void (*kernel)(ScoreArgs);
+  int rows, keys, groups;
+};
+template <int HD>
+ScorePlan score_plan(int rows) {
+  constexpr int DQ = HD >= 128 ? HD / 128 : 1;
+  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, 16, 16, kWaves / DQ};
+  return {scores_kernel<HD, 1, 2, 4>, 64, 32, kWaves};
 }
 
 Workspace g_weights_ws;
@@ -196,24 +418,27 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     Scores &s = a.s;
     s.rows = n * heads;
     s.heads = heads;
-    s.splits = 1;
     s.pos0 = qpos0 + r0;
     s.window = win;
     s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
     s.end = s.pos0 + n;
     s.stride = (size_t)((s.end - s.first + 3) & ~3);
+    const ScorePlan plan = head_dim == 64    ? score_plan<64>(s.rows)
+                           : head_dim == 128 ? score_plan<128>(s.rows)
+                           : head_dim == 256 ? score_plan<256>(s.rows)
+                                             : score_plan<512>(s.rows);
+    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(s.end - s.first, plan.keys * plan.groups);
+    s.splits = 2 * cu_count() / blocks;
+    if (s.splits > steps) s.splits = steps;
+    if (s.splits > kMaxSplits) s.splits = kMaxSplits;
+    if (s.splits < 1) s.splits = 1;
     const size_t scores = s.rows * s.stride, ml = (size_t)s.splits * s.rows * 2;
     void *mem = nullptr;
     if ((rc = g_weights_ws.get((scores + ml + weight_part_floats(s.rows, s.end - s.first)) * 4, &mem, who)))
       return rc;
     s.score = static_cast<float *>(mem);
     s.ml = reinterpret_cast<float2 *>(s.score + scores);
-    switch (head_dim) {
-      case 64: hipLaunchKernelGGL(scores_kernel<64>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      case 128: hipLaunchKernelGGL(scores_kernel<128>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      case 256: hipLaunchKernelGGL(scores_kernel<256>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-      default: hipLaunchKernelGGL(scores_kernel<512>, dim3(s.rows), dim3(256), 0, stream(), a); break;
-    }
+    hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(64 * kWaves), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");
     rc = launch_weights(s, keylen, s.score + scores + ml, r0 ? weights : before, weights);
     if (rc) return rc;

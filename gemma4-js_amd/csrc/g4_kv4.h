@@ -16,7 +16,7 @@ int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *w
 // from key on).
 struct Scores {
   float *score;
-  float2 *ml;  // [splits][rows]
+  float2 *ml;  // [rows][splits]
   size_t stride;
   int rows, heads, splits;
   int first, end, pos0, window;  // keys first .. end - 1 are seen by some row
