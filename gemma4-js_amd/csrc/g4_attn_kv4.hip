@@ -39,10 +39,18 @@ __device__ __forceinline__ Scale scale_pair(float a, float b) {
   const half2_t s = __builtin_convertvector((f32x2_t){a, b}, half2_t);
   return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}};
 }
+// (mask and exponent in registers, so that one instruction takes both)
+struct Magic {
+  uint32_t mask, exponent;
+  __device__ __forceinline__ Magic() {
+    asm("v_mov_b32 %0, 0x03c003c0" : "=v"(mask));
+    asm("s_mov_b32 %0, 0x4c004c00" : "=s"(exponent));
+  }
+};
 template <int T>
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, const Scale &x) {
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, const Scale &x, const Magic &mg) {
   const uint32_t sh = T == 0 ? w << 6 : T == 1 ? w << 2 : T == 2 ? w >> 2 : w >> 6;
-  const half2_t h = __builtin_bit_cast(half2_t, (sh & 0x03c003c0u) | 0x4c004c00u);
+  const half2_t h = __builtin_bit_cast(half2_t, (sh & mg.mask) | mg.exponent);
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(h, x.s, x.c));
 }
 
@@ -165,11 +173,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   // q: a thread takes 8 values of a row, whose largest gets the exponent 13
   {
     constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    constexpr int N = (R + PASS - 1) / PASS;
     const int wd = t % TW;
-    for (int r = t / TW; r < R; r += PASS) {
-      const int row = min(R0 + r, S.rows - 1);
+    f32x4 qx[N][2];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = min(R0 + min(t / TW + i * PASS, R - 1), S.rows - 1);
       const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 8 * wd);
-      const f32x4 x0 = p[0], x1 = p[1];
+      qx[i][0] = p[0];
+      qx[i][1] = p[1];
+    }
+#pragma unroll
+    for (int pass = 0; pass < N; ++pass) {
+      const int r = t / TW + pass * PASS;
+      const f32x4 x0 = qx[pass][0], x1 = qx[pass][1];
       int top = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -177,6 +194,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
       for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
       const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      if (r >= R) break;
       if (wd == 0) xq[r] = e - 21;  // (8 of the scales)
       u32x4 hi4, lo4;
 #pragma unroll
@@ -208,6 +226,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
+  const Magic mg;
   const int turns = (t1 - t0 + KG - 1) / KG;
   for (int it = 0; it < turns; ++it) {
     const int step = t0 + kg + it * KG, key0 = lo + step * kStep;
@@ -259,8 +278,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
           for (int T = 0; T < 2; ++T) {
             const uint32_t wd = kr[T][n];
             kv[T] = __builtin_bit_cast(
-                half8_t, (u32x4){value_pair<0>(wd, x[T]), value_pair<1>(wd, x[T]), value_pair<2>(wd, x[T]),
-                                 value_pair<3>(wd, x[T])});
+                half8_t, (u32x4){value_pair<0>(wd, x[T], mg), value_pair<1>(wd, x[T], mg), value_pair<2>(wd, x[T], mg),
+                                 value_pair<3>(wd, x[T], mg)});
           }
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
@@ -410,8 +429,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
           auto tile = [&](auto T) {
             constexpr int e = decltype(T)::value;
             const half8_t vv = __builtin_bit_cast(
-                half8_t, (u32x4){value_pair<e>(d[0], vx[0]), value_pair<e>(d[1], vx[1]), value_pair<e>(d[2], vx[2]),
-                                 value_pair<e>(d[3], vx[3])});
+                half8_t, (u32x4){value_pair<e>(d[0], vx[0], mg), value_pair<e>(d[1], vx[1], mg), value_pair<e>(d[2], vx[2], mg),
+                                 value_pair<e>(d[3], vx[3], mg)});
             const int n = 8 * i + 4 * h + e;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
