@@ -47,58 +47,94 @@ struct SumArgs {
   float *part;  // [groups][end - first], or null
 };
 
+constexpr int kBatch = 16;  // loads of a thread that are under way together
+
+// A thread per key adds up to 64 rows; blockIdx.y counts these groups.  The first rows' scores are
+// loaded before the rows' maxima and sums are known.
 __global__ __launch_bounds__(256) void weights_kernel(SumArgs a) {
-  __shared__ float2 stat[kGroup];  // maximum, 1 / sum
+  __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
   const Scores &s = a.s;
-  const int t = threadIdx.x, r0 = blockIdx.y * kGroup;
+  const int t = threadIdx.x, r0 = blockIdx.y * kGroup, n = min(kGroup, s.rows - r0);
   const int key = blockIdx.x * 256 + t + (a.part ? s.first : 0);
-  const int n = min(kGroup, s.rows - r0);
-  {
+  const bool any = key >= s.first && key < s.end;
+  const float *p = s.score + (size_t)r0 * s.stride + (any ? key - s.first : 0);
+  float x[kBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) x[i] = p[(size_t)min(i0 + i, n - 1) * s.stride];
+  };
+  const float before = !a.part && a.before && key < a.keylen ? a.before[key] : 0.f;
+  if (n > 0) {
+    load(0);
     int lanes = 4;  // per row
     while (lanes < 64 && lanes * 2 * n <= 256) lanes *= 2;
-    const int i = t / lanes;
-    const float2 *ml = s.ml + (size_t)(r0 + min(i, n - 1)) * s.splits;
+    const int i = t / lanes, row = r0 + min(i, n - 1);
+    const float2 *ml = s.ml + (size_t)row * s.splits;
     float m = kNoScore, l = 0.f;
-    for (int p = t % lanes; p < s.splits; p += lanes) {
-      const float2 x = ml[p];
-      const float mn = fmaxf(m, x.x);
-      l = l * __builtin_amdgcn_exp2f(m - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
+    for (int p0 = t % lanes; p0 < s.splits; p0 += 4 * lanes) {
+      float2 y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = ml[min(p0 + e * lanes, s.splits - 1)];
+      float mn = m;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mn = fmaxf(mn, y[e].x);
+      l *= __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (p0 + e * lanes < s.splits) l = fmaf(y[e].y, __builtin_amdgcn_exp2f(y[e].x - mn), l);
       m = mn;
     }
     for (int o = 1; o < lanes; o <<= 1) {
       const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
-      const float x = l * __builtin_amdgcn_exp2f(m - mn), y = l2 * __builtin_amdgcn_exp2f(m2 - mn);
-      l = (t & o) ? y + x : x + y;
+      const float u = l * __builtin_amdgcn_exp2f(m - mn), v = l2 * __builtin_amdgcn_exp2f(m2 - mn);
+      l = (t & o) ? v + u : u + v;
       m = mn;
     }
-    if (t % lanes == 0 && i < n) stat[i] = make_float2(m, 1.f / l);
+    if (t % lanes == 0 && i < n) {
+      const int pos = s.pos0 + row / s.heads;
+      stat[i] = make_float4(m, 1.f / l, __int_as_float(pos),
+                            __int_as_float(s.window > 0 ? pos - s.window : -1));
+    }
   }
   __syncthreads();
   float sum = 0.f;
-  if (key >= s.first && key < s.end) {
-    const float *p = s.score + (size_t)r0 * s.stride + (key - s.first);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const int pos = s.pos0 + (r0 + i) / s.heads;
-      const bool sees = key <= pos && (s.window == 0 || key > pos - s.window);
-      const float w = __builtin_amdgcn_exp2f(p[(size_t)i * s.stride] - stat[i].x) * stat[i].y;
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float4 st = stat[min(i0 + i, n - 1)];
+      const bool sees = i0 + i < n && key <= __float_as_int(st.z) && key > __float_as_int(st.w);
+      const float w = __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
       if (sees) sum += w;
     }
+    if (i0 + kBatch < n) load(i0 + kBatch);
   }
+  if (!any) sum = 0.f;
   if (a.part) {
-    if (key < s.end) a.part[(size_t)blockIdx.y * (s.end - s.first) + (key - s.first)] = sum;
+    if (any) a.part[(size_t)blockIdx.y * (s.end - s.first) + (key - s.first)] = sum;
   } else if (key < a.keylen) {
-    a.weights[key] = (a.before ? a.before[key] : 0.f) + sum;
+    a.weights[key] = before + sum;
   }
 }
 
-__global__ __launch_bounds__(256) void weights_join_kernel(SumArgs a, int groups) {
-  const int key = blockIdx.x * 256 + threadIdx.x;
+// Adds the groups of a key, 8 of them under way together.
+__global__ __launch_bounds__(64) void weights_join_kernel(SumArgs a, int groups) {
+  const int key = blockIdx.x * 64 + threadIdx.x;
   if (key >= a.keylen) return;
+  const float before = a.before ? a.before[key] : 0.f;
   float sum = 0.f;
-  if (key >= a.s.first && key < a.s.end)
-    for (int g = 0; g < groups; ++g) sum += a.part[(size_t)g * (a.s.end - a.s.first) + (key - a.s.first)];
-  a.weights[key] = (a.before ? a.before[key] : 0.f) + sum;
+  if (key >= a.s.first && key < a.s.end) {
+    const size_t step = a.s.end - a.s.first;
+    const float *p = a.part + (key - a.s.first);
+    for (int g = 0; g < groups; g += kBatch) {
+      float x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) x[i] = p[min(g + i, groups - 1) * step];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (g + i < groups) sum += x[i];
+    }
+  }
+  a.weights[key] = before + sum;
 }
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
@@ -116,7 +152,7 @@ int launch_weights(const Scores &s, int keylen, float *part, const float *before
                      stream(), a);
   G4_LAUNCH_CHECK("weights_kernel");
   if (!a.part) return G4_OK;
-  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen, 256)), dim3(256), 0, stream(), a, groups);
+  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen, 64)), dim3(64), 0, stream(), a, groups);
   G4_LAUNCH_CHECK("weights_join_kernel");
   return G4_OK;
 }
