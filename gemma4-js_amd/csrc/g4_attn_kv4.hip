@@ -16,6 +16,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
+constexpr float kSlack = 8.f;               // how far (log 2) a score may pass its row's reference
 constexpr int kStep = 32;                   // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kMaxSplits = 256;
@@ -76,6 +77,8 @@ __device__ __forceinline__ bool plain_scale(uint32_t bits) {
 }
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+// Rows of q whose exponent a factor of FP32 holds with all its bits.
+__device__ __forceinline__ bool usual_row(int e) { return e >= -120; }
 // 2^(8 - e) for -100 <= e <= 127
 __device__ __forceinline__ float pow2_8_minus(int e) { return __int_as_float((135 - e) << 23); }
 __device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7) - 127, -100); }
@@ -125,7 +128,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 
   uint32_t kr[2][KW], ksr[2][KS], vr[8][VW], vsr[8];
   auto load_k = [&](int step) {
-    const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * kStep), last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
     const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
 #pragma unroll
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     }
   };
   auto load_v = [&](int step) {
-    const int k0 = lo + min(step, steps - 1) * kStep, last = hi - 1 - k0;
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * kStep), last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
     const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
 #pragma unroll
@@ -169,6 +172,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   };
   load_k(t0 + kg);
   load_v(t0 + kg);
+  asm volatile("" ::: "memory");
 
   // q: a thread takes 8 values of a row, whose largest gets the exponent 13
   {
@@ -214,18 +218,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   __syncthreads();
 
   int pos[RT], xe[RT];
-  float m[RT], l[RT], E[RT];
+  float xf[RT], m[RT], l[RT], E[RT];
+  bool usual = true;
   f32x4 o[RT][VD];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     pos[r] = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
     xe[r] = xq[16 * r + c];
+    xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
+    usual = usual && usual_row(xe[r]);
     m[r] = kNoScore;
     l[r] = 0.f;
     E[r] = -1000.f;  // outputs are held times 2^(21 - E)
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
+  uint32_t none = 0;  // bit 4 r + v: register v of row tile r holds no numbers
   const Magic mg;
   const int turns = (t1 - t0 + KG - 1) / KG;
   for (int it = 0; it < turns; ++it) {
@@ -234,13 +242,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     // the keys' exponents, where a scale needs them
     uint32_t ke[2] = {0, 0};  // a byte each
     float kmul[2] = {256.f, 256.f};
+    bool kplain = usual;
     {
-      bool plain = true;
 #pragma unroll
       for (int T = 0; T < 2; ++T)
 #pragma unroll
-        for (int J = 0; J < KS; ++J) plain = plain && plain_scale(ksr[T][J]);
-      if (!__all(plain)) {
+        for (int J = 0; J < KS; ++J) kplain = kplain && plain_scale(ksr[T][J]);
+      kplain = __all(kplain);
+      if (!kplain) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
           int top = 0;
@@ -300,7 +309,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
         for (int T = 0; T < 2; ++T)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            s[r][T][i] = ldexpf((sh[r][T][i] + sl[r][T][i]) * kLog2e, xe[r] + byte_of(ke[T], i));
+            s[r][T][i] = (sh[r][T][i] + sl[r][T][i]) * xf[r];
+      if (!kplain) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[r][T][i] = ldexpf(s[r][T][i], (usual_row(xe[r]) ? 0 : xe[r]) + byte_of(ke[T], i));
+      }
     }
     load_k(step + KG);
     if constexpr (DQ > 1) {
@@ -378,10 +396,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
       }
       float tm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
       // (fmaxf drops a NaN score, whose weight is NaN.)
-      const float mn = fmaxf(m[r], group_max(tm));
+      tm = group_max(tm);
+      const float mn = tm > m[r] + kSlack ? tm : m[r];
       const float corr = __builtin_amdgcn_exp2f(m[r] - mn);
       float E2 = E[r] + fmaxf(ceilf(m[r] - mn), -1000.f);
-      float bound = 0.f;
+      float bound = kSlack;
       if (!vplain) {
         bound = -INFINITY;
 #pragma unroll
@@ -449,14 +468,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     if (!vplain && __any(odd != 0)) {  // rows that see such a key: NaN in its dims
 #pragma unroll
       for (int r = 0; r < RT; ++r)
-        for (int g2 = 0; g2 < 4; ++g2) {
-          const uint32_t sees = __shfl((int)seen[r], 16 * g2 + c, 64);
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (__shfl((int)odd, 16 * g2 + 4 * g + v, 64) & sees) {
-#pragma unroll
-              for (int n = 0; n < VD; ++n) o[r][n][v] = __int_as_float(0x7fc00000);
-            }
+        for (int i = 0; i < 16; ++i) {  // keys of lanes (., i / 4), dims of register i % 4
+          const uint32_t bad = (uint32_t)__shfl((int)odd, 16 * (i >> 2) + 4 * g + (i & 3), 64);
+          if (bad & (uint32_t)__shfl((int)seen[r], 16 * (i >> 2) + c, 64)) none |= 1u << (4 * r + (i & 3));
         }
     }
     load_v(step + KG);
@@ -487,7 +501,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     if (!whole && L == 0.f) f = 0.f;
     f = ldexpf(f, (int)E[r] - 21);
 #pragma unroll
-    for (int n = 0; n < VD; ++n) o[r][n] *= f;
+    for (int v = 0; v < 4; ++v) {
+      const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
+#pragma unroll
+      for (int n = 0; n < VD; ++n) o[r][n][v] *= fv;
+    }
     // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
     float *mine = &sm.o[c][dq * DW + 4 * g * VD];
 #pragma unroll
@@ -519,6 +537,426 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
         for (int n = 0; n < VD; n += 4)
           *reinterpret_cast<f32x4 *>(p + v * VD + n) =
               (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]};
+    }
+  }
+}
+
+// Many rows: a block owns 16 RT rows and a run of 32-key steps; its four waves share the head dim
+// both for the scores and for the outputs, so that each value of the cache is unpacked once for
+// all rows.  The waves' partial scores go through LDS; wave w < RT adds those of rows 16 w .. + 15, in
+// order, does their softmax and leaves the weights in LDS for all four.  The next step's scores are
+// formed beside the softmax.
+template <int HD, int RT>
+__global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_kernel(Kv4Args a) {
+  constexpr int DW = HD / kWaves, R = 16 * RT, NT = 2, KEYS = 16 * NT;
+  constexpr int KN = DW / 32;         // words of a key per lane, and products
+  constexpr int VD = DW / 16;         // dims per lane, and output tiles
+  static_assert(DW == 128 || DW == 64, "one scale of a key per lane");
+  __shared__ f32x4 sx[kWaves][RT][NT][64];
+  __shared__ u32x4 sp[NT / 2][RT][2][64];
+  __shared__ u32x4 sql[kWaves][KN][RT][64];  // q's lower parts, which no registers are left for
+  __shared__ float sf[R];
+  __shared__ int stop[kWaves][R];           // q's largest
+  __shared__ int sve[kWaves][KEYS];         // v's exponents, where not all scales are plain
+  __shared__ int splain[kWaves];
+  const Scores &S = a.s;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int R0 = blockIdx.x * R, split = blockIdx.y;
+  const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
+  int lo = S.first;
+  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
+  const int per = (steps + S.splits - 1) / S.splits;
+  const int t0 = split * per, t1 = min(t0 + per, steps);
+
+  uint32_t kr[NT][KN], ksr[NT], vr[NT / 2][8], vsr[NT / 2][8];
+  auto load_k = [&](int step) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + w * (DW / 2);
+    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16) + w * (DW / 16);
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      const uint32_t r = (uint32_t)min(16 * T + c, last);
+      if constexpr (DW == 128) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (r * (HD / 2) + g * 16));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kr[T][i] = x[i];
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p + (r * (HD / 2) + g * 8));
+        kr[T][0] = x.x;
+        kr[T][1] = x.y;
+      }
+      ksr[T] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + g * DW / 128 * 2));
+    }
+  };
+  auto load_v = [&](int step) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + w * (DW / 2);
+#pragma unroll
+    for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t r = (uint32_t)min(32 * b + 16 * (j >> 2) + 4 * g + (j & 3), last);
+        const char *pr = p + (r * (HD / 2) + c * (DW / 32));
+        if constexpr (DW == 128) vr[b][j] = *reinterpret_cast<const uint32_t *>(pr);
+        else vr[b][j] = *reinterpret_cast<const uint16_t *>(pr);
+      }
+  };
+  auto load_vs = [&](int step) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
+    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + w * (DW / 16);
+#pragma unroll
+    for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t r = (uint32_t)min(32 * b + 16 * (j >> 2) + 4 * g + (j & 3), last);
+        vsr[b][j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
+      }
+  };
+  load_k(t0);
+
+  // q: lane (c, g) holds its row's dims g DW / 4 + 8 n .. + 7 of the wave's
+  half8_t qh[RT][KN];
+  int xe[RT];
+  float xf[RT];
+  bool usual = true;
+  {
+    f32x4 x[RT][KN][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = min(R0 + 16 * r + c, S.rows - 1);
+      int top = 0;
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + w * DW + g * (DW / 4) + 8 * n);
+        x[r][n][0] = p[0];
+        x[r][n][1] = p[1];
+      }
+#pragma unroll
+      for (int n = 0; n < KN; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = max(top, max(__float_as_int(x[r][n][0][i]) & 0x7fffffff, __float_as_int(x[r][n][1][i]) & 0x7fffffff));
+      top = max(top, __shfl_xor(top, 16, 64));
+      top = max(top, __shfl_xor(top, 32, 64));
+      if (g == 0) stop[w][16 * r + c] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      int top = 0;
+#pragma unroll
+      for (int d = 0; d < kWaves; ++d) top = max(top, stop[d][16 * r + c]);
+      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      xe[r] = e - 21;  // (8 of the scales)
+      xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
+      usual = usual && usual_row(xe[r]);
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        u32x4 h4, l4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2_t z = {ldexpf(x[r][n][0][i], 13 - e), ldexpf(x[r][n][1][i], 13 - e)};
+          const half2_t h = __builtin_convertvector(z, half2_t);
+          h4[i] = __builtin_bit_cast(uint32_t, h);
+          l4[i] = __builtin_bit_cast(
+              uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
+        }
+        qh[r][n] = __builtin_bit_cast(half8_t, h4);
+        sql[w][n][r][lane] = l4;
+      }
+    }
+  }
+  const Magic mg;
+  // partial scores of a step, as they are (log 2 units)
+  f32x4 s[RT][NT];
+  auto scores = [&](int next) {
+    uint32_t ke[NT] = {};
+    float kmul[NT];
+    bool plain = true;
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      kmul[T] = 256.f;
+      plain = plain && plain_scale(ksr[T]);
+    }
+    plain = __all(plain && usual);
+    if (!plain) {
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        int top = (int)(ksr[T] & 0x7fffu);
+        top = max(top, __shfl_xor(top, 16, 64));
+        top = max(top, __shfl_xor(top, 32, 64));
+        const int e = min(scale_exponent(top), 127);
+        kmul[T] = pow2_8_minus(e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e, 4 * g + i, 64) & 255) << (8 * i);
+      }
+    }
+    Scale x[NT];
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      const float f = bf16_to_f32(ksr[T]) * kmul[T];
+      x[T] = scale_pair(f, f);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int n = 0; n < KN; ++n) {
+      half8_t ql[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) ql[r] = __builtin_bit_cast(half8_t, sql[w][n][r][lane]);
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        const uint32_t wd = kr[T][n];
+        const half8_t kv = __builtin_bit_cast(
+            half8_t, (u32x4){value_pair<0>(wd, x[T], mg), value_pair<1>(wd, x[T], mg), value_pair<2>(wd, x[T], mg),
+                             value_pair<3>(wd, x[T], mg)});
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[r][n], s[r][T], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[r], s[r][T], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_k(next);
+#pragma unroll
+    for (int T = 0; T < NT; ++T)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][T] *= xf[r];
+    if (!plain) {
+#pragma unroll
+      for (int T = 0; T < NT; ++T)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][T][i] = ldexpf(s[r][T][i], (usual_row(xe[r]) ? 0 : xe[r]) + byte_of(ke[T], i));
+    }
+  };
+
+  float m = kNoScore, l = 0.f, E = -1000.f;  // of row 16 w + c
+  uint32_t none = 0;  // bit 4 r + v: register v of row tile r holds no numbers
+  f32x4 o[RT][VD];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const int my_row = R0 + 16 * min(w, RT - 1) + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
+  if (t0 < t1) scores(t0 + 1);
+  load_vs(t0);
+  load_v(t0);
+  asm volatile("" ::: "memory");  // (else the loads move into the loop, with an address of 64 bits each)
+  for (int step = t0; step < t1; ++step) {
+    const int key0 = lo + step * KEYS;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int T = 0; T < NT; ++T) sx[w][r][T][lane] = s[r][T];
+    // v's exponents, of all waves where one has a scale that is not plain
+    uint32_t odd[NT / 2] = {};  // keys of which this lane's dims are no numbers
+    {
+      bool plain = true;
+#pragma unroll
+      for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) plain = plain && plain_scale(vsr[b][j]);
+      plain = __all(plain);
+      if (lane == 0) splain[w] = plain;
+      if (!plain) {
+#pragma unroll
+        for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((vsr[b][j] & 0x7fffu) >= 0x7f80u) {
+              odd[b] |= 1u << j;
+              vsr[b][j] = 0;
+            }
+      }
+#pragma unroll
+      for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (plain) continue;
+          const int e = scale_exponent(row_max((int)(vsr[b][j] & 0x7fffu)));
+          if (c == 0) sve[w][32 * b + 16 * (j >> 2) + 4 * g + (j & 3)] = e;
+        }
+      if (plain && lane < KEYS) sve[w][lane] = 0;
+    }
+    __syncthreads();
+    const bool plain = splain[0] && splain[1] && splain[2] && splain[3];
+    f32x4 x[NT];
+    // this wave's rows: the scores of the four, in order
+    if (w < RT) {
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        x[T] = sx[0][w][T][lane];
+#pragma unroll
+        for (int d = 1; d < kWaves; ++d) x[T] += sx[d][w][T][lane];
+      }
+    }
+    if (step + 1 < t1) scores(step + 2);
+    if (w < RT) {
+      const bool inner = key0 + KEYS - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
+      if (!inner) {
+#pragma unroll
+        for (int T = 0; T < NT; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * T + 4 * g + i;
+            if (key > my_pos || (S.window > 0 && key <= my_pos - S.window)) x[T][i] = -INFINITY;
+          }
+      }
+      if (S.score && my_row < S.rows) {
+#pragma unroll
+        for (int T = 0; T < NT; ++T) {
+          const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
+          if (at < S.stride)
+            *reinterpret_cast<float4 *>(S.score + (size_t)my_row * S.stride + at) =
+                make_float4(x[T][0], x[T][1], x[T][2], x[T][3]);
+        }
+      }
+      float tm = kNoScore;
+#pragma unroll
+      for (int T = 0; T < NT; ++T) tm = fmaxf(tm, fmaxf(fmaxf(x[T][0], x[T][1]), fmaxf(x[T][2], x[T][3])));
+      // (fmaxf drops a NaN score, whose weight is NaN.)
+      tm = group_max(tm);
+      const float mn = tm > m + kSlack ? tm : m;
+      const float corr = __builtin_amdgcn_exp2f(m - mn);
+      float E2 = E + fmaxf(ceilf(m - mn), -1000.f), bound = kSlack;
+      uint32_t ve[NT] = {};  // a byte each
+      if (!plain) {
+        bound = -INFINITY;
+#pragma unroll
+        for (int T = 0; T < NT; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 16 * T + 4 * g + i;
+            const int e = max(max(sve[0][at], sve[1][at]), max(sve[2][at], sve[3][at]));
+            ve[T] |= (uint32_t)(e & 255) << (8 * i);
+            bound = fmaxf(bound, (float)e + ceilf(x[T][i] - mn));
+          }
+        bound = group_max(bound);
+      }
+      E2 = fmaxf(fmaxf(E2, bound), -1000.f);
+      const int up = 13 - (int)E2;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < NT / 2; ++b) {
+        u32x4 h4, l4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int T = 2 * b + (j >> 1), i = 2 * (j & 1);
+          const float p0 = __builtin_amdgcn_exp2f(x[T][i] - mn), p1 = __builtin_amdgcn_exp2f(x[T][i + 1] - mn);
+          sum += p0;
+          sum += p1;
+          const f32x2_t z = {ldexpf(p0, up + byte_of(ve[T], i)), ldexpf(p1, up + byte_of(ve[T], i + 1))};
+          const half2_t h = __builtin_convertvector(z, half2_t);
+          h4[j] = __builtin_bit_cast(uint32_t, h);
+          l4[j] = __builtin_bit_cast(
+              uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
+        }
+        sp[b][w][0][lane] = h4;
+        sp[b][w][1][lane] = l4;
+      }
+      l = fmaf(l, corr, sum);
+      if (g == 0) sf[16 * w + c] = ldexpf(corr, (int)(E - E2));
+      m = mn;
+      E = E2;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float f = sf[16 * r + c];
+      if (__any(f != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < VD; ++n) o[r][n] *= f;
+      }
+    }
+    Scale vx[NT / 2][4];
+#pragma unroll
+    for (int b = 0; b < NT / 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f0 = 256.f, f1 = 256.f;
+        if (!plain) {
+          const int at = 32 * b + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
+          f0 = pow2_8_minus(max(max(sve[0][at], sve[1][at]), max(sve[2][at], sve[3][at])));
+          f1 = pow2_8_minus(max(max(sve[0][at + 1], sve[1][at + 1]), max(sve[2][at + 1], sve[3][at + 1])));
+        }
+        vx[b][j] = scale_pair(bf16_to_f32(vsr[b][2 * j]) * f0, bf16_to_f32(vsr[b][2 * j + 1]) * f1);
+      }
+    load_vs(step + 1);  // (which the next step looks at first)
+#pragma unroll
+    for (int b = 0; b < NT / 2; ++b) {
+      half8_t ph[RT], pl[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        ph[r] = __builtin_bit_cast(half8_t, sp[b][r][0][lane]);
+        pl[r] = __builtin_bit_cast(half8_t, sp[b][r][1][lane]);
+      }
+#pragma unroll
+      for (int h = 0; h < VD / 4; ++h) {
+        uint32_t d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          d[j] = __builtin_amdgcn_perm(vr[b][2 * j + 1], vr[b][2 * j], h ? 0x07060302u : 0x05040100u);
+        auto tile = [&](auto T) {
+          constexpr int e = decltype(T)::value;
+          const half8_t vv = __builtin_bit_cast(
+              half8_t, (u32x4){value_pair<e>(d[0], vx[b][0], mg), value_pair<e>(d[1], vx[b][1], mg),
+                               value_pair<e>(d[2], vx[b][2], mg), value_pair<e>(d[3], vx[b][3], mg)});
+          const int n = 4 * h + e;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
+        };
+        tile(std::integral_constant<int, 0>());
+        tile(std::integral_constant<int, 1>());
+        tile(std::integral_constant<int, 2>());
+        tile(std::integral_constant<int, 3>());
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (__any(odd[0] != 0)) {  // rows that see such a key: NaN in its dims
+      for (int i = 0; i < 16 * NT / 2; ++i) {  // keys of lanes (., i / 4 % 4), dims of register i % 4
+        const uint32_t bad = (uint32_t)__shfl((int)odd[i >> 4], 16 * (i >> 2 & 3) + 4 * g + (i & 3), 64);
+        for (int j = 0; j < 8; ++j) {
+          const int key = key0 + 32 * (i >> 4) + 16 * (j >> 2) + 4 * (i >> 2 & 3) + (j & 3);
+          for (int r = 0; r < RT; ++r) {
+            const int pos = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
+            if ((bad >> j & 1) && key <= pos && (S.window == 0 || key > pos - S.window)) none |= 1u << (4 * r + (i & 3));
+          }
+        }
+      }
+    }
+    load_v(step + 1);
+  }
+
+  const bool whole = S.splits == 1;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (S.ml && w < RT && g == 0 && my_row < S.rows) S.ml[(size_t)my_row * S.splits + split] = make_float2(m, l);
+  // (a split of which the row sees nothing: 0, not 0 / 0)
+  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)E - 21);
+  __syncthreads();  // (sf is read to the last step's end)
+  if (w < RT && g == 0) sf[16 * w + c] = fin;
+  __syncthreads();
+  float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = R0 + 16 * r + c;
+    if (row >= S.rows) continue;
+    const float f = sf[16 * r + c];
+    // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
+    float *p = out + (size_t)row * HD + w * DW + 4 * g * VD;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
+#pragma unroll
+      for (int n = 0; n < VD; n += 4)
+        *reinterpret_cast<f32x4 *>(p + v * VD + n) =
+            (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * fv;
     }
   }
 }
@@ -567,19 +1005,62 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
   reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[blockIdx.y * U + u] = y;
 }
 
+// The same for up to 8 splits of many rows: a thread per 16-byte unit.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
+  constexpr int MOST = 8;
+  const Scores &S = a.s;
+  const size_t unit = (size_t)blockIdx.x * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
+  if (unit >= units) return;
+  const float2 *ml = S.ml + unit / (HD / 4) * S.splits;
+  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part) + unit;
+  f32x4 x[MOST];
+  float e[MOST];
+  float M = kNoScore, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    x[i] = p[min(i, S.splits - 1) * units];
+    M = fmaxf(M, ml[min(i, S.splits - 1)].x);
+  }
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const float2 z = ml[min(i, S.splits - 1)];
+    e[i] = i < S.splits ? z.y * __builtin_amdgcn_exp2f(z.x - M) : 0.f;
+    L += e[i];
+  }
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) y += e[i] * x[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] /= L;
+  reinterpret_cast<f32x4 *>(a.y)[unit] = y;
+}
+
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 Workspace g_kv4_ws;
 
-// n query rows from row0 on; `before` and `weights` of this call.
-template <int HD, int RT>
+// The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per CU.
+struct Plan {
+  void (*kernel)(Kv4Args);
+  int rows, keys, per_cu;
+};
+template <int HD>
+Plan plan_of(int rows) {
+  if (rows <= 16) return {attn_kv4_kernel<HD, 1>, 16, kStep * kGroups<HD>, 2};
+  if constexpr (HD >= 256) return {attn_kv4_rows_kernel<HD, 2>, 32, 32, 2};
+  else return {attn_kv4_kernel<HD, 2>, 32, kStep * kGroups<HD>, 2};
+}
+
+// The rows of a.s, all at once; `before` and `weights` of this call.
+template <int HD>
 int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   Scores &s = a.s;
-  const int blocks = cdiv(s.rows, 16 * RT);
-  const int keys = s.window > 0 ? min(s.end - s.first, s.window + 16 * RT) : s.end - s.first;
-  const int steps = cdiv(keys, kStep);
-  int splits = 2 * cu_count() / blocks;
-  if (splits > cdiv(steps, kGroups<HD>)) splits = cdiv(steps, kGroups<HD>);
+  const Plan plan = plan_of<HD>(s.rows);
+  const int blocks = cdiv(s.rows, plan.rows);
+  const int keys = s.window > 0 ? min(s.end - s.first, s.window + plan.rows) : s.end - s.first;
+  int splits = plan.per_cu * cu_count() / blocks;
+  if (splits > cdiv(keys, plan.keys)) splits = cdiv(keys, plan.keys);
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 1) splits = 1;
   s.splits = splits;
@@ -594,20 +1075,18 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     s.score = weights ? a.part + n_part : nullptr;
     s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
   }
-  hipLaunchKernelGGL((attn_kv4_kernel<HD, RT>), dim3(blocks, splits), dim3(64 * kWaves), 0, stream(), a);
+  hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(64 * kWaves), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
   if (splits > 1) {
-    hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 64), dim3(256), 0, stream(), a);
+    if (s.rows >= 64 && splits <= 8)
+      hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3((unsigned)(((size_t)s.rows * (HD / 4) + 255) / 256)), dim3(256),
+                         0, stream(), a);
+    else
+      hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 64), dim3(256), 0, stream(), a);
     G4_LAUNCH_CHECK("attn_kv4_merge_kernel");
   }
   if (!weights) return G4_OK;
   return launch_weights(s, keylen, a.part + n_part + n_score + n_ml, before, weights);
-}
-
-template <int HD>
-int launch_hd(const Kv4Args &a, int keylen, const float *before, float *weights) {
-  return a.s.rows <= 16 ? launch_rows<HD, 1>(a, keylen, before, weights)
-                        : launch_rows<HD, 2>(a, keylen, before, weights);
 }
 
 }  // namespace
@@ -661,10 +1140,10 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
     s.stride = (size_t)((s.end - s.first + 3) & ~3);
     const float *b = r0 ? weights : before;
     switch (head_dim) {
-      case 64: rc = launch_hd<64>(a, keylen, b, weights); break;
-      case 128: rc = launch_hd<128>(a, keylen, b, weights); break;
-      case 256: rc = launch_hd<256>(a, keylen, b, weights); break;
-      default: rc = launch_hd<512>(a, keylen, b, weights); break;
+      case 64: rc = launch_rows<64>(a, keylen, b, weights); break;
+      case 128: rc = launch_rows<128>(a, keylen, b, weights); break;
+      case 256: rc = launch_rows<256>(a, keylen, b, weights); break;
+      default: rc = launch_rows<512>(a, keylen, b, weights); break;
     }
     if (rc) return rc;
   }
