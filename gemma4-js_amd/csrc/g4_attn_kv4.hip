@@ -28,6 +28,9 @@ struct Kv4Args {
   float *y;
   float *part;  // [splits][rows][hd], each split's outputs
   Scores s;     // score null: not kept
+  // attn_kv4_rows_kernel's row blocks to do again, marked with the call
+  uint32_t *redo, call;
+  int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
 // Eight values of a cache as FP16, in pairs (0, 4) (1, 5) (2, 6) (3, 7) of the word's nibbles or of
@@ -70,10 +73,11 @@ __device__ __forceinline__ int row_max(int v) {
   return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
 }
 
+constexpr uint32_t kLeastScale = (127 - 12) << 7, kPlainScales = 15 << 7;
 // Scales within these bounds (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
 // exponent of their row's largest taken out, which then goes to the score or the weight.
 __device__ __forceinline__ bool plain_scale(uint32_t bits) {
-  return (bits & 0x7fffu) - (uint32_t)((127 - 12) << 7) < (uint32_t)(15 << 7);
+  return (bits & 0x7fffu) - kLeastScale < kPlainScales;
 }
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
@@ -118,6 +122,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
+  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] != a.call) return;
   // the rows' positions, and the keys that some of them see
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
   int lo = S.first;
@@ -541,24 +546,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   }
 }
 
-// Many rows: a block owns 16 RT rows and a run of 32-key steps; its four waves share the head dim
-// both for the scores and for the outputs, so that each value of the cache is unpacked once for
-// all rows.  The waves' partial scores go through LDS; wave w < RT adds those of rows 16 w .. + 15, in
-// order, does their softmax and leaves the weights in LDS for all four.  The next step's scores are
-// formed beside the softmax.
-template <int HD, int RT>
-__global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_kernel(Kv4Args a) {
-  constexpr int DW = HD / kWaves, R = 16 * RT, NT = 2, KEYS = 16 * NT;
+// Many rows of a cache whose scales all are plain: a block owns 16 RT rows and a run of 32-key steps;
+// its W waves share the head dim both for the scores and for the outputs, so that each value of the
+// cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave w < RT adds
+// those of rows 16 w .. + 15, in order, does their softmax and leaves the weights in LDS for all.
+// The next step's scores are formed before, so that one barrier per step makes both known.
+// A block that meets another scale (or a q below 2^-99) says so in `redo`, and attn_kv4_kernel does
+// its rows again.
+template <int HD, int RT, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
+  constexpr int DW = HD / W, R = 16 * RT, NT = 2, KEYS = 16 * NT;
   constexpr int KN = DW / 32;         // words of a key per lane, and products
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
   static_assert(DW == 128 || DW == 64, "one scale of a key per lane");
-  __shared__ f32x4 sx[kWaves][RT][NT][64];
-  __shared__ u32x4 sp[NT / 2][RT][2][64];
-  __shared__ u32x4 sql[kWaves][KN][RT][64];  // q's lower parts, which no registers are left for
-  __shared__ float sf[R];
-  __shared__ int stop[kWaves][R];           // q's largest
-  __shared__ int sve[kWaves][KEYS];         // v's exponents, where not all scales are plain
-  __shared__ int splain[kWaves];
+  // (two of each: what the step's readers may still look at, and the next)
+  __shared__ f32x4 sx[2][W][RT][NT][64];
+  __shared__ u32x4 sp[2][RT][2][64];
+  __shared__ float sf[2][R];
+  __shared__ int stop[W][R], sxq[R];  // q's largest, q's exponents
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -569,8 +574,9 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
   const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
   const int per = (steps + S.splits - 1) / S.splits;
   const int t0 = split * per, t1 = min(t0 + per, steps);
+  uint32_t beyond = 0;  // the scales' largest distance from the least plain one
 
-  uint32_t kr[NT][KN], ksr[NT], vr[NT / 2][8], vsr[NT / 2][8];
+  uint32_t kr[NT][KN], ksr[NT], vr[8], vsr[8];
   auto load_k = [&](int step) {
     const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + w * (DW / 2);
@@ -594,33 +600,26 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
     const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + w * (DW / 2);
 #pragma unroll
-    for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t r = (uint32_t)min(32 * b + 16 * (j >> 2) + 4 * g + (j & 3), last);
-        const char *pr = p + (r * (HD / 2) + c * (DW / 32));
-        if constexpr (DW == 128) vr[b][j] = *reinterpret_cast<const uint32_t *>(pr);
-        else vr[b][j] = *reinterpret_cast<const uint16_t *>(pr);
-      }
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
+      const char *pr = p + (r * (HD / 2) + c * (DW / 32));
+      if constexpr (DW == 128) vr[j] = *reinterpret_cast<const uint32_t *>(pr);
+      else vr[j] = *reinterpret_cast<const uint16_t *>(pr);
+    }
   };
   auto load_vs = [&](int step) {
     const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
     const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + w * (DW / 16);
 #pragma unroll
-    for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t r = (uint32_t)min(32 * b + 16 * (j >> 2) + 4 * g + (j & 3), last);
-        vsr[b][j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
-      }
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
+      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
+    }
   };
   load_k(t0);
 
   // q: lane (c, g) holds its row's dims g DW / 4 + 8 n .. + 7 of the wave's
-  half8_t qh[RT][KN];
-  int xe[RT];
-  float xf[RT];
-  bool usual = true;
+  half8_t qh[RT][KN], ql[RT][KN];
   {
     f32x4 x[RT][KN][2];
 #pragma unroll
@@ -647,11 +646,10 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
     for (int r = 0; r < RT; ++r) {
       int top = 0;
 #pragma unroll
-      for (int d = 0; d < kWaves; ++d) top = max(top, stop[d][16 * r + c]);
+      for (int d = 0; d < W; ++d) top = max(top, stop[d][16 * r + c]);
       const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
-      xe[r] = e - 21;  // (8 of the scales)
-      xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
-      usual = usual && usual_row(xe[r]);
+      if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of the scales)
+      beyond = max(beyond, usual_row(e - 21) ? 0u : ~0u);
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         u32x4 h4, l4;
@@ -664,48 +662,25 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
               uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
         }
         qh[r][n] = __builtin_bit_cast(half8_t, h4);
-        sql[w][n][r][lane] = l4;
+        ql[r][n] = __builtin_bit_cast(half8_t, l4);
       }
     }
   }
   const Magic mg;
-  // partial scores of a step, as they are (log 2 units)
-  f32x4 s[RT][NT];
-  auto scores = [&](int next) {
-    uint32_t ke[NT] = {};
-    float kmul[NT];
-    bool plain = true;
-#pragma unroll
-    for (int T = 0; T < NT; ++T) {
-      kmul[T] = 256.f;
-      plain = plain && plain_scale(ksr[T]);
-    }
-    plain = __all(plain && usual);
-    if (!plain) {
-#pragma unroll
-      for (int T = 0; T < NT; ++T) {
-        int top = (int)(ksr[T] & 0x7fffu);
-        top = max(top, __shfl_xor(top, 16, 64));
-        top = max(top, __shfl_xor(top, 32, 64));
-        const int e = min(scale_exponent(top), 127);
-        kmul[T] = pow2_8_minus(e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e, 4 * g + i, 64) & 255) << (8 * i);
-      }
-    }
+  // partial scores of a step into LDS
+  auto scores = [&](int step) {
     Scale x[NT];
+    f32x4 s[RT][NT];
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
-      const float f = bf16_to_f32(ksr[T]) * kmul[T];
+      beyond = max(beyond, ksr[T] - kLeastScale);
+      const float f = bf16_to_f32(ksr[T]) * 256.f;
       x[T] = scale_pair(f, f);
 #pragma unroll
       for (int r = 0; r < RT; ++r) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
-    for (int n = 0; n < KN; ++n) {
-      half8_t ql[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) ql[r] = __builtin_bit_cast(half8_t, sql[w][n][r][lane]);
+    for (int n = 0; n < KN; ++n)
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
         const uint32_t wd = kr[T][n];
@@ -713,89 +688,45 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
             half8_t, (u32x4){value_pair<0>(wd, x[T], mg), value_pair<1>(wd, x[T], mg), value_pair<2>(wd, x[T], mg),
                              value_pair<3>(wd, x[T], mg)});
 #pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[r][n], s[r][T], 0, 0, 0);
+#pragma unroll
         for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[r][n], s[r][T], 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[r], s[r][T], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    load_k(next);
+    load_k(step + 1);
 #pragma unroll
-    for (int T = 0; T < NT; ++T)
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) s[r][T] *= xf[r];
-    if (!plain) {
-#pragma unroll
-      for (int T = 0; T < NT; ++T)
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][T][i] = ldexpf(s[r][T][i], (usual_row(xe[r]) ? 0 : xe[r]) + byte_of(ke[T], i));
-    }
+      for (int T = 0; T < NT; ++T) sx[(step - t0) & 1][w][r][T][lane] = s[r][T];
   };
 
-  float m = kNoScore, l = 0.f, E = -1000.f;  // of row 16 w + c
-  uint32_t none = 0;  // bit 4 r + v: register v of row tile r holds no numbers
-  f32x4 o[RT][VD];
+  float m = kNoScore, l = 0.f;  // of row 16 w + c
+  f32x4 o[RT][VD];              // outputs times 2^(21 - kSlack)
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int my_row = R0 + 16 * min(w, RT - 1) + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
-  if (t0 < t1) scores(t0 + 1);
   load_vs(t0);
   load_v(t0);
-  asm volatile("" ::: "memory");  // (else the loads move into the loop, with an address of 64 bits each)
+  __syncthreads();
+  const float my_factor = ldexpf(kLog2e, sxq[16 * min(w, RT - 1) + c]);
+  if (t0 < t1) scores(t0);
+  asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
+  __syncthreads();
   for (int step = t0; step < t1; ++step) {
-    const int key0 = lo + step * KEYS;
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int T = 0; T < NT; ++T) sx[w][r][T][lane] = s[r][T];
-    // v's exponents, of all waves where one has a scale that is not plain
-    uint32_t odd[NT / 2] = {};  // keys of which this lane's dims are no numbers
-    {
-      bool plain = true;
-#pragma unroll
-      for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) plain = plain && plain_scale(vsr[b][j]);
-      plain = __all(plain);
-      if (lane == 0) splain[w] = plain;
-      if (!plain) {
-#pragma unroll
-        for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((vsr[b][j] & 0x7fffu) >= 0x7f80u) {
-              odd[b] |= 1u << j;
-              vsr[b][j] = 0;
-            }
-      }
-#pragma unroll
-      for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (plain) continue;
-          const int e = scale_exponent(row_max((int)(vsr[b][j] & 0x7fffu)));
-          if (c == 0) sve[w][32 * b + 16 * (j >> 2) + 4 * g + (j & 3)] = e;
-        }
-      if (plain && lane < KEYS) sve[w][lane] = 0;
-    }
-    __syncthreads();
-    const bool plain = splain[0] && splain[1] && splain[2] && splain[3];
-    f32x4 x[NT];
-    // this wave's rows: the scores of the four, in order
+    const int key0 = lo + step * KEYS, at = (step - t0) & 1;
+    if (step + 1 < t1) scores(step + 1);
     if (w < RT) {
+      // this wave's rows: the scores of all, in order
+      float x[NT][4];
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
-        x[T] = sx[0][w][T][lane];
+        f32x4 y = sx[at][0][w][T][lane];
 #pragma unroll
-        for (int d = 1; d < kWaves; ++d) x[T] += sx[d][w][T][lane];
+        for (int d = 1; d < W; ++d) y += sx[at][d][w][T][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[T][i] = y[i] * my_factor;
       }
-    }
-    if (step + 1 < t1) scores(step + 2);
-    if (w < RT) {
       const bool inner = key0 + KEYS - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
       if (!inner) {
 #pragma unroll
@@ -809,10 +740,10 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
       if (S.score && my_row < S.rows) {
 #pragma unroll
         for (int T = 0; T < NT; ++T) {
-          const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
-          if (at < S.stride)
-            *reinterpret_cast<float4 *>(S.score + (size_t)my_row * S.stride + at) =
-                make_float4(x[T][0], x[T][1], x[T][2], x[T][3]);
+          const size_t to = (size_t)(key0 + 16 * T + 4 * g - S.first);
+          if (to < S.stride)
+            *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + to) =
+                (f32x4){x[T][0], x[T][1], x[T][2], x[T][3]};
         }
       }
       float tm = kNoScore;
@@ -822,142 +753,97 @@ __global__ __launch_bounds__(64 * kWaves, RT > 2 ? 1 : 2) void attn_kv4_rows_ker
       tm = group_max(tm);
       const float mn = tm > m + kSlack ? tm : m;
       const float corr = __builtin_amdgcn_exp2f(m - mn);
-      float E2 = E + fmaxf(ceilf(m - mn), -1000.f), bound = kSlack;
-      uint32_t ve[NT] = {};  // a byte each
-      if (!plain) {
-        bound = -INFINITY;
-#pragma unroll
-        for (int T = 0; T < NT; ++T)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = 16 * T + 4 * g + i;
-            const int e = max(max(sve[0][at], sve[1][at]), max(sve[2][at], sve[3][at]));
-            ve[T] |= (uint32_t)(e & 255) << (8 * i);
-            bound = fmaxf(bound, (float)e + ceilf(x[T][i] - mn));
-          }
-        bound = group_max(bound);
-      }
-      E2 = fmaxf(fmaxf(E2, bound), -1000.f);
-      const int up = 13 - (int)E2;
       float sum = 0.f;
+      u32x4 h4, l4;
 #pragma unroll
-      for (int b = 0; b < NT / 2; ++b) {
-        u32x4 h4, l4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int T = 2 * b + (j >> 1), i = 2 * (j & 1);
-          const float p0 = __builtin_amdgcn_exp2f(x[T][i] - mn), p1 = __builtin_amdgcn_exp2f(x[T][i + 1] - mn);
-          sum += p0;
-          sum += p1;
-          const f32x2_t z = {ldexpf(p0, up + byte_of(ve[T], i)), ldexpf(p1, up + byte_of(ve[T], i + 1))};
-          const half2_t h = __builtin_convertvector(z, half2_t);
-          h4[j] = __builtin_bit_cast(uint32_t, h);
-          l4[j] = __builtin_bit_cast(
-              uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
-        }
-        sp[b][w][0][lane] = h4;
-        sp[b][w][1][lane] = l4;
+      for (int j = 0; j < 4; ++j) {
+        const int T = j >> 1, i = 2 * (j & 1);
+        const float p0 = __builtin_amdgcn_exp2f(x[T][i] - mn), p1 = __builtin_amdgcn_exp2f(x[T][i + 1] - mn);
+        sum += p0;
+        sum += p1;
+        const f32x2_t z = {p0 * 32.f, p1 * 32.f};  // 2^(13 - kSlack)
+        const half2_t h = __builtin_convertvector(z, half2_t);
+        h4[j] = __builtin_bit_cast(uint32_t, h);
+        l4[j] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
       }
+      sp[at][w][0][lane] = h4;
+      sp[at][w][1][lane] = l4;
       l = fmaf(l, corr, sum);
-      if (g == 0) sf[16 * w + c] = ldexpf(corr, (int)(E - E2));
+      if (g == 0) sf[at][16 * w + c] = corr;
       m = mn;
-      E = E2;
     }
+    Scale vx[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      beyond = max(beyond, max(vsr[2 * j] - kLeastScale, vsr[2 * j + 1] - kLeastScale));
+      vx[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * 256.f, bf16_to_f32(vsr[2 * j + 1]) * 256.f);
+    }
+    load_vs(step + 1);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float f = sf[16 * r + c];
+      const float f = sf[at][16 * r + c];
       if (__any(f != 1.f)) {
 #pragma unroll
         for (int n = 0; n < VD; ++n) o[r][n] *= f;
       }
     }
-    Scale vx[NT / 2][4];
+    half8_t ph[RT], pl[RT];
 #pragma unroll
-    for (int b = 0; b < NT / 2; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f0 = 256.f, f1 = 256.f;
-        if (!plain) {
-          const int at = 32 * b + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-          f0 = pow2_8_minus(max(max(sve[0][at], sve[1][at]), max(sve[2][at], sve[3][at])));
-          f1 = pow2_8_minus(max(max(sve[0][at + 1], sve[1][at + 1]), max(sve[2][at + 1], sve[3][at + 1])));
-        }
-        vx[b][j] = scale_pair(bf16_to_f32(vsr[b][2 * j]) * f0, bf16_to_f32(vsr[b][2 * j + 1]) * f1);
-      }
-    load_vs(step + 1);  // (which the next step looks at first)
-#pragma unroll
-    for (int b = 0; b < NT / 2; ++b) {
-      half8_t ph[RT], pl[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        ph[r] = __builtin_bit_cast(half8_t, sp[b][r][0][lane]);
-        pl[r] = __builtin_bit_cast(half8_t, sp[b][r][1][lane]);
-      }
-#pragma unroll
-      for (int h = 0; h < VD / 4; ++h) {
-        uint32_t d[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          d[j] = __builtin_amdgcn_perm(vr[b][2 * j + 1], vr[b][2 * j], h ? 0x07060302u : 0x05040100u);
-        auto tile = [&](auto T) {
-          constexpr int e = decltype(T)::value;
-          const half8_t vv = __builtin_bit_cast(
-              half8_t, (u32x4){value_pair<e>(d[0], vx[b][0], mg), value_pair<e>(d[1], vx[b][1], mg),
-                               value_pair<e>(d[2], vx[b][2], mg), value_pair<e>(d[3], vx[b][3], mg)});
-          const int n = 4 * h + e;
-#pragma unroll
-          for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
-        };
-        tile(std::integral_constant<int, 0>());
-        tile(std::integral_constant<int, 1>());
-        tile(std::integral_constant<int, 2>());
-        tile(std::integral_constant<int, 3>());
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int r = 0; r < RT; ++r) {
+      ph[r] = __builtin_bit_cast(half8_t, sp[at][r][0][lane]);
+      pl[r] = __builtin_bit_cast(half8_t, sp[at][r][1][lane]);
     }
-    if (__any(odd[0] != 0)) {  // rows that see such a key: NaN in its dims
-      for (int i = 0; i < 16 * NT / 2; ++i) {  // keys of lanes (., i / 4 % 4), dims of register i % 4
-        const uint32_t bad = (uint32_t)__shfl((int)odd[i >> 4], 16 * (i >> 2 & 3) + 4 * g + (i & 3), 64);
-        for (int j = 0; j < 8; ++j) {
-          const int key = key0 + 32 * (i >> 4) + 16 * (j >> 2) + 4 * (i >> 2 & 3) + (j & 3);
-          for (int r = 0; r < RT; ++r) {
-            const int pos = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
-            if ((bad >> j & 1) && key <= pos && (S.window == 0 || key > pos - S.window)) none |= 1u << (4 * r + (i & 3));
-          }
-        }
-      }
+#pragma unroll
+    for (int h = 0; h < VD / 4; ++h) {
+      uint32_t d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = __builtin_amdgcn_perm(vr[2 * j + 1], vr[2 * j], h ? 0x07060302u : 0x05040100u);
+      auto tile = [&](auto T) {
+        constexpr int e = decltype(T)::value;
+        const half8_t vv = __builtin_bit_cast(
+            half8_t, (u32x4){value_pair<e>(d[0], vx[0], mg), value_pair<e>(d[1], vx[1], mg),
+                             value_pair<e>(d[2], vx[2], mg), value_pair<e>(d[3], vx[3], mg)});
+        const int n = 4 * h + e;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
+      };
+      tile(std::integral_constant<int, 0>());
+      tile(std::integral_constant<int, 1>());
+      tile(std::integral_constant<int, 2>());
+      tile(std::integral_constant<int, 3>());
     }
     load_v(step + 1);
   }
 
+  // (q's below the usual are all waves' matter, and rows that lie behind their split's keys too)
+  if (__any(beyond >= kPlainScales) && lane == 0) a.redo[blockIdx.x] = a.call;
   const bool whole = S.splits == 1;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (S.ml && w < RT && g == 0 && my_row < S.rows) S.ml[(size_t)my_row * S.splits + split] = make_float2(m, l);
   // (a split of which the row sees nothing: 0, not 0 / 0)
-  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)E - 21);
+  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 21);
   __syncthreads();  // (sf is read to the last step's end)
-  if (w < RT && g == 0) sf[16 * w + c] = fin;
+  if (w < RT && g == 0) sf[0][16 * w + c] = fin;
   __syncthreads();
   float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int row = R0 + 16 * r + c;
     if (row >= S.rows) continue;
-    const float f = sf[16 * r + c];
+    const float f = sf[0][16 * r + c];
     // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
     float *p = out + (size_t)row * HD + w * DW + 4 * g * VD;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
       for (int n = 0; n < VD; n += 4)
         *reinterpret_cast<f32x4 *>(p + v * VD + n) =
-            (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * fv;
-    }
+            (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * f;
   }
 }
 
@@ -1038,18 +924,22 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-Workspace g_kv4_ws;
+Workspace g_kv4_ws, g_redo_ws;
+uint32_t g_call = 0;
 
-// The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per CU.
+// The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per
+// CU and threads.
 struct Plan {
   void (*kernel)(Kv4Args);
-  int rows, keys, per_cu;
+  void (*again)(Kv4Args);  // of 32 rows per block, where the first one may leave some undone
+  int rows, keys, per_cu, threads;
 };
 template <int HD>
 Plan plan_of(int rows) {
-  if (rows <= 16) return {attn_kv4_kernel<HD, 1>, 16, kStep * kGroups<HD>, 2};
-  if constexpr (HD >= 256) return {attn_kv4_rows_kernel<HD, 2>, 32, 32, 2};
-  else return {attn_kv4_kernel<HD, 2>, 32, kStep * kGroups<HD>, 2};
+  if (rows <= 16) return {attn_kv4_kernel<HD, 1>, nullptr, 16, kStep * kGroups<HD>, 2, 64 * kWaves};
+  if constexpr (HD == 512) return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2>, 64, 32, 1, 512};
+  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 4, 4>, attn_kv4_kernel<HD, 2>, 64, 32, 1, 256};
+  else return {attn_kv4_kernel<HD, 2>, nullptr, 32, kStep * kGroups<HD>, 2, 64 * kWaves};
 }
 
 // The rows of a.s, all at once; `before` and `weights` of this call.
@@ -1075,8 +965,21 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     s.score = weights ? a.part + n_part : nullptr;
     s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
   }
-  hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(64 * kWaves), 0, stream(), a);
+  if (plan.again) {
+    // (a recording keeps its number: a block that one replay marked is done again by all, which
+    // changes nothing but the time)
+    void *mem = nullptr;
+    if (int rc = g_redo_ws.get((size_t)blocks * 4, &mem, "g4_attention_kv4")) return rc;
+    a.redo = static_cast<uint32_t *>(mem);
+    a.call = ++g_call;
+  }
+  hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(plan.threads), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
+  if (plan.again) {
+    a.redo_rows = plan.rows;
+    hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 32), splits), dim3(64 * kWaves), 0, stream(), a);
+    G4_LAUNCH_CHECK("attn_kv4_kernel");
+  }
   if (splits > 1) {
     if (s.rows >= 64 && splits <= 8)
       hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3((unsigned)(((size_t)s.rows * (HD / 4) + 255) / 256)), dim3(256),
