@@ -13,6 +13,7 @@ namespace {
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
@@ -33,6 +34,9 @@ struct Kv4Args {
   int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
+// BF16 bits of the least plain scale, 2^-12, and how many there are, below 8.
+constexpr uint16_t kLeastScale = (127 - 12) << 7, kPlainScales = 15 << 7;
+
 // Eight values of a cache as FP16, in pairs (0, 4) (1, 5) (2, 6) (3, 7) of the word's nibbles or of
 // two words' halves: a nibble n in the mantissa's upper four bits under the exponent of 16 is
 // 16 + n, and (16 + n) s - 24 s = (n - 8) s is exact in one fused step: s has 8 bits, 24 s 10.
@@ -51,6 +55,16 @@ struct Magic {
     asm("s_mov_b32 %0, 0x4c004c00" : "=s"(exponent));
   }
 };
+// The same for two BF16 scales as they are: FP16 bits by whole numbers, and how far they lie from the
+// least plain one, kept as the largest seen (a plain scale times 2^8 is a normal FP16 number).
+__device__ __forceinline__ Scale plain_pair(uint32_t lo, uint32_t hi, ushort2_t &beyond) {
+  const ushort2_t u = __builtin_bit_cast(ushort2_t, __builtin_amdgcn_perm(hi, lo, 0x05040100u));
+  const ushort2_t d = u - (ushort2_t){kLeastScale, kLeastScale};
+  beyond = __builtin_elementwise_max(beyond, d);
+  constexpr uint16_t least = (kLeastScale - ((127 - 8 - 15) << 7)) << 3;
+  const half2_t s = __builtin_bit_cast(half2_t, (ushort2_t)(d * (ushort2_t){8, 8} + (ushort2_t){least, least}));
+  return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}};
+}
 template <int T>
 __device__ __forceinline__ uint32_t value_pair(uint32_t w, const Scale &x, const Magic &mg) {
   const uint32_t sh = T == 0 ? w << 6 : T == 1 ? w << 2 : T == 2 ? w >> 2 : w >> 6;
@@ -73,11 +87,10 @@ __device__ __forceinline__ int row_max(int v) {
   return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
 }
 
-constexpr uint32_t kLeastScale = (127 - 12) << 7, kPlainScales = 15 << 7;
-// Scales within these bounds (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
+// Plain scales (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
 // exponent of their row's largest taken out, which then goes to the score or the weight.
 __device__ __forceinline__ bool plain_scale(uint32_t bits) {
-  return (bits & 0x7fffu) - kLeastScale < kPlainScales;
+  return (bits & 0x7fffu) - (uint32_t)kLeastScale < kPlainScales;
 }
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
@@ -575,6 +588,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   __shared__ f32x4 sx[2][W][RT][NT][64];
   __shared__ u32x4 sp[2][RT][2][64];
   __shared__ float sf[2][R];
+  __shared__ int smoved[2][4];        // whether some row's reference moved
+  static_assert(RT <= 4, "a flag per row tile");
   __shared__ int stop[W][R], sxq[R];  // q's largest, q's exponents
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -586,7 +601,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
   const int per = (steps + S.splits - 1) / S.splits;
   const int t0 = split * per, t1 = min(t0 + per, steps);
-  uint32_t beyond = 0;  // the scales' largest distance from the least plain one
+  ushort2_t beyond = {0, 0};  // the scales' largest distance from the least plain one
 
   uint32_t kr[NT][KN], ksr[NT], vr[8], vsr[8];
   auto load_k = [&](int step) {
@@ -661,7 +676,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       for (int d = 0; d < W; ++d) top = max(top, stop[d][16 * r + c]);
       const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of the scales)
-      beyond = max(beyond, usual_row(e - 21) ? 0u : ~0u);
+      if (!usual_row(e - 21)) beyond = (ushort2_t){0xffff, 0xffff};
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         u32x4 h4, l4;
@@ -685,9 +700,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
     f32x4 s[RT][NT];
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
-      beyond = max(beyond, ksr[T] - kLeastScale);
-      const float f = bf16_to_f32(ksr[T]) * 256.f;
-      x[T] = scale_pair(f, f);
+      x[T] = plain_pair(ksr[T], ksr[T], beyond);
 #pragma unroll
       for (int r = 0; r < RT; ++r) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -784,29 +797,31 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       sp[at][w][1][lane] = l4;
       l = fmaf(l, corr, sum);
       if (g == 0) sf[at][16 * w + c] = corr;
+      const bool moved = __any(corr != 1.f);
+      if (lane == 0) smoved[at][w] = moved;
       m = mn;
     }
     Scale vx[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      beyond = max(beyond, max(vsr[2 * j] - kLeastScale, vsr[2 * j + 1] - kLeastScale));
-      vx[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * 256.f, bf16_to_f32(vsr[2 * j + 1]) * 256.f);
-    }
+    for (int j = 0; j < 4; ++j) vx[j] = plain_pair(vsr[2 * j], vsr[2 * j + 1], beyond);
     load_vs(step + 1);
     __syncthreads();
+    int moved = 0;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const float f = sf[at][16 * r + c];
-      if (__any(f != 1.f)) {
-#pragma unroll
-        for (int n = 0; n < VD; ++n) o[r][n] *= f;
-      }
-    }
+    for (int r = 0; r < RT; ++r) moved |= smoved[at][r];
     half8_t ph[RT], pl[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       ph[r] = __builtin_bit_cast(half8_t, sp[at][r][0][lane]);
       pl[r] = __builtin_bit_cast(half8_t, sp[at][r][1][lane]);
+    }
+    if (__builtin_amdgcn_readfirstlane(moved)) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float f = sf[at][16 * r + c];
+#pragma unroll
+        for (int n = 0; n < VD; ++n) o[r][n] *= f;
+      }
     }
 #pragma unroll
     for (int h = 0; h < VD / 4; ++h) {
@@ -834,7 +849,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   }
 
   // (q's below the usual are all waves' matter, and rows that lie behind their split's keys too)
-  if (__any(beyond >= kPlainScales) && lane == 0) a.redo[blockIdx.x] = a.call;
+  if (__any(max(beyond[0], beyond[1]) >= kPlainScales) && lane == 0) a.redo[blockIdx.x] = a.call;
   const bool whole = S.splits == 1;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -905,10 +920,10 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
   reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[blockIdx.y * U + u] = y;
 }
 
-// The same for up to 8 splits of many rows: a thread per 16-byte unit.
+// The same for up to 16 splits of many rows: a thread per 16-byte unit.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
-  constexpr int MOST = 8;
+  constexpr int MOST = 16;
   const Scores &S = a.s;
   const size_t unit = (size_t)blockIdx.x * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
   if (unit >= units) return;
@@ -995,7 +1010,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     G4_LAUNCH_CHECK("attn_kv4_kernel");
   }
   if (splits > 1) {
-    if (s.rows >= 64 && splits <= 8)
+    if (s.rows >= 64 && splits <= 16)
       hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3((unsigned)(((size_t)s.rows * (HD / 4) + 255) / 256)), dim3(256),
                          0, stream(), a);
     else

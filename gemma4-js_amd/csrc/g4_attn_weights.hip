@@ -36,7 +36,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
-constexpr int kGroup = 64;                  // rows that a block adds up
+constexpr int kGroup = 32;                  // rows that a block adds up
 constexpr int kMaxSplits = 512;
 
 struct SumArgs {
@@ -49,7 +49,7 @@ struct SumArgs {
 
 constexpr int kBatch = 16;  // loads of a thread that are under way together
 
-// A thread per key adds up to 64 rows; blockIdx.y counts these groups.  The first rows' scores are
+// A thread per key adds up to 32 rows; blockIdx.y counts these groups.  The first rows' scores are
 // loaded before the rows' maxima and sums are known.
 __global__ __launch_bounds__(256) void weights_kernel(SumArgs a) {
   __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
@@ -168,6 +168,9 @@ constexpr int kWaves = 4;
 struct ScoreArgs {
   const float *q, *k;
   Scores s;
+  // scores_rows_kernel's row blocks to do again, marked with the call
+  uint32_t *redo, call;
+  int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
 // Eight FP32 values, times `up`, as sums of two FP16 values.
@@ -214,6 +217,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
+  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] != a.call) return;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
   int lo = S.first;
   if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
@@ -403,19 +407,200 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   }
 }
 
-// The plan's shape: rows per block, keys per step, key groups.
+// Many rows: a block owns 16 RT rows and a run of 32-key steps; its W waves share the head dim, so that
+// each k is split into its two values once for all rows, with q in registers.  The waves' partial
+// scores go through LDS; wave w adds those of rows 16 (w % RT) .. and, of these, keys 16 (w / RT) ..
+// in order and keeps the running maximum and sum of its own.  A block in which a key's largest value
+// is outside 2^-10 .. 2^7 (times 2^8: 2^-2 .. 2^15) or a q below 2^-99 says so in `redo`, and
+// scores_kernel does its rows again.
+template <int HD, int RT, int W>
+__global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
+  constexpr int DW = HD / W, KN = DW / 32, R = 16 * RT, NT = W / RT, KEYS = 16 * NT;
+  static_assert(W % RT == 0, "a tile per wave");
+  __shared__ f32x4 sx[2][W][RT][NT][64];
+  __shared__ float stop[2][W][KEYS];  // the keys' largest values
+  __shared__ int sq[W][R], sxq[R];    // q's largest, q's exponents
+  __shared__ float2 wml[NT][R];
+  const Scores &S = a.s;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  int R0 = blockIdx.x * R, split = blockIdx.y;
+  if (S.splits % 8 == 0) {  // blocks are dealt to the 8 XCDs in turn: a split's to one, whose L2 holds its keys
+    const int b = blockIdx.y * gridDim.x + blockIdx.x, n = b / 8;
+    split = n / (int)gridDim.x * 8 + b % 8;
+    R0 = n % (int)gridDim.x * R;
+  }
+  const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
+  int lo = S.first;
+  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
+  const int per = (steps + S.splits - 1) / S.splits;
+  const int t0 = split * per, t1 = min(t0 + per, steps);
+  bool fits = true;
+
+  f32x4 kr[NT][KN][2];
+  auto load_k = [&](int step) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
+    const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + w * DW);
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 8 * g) * 4;
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        kr[T][n][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
+        kr[T][n][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
+      }
+    }
+  };
+  load_k(t0);
+  // q: lane (c, g) holds its row's dims 32 n + 8 g .. + 7 of the wave's
+  half8_t qh[RT][KN], ql[RT][KN];
+  {
+    f32x4 x[RT][KN][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = min(R0 + 16 * r + c, S.rows - 1);
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + w * DW + 32 * n + 8 * g);
+        x[r][n][0] = p[0];
+        x[r][n][1] = p[1];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      int top = 0;  // as bits, where NaN > infinity > numbers
+#pragma unroll
+      for (int n = 0; n < KN; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = max(top, max(__float_as_int(x[r][n][0][i]) & 0x7fffffff, __float_as_int(x[r][n][1][i]) & 0x7fffffff));
+      top = max(top, __shfl_xor(top, 16, 64));
+      top = max(top, __shfl_xor(top, 32, 64));
+      if (g == 0) sq[w][16 * r + c] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      int top = 0;
+#pragma unroll
+      for (int d = 0; d < W; ++d) top = max(top, sq[d][16 * r + c]);
+      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of k's)
+      fits = fits && e >= -99;
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        f32x4 x0 = x[r][n][0], x1 = x[r][n][1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x0[i] = ldexpf(x0[i], 13 - e), x1[i] = ldexpf(x1[i], 13 - e);
+        halves(x0, x1, 1.f, qh[r][n], ql[r][n]);
+      }
+    }
+  }
+  auto scores = [&](int step) {
+    f32x4 s[RT][NT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int T = 0; T < NT; ++T) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int at = (step - t0) & 1;
+#pragma unroll
+    for (int T = 0; T < NT; ++T) {
+      float top = 0.f;
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        half8_t kh, kl;
+        top = fmaxf(top, largest(kr[T][n][0], kr[T][n][1]));
+        halves(kr[T][n][0], kr[T][n][1], 256.f, kh, kl);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[r][n], s[r][T], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[r][n], s[r][T], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[r][n], s[r][T], 0, 0, 0);
+      }
+      top = group_max(top);
+      if (g == 0) stop[at][w][16 * T + c] = top;
+    }
+    load_k(step + 1);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int T = 0; T < NT; ++T) sx[at][w][r][T][lane] = s[r][T];
+  };
+
+  // this wave's rows and keys
+  const int mr = w % RT, mt = w / RT;
+  const int my_row = R0 + 16 * mr + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
+  float m = kNoScore, l = 0.f;
+  if (t0 < t1) scores(t0);
+  asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
+  __syncthreads();
+  const float factor = ldexpf(kLog2e, sxq[16 * mr + c]);
+  for (int step = t0; step < t1; ++step) {
+    const int key0 = lo + step * KEYS, at = (step - t0) & 1;
+    if (step + 1 < t1) scores(step + 1);
+    f32x4 x = sx[at][0][mr][mt][lane];
+#pragma unroll
+    for (int d = 1; d < W; ++d) x += sx[at][d][mr][mt][lane];
+    x *= factor;
+    if (lane < KEYS) {
+      float top = stop[at][0][lane];
+#pragma unroll
+      for (int d = 1; d < W; ++d) top = fmaxf(top, stop[at][d][lane]);
+      // (keys without numbers give scores that are none either way)
+      fits = fits && (top == 0.f || (top >= 0x1p-10f && top < 128.f) || !(top < INFINITY));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = key0 + 16 * mt + 4 * g + i;
+      if (key > my_pos || (S.window > 0 && key <= my_pos - S.window)) x[i] = -INFINITY;
+    }
+    const size_t to = (size_t)(key0 + 16 * mt + 4 * g - S.first);
+    if (my_row < S.rows && to < S.stride) *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + to) = x;
+    // (fmaxf drops a NaN score, whose weight is NaN; a lane's maximum is its own until the end)
+    const float mn = fmaxf(fmaxf(fmaxf(m, x[0]), fmaxf(x[1], x[2])), x[3]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(x[i] - mn);
+    l = fmaf(l, __builtin_amdgcn_exp2f(m - mn), sum);
+    m = mn;
+    __syncthreads();
+  }
+  if (!__all(fits) && lane == 0) a.redo[R0 / R] = a.call;
+  const float M = group_max(m);
+  l *= __builtin_amdgcn_exp2f(m - M);
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) wml[mt][16 * mr + c] = make_float2(M, l);
+  __syncthreads();
+  if (t < R && R0 + t < S.rows) {
+    float Mx = kNoScore, L = 0.f;
+    for (int i = 0; i < NT; ++i) Mx = fmaxf(Mx, wml[i][t].x);
+    for (int i = 0; i < NT; ++i) L = fmaf(wml[i][t].y, __builtin_amdgcn_exp2f(wml[i][t].x - Mx), L);
+    S.ml[(size_t)(R0 + t) * S.splits + split] = make_float2(Mx, L);
+  }
+}
+
+// The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per CU
+// and threads.
 struct ScorePlan {
   void (*kernel)(ScoreArgs);
-  int rows, keys, groups;
+  void (*again)(ScoreArgs);  // of 64 rows per block, where the first one may leave some undone
+  int rows, keys, per_cu, threads;
 };
 template <int HD>
 ScorePlan score_plan(int rows) {
   constexpr int DQ = HD >= 128 ? HD / 128 : 1;
-  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, 16, 16, kWaves / DQ};
-  return {scores_kernel<HD, 1, 2, 4>, 64, 32, kWaves};
+  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, nullptr, 16, 16 * kWaves / DQ, 2, 64 * kWaves};
+  if constexpr (HD == 512)
+    return {scores_rows_kernel<HD, 4, 8>, scores_kernel<HD, 1, 2, 4>, 64, 32, 1, 512};
+  else
+    return {scores_kernel<HD, 1, 2, 4>, nullptr, 64, 32 * kWaves, 2, 64 * kWaves};
 }
 
-Workspace g_weights_ws;
+Workspace g_weights_ws, g_score_redo_ws;
+uint32_t g_score_call = 0;
 
 }  // namespace
 }  // namespace g4
@@ -463,10 +648,11 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
                            : head_dim == 128 ? score_plan<128>(s.rows)
                            : head_dim == 256 ? score_plan<256>(s.rows)
                                              : score_plan<512>(s.rows);
-    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(s.end - s.first, plan.keys * plan.groups);
-    s.splits = 2 * cu_count() / blocks;
+    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(s.end - s.first, plan.keys);
+    s.splits = plan.per_cu * cu_count() / blocks;
     if (s.splits > steps) s.splits = steps;
     if (s.splits > kMaxSplits) s.splits = kMaxSplits;
+    if (plan.again && s.splits > 8 && s.splits % 8 <= s.splits / 8) s.splits = s.splits / 8 * 8;
     if (s.splits < 1) s.splits = 1;
     const size_t scores = s.rows * s.stride, ml = (size_t)s.splits * s.rows * 2;
     void *mem = nullptr;
@@ -474,8 +660,21 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
       return rc;
     s.score = static_cast<float *>(mem);
     s.ml = reinterpret_cast<float2 *>(s.score + scores);
-    hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(64 * kWaves), 0, stream(), a);
+    if (plan.again) {
+      // (a recording keeps its number: a block that one replay marked is done again by all, which
+      // changes nothing but the time)
+      void *redo = nullptr;
+      if ((rc = g_score_redo_ws.get((size_t)blocks * 4, &redo, who))) return rc;
+      a.redo = static_cast<uint32_t *>(redo);
+      a.call = ++g_score_call;
+    }
+    hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(plan.threads), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");
+    if (plan.again) {
+      a.redo_rows = plan.rows;
+      hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 64), s.splits), dim3(64 * kWaves), 0, stream(), a);
+      G4_LAUNCH_CHECK("scores_kernel");
+    }
     rc = launch_weights(s, keylen, s.score + scores + ml, r0 ? weights : before, weights);
     if (rc) return rc;
   }
