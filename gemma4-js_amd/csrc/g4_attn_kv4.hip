@@ -254,6 +254,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   uint32_t none = 0;  // bit 4 r + v: register v of row tile r holds no numbers
   const Magic mg;
   const int turns = (t1 - t0 + KG - 1) / KG;
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the waits in the loop then count its own loads
   for (int it = 0; it < turns; ++it) {
     const int step = t0 + kg + it * KG, key0 = lo + step * kStep;
     const bool mine = step < t1;
@@ -738,6 +739,9 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const float my_factor = ldexpf(kLog2e, sxq[16 * min(w, RT - 1) + c]);
   if (t0 < t1) scores(t0);
   asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
+  // Everything loaded so far has to be there: a wait in the loop counts the loads behind the one it
+  // is for, and would count by the loop's entry, where k's are the last, in every turn.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   for (int step = t0; step < t1; ++step) {
     const int key0 = lo + step * KEYS, at = (step - t0) & 1;

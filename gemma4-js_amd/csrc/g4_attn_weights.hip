@@ -535,6 +535,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   float m = kNoScore, l = 0.f;
   if (t0 < t1) scores(t0);
   asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the waits in the loop then count its own loads
   __syncthreads();
   const float factor = ldexpf(kLog2e, sxq[16 * mr + c]);
   for (int step = t0; step < t1; ++step) {
