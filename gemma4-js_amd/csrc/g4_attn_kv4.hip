@@ -586,8 +586,14 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
   static_assert(DW == 128 || DW == 64, "one scale of a key per lane");
   // (two of each: what the step's readers may still look at, and the next)
-  __shared__ f32x4 sx[2][W][RT][NT][64];
-  __shared__ u32x4 sp[2][RT][2][64];
+  union Smem {
+    struct {
+      f32x4 sx[2][W][RT][NT][64];
+      u32x4 sp[2][RT][2][64];
+    };
+    float rows[R][HD + 4];  // q and the outputs, on their way from and to whole lines of memory
+  };
+  __shared__ Smem sm;
   __shared__ float sf[2][R];
   __shared__ int smoved[2][4];        // whether some row's reference moved
   static_assert(RT <= 4, "a flag per row tile");
@@ -649,14 +655,26 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   // q: lane (c, g) holds its row's dims g DW / 4 + 8 n .. + 7 of the wave's
   half8_t qh[RT][KN], ql[RT][KN];
   {
+    constexpr int U = R * HD / 4 / (64 * W);
+    f32x4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = t + 64 * W * i, row = min(R0 + u / (HD / 4), S.rows - 1);
+      y[i] = *reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + u % (HD / 4) * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = t + 64 * W * i;
+      *reinterpret_cast<f32x4 *>(&sm.rows[u / (HD / 4)][u % (HD / 4) * 4]) = y[i];
+    }
+    __syncthreads();
     f32x4 x[RT][KN][2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int row = min(R0 + 16 * r + c, S.rows - 1);
       int top = 0;
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + w * DW + g * (DW / 4) + 8 * n);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + g * (DW / 4) + 8 * n]);
         x[r][n][0] = p[0];
         x[r][n][1] = p[1];
       }
@@ -723,7 +741,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) sx[(step - t0) & 1][w][r][T][lane] = s[r][T];
+      for (int T = 0; T < NT; ++T) sm.sx[(step - t0) & 1][w][r][T][lane] = s[r][T];
   };
 
   float m = kNoScore, l = 0.f;  // of row 16 w + c
@@ -751,9 +769,9 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       float x[NT][4];
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
-        f32x4 y = sx[at][0][w][T][lane];
+        f32x4 y = sm.sx[at][0][w][T][lane];
 #pragma unroll
-        for (int d = 1; d < W; ++d) y += sx[at][d][w][T][lane];
+        for (int d = 1; d < W; ++d) y += sm.sx[at][d][w][T][lane];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[T][i] = y[i] * my_factor;
       }
@@ -797,8 +815,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
         l4[j] = __builtin_bit_cast(
             uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
       }
-      sp[at][w][0][lane] = h4;
-      sp[at][w][1][lane] = l4;
+      sm.sp[at][w][0][lane] = h4;
+      sm.sp[at][w][1][lane] = l4;
       l = fmaf(l, corr, sum);
       if (g == 0) sf[at][16 * w + c] = corr;
       const bool moved = __any(corr != 1.f);
@@ -816,8 +834,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
     half8_t ph[RT], pl[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      ph[r] = __builtin_bit_cast(half8_t, sp[at][r][0][lane]);
-      pl[r] = __builtin_bit_cast(half8_t, sp[at][r][1][lane]);
+      ph[r] = __builtin_bit_cast(half8_t, sm.sp[at][r][0][lane]);
+      pl[r] = __builtin_bit_cast(half8_t, sm.sp[at][r][1][lane]);
     }
     if (__builtin_amdgcn_readfirstlane(moved)) {
 #pragma unroll
@@ -866,17 +884,21 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int row = R0 + 16 * r + c;
-    if (row >= S.rows) continue;
     const float f = sf[0][16 * r + c];
     // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
-    float *p = out + (size_t)row * HD + w * DW + 4 * g * VD;
 #pragma unroll
     for (int v = 0; v < 4; ++v)
 #pragma unroll
       for (int n = 0; n < VD; n += 4)
-        *reinterpret_cast<f32x4 *>(p + v * VD + n) =
+        *reinterpret_cast<f32x4 *>(&sm.rows[16 * r + c][w * DW + (4 * g + v) * VD + n]) =
             (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]} * f;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int u = t; u < R * HD / 4; u += 64 * W) {
+    const int row = u / (HD / 4), d = u % (HD / 4) * 4;
+    if (R0 + row < S.rows)
+      *reinterpret_cast<f32x4 *>(out + (size_t)(R0 + row) * HD + d) = *reinterpret_cast<const f32x4 *>(&sm.rows[row][d]);
   }
 }
 

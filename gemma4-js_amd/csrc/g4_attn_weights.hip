@@ -417,7 +417,11 @@ template <int HD, int RT, int W>
 __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   constexpr int DW = HD / W, KN = DW / 32, R = 16 * RT, NT = W / RT, KEYS = 16 * NT;
   static_assert(W % RT == 0, "a tile per wave");
-  __shared__ f32x4 sx[2][W][RT][NT][64];
+  union Smem {
+    f32x4 sx[2][W][RT][NT][64];
+    float rows[R][HD + 4];  // q, on its way from whole lines of memory
+  };
+  __shared__ Smem sm;
   __shared__ float stop[2][W][KEYS];  // the keys' largest values
   __shared__ int sq[W][R], sxq[R];    // q's largest, q's exponents
   __shared__ float2 wml[NT][R];
@@ -456,13 +460,25 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   // q: lane (c, g) holds its row's dims 32 n + 8 g .. + 7 of the wave's
   half8_t qh[RT][KN], ql[RT][KN];
   {
+    constexpr int U = R * HD / 4 / (64 * W);
+    f32x4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = t + 64 * W * i, row = min(R0 + u / (HD / 4), S.rows - 1);
+      y[i] = *reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + u % (HD / 4) * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = t + 64 * W * i;
+      *reinterpret_cast<f32x4 *>(&sm.rows[u / (HD / 4)][u % (HD / 4) * 4]) = y[i];
+    }
+    __syncthreads();
     f32x4 x[RT][KN][2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int row = min(R0 + 16 * r + c, S.rows - 1);
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + w * DW + 32 * n + 8 * g);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + 32 * n + 8 * g]);
         x[r][n][0] = p[0];
         x[r][n][1] = p[1];
       }
@@ -526,7 +542,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) sx[at][w][r][T][lane] = s[r][T];
+      for (int T = 0; T < NT; ++T) sm.sx[at][w][r][T][lane] = s[r][T];
   };
 
   // this wave's rows and keys
@@ -541,9 +557,9 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   for (int step = t0; step < t1; ++step) {
     const int key0 = lo + step * KEYS, at = (step - t0) & 1;
     if (step + 1 < t1) scores(step + 1);
-    f32x4 x = sx[at][0][mr][mt][lane];
+    f32x4 x = sm.sx[at][0][mr][mt][lane];
 #pragma unroll
-    for (int d = 1; d < W; ++d) x += sx[at][d][mr][mt][lane];
+    for (int d = 1; d < W; ++d) x += sm.sx[at][d][mr][mt][lane];
     x *= factor;
     if (lane < KEYS) {
       float top = stop[at][0][lane];
