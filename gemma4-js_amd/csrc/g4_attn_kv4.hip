@@ -404,13 +404,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
         }
       }
       const int row = R0 + 16 * r + c;
-      if (S.score && mine && dq == 0 && row < S.rows) {
+      if (S.score && mine && dq == 0) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-          const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
-          if (at < S.stride)
-            *reinterpret_cast<float4 *>(S.score + (size_t)row * S.stride + at) =
-                make_float4(x[4 * T], x[4 * T + 1], x[4 * T + 2], x[4 * T + 3]);
+          *reinterpret_cast<float4 *>(S.score + (size_t)row * S.stride + (key0 + 16 * T + 4 * g - S.first)) =
+              make_float4(x[4 * T], x[4 * T + 1], x[4 * T + 2], x[4 * T + 3]);
         }
       }
       float tm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -785,14 +783,11 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
             if (key > my_pos || (S.window > 0 && key <= my_pos - S.window)) x[T][i] = -INFINITY;
           }
       }
-      if (S.score && my_row < S.rows) {
+      if (S.score) {
 #pragma unroll
-        for (int T = 0; T < NT; ++T) {
-          const size_t to = (size_t)(key0 + 16 * T + 4 * g - S.first);
-          if (to < S.stride)
-            *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + to) =
-                (f32x4){x[T][0], x[T][1], x[T][2], x[T][3]};
-        }
+        for (int T = 0; T < NT; ++T)
+          *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + (key0 + 16 * T + 4 * g - S.first)) =
+              (f32x4){x[T][0], x[T][1], x[T][2], x[T][3]};
       }
       float tm = kNoScore;
 #pragma unroll
@@ -1011,7 +1006,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   s.splits = splits;
   const bool ml = weights || splits > 1;
   const size_t n_part = splits > 1 ? (size_t)splits * s.rows * HD : 0, n_ml = ml ? (size_t)splits * s.rows * 2 : 0;
-  const size_t n_score = weights ? s.rows * s.stride : 0;
+  const size_t n_score = weights ? score_floats(s.rows, s.stride) : 0;
   const size_t n_sum = weights ? weight_part_floats(s.rows, s.end - s.first) : 0;
   if (n_part + n_ml + n_score + n_sum) {
     void *mem = nullptr;
@@ -1095,7 +1090,7 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
     s.window = win;
     s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
     s.end = s.pos0 + n;
-    s.stride = (size_t)((s.end - s.first + 3) & ~3);
+    s.stride = score_stride(s.end - s.first);
     const float *b = r0 ? weights : before;
     switch (head_dim) {
       case 64: rc = launch_rows<64>(a, keylen, b, weights); break;

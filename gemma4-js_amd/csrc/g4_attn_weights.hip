@@ -141,6 +141,8 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace
 
+size_t score_stride(int keys) { return (size_t)((keys + 3) & ~3) + 32; }
+size_t score_floats(int rows, size_t stride) { return (size_t)((rows + 63) & ~63) * stride; }
 size_t weight_part_floats(int rows, int keys) {
   return rows > kGroup ? (size_t)cdiv(rows, kGroup) * keys : 0;
 }
@@ -376,8 +378,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
       float tm = kNoScore;
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
-        const size_t at = (size_t)(key0 + 16 * T + 4 * g - S.first);
-        if (row < S.rows && at < S.stride) *reinterpret_cast<f32x4 *>(S.score + (size_t)row * S.stride + at) = s[r][T];
+        *reinterpret_cast<f32x4 *>(S.score + (size_t)row * S.stride + (key0 + 16 * T + 4 * g - S.first)) = s[r][T];
         tm = fmaxf(tm, fmaxf(fmaxf(s[r][T][0], s[r][T][1]), fmaxf(s[r][T][2], s[r][T][3])));
       }
       // (fmaxf drops a NaN score, whose weight is NaN.)
@@ -442,8 +443,11 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const int t0 = split * per, t1 = min(t0 + per, steps);
   bool fits = true;
 
-  f32x4 kr[NT][KN][2];
-  auto load_k = [&](int step) {
+  struct Keys {
+    f32x4 x[NT][KN][2];
+  };
+  Keys ka, kb;  // of the next step and the one after it
+  auto load_k = [&](int step, Keys &kr) {
     const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + w * DW);
 #pragma unroll
@@ -451,12 +455,12 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 8 * g) * 4;
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
-        kr[T][n][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
-        kr[T][n][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
+        kr.x[T][n][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
+        kr.x[T][n][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
       }
     }
   };
-  load_k(t0);
+  load_k(t0, ka);
   // q: lane (c, g) holds its row's dims 32 n + 8 g .. + 7 of the wave's
   half8_t qh[RT][KN], ql[RT][KN];
   {
@@ -513,7 +517,9 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       }
     }
   }
-  auto scores = [&](int step) {
+  auto scores = [&](int step, const Keys &kr, Keys &next) {
+    load_k(step + 1, next);
+    __builtin_amdgcn_sched_barrier(0);  // (before this step's are split)
     f32x4 s[RT][NT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -526,8 +532,8 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         half8_t kh, kl;
-        top = fmaxf(top, largest(kr[T][n][0], kr[T][n][1]));
-        halves(kr[T][n][0], kr[T][n][1], 256.f, kh, kl);
+        top = fmaxf(top, largest(kr.x[T][n][0], kr.x[T][n][1]));
+        halves(kr.x[T][n][0], kr.x[T][n][1], 256.f, kh, kl);
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[r][n], s[r][T], 0, 0, 0);
 #pragma unroll
@@ -538,7 +544,6 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       top = group_max(top);
       if (g == 0) stop[at][w][16 * T + c] = top;
     }
-    load_k(step + 1);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -549,14 +554,14 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const int mr = w % RT, mt = w / RT;
   const int my_row = R0 + 16 * mr + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
   float m = kNoScore, l = 0.f;
-  if (t0 < t1) scores(t0);
+  if (t0 < t1) scores(t0, ka, kb);
   asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the waits in the loop then count its own loads
   __syncthreads();
   const float factor = ldexpf(kLog2e, sxq[16 * mr + c]);
-  for (int step = t0; step < t1; ++step) {
+  auto turn = [&](int step, const Keys &kr, Keys &next) {
     const int key0 = lo + step * KEYS, at = (step - t0) & 1;
-    if (step + 1 < t1) scores(step + 1);
+    if (step + 1 < t1) scores(step + 1, kr, next);
     f32x4 x = sm.sx[at][0][mr][mt][lane];
 #pragma unroll
     for (int d = 1; d < W; ++d) x += sm.sx[at][d][mr][mt][lane];
@@ -573,8 +578,8 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       const int key = key0 + 16 * mt + 4 * g + i;
       if (key > my_pos || (S.window > 0 && key <= my_pos - S.window)) x[i] = -INFINITY;
     }
-    const size_t to = (size_t)(key0 + 16 * mt + 4 * g - S.first);
-    if (my_row < S.rows && to < S.stride) *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + to) = x;
+    // (stored by all: behind a condition, the next wait for a load would wait for it too)
+    *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + (key0 + 16 * mt + 4 * g - S.first)) = x;
     // (fmaxf drops a NaN score, whose weight is NaN; a lane's maximum is its own until the end)
     const float mn = fmaxf(fmaxf(fmaxf(m, x[0]), fmaxf(x[1], x[2])), x[3]);
     float sum = 0.f;
@@ -583,6 +588,10 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     l = fmaf(l, __builtin_amdgcn_exp2f(m - mn), sum);
     m = mn;
     __syncthreads();
+  };
+  for (int step = t0; step < t1; step += 2) {
+    turn(step, kb, ka);
+    if (step + 1 < t1) turn(step + 1, ka, kb);
   }
   if (!__all(fits) && lane == 0) a.redo[R0 / R] = a.call;
   const float M = group_max(m);
@@ -660,7 +669,7 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     s.window = win;
     s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
     s.end = s.pos0 + n;
-    s.stride = (size_t)((s.end - s.first + 3) & ~3);
+    s.stride = score_stride(s.end - s.first);
     const ScorePlan plan = head_dim == 64    ? score_plan<64>(s.rows)
                            : head_dim == 128 ? score_plan<128>(s.rows)
                            : head_dim == 256 ? score_plan<256>(s.rows)
@@ -671,7 +680,7 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     if (s.splits > kMaxSplits) s.splits = kMaxSplits;
     if (plan.again && s.splits > 8 && s.splits % 8 <= s.splits / 8) s.splits = s.splits / 8 * 8;
     if (s.splits < 1) s.splits = 1;
-    const size_t scores = s.rows * s.stride, ml = (size_t)s.splits * s.rows * 2;
+    const size_t scores = score_floats(s.rows, s.stride), ml = (size_t)s.splits * s.rows * 2;
     void *mem = nullptr;
     if ((rc = g_weights_ws.get((scores + ml + weight_part_floats(s.rows, s.end - s.first)) * 4, &mem, who)))
       return rc;

@@ -14,6 +14,8 @@ int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *w
 // units of log 2, and (maximum, sum of 2^(score - maximum)) of each row and key split.  Query row
 // i sits at position pos0 + i; a key is seen at positions key .. key + window - 1 (window 0: all
 // from key on).
+// Kernels of up to 64 rows and 32 keys per step store whole blocks: what score_stride and
+// score_floats add to the rows and keys is theirs.
 struct Scores {
   float *score;
   float2 *ml;  // [rows][splits]
@@ -21,6 +23,9 @@ struct Scores {
   int rows, heads, splits;
   int first, end, pos0, window;  // keys first .. end - 1 are seen by some row
 };
+
+size_t score_stride(int keys);
+size_t score_floats(int rows, size_t stride);
 
 // weights[key] = before[key] + sum over the rows of 2^(score - max) / sum, for all keys < keylen;
 // `part` holds weight_part_floats(rows, end - first).
