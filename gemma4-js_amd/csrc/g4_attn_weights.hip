@@ -233,9 +233,9 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
     const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + dq * DW);
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
-      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 8 * g) * 4;
+      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 4 * g) * 4;
       x[T][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
-      x[T][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
+      x[T][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 64);
     }
   };
   load_k(t0 + kg, 0, kr[0]);
@@ -244,8 +244,8 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
     const int wd = t % TW;
     for (int r = t / TW; r < R; r += PASS) {
       const int row = min(R0 + r, S.rows - 1);
-      const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 8 * wd);
-      f32x4 x0 = p[0], x1 = p[1];
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 32 * (wd >> 2) + 4 * (wd & 3));
+      f32x4 x0 = p[0], x1 = p[4];
       int top = 0;  // as bits, where NaN > infinity > numbers
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -411,9 +411,10 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 // Many rows: a block owns 16 RT rows and a run of 32-key steps; its W waves share the head dim, so that
 // each k is split into its two values once for all rows, with q in registers.  The waves' partial
 // scores go through LDS; wave w adds those of rows 16 (w % RT) .. and, of these, keys 16 (w / RT) ..
-// in order and keeps the running maximum and sum of its own.  A block in which a key's largest value
-// is outside 2^-10 .. 2^7 (times 2^8: 2^-2 .. 2^15) or a q below 2^-99 says so in `redo`, and
-// scores_kernel does its rows again.
+// in order and keeps the running maximum and sum of its own.
+// k times 2^8 in FP16 ends at 2^-24: what is lost of each is 2^-33, which 512 q below 16 make less
+// than 10^-6 of a score.  A block with a k of 128 or more, with larger q and a key that is below
+// 2^-10 throughout, or with a q below 2^-99, says so in `redo`, and scores_kernel does its rows again.
 template <int HD, int RT, int W>
 __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   constexpr int DW = HD / W, KN = DW / 32, R = 16 * RT, NT = W / RT, KEYS = 16 * NT;
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
   const int per = (steps + S.splits - 1) / S.splits;
   const int t0 = split * per, t1 = min(t0 + per, steps);
-  bool fits = true;
+  bool fits = true, large = false;  // large: some q of 16 or more, for which small k matter
 
   struct Keys {
     f32x4 x[NT][KN][2];
@@ -452,16 +453,17 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + w * DW);
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
-      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 8 * g) * 4;
+      const uint32_t at = (uint32_t)(min(16 * T + c, last) * HD + 4 * g) * 4;
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         kr.x[T][n][0] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n);
-        kr.x[T][n][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 16);
+        kr.x[T][n][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 64);
       }
     }
   };
   load_k(t0, ka);
-  // q: lane (c, g) holds its row's dims 32 n + 8 g .. + 7 of the wave's
+  // q: lane (c, g) holds its row's dims 32 n + 4 g .. + 3 and + 16 .. + 19 of the wave's, k alike: a
+  // load takes 64 consecutive bytes of each key
   half8_t qh[RT][KN], ql[RT][KN];
   {
     constexpr int U = R * HD / 4 / (64 * W);
@@ -482,9 +484,9 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     for (int r = 0; r < RT; ++r) {
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + 32 * n + 8 * g]);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + 32 * n + 4 * g]);
         x[r][n][0] = p[0];
-        x[r][n][1] = p[1];
+        x[r][n][1] = p[4];
       }
     }
 #pragma unroll
@@ -508,6 +510,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of k's)
       fits = fits && e >= -99;
+      large = large || e >= 4;
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         f32x4 x0 = x[r][n][0], x1 = x[r][n][1];
@@ -517,6 +520,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       }
     }
   }
+  large = __any(large);
   auto scores = [&](int step, const Keys &kr, Keys &next) {
     load_k(step + 1, next);
     __builtin_amdgcn_sched_barrier(0);  // (before this step's are split)
@@ -541,8 +545,11 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[r][n], s[r][T], 0, 0, 0);
       }
-      top = group_max(top);
-      if (g == 0) stop[at][w][16 * T + c] = top;
+      fits = fits && (top < 128.f || !(top < INFINITY));  // (what is no number gives scores that are none)
+      if (large) {
+        top = group_max(top);
+        if (g == 0) stop[at][w][16 * T + c] = top;
+      }
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -561,17 +568,18 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const float factor = ldexpf(kLog2e, sxq[16 * mr + c]);
   auto turn = [&](int step, const Keys &kr, Keys &next) {
     const int key0 = lo + step * KEYS, at = (step - t0) & 1;
-    if (step + 1 < t1) scores(step + 1, kr, next);
-    f32x4 x = sm.sx[at][0][mr][mt][lane];
+    f32x4 y[W];  // (loaded before the next step's products)
 #pragma unroll
-    for (int d = 1; d < W; ++d) x += sm.sx[at][d][mr][mt][lane];
+    for (int d = 0; d < W; ++d) y[d] = sm.sx[at][d][mr][mt][lane];
+    scores(step + 1, kr, next);  // (behind the last one: its keys once more, looked at by nobody)
+    f32x4 x = y[0];
+#pragma unroll
+    for (int d = 1; d < W; ++d) x += y[d];
     x *= factor;
-    if (lane < KEYS) {
+    if (large && lane < KEYS) {
       float top = stop[at][0][lane];
-#pragma unroll
       for (int d = 1; d < W; ++d) top = fmaxf(top, stop[at][d][lane]);
-      // (keys without numbers give scores that are none either way)
-      fits = fits && (top == 0.f || (top >= 0x1p-10f && top < 128.f) || !(top < INFINITY));
+      fits = fits && (top == 0.f || top >= 0x1p-10f);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
