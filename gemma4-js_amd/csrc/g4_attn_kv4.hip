@@ -19,7 +19,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
 constexpr float kSlack = 8.f;               // how far (log 2) a score may pass its row's reference
 constexpr int kStep = 32;                   // keys of a wave's step
-constexpr int kWaves = 4;
 constexpr int kMaxSplits = 256;
 
 struct Kv4Args {
@@ -103,8 +102,13 @@ __device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7)
 // Dims that a wave works on; the waves of a key group share the head dim.
 template <int HD>
 constexpr int kDims = HD > 256 ? 256 : HD;
-template <int HD>
-constexpr int kGroups = kWaves / (HD / kDims<HD>);  // key groups of a block
+template <int HD, int W>
+constexpr int kGroups = W / (HD / kDims<HD>);  // key groups of a block
+
+// x of lane c ^ 8 of each 16
+__device__ __forceinline__ float other_half(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));  // row_ror:8
+}
 
 // A block owns 16 RT rows of [qrows * heads, hd] and a run of 32-key steps, which its key groups
 // take in turn; lane (c, g) of a wave works for row c throughout:
@@ -113,20 +117,23 @@ constexpr int kGroups = kWaves / (HD / kDims<HD>);  // key groups of a block
 //   softmax           running maximum and sum per row
 //   O^T += V^T . P^T  the lane's weights are its operand as they are, FP16 hi + lo; a lane unpacks
 //                     DW / 16 dims of 8 keys
-template <int HD, int RT>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
-  constexpr int DW = kDims<HD>, DQ = HD / DW, KG = kGroups<HD>;
+// PAIR: 8 rows, lanes c and c + 8 both working for row c, with the hi part in the first and the lo
+// part in the second one, so that one product does both.
+template <int HD, int RT, bool PAIR, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
+  constexpr int DW = kDims<HD>, DQ = HD / DW, KG = kGroups<HD, W>;
+  static_assert(!PAIR || RT == 1, "one tile");
   constexpr int KW = DW / 32;                  // words of a key per lane, and products
   constexpr int KS = DW >= 128 ? DW / 128 : 1; // scales of a key per lane
   constexpr int VD = DW / 16;                  // dims per lane, and output tiles
   constexpr int VW = VD >= 8 ? VD / 8 : 1;     // words of them (64: half a word)
-  constexpr int R = 16 * RT, OS = HD + 4;
+  constexpr int R = PAIR ? 8 : 16 * RT, OR = PAIR ? 8 : 16, OS = HD + 4;
   union Smem {
     struct {
-      u32x4 q[2][RT][HD / 32][64];
+      u32x4 q[PAIR ? 1 : 2][RT][HD / 32][64];
       f32x4 sx[DQ > 1 ? 2 : 0][KG][DQ][RT][2][64];  // the waves' scores, two buffers
     } loop;
-    float o[16][OS];
+    float o[KG / 2][OR][OS];
   };
   __shared__ Smem sm;
   __shared__ int xq[R];
@@ -134,6 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
+  const int cr = PAIR ? c & 7 : c;  // the lane's row of a tile
   const int R0 = blockIdx.x * R, split = blockIdx.y;
   if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] != a.call) return;
   // the rows' positions, and the keys that some of them see
@@ -194,7 +202,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 
   // q: a thread takes 8 values of a row, whose largest gets the exponent 13
   {
-    constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    constexpr int TW = HD / 8, PASS = 64 * W / TW;
     constexpr int N = (R + PASS - 1) / PASS;
     const int wd = t % TW;
     f32x4 qx[N][2];
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
       const int n = HD >= 128 ? (wd >> 4) * 4 + (wd & 3) : wd & 1;
       const int at = HD >= 128 ? (wd >> 2) & 3 : wd >> 1;
       sm.loop.q[0][r >> 4][n][(r & 15) + 16 * at] = hi4;
-      sm.loop.q[1][r >> 4][n][(r & 15) + 16 * at] = lo4;
+      sm.loop.q[PAIR ? 0 : 1][r >> 4][n][(r & 15) + 16 * at + (PAIR ? 8 : 0)] = lo4;
     }
   }
   __syncthreads();
@@ -241,8 +249,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   f32x4 o[RT][VD];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    pos[r] = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
-    xe[r] = xq[16 * r + c];
+    pos[r] = S.pos0 + min(R0 + 16 * r + cr, S.rows - 1) / S.heads;
+    xe[r] = xq[16 * r + cr];
     xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
     usual = usual && usual_row(xe[r]);
     m[r] = kNoScore;
@@ -312,11 +320,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
             const half8_t qh = __builtin_bit_cast(half8_t, sm.loop.q[0][r][dq * KW + n][lane]);
-            const half8_t ql = __builtin_bit_cast(half8_t, sm.loop.q[1][r][dq * KW + n][lane]);
 #pragma unroll
-            for (int T = 0; T < 2; ++T) {
-              sh[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], qh, sh[r][T], 0, 0, 0);
-              sl[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], ql, sl[r][T], 0, 0, 0);
+            for (int T = 0; T < 2; ++T) sh[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], qh, sh[r][T], 0, 0, 0);
+            if constexpr (!PAIR) {
+              const half8_t ql = __builtin_bit_cast(half8_t, sm.loop.q[1][r][dq * KW + n][lane]);
+#pragma unroll
+              for (int T = 0; T < 2; ++T)
+                sl[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[T], ql, sl[r][T], 0, 0, 0);
             }
           }
           if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (else all is unpacked at once, and spilled)
@@ -328,7 +338,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
         for (int T = 0; T < 2; ++T)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            s[r][T][i] = (sh[r][T][i] + sl[r][T][i]) * xf[r];
+            s[r][T][i] = (sh[r][T][i] + (PAIR ? other_half(sh[r][T][i]) : sl[r][T][i])) * xf[r];
       if (!kplain) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
@@ -403,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
           }
         }
       }
-      const int row = R0 + 16 * r + c;
+      const int row = R0 + 16 * r + cr;
       if (S.score && mine && dq == 0) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
@@ -442,6 +452,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
         h4[j] = __builtin_bit_cast(uint32_t, h);
         l4[j] = __builtin_bit_cast(
             uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
+        if (PAIR && c >= 8) h4[j] = l4[j];
       }
       ph[r] = __builtin_bit_cast(half8_t, h4);
       pl[r] = __builtin_bit_cast(half8_t, l4);
@@ -471,7 +482,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
-              o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+              if constexpr (!PAIR) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
             }
           };
           tile(std::integral_constant<int, 0>());
@@ -493,12 +504,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     load_v(step + KG);
   }
 
-  // the key groups' sums, in order, through LDS
+  // the key groups' sums through LDS, the upper half of the groups to the lower one
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
-    if (g == 0 && dq == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
+    if (g == 0 && dq == 0) wml[kg][16 * r + cr] = make_float2(m[r], l[r]);
   }
   __syncthreads();
   const bool whole = S.splits == 1;
@@ -507,11 +518,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
   for (int r = 0; r < RT; ++r) {
     float M = kNoScore, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][16 * r + c].x);
+    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][16 * r + cr].x);
 #pragma unroll
     for (int i = 0; i < KG; ++i)
-      L = fmaf(wml[i][16 * r + c].y, __builtin_amdgcn_exp2f(wml[i][16 * r + c].x - M), L);
-    const int row = R0 + 16 * r + c;
+      L = fmaf(wml[i][16 * r + cr].y, __builtin_amdgcn_exp2f(wml[i][16 * r + cr].x - M), L);
+    const int row = R0 + 16 * r + cr;
     if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)row * S.splits + split] = make_float2(M, L);
     // (a split of which the row sees nothing: 0, not 0 / 0)
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
@@ -521,32 +532,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kv4_kernel(Kv4Args a) {
     for (int v = 0; v < 4; ++v) {
       const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
 #pragma unroll
-      for (int n = 0; n < VD; ++n) o[r][n][v] *= fv;
+      for (int n = 0; n < VD; ++n) {
+        if (PAIR) o[r][n][v] += other_half(o[r][n][v]);
+        o[r][n][v] *= fv;
+      }
     }
     // lane (c, g): tile n, register v holds dim (4 g + v) VD + n of the wave's
-    float *mine = &sm.o[c][dq * DW + 4 * g * VD];
 #pragma unroll
-    for (int i = KG - 1; i >= 1; --i) {
-      if (kg == i)
+    for (int half = KG / 2; half >= 1; half /= 2) {
+      float *at = &sm.o[kg & (half - 1)][cr][dq * DW + 4 * g * VD];
+      if (kg >= half && kg < 2 * half && c == cr)
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
           for (int n = 0; n < VD; n += 4)
-            *reinterpret_cast<f32x4 *>(mine + v * VD + n) =
+            *reinterpret_cast<f32x4 *>(at + v * VD + n) =
                 (f32x4){o[r][n][v], o[r][n + 1][v], o[r][n + 2][v], o[r][n + 3][v]};
       __syncthreads();
-      if (kg == 0)
+      if (kg < half)
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
           for (int n = 0; n < VD; n += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(mine + v * VD + n);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(at + v * VD + n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[r][n + e][v] += x[e];
           }
-      __syncthreads();
+      if (half > 1 || r + 1 < RT) __syncthreads();
     }
-    if (kg == 0 && row < S.rows) {
+    if (kg == 0 && c == cr && row < S.rows) {
       float *p = out + (size_t)row * HD + dq * DW + 4 * g * VD;
 #pragma unroll
       for (int v = 0; v < 4; ++v)
@@ -986,10 +1000,11 @@ struct Plan {
 };
 template <int HD>
 Plan plan_of(int rows) {
-  if (rows <= 16) return {attn_kv4_kernel<HD, 1>, nullptr, 16, kStep * kGroups<HD>, 2, 64 * kWaves};
-  if constexpr (HD == 512) return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2>, 64, 32, 1, 512};
-  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 4, 4>, attn_kv4_kernel<HD, 2>, 64, 32, 1, 256};
-  else return {attn_kv4_kernel<HD, 2>, nullptr, 32, kStep * kGroups<HD>, 2, 64 * kWaves};
+  if (rows <= 8) return {attn_kv4_kernel<HD, 1, true, 4>, nullptr, 8, kStep * kGroups<HD, 4>, 2, 256};
+  if (rows <= 16) return {attn_kv4_kernel<HD, 1, false, 4>, nullptr, 16, kStep * kGroups<HD, 4>, 2, 256};
+  if constexpr (HD == 512) return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 512};
+  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 4, 4>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 256};
+  else return {attn_kv4_kernel<HD, 2, false, 4>, nullptr, 32, kStep * kGroups<HD, 4>, 2, 256};
 }
 
 // The rows of a.s, all at once; `before` and `weights` of this call.
@@ -1027,7 +1042,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   G4_LAUNCH_CHECK("attn_kv4_kernel");
   if (plan.again) {
     a.redo_rows = plan.rows;
-    hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 32), splits), dim3(64 * kWaves), 0, stream(), a);
+    hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 32), splits), dim3(256), 0, stream(), a);
     G4_LAUNCH_CHECK("attn_kv4_kernel");
   }
   if (splits > 1) {
