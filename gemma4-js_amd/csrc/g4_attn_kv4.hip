@@ -14,12 +14,13 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
 constexpr float kSlack = 8.f;               // how far (log 2) a score may pass its row's reference
 constexpr int kStep = 32;                   // keys of a wave's step
-constexpr int kMaxSplits = 256;
+constexpr int kMaxSplits = 512;
 
 struct Kv4Args {
   const float *q;
@@ -88,9 +89,6 @@ __device__ __forceinline__ int row_max(int v) {
 
 // Plain scales (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
 // exponent of their row's largest taken out, which then goes to the score or the weight.
-__device__ __forceinline__ bool plain_scale(uint32_t bits) {
-  return (bits & 0x7fffu) - (uint32_t)kLeastScale < kPlainScales;
-}
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 // Rows of q whose exponent a factor of FP32 holds with all its bits.
@@ -153,48 +151,63 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   const int t0 = split * per, t1 = min(t0 + per, steps);
 
   uint32_t kr[2][KW], ksr[2][KS], vr[8][VW], vsr[8];
+  // Loads by an offset per lane from a step's first row; rows behind the last key give zeros, which
+  // `look_*` makes 1 among the scales.
+  const int row_k = c, row_v = 4 * g;
+  const uint32_t at_k = row_k * (HD / 2) + dq * (DW / 2) + g * (DW >= 128 ? 16 : 8);
+  const uint32_t at_ks = row_k * (HD / 16) + dq * (DW / 16) + (DW >= 128 ? g : g >> 1) * 2;
+  const uint32_t at_v = row_v * (HD / 2) + dq * (DW / 2) + c * (DW / 32);
+  const uint32_t at_vs = row_v * (HD / 16) + dq * (DW / 16) + c * DW / 512 * 2;
+  auto rows_of = [&](const void *plane, int step, int bytes) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * kStep);
+    char *p = const_cast<char *>(static_cast<const char *>(plane)) + (size_t)k0 * bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, min(hi - k0, kStep) * bytes, 0x00020000);
+  };
   auto load_k = [&](int step) {
-    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * kStep), last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
-    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
+    const auto p = rows_of(a.k, step, HD / 2), ps = rows_of(a.ks, step, HD / 16);
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
-      const uint32_t r = (uint32_t)min(16 * T + c, last);
-      if constexpr (DW >= 128) {
 #pragma unroll
-        for (int J = 0; J < KS; ++J) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (r * (HD / 2) + g * 16) + 64 * J);
+      for (int J = 0; J < KS; ++J) {
+        if constexpr (DW >= 128) {
+          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(p, at_k + 64 * J + 16 * T * (HD / 2), 0, 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) kr[T][4 * J + i] = x[i];
-          ksr[T][J] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + g * 2) + 8 * J);
+        } else {
+          const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(p, at_k + 16 * T * (HD / 2), 0, 0);
+          kr[T][0] = x[0];
+          kr[T][1] = x[1];
         }
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(p + (r * (HD / 2) + g * 8));
-        kr[T][0] = x.x;
-        kr[T][1] = x.y;
-        ksr[T][0] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + (g >> 1) * 2));
+        ksr[T][J] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ps, at_ks + 8 * J + 16 * T * (HD / 16), 0, 0);
       }
     }
   };
   auto load_v = [&](int step) {
-    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * kStep), last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + dq * (DW / 2);
-    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + dq * (DW / 16);
+    const auto p = rows_of(a.v, step, HD / 2), ps = rows_of(a.vs, step, HD / 16);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
-      const char *pr = p + (r * (HD / 2) + c * (DW / 32));
+      const uint32_t at = at_v + (16 * (j >> 2) + (j & 3)) * (HD / 2);
       if constexpr (DW == 256) {
-        const uint2 x = *reinterpret_cast<const uint2 *>(pr);
-        vr[j][0] = x.x;
-        vr[j][1] = x.y;
+        const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(p, at, 0, 0);
+        vr[j][0] = x[0];
+        vr[j][1] = x[1];
       } else if constexpr (DW == 128) {
-        vr[j][0] = *reinterpret_cast<const uint32_t *>(pr);
+        vr[j][0] = __builtin_amdgcn_raw_buffer_load_b32(p, at, 0, 0);
       } else {
-        vr[j][0] = *reinterpret_cast<const uint16_t *>(pr);
+        vr[j][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(p, at, 0, 0);
       }
-      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
+      vsr[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ps, at_vs + (16 * (j >> 2) + (j & 3)) * (HD / 16), 0, 0);
     }
+  };
+  auto look_k = [&](int last) {
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int J = 0; J < KS; ++J) ksr[T][J] = 16 * T + row_k > last ? 0x3f80u : ksr[T][J];
+  };
+  auto look_v = [&](int last) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vsr[j] = 16 * (j >> 2) + row_v + (j & 3) > last ? 0x3f80u : vsr[j];
   };
   load_k(t0 + kg);
   load_v(t0 + kg);
@@ -266,16 +279,19 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   for (int it = 0; it < turns; ++it) {
     const int step = t0 + kg + it * KG, key0 = lo + step * kStep;
     const bool mine = step < t1;
+    const int last = hi - 1 - (lo + min(step, steps - 1) * kStep);  // row of the step
+    if (last < kStep - 1) look_k(last);
     // the keys' exponents, where a scale needs them
     uint32_t ke[2] = {0, 0};  // a byte each
-    float kmul[2] = {256.f, 256.f};
-    bool kplain = usual;
+    Scale x[2][KS];
+    bool kplain;
     {
+      ushort2_t beyond = {0, 0};
 #pragma unroll
       for (int T = 0; T < 2; ++T)
 #pragma unroll
-        for (int J = 0; J < KS; ++J) kplain = kplain && plain_scale(ksr[T][J]);
-      kplain = __all(kplain);
+        for (int J = 0; J < KS; ++J) x[T][J] = plain_pair(ksr[T][J], ksr[T][J], beyond);
+      kplain = __all(usual && beyond[0] < kPlainScales);
       if (!kplain) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
@@ -285,7 +301,11 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
           top = max(top, __shfl_xor(top, 16, 64));
           top = max(top, __shfl_xor(top, 32, 64));
           const int e = min(scale_exponent(top), 127);
-          kmul[T] = pow2_8_minus(e);
+#pragma unroll
+          for (int J = 0; J < KS; ++J) {
+            const float f = bf16_to_f32(ksr[T][J]) * pow2_8_minus(e);
+            x[T][J] = scale_pair(f, f);
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e, 4 * g + i, 64) & 255) << (8 * i);
         }
@@ -300,12 +320,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
         for (int T = 0; T < 2; ++T) sh[r][T] = sl[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int J = 0; J < KS; ++J) {
-        Scale x[2];
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          const float f = bf16_to_f32(ksr[T][J]) * kmul[T];
-          x[T] = scale_pair(f, f);
-        }
 #pragma unroll
         for (int i = 0; i < KW / KS; ++i) {
           const int n = J * (KW / KS) + i;
@@ -314,8 +328,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
           for (int T = 0; T < 2; ++T) {
             const uint32_t wd = kr[T][n];
             kv[T] = __builtin_bit_cast(
-                half8_t, (u32x4){value_pair<0>(wd, x[T], mg), value_pair<1>(wd, x[T], mg), value_pair<2>(wd, x[T], mg),
-                                 value_pair<3>(wd, x[T], mg)});
+                half8_t, (u32x4){value_pair<0>(wd, x[T][J], mg), value_pair<1>(wd, x[T][J], mg), value_pair<2>(wd, x[T][J], mg),
+                                 value_pair<3>(wd, x[T][J], mg)});
           }
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
@@ -367,16 +381,17 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
     }
 
     // v's exponents: keys 4 g + i of each half, as the weights are held
+    if (last < kStep - 1) look_v(last);
     uint32_t ve[2] = {0, 0};
     Scale vx[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      vx[j] = scale_pair(bf16_to_f32(vsr[2 * j]) * 256.f, bf16_to_f32(vsr[2 * j + 1]) * 256.f);
     uint32_t odd = 0;  // keys of which this lane's dims are no numbers
-    bool vplain = true;
+    bool vplain;
+    {
+      ushort2_t beyond = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vplain = vplain && plain_scale(vsr[j]);
-    vplain = __all(vplain);
+      for (int j = 0; j < 4; ++j) vx[j] = plain_pair(vsr[2 * j], vsr[2 * j + 1], beyond);
+      vplain = __all(max(beyond[0], beyond[1]) < kPlainScales);
+    }
     if (!vplain) {
       float f[8];
 #pragma unroll
@@ -912,10 +927,11 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
 }
 
 // Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
-// one row's 64 dims; thread (j, u) adds splits j, j + 16, .. of 16-byte unit u in order.
+// one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
+// under way together and before their weights are known.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
-  constexpr int U = 16, G = 256 / U;
+  constexpr int U = 8, G = 256 / U, N = 8, PER = kMaxSplits / 256;
   const Scores &S = a.s;
   const int t = threadIdx.x, u = t % U, j = t / U, row = blockIdx.x;
   __shared__ float wt[kMaxSplits];
@@ -923,26 +939,40 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
   __shared__ f32x4 sums[G][U];
   const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + blockIdx.y * U + u;
   const size_t step = (size_t)S.rows * HD / 4;
-  f32x4 x[4];
+  f32x4 x[N];
+  auto load = [&](int s0) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = p[min(j + G * i, S.splits - 1) * step];
-  const float2 ml = t < S.splits ? S.ml[(size_t)row * S.splits + t] : make_float2(kNoScore, 0.f);
-  float M = ml.x;
+    for (int i = 0; i < N; ++i) x[i] = p[min(s0 + G * i, S.splits - 1) * step];
+  };
+  float2 ml[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) ml[i] = S.ml[(size_t)row * S.splits + min(t + 256 * i, S.splits - 1)];
+  load(j);
+  float M = ml[0].x;
+#pragma unroll
+  for (int i = 1; i < PER; ++i) M = fmaxf(M, ml[i].x);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   if ((t & 63) == 0) wmax[t >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-  const float e = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
-  wt[t] = e;
+  float e = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const float z = t + 256 * i < S.splits ? ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - M) : 0.f;
+    wt[t + 256 * i] = z;
+    e += z;
+  }
   const float L = wave_sum(e);
   if ((t & 63) == 0) wsum[t >> 6] = L;
   __syncthreads();
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = j; s0 < S.splits; s0 += G * N) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (j + G * i < S.splits) y += wt[j + G * i] * x[i];
-  for (int s = j + 4 * G; s < S.splits; s += G) y += wt[s] * p[s * step];
+    for (int i = 0; i < N; ++i)
+      if (s0 + G * i < S.splits) y += wt[s0 + G * i] * x[i];
+    if (s0 + G * N < S.splits) load(s0 + G * N);
+  }
   sums[j][u] = y;
   __syncthreads();
   if (j > 0) return;
@@ -1014,8 +1044,14 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   const Plan plan = plan_of<HD>(s.rows);
   const int blocks = cdiv(s.rows, plan.rows);
   const int keys = s.window > 0 ? min(s.end - s.first, s.window + plan.rows) : s.end - s.first;
-  int splits = plan.per_cu * cu_count() / blocks;
-  if (splits > cdiv(keys, plan.keys)) splits = cdiv(keys, plan.keys);
+  // A block per CU, or as many as fit where each then has several turns: the join of their outputs
+  // costs more than a shorter loop gains.  One token, us: 16001 keys of 512, 251 splits of one turn
+  // 14.7, 126 of two 16.4; 32003 with weights 256 of two 20.9, 512 of one 24.9; 131072 512 of
+  // four 29.1, 256 of eight 30.7.
+  const int turns = cdiv(keys, plan.keys);
+  int splits = cu_count() / blocks;
+  if (turns >= 4 * plan.per_cu * splits) splits = plan.per_cu * cu_count() / blocks;
+  if (splits > turns) splits = turns;
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 1) splits = 1;
   s.splits = splits;
@@ -1050,7 +1086,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
       hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3((unsigned)(((size_t)s.rows * (HD / 4) + 255) / 256)), dim3(256),
                          0, stream(), a);
     else
-      hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 64), dim3(256), 0, stream(), a);
+      hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 32), dim3(256), 0, stream(), a);
     G4_LAUNCH_CHECK("attn_kv4_merge_kernel");
   }
   if (!weights) return G4_OK;
