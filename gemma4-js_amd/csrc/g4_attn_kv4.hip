@@ -18,7 +18,10 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
-constexpr float kSlack = 8.f;               // how far (log 2) a score may pass its row's reference
+// How far (log 2) a score may pass its row's reference before the outputs are scaled again.  Weights
+// are split into two FP16 values times 2^(15 - kSlack), so one is held to 2^-22 of it, or to 2^-38 of
+// its row's largest if that is more.
+constexpr float kSlack = 2.f;
 constexpr int kStep = 32;                   // keys of a wave's step
 constexpr int kMaxSplits = 512;
 
@@ -29,8 +32,10 @@ struct Kv4Args {
   float *y;
   float *part;  // [splits][rows][hd], each split's outputs
   Scores s;     // score null: not kept
-  // attn_kv4_rows_kernel's row blocks to do again, marked with the call
-  uint32_t *redo, call;
+  // attn_kv4_rows_kernel's row blocks to do again: set by a block, and with one split also cleared;
+  // with several, all are 0 between calls, as the splits' join leaves them
+  uint32_t *redo;
+  int blocks;
   int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
@@ -87,8 +92,6 @@ __device__ __forceinline__ int row_max(int v) {
   return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
 }
 
-// Plain scales (2^-12 <= s < 8) are taken as they are, times 2^8; others with the
-// exponent of their row's largest taken out, which then goes to the score or the weight.
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 // Rows of q whose exponent a factor of FP32 holds with all its bits.
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int cr = PAIR ? c & 7 : c;  // the lane's row of a tile
   const int R0 = blockIdx.x * R, split = blockIdx.y;
-  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] != a.call) return;
+  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] == 0) return;
   // the rows' positions, and the keys that some of them see
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
   int lo = S.first;
@@ -236,7 +239,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
         top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
 #pragma unroll
       for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
-      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (r >= R) break;
       if (wd == 0) xq[r] = e - 21;  // (8 of the scales)
       u32x4 hi4, lo4;
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
     usual = usual && usual_row(xe[r]);
     m[r] = kNoScore;
     l[r] = 0.f;
-    E[r] = -1000.f;  // outputs are held times 2^(21 - E)
+    E[r] = -1000.f;  // outputs are held times 2^(23 - E)
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
@@ -451,7 +454,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
       }
       E2 = fmaxf(fmaxf(E2, bound), -1000.f);
       float p[8], sum = 0.f;
-      const int up = 13 - (int)E2;
+      const int up = 15 - (int)E2;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         p[j] = __builtin_amdgcn_exp2f(x[j] - mn);
@@ -542,7 +545,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
     // (a split of which the row sees nothing: 0, not 0 / 0)
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
     if (!whole && L == 0.f) f = 0.f;
-    f = ldexpf(f, (int)E[r] - 21);
+    f = ldexpf(f, (int)E[r] - 23);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
@@ -720,7 +723,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       int top = 0;
 #pragma unroll
       for (int d = 0; d < W; ++d) top = max(top, stop[d][16 * r + c]);
-      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of the scales)
       if (!usual_row(e - 21)) beyond = (ushort2_t){0xffff, 0xffff};
 #pragma unroll
@@ -771,8 +774,9 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       for (int T = 0; T < NT; ++T) sm.sx[(step - t0) & 1][w][r][T][lane] = s[r][T];
   };
 
+  constexpr float kWeight = 1 << (15 - (int)kSlack);
   float m = kNoScore, l = 0.f;  // of row 16 w + c
-  f32x4 o[RT][VD];              // outputs times 2^(21 - kSlack)
+  f32x4 o[RT][VD];              // outputs times 2^(23 - kSlack)
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -833,7 +837,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
         const float p0 = __builtin_amdgcn_exp2f(x[T][i] - mn), p1 = __builtin_amdgcn_exp2f(x[T][i + 1] - mn);
         sum += p0;
         sum += p1;
-        const f32x2_t z = {p0 * 32.f, p1 * 32.f};  // 2^(13 - kSlack)
+        const f32x2_t z = {p0 * kWeight, p1 * kWeight};
         const half2_t h = __builtin_convertvector(z, half2_t);
         h4[j] = __builtin_bit_cast(uint32_t, h);
         l4[j] = __builtin_bit_cast(
@@ -894,16 +898,22 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
     load_v(step + 1);
   }
 
-  // (q's below the usual are all waves' matter, and rows that lie behind their split's keys too)
-  if (__any(max(beyond[0], beyond[1]) >= kPlainScales) && lane == 0) a.redo[blockIdx.x] = a.call;
+  const bool again = __any(max(beyond[0], beyond[1]) >= kPlainScales);
+  if (lane == 0) stop[w][0] = again;
   const bool whole = S.splits == 1;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (S.ml && w < RT && g == 0 && my_row < S.rows) S.ml[(size_t)my_row * S.splits + split] = make_float2(m, l);
   // (a split of which the row sees nothing: 0, not 0 / 0)
-  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 21);
+  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 23);
   __syncthreads();  // (sf is read to the last step's end)
   if (w < RT && g == 0) sf[0][16 * w + c] = fin;
+  if (t == 0) {
+    int some = 0;
+#pragma unroll
+    for (int d = 0; d < W; ++d) some |= stop[d][0];
+    if (whole || some) a.redo[blockIdx.x] = some;
+  }
   __syncthreads();
   float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
 #pragma unroll
@@ -926,6 +936,10 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   }
 }
 
+__device__ __forceinline__ void clear_redo(const Kv4Args &a) {
+  for (int i = threadIdx.x; i < a.blocks; i += 256) a.redo[i] = 0;
+}
+
 // Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
 // one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
 // under way together and before their weights are known.
@@ -944,6 +958,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = p[min(s0 + G * i, S.splits - 1) * step];
   };
+  if (row == 0 && blockIdx.y == 0) clear_redo(a);
   float2 ml[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) ml[i] = S.ml[(size_t)row * S.splits + min(t + 256 * i, S.splits - 1)];
@@ -991,6 +1006,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
   constexpr int MOST = 16;
   const Scores &S = a.s;
   const size_t unit = (size_t)blockIdx.x * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
+  if (blockIdx.x == 0) clear_redo(a);
   if (unit >= units) return;
   const float2 *ml = S.ml + unit / (HD / 4) * S.splits;
   const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part) + unit;
@@ -1019,7 +1035,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 Workspace g_kv4_ws, g_redo_ws;
-uint32_t g_call = 0;
+constexpr int kMostMarks = 512;  // row blocks of a call of several splits: no more than fit at once
 
 // The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per
 // CU and threads.
@@ -1053,7 +1069,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   if (turns >= 4 * plan.per_cu * splits) splits = plan.per_cu * cu_count() / blocks;
   if (splits > turns) splits = turns;
   if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits < 1) splits = 1;
+  if (splits < 1 || blocks > kMostMarks) splits = 1;
   s.splits = splits;
   const bool ml = weights || splits > 1;
   const size_t n_part = splits > 1 ? (size_t)splits * s.rows * HD : 0, n_ml = ml ? (size_t)splits * s.rows * 2 : 0;
@@ -1067,12 +1083,11 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
   }
   if (plan.again) {
-    // (a recording keeps its number: a block that one replay marked is done again by all, which
-    // changes nothing but the time)
+    // (the marks of calls with one split lie behind the others: they are not left 0)
     void *mem = nullptr;
-    if (int rc = g_redo_ws.get((size_t)blocks * 4, &mem, "g4_attention_kv4")) return rc;
-    a.redo = static_cast<uint32_t *>(mem);
-    a.call = ++g_call;
+    if (int rc = g_redo_ws.get((size_t)(kMostMarks + blocks) * 4, &mem, "g4_attention_kv4")) return rc;
+    a.redo = static_cast<uint32_t *>(mem) + (splits > 1 ? 0 : kMostMarks);
+    a.blocks = blocks;
   }
   hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(plan.threads), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
@@ -1107,10 +1122,13 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
   if (before && !weights) return fail(G4_E_ARG, "%s: before without weights", who);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(y)) & 15)
     return fail(G4_E_ARG, "%s: q and y must be 16-byte aligned", who);
+  const int head_dim = cache->head_dim;
+  const size_t qn = (size_t)qrows * heads * head_dim * 4, wn = weights ? (size_t)keylen * 4 : 0;
+  if (overlap(q, qn, y, qn) || overlap(q, qn, weights, wn) || overlap(y, qn, weights, wn) ||
+      (before && overlap(y, qn, before, wn)))
+    return fail(G4_E_ARG, "%s: y or weights overlaps another argument", who);
   G4_CHECK_INIT();
   if (keylen == 0) return ok();
-  const int head_dim = cache->head_dim;
-  const size_t qn = (size_t)qrows * heads * head_dim * 4;
   int rc = check_kv4_memory(cache, keylen, true, true, "g4_attention_kv4 cache");
   if (!rc && qrows) rc = check_device_range(q, qn, "g4_attention_kv4 q");
   if (!rc && qrows) rc = check_device_range(y, qn, "g4_attention_kv4 y");

@@ -18,9 +18,7 @@ int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int
   if (qpos0 < 0 || qpos0 > keylen - qrows || (sliding && window <= 0))
     return fail(G4_E_ARG, "%s: keylen %d must cover query positions %d.. + %d (window %d)", who,
                 keylen, qpos0, qrows, window);
-  const uintptr_t b = reinterpret_cast<uintptr_t>(before), w = reinterpret_cast<uintptr_t>(weights);
-  const uintptr_t bytes = (uintptr_t)keylen * 4;
-  if (before && weights && before != weights && (b < w ? w - b : b - w) < bytes)
+  if (before && weights && before != weights && overlap(before, (size_t)keylen * 4, weights, (size_t)keylen * 4))
     return fail(G4_E_ARG, "%s: before overlaps weights", who);
   return G4_OK;
 }
@@ -54,6 +52,8 @@ constexpr int kBatch = 16;  // loads of a thread that are under way together
 __global__ __launch_bounds__(256) void weights_kernel(SumArgs a) {
   __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
   const Scores &s = a.s;
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < s.n_marks; i += 256) s.marks[i] = 0;
   const int t = threadIdx.x, r0 = blockIdx.y * kGroup, n = min(kGroup, s.rows - r0);
   const int key = blockIdx.x * 256 + t + (a.part ? s.first : 0);
   const bool any = key >= s.first && key < s.end;
@@ -170,8 +170,8 @@ constexpr int kWaves = 4;
 struct ScoreArgs {
   const float *q, *k;
   Scores s;
-  // scores_rows_kernel's row blocks to do again, marked with the call
-  uint32_t *redo, call;
+  // scores_rows_kernel's row blocks to do again; all 0 between calls, as weights_kernel leaves them
+  uint32_t *redo;
   int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
-  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] != a.call) return;
+  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] == 0) return;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
   int lo = S.first;
   if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
         top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
 #pragma unroll
       for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
-      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (wd == 0) xq[r] = e - 13;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x0[i] = ldexpf(x0[i], 13 - e), x1[i] = ldexpf(x1[i], 13 - e);
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
       int top = 0;
 #pragma unroll
       for (int d = 0; d < W; ++d) top = max(top, sq[d][16 * r + c]);
-      const int e = top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+      const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of k's)
       fits = fits && e >= -99;
       large = large || e >= 4;
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     turn(step, kb, ka);
     if (step + 1 < t1) turn(step + 1, ka, kb);
   }
-  if (!__all(fits) && lane == 0) a.redo[R0 / R] = a.call;
+  if (!__all(fits) && lane == 0) a.redo[R0 / R] = 1;
   const float M = group_max(m);
   l *= __builtin_amdgcn_exp2f(m - M);
   l += __shfl_xor(l, 16, 64);
@@ -634,7 +634,6 @@ ScorePlan score_plan(int rows) {
 }
 
 Workspace g_weights_ws, g_score_redo_ws;
-uint32_t g_score_call = 0;
 
 }  // namespace
 }  // namespace g4
@@ -650,6 +649,9 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
   if (int rc = check_weighted(qrows, heads, keylen, qpos0, sliding, window, before, weights, who)) return rc;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k)) & 15)
     return fail(G4_E_ARG, "%s: q and k must be 16-byte aligned", who);
+  if (overlap(weights, (size_t)keylen * 4, q, (size_t)qrows * heads * head_dim * 4) ||
+      overlap(weights, (size_t)keylen * 4, k, (size_t)keylen * head_dim * 4))
+    return fail(G4_E_ARG, "%s: weights overlaps q or k", who);
   G4_CHECK_INIT();
   if (keylen == 0) return ok();
   int rc = check_device_range(weights, (size_t)keylen * 4, "g4_attention_weights weights");
@@ -695,12 +697,11 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     s.score = static_cast<float *>(mem);
     s.ml = reinterpret_cast<float2 *>(s.score + scores);
     if (plan.again) {
-      // (a recording keeps its number: a block that one replay marked is done again by all, which
-      // changes nothing but the time)
       void *redo = nullptr;
       if ((rc = g_score_redo_ws.get((size_t)blocks * 4, &redo, who))) return rc;
       a.redo = static_cast<uint32_t *>(redo);
-      a.call = ++g_score_call;
+      s.marks = a.redo;
+      s.n_marks = blocks;
     }
     hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(plan.threads), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");

@@ -1,5 +1,6 @@
 // The rows of a cache to keep: the first ones, the latest ones and the heaviest of the others.
 #include "g4_internal.h"
+#include "g4_kv4.h"
 
 namespace g4 {
 namespace {
@@ -354,9 +355,11 @@ G4_API int g4_cache_evict(const float *weights, size_t stride, int sets, int len
   if (stride < (size_t)len || stride > (size_t(1) << 52))
     return fail(G4_E_ARG, "g4_cache_evict: stride %zu of %d rows", stride, len);
   const size_t n = sets > 0 ? (sets - 1) * stride + len : 0;
-  const uintptr_t w = reinterpret_cast<uintptr_t>(weights), k = reinterpret_cast<uintptr_t>(kept);
-  if (kept && kept != weights && (w < k ? k - w : w - k) < n * 4)
+  if (kept && kept != weights && overlap(weights, n * 4, kept, n * 4))
     return fail(G4_E_ARG, "g4_cache_evict: kept overlaps weights");
+  const size_t n_rows = (size_t)sets * keep * 4;
+  if (overlap(rows, n_rows, weights, n * 4) || (kept && overlap(rows, n_rows, kept, n * 4)))
+    return fail(G4_E_ARG, "g4_cache_evict: rows overlaps weights or kept");
   G4_CHECK_INIT();
   if (sets == 0 || len == 0) return ok();
   int rc = check_device_range(weights, n * 4, "g4_cache_evict weights");

@@ -22,6 +22,8 @@ struct Scores {
   size_t stride;
   int rows, heads, splits;
   int first, end, pos0, window;  // keys first .. end - 1 are seen by some row
+  uint32_t *marks;               // that weights_kernel clears
+  int n_marks;
 };
 
 size_t score_stride(int keys);
@@ -37,5 +39,11 @@ int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int
                    const float *before, const float *weights, const char *who);
 // Query rows whose scores are kept at once.
 int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window);
+
+// Whether two ranges of bytes have some in common; none where one is empty.
+inline bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na && nb && (x < y ? y - x < na : x - y < nb);
+}
 
 }  // namespace g4

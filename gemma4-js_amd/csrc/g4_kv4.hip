@@ -31,6 +31,19 @@ int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *w
 
 namespace {
 
+// The n FP32 rows at k or v against rows at .. of the cache's planes.
+bool overlaps_cache(const g4_kv4 *c, int at, int n, const float *k, const float *v) {
+  const size_t row = c->head_dim, first = at, bytes = (size_t)n * row * 4;
+  for (const float *x : {k, v}) {
+    if (!x) continue;
+    for (const uint32_t *p : {c->k, c->v})
+      if (overlap(x, bytes, p + first * row / 8, n * row / 2)) return true;
+    for (const uint16_t *p : {c->k_scales, c->v_scales})
+      if (overlap(x, bytes, p + first * row / 32, n * row / 16)) return true;
+  }
+  return false;
+}
+
 constexpr long kMaxBlocks = 1 << 23;  // of a launch, which has less than 2^32 threads
 
 struct Rows4 {
@@ -123,6 +136,7 @@ G4_API int g4_kv4_append(const g4_kv4 *c, const float *k, const float *v, int n,
   if (int rc = check_kv4(c, at, n, "g4_kv4_append")) return rc;
   if (unaligned(k) || unaligned(v))
     return fail(G4_E_ARG, "g4_kv4_append: k and v must be 16-byte aligned");
+  if (overlaps_cache(c, at, n, k, v)) return fail(G4_E_ARG, "g4_kv4_append: k or v overlaps the cache");
   G4_CHECK_INIT();
   if (n == 0) return ok();
   const size_t bytes = (size_t)n * c->head_dim * 4;
@@ -141,6 +155,8 @@ G4_API int g4_kv4_read(const g4_kv4 *c, int at, int n, float *k, float *v) {
   if (int rc = check_kv4(c, at, n, "g4_kv4_read")) return rc;
   if (unaligned(k) || unaligned(v))
     return fail(G4_E_ARG, "g4_kv4_read: k and v must be 16-byte aligned");
+  if (overlaps_cache(c, at, n, k, v) || (k && v && overlap(k, (size_t)n * c->head_dim * 4, v, (size_t)n * c->head_dim * 4)))
+    return fail(G4_E_ARG, "g4_kv4_read: k or v overlaps the cache or the other");
   G4_CHECK_INIT();
   if (n == 0 || (!k && !v)) return ok();
   const size_t bytes = (size_t)n * c->head_dim * 4;

@@ -451,8 +451,10 @@ int g4_cache_rows(float *const *dst, const float *const *src, const int *widths,
  *   g4_cache_rows of the rows that it lists, over FP32 planes or over the four planes
  *   of g4_kv4 (rows of 4-byte units: head_dim / 8 of codes, head_dim / 64 of scales).
  * Rows keep the RoPE of their own positions; qpos0 counts cache rows.
- * Arguments are checked before anything else, so a refusal needs no device.  All can
- * be recorded; those with scratch need one earlier call of those sizes for it. */
+ * Arguments are checked before anything else, so a refusal needs no device.  What is
+ * written overlaps no other argument, unless it says so.  All can be recorded:
+ * g4_attention_kv4, g4_attention_weights and g4_cache_evict of more than 16384 rows
+ * after one call outside a recorder of the same sizes, for their scratch. */
 
 /* One layer's k and v rows in 4 bits, in the caller's device memory (no handle: the
  * struct is read during each call).  Values are (nibble - 8) * scale, as g4_w4_load's:
@@ -483,16 +485,20 @@ int g4_kv4_read(const g4_kv4 *cache, int at, int n, float *k, float *v);
  *   weights[key] = before[key] + the weight of that key, summed over rows and heads,
  * before NULL counting as zeros; it may be weights itself, but not overlap it otherwise.
  * Rows that a query row does not see have no influence on it, whatever they hold.
- * heads <= 8; qrows <= 2^20; keylen <= 2^28; q and y 16-byte aligned.  A q, k or
- * v that lies more than 2^36 below the largest of its row (of q: of its head) is kept
- * to that precision. */
+ * heads <= 8; qrows <= 2^20; keylen <= 2^28; q and y 16-byte aligned.
+ * Products are of FP16 pairs with sums in FP32: a q and a weight are held to 2^-22 of
+ * them, or to 2^-38 of their row's largest if that is more; k and v as they are, but for
+ * values whose scale is less than 2^-25 of their row's largest, which lose bits.  A q or k
+ * without a number gives the row NaN, a v whose scale is none (an infinite one too) its
+ * 32 dims. */
 int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int heads, int keylen,
                      int qpos0, int sliding, int window, float *y, const float *before,
                      float *weights);
 
 /* Those weights over FP32 keys: k [keylen, head_dim], rows and masks as g4_attention's,
- * before and weights as above.  head_dim 64, 128, 256 or 512; heads, qrows and keylen
- * as above; q and k 16-byte aligned. */
+ * before and weights as above, q held as it is there, k to 2^-22 of it or 2^-23 of its
+ * row's largest; a k that is no number gives the rows that see it NaN.  head_dim 64,
+ * 128, 256 or 512; heads, qrows and keylen as above; q and k 16-byte aligned. */
 int g4_attention_weights(const float *q, const float *k, int qrows, int heads, int head_dim,
                          int keylen, int qpos0, int sliding, int window, const float *before,
                          float *weights);

@@ -159,13 +159,13 @@ def test_two_recordings_and_eager_calls_share_scratch(g4):
             call()
         recs.append(enc.cmdbuf)
     big = g4.Kv4Cache(20000, 512)
-    bq = g4.Buffer(100 * HEADS * 512 * 4)
+    bq, by = (g4.Buffer(100 * HEADS * 512 * 4) for _ in range(2))
     for _ in range(3):
         for (_, bufs, _), rec in zip(calls, recs):
             for b in bufs:
                 b.upload(np.zeros(b.nbytes // 4, np.float32))
             rec.submit()
-            big.attention(bq, 100, HEADS, 20000, 19900, False, 0, bq, g4.Buffer(80000))
+            big.attention(bq, 100, HEADS, 20000, 19900, False, 0, by, g4.Buffer(80000))
         calls[2][0]()
         for _, bufs, want in calls:
             for b, a in zip(bufs, want):
@@ -203,7 +203,7 @@ q, y, w, k = g4.Buffer(40 * 8 * 256 * 4), g4.Buffer(40 * 8 * 256 * 4), g4.Buffer
 rows = g4.Buffer(300000 * 4)
 calls = [lambda: c.attention(q, 40, 8, 9000, 8960, False, 0, y, w),
          lambda: g4.attention_weights(q, k, 40, 8, 256, 9000, 8960, False, 0, w)]
-free = [lambda: c.append(k, k, 5, 7), lambda: c.read(3, 4, y, y), lambda: g4.cache_evict(w, 3, 1000, 900, 4, 8, rows, w)]
+free = [lambda: c.append(k, k, 5, 7), lambda: c.read(3, 4, y, q), lambda: g4.cache_evict(w, 3, 1000, 900, 4, 8, rows, w)]
 for call in calls:
     with g4.Encoder() as enc:
         try:

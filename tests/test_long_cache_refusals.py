@@ -93,3 +93,34 @@ def test_evict_overlap(kept):
 def test_cache_of_other_buffers():
     with pytest.raises(ValueError):
         g4hip.Kv4Cache(8, 64, [16, 16])
+
+
+@pytest.mark.parametrize("y,w", [(65536, 1 << 20), (65536 + 2 * 8 * 256 * 4 - 16, 1 << 20), (1 << 20, 65536 + 12),
+                                 (1 << 20, (1 << 20) + 2 * 8 * 256 * 4 - 4), (1 << 20, (1 << 20) - 196)])
+def test_attention_kv4_overlaps(y, w):
+    # 2 rows of 8 * 256 at q and y, 50 weights
+    refused(g4hip.lib().g4_attention_kv4(65536, cache(), 2, 8, 50, 40, 0, 0, y, None, w), "overlaps")
+    refused(g4hip.lib().g4_attention_kv4(65536, cache(), 2, 8, 50, 40, 0, 0, y, y + 16, w), "overlaps")
+
+
+@pytest.mark.parametrize("w", [65536, 65536 - 196, 65536 + 2 * 8 * 256 * 4 - 4, (1 << 20) - 4, (1 << 20) + 50 * 1024 - 4])
+def test_attention_weights_overlaps(w):
+    refused(g4hip.lib().g4_attention_weights(65536, 1 << 20, 2, 8, 256, 50, 40, 0, 0, None, w), "overlaps")
+
+
+@pytest.mark.parametrize("rows,kept", [(4096, None), (4096 + 116, None), (4096 - 36, 1 << 20), ((1 << 20) + 8, 1 << 20)])
+def test_evict_rows_overlap(rows, kept):
+    # 2 sets of 10 at a stride of 20: 30 weights; 2 * 5 rows
+    refused(g4hip.lib().g4_cache_evict(4096, 20, 2, 10, 5, 0, 0, rows, kept), "overlaps")
+
+
+def test_kv4_rows_overlap_their_cache():
+    # rows 3 .. 6 of 256: 512 bytes of codes, 64 of scales
+    planes = [1 << 20, 2 << 20, 3 << 20, 4 << 20]
+    L = g4hip.lib()
+    for p, row in zip(planes, (128, 128, 16, 16)):
+        for x in (p + 3 * row, p + 7 * row - 16, p + 3 * row - 4096 + 16):
+            for k, v in ((x, 16 << 20), (16 << 20, x)):
+                refused(L.g4_kv4_append(cache(100, 256, *planes), k, v, 4, 3), "overlaps")
+                refused(L.g4_kv4_read(cache(100, 256, *planes), 3, 4, k, v), "overlaps")
+    refused(L.g4_kv4_read(cache(100, 256, *planes), 3, 4, 16 << 20, (16 << 20) + 4080), "overlaps")
