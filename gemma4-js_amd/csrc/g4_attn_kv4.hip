@@ -15,6 +15,7 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t any_u16 __attribute__((may_alias));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
@@ -48,9 +49,9 @@ constexpr uint16_t kLeastScale = (127 - 12) << 7, kPlainScales = 15 << 7;
 struct Scale {
   half2_t s, c;  // s and -24 s
 };
+__device__ __forceinline__ Scale scale_of(half2_t s) { return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}}; }
 __device__ __forceinline__ Scale scale_pair(float a, float b) {
-  const half2_t s = __builtin_convertvector((f32x2_t){a, b}, half2_t);
-  return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}};
+  return scale_of(__builtin_convertvector((f32x2_t){a, b}, half2_t));
 }
 // (mask and exponent in registers, so that one instruction takes both)
 struct Magic {
@@ -67,8 +68,7 @@ __device__ __forceinline__ Scale plain_pair(uint32_t lo, uint32_t hi, ushort2_t 
   const ushort2_t d = u - (ushort2_t){kLeastScale, kLeastScale};
   beyond = __builtin_elementwise_max(beyond, d);
   constexpr uint16_t least = (kLeastScale - ((127 - 8 - 15) << 7)) << 3;
-  const half2_t s = __builtin_bit_cast(half2_t, (ushort2_t)(d * (ushort2_t){8, 8} + (ushort2_t){least, least}));
-  return {s, s * (half2_t){(_Float16)-24.f, (_Float16)-24.f}};
+  return scale_of(__builtin_bit_cast(half2_t, (ushort2_t)(d * (ushort2_t){8, 8} + (ushort2_t){least, least})));
 }
 template <int T>
 __device__ __forceinline__ uint32_t value_pair(uint32_t w, const Scale &x, const Magic &mg) {
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   constexpr int DW = HD / W, R = 16 * RT, NT = 2, KEYS = 16 * NT;
   constexpr int KN = DW / 32;         // words of a key per lane, and products
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
-  static_assert(DW == 128 || DW == 64, "one scale of a key per lane");
+  static_assert(DW == 64, "32 bytes of a row per wave");
   // (two of each: what the step's readers may still look at, and the next)
   union Smem {
     struct {
@@ -624,6 +624,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
     float rows[R][HD + 4];  // q and the outputs, on their way from and to whole lines of memory
   };
   __shared__ Smem sm;
+  __shared__ u32x4 sv[W][64];         // v's codes of a step
   __shared__ float sf[2][R];
   __shared__ int smoved[2][4];        // whether some row's reference moved
   static_assert(RT <= 4, "a flag per row tile");
@@ -640,49 +641,36 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const int t0 = split * per, t1 = min(t0 + per, steps);
   ushort2_t beyond = {0, 0};  // the scales' largest distance from the least plain one
 
-  uint32_t kr[NT][KN], ksr[NT], vr[8], vsr[8];
+  // A lane loads 16 bytes and a scale of a key, and of a v: lane (c, g) key 16 (g / 2) + c, bytes
+  // 16 (g % 2) .. of the wave's 32, of which the lanes' halves then swap 8; as v's, lane l those of
+  // slot l / 2 = 4 j + g that holds key 16 (j / 4) + 4 g + j % 4, by LDS to lanes (., g) as their
+  // j-th; and the scale of slot 4 (c % 8) + g and of dims 32 (c / 8) ...  Rows behind the last key
+  // give zeros, whose scales are made 1.
+  u32x4 kr, vr;
+  uint32_t ksr, vsr;
+  const auto slot_row = [](int j, int gg) { return 16 * (j >> 2) + 4 * gg + (j & 3); };
+  const int row_k = 16 * (g >> 1) + c, row_v = slot_row(lane >> 3, lane >> 1 & 3), row_vs = slot_row(c & 7, g);
+  const uint32_t at_k = row_k * (HD / 2) + w * (DW / 2) + (g & 1) * 16;
+  const uint32_t at_ks = row_k * (HD / 16) + w * (DW / 16) + (g & 1) * 2;
+  const uint32_t at_v = row_v * (HD / 2) + w * (DW / 2) + (lane & 1) * 16;
+  const uint32_t at_vs = row_vs * (HD / 16) + w * (DW / 16) + (c >> 3) * 2;
+  auto rows_of = [&](const void *plane, int step, int bytes) {
+    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS);
+    char *p = const_cast<char *>(static_cast<const char *>(plane)) + (size_t)k0 * bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, min(hi - k0, KEYS) * bytes, 0x00020000);
+  };
   auto load_k = [&](int step) {
-    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.k) + (size_t)k0 * (HD / 2) + w * (DW / 2);
-    const char *ps = reinterpret_cast<const char *>(a.ks) + (size_t)k0 * (HD / 16) + w * (DW / 16);
-#pragma unroll
-    for (int T = 0; T < NT; ++T) {
-      const uint32_t r = (uint32_t)min(16 * T + c, last);
-      if constexpr (DW == 128) {
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (r * (HD / 2) + g * 16));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kr[T][i] = x[i];
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(p + (r * (HD / 2) + g * 8));
-        kr[T][0] = x.x;
-        kr[T][1] = x.y;
-      }
-      ksr[T] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + g * DW / 128 * 2));
-    }
+    kr = __builtin_amdgcn_raw_buffer_load_b128(rows_of(a.k, step, HD / 2), at_k, 0, 0);
+    ksr = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows_of(a.ks, step, HD / 16), at_ks, 0, 0);
   };
   auto load_v = [&](int step) {
-    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
-    const char *p = reinterpret_cast<const char *>(a.v) + (size_t)k0 * (HD / 2) + w * (DW / 2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
-      const char *pr = p + (r * (HD / 2) + c * (DW / 32));
-      if constexpr (DW == 128) vr[j] = *reinterpret_cast<const uint32_t *>(pr);
-      else vr[j] = *reinterpret_cast<const uint16_t *>(pr);
-    }
+    vr = __builtin_amdgcn_raw_buffer_load_b128(rows_of(a.v, step, HD / 2), at_v, 0, 0);
+    vsr = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows_of(a.vs, step, HD / 16), at_vs, 0, 0);
   };
-  auto load_vs = [&](int step) {
-    const int k0 = __builtin_amdgcn_readfirstlane(lo + min(step, steps - 1) * KEYS), last = hi - 1 - k0;
-    const char *ps = reinterpret_cast<const char *>(a.vs) + (size_t)k0 * (HD / 16) + w * (DW / 16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t r = (uint32_t)min(16 * (j >> 2) + 4 * g + (j & 3), last);
-      vsr[j] = *reinterpret_cast<const uint16_t *>(ps + (r * (HD / 16) + c * DW / 512 * 2));
-    }
-  };
+  auto last_row = [&](int step) { return hi - 1 - (lo + min(step, steps - 1) * KEYS); };
   load_k(t0);
 
-  // q: lane (c, g) holds its row's dims g DW / 4 + 8 n .. + 7 of the wave's
+  // q: lane (c, g) holds its row's dims 32 (g % 2) + 16 (g / 2) + 8 n .. + 7 of the wave's, as k's are
   half8_t qh[RT][KN], ql[RT][KN];
   {
     constexpr int U = R * HD / 4 / (64 * W);
@@ -704,7 +692,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       int top = 0;
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + g * (DW / 4) + 8 * n]);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(&sm.rows[16 * r + c][w * DW + 32 * (g & 1) + 16 * (g >> 1) + 8 * n]);
         x[r][n][0] = p[0];
         x[r][n][1] = p[1];
       }
@@ -745,19 +733,31 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const Magic mg;
   // partial scores of a step into LDS
   auto scores = [&](int step) {
+    if (row_k > last_row(step)) ksr = 0x3f80u;
     Scale x[NT];
+    uint32_t kw[NT][KN];
     f32x4 s[RT][NT];
+    {
+      const uint32_t both = __builtin_bit_cast(uint32_t, plain_pair(ksr, ksr, beyond).s);
+      const auto y = __builtin_amdgcn_permlane32_swap(both, both, false, false);
 #pragma unroll
-    for (int T = 0; T < NT; ++T) {
-      x[T] = plain_pair(ksr[T], ksr[T], beyond);
+      for (int T = 0; T < NT; ++T) x[T] = scale_of(__builtin_bit_cast(half2_t, (uint32_t)y[T]));
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        const auto z = __builtin_amdgcn_permlane32_swap(kr[n], kr[n + 2], false, false);
+#pragma unroll
+        for (int T = 0; T < NT; ++T) kw[T][n] = z[T];
+      }
+    }
+#pragma unroll
+    for (int T = 0; T < NT; ++T)
 #pragma unroll
       for (int r = 0; r < RT; ++r) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
 #pragma unroll
     for (int n = 0; n < KN; ++n)
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
-        const uint32_t wd = kr[T][n];
+        const uint32_t wd = kw[T][n];
         const half8_t kv = __builtin_bit_cast(
             half8_t, (u32x4){value_pair<0>(wd, x[T], mg), value_pair<1>(wd, x[T], mg), value_pair<2>(wd, x[T], mg),
                              value_pair<3>(wd, x[T], mg)});
@@ -782,7 +782,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int my_row = R0 + 16 * min(w, RT - 1) + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
-  load_vs(t0);
   load_v(t0);
   __syncthreads();
   const float my_factor = ldexpf(kLog2e, sxq[16 * min(w, RT - 1) + c]);
@@ -794,6 +793,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   __syncthreads();
   for (int step = t0; step < t1; ++step) {
     const int key0 = lo + step * KEYS, at = (step - t0) & 1;
+    // (formed by all waves first: behind the softmax, by those that do it, 105.5 us for 97.6)
     if (step + 1 < t1) scores(step + 1);
     if (w < RT) {
       // this wave's rows: the scores of all, in order
@@ -851,10 +851,25 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       if (lane == 0) smoved[at][w] = moved;
       m = mn;
     }
+    if (row_vs > last_row(step)) vsr = 0x3f80u;
     Scale vx[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vx[j] = plain_pair(vsr[2 * j], vsr[2 * j + 1], beyond);
-    load_vs(step + 1);
+    {
+      // keys j and j + 1 of even j's lane, then from there to all of its 8
+      const uint32_t next = __builtin_amdgcn_update_dpp(0, (int)vsr, 0xB1, 0xf, 0xf, true);
+      const int both = __builtin_bit_cast(int, plain_pair(vsr, next, beyond).s);
+      auto of = [&](auto j) {
+        constexpr int at = 0x150 + 2 * decltype(j)::value;  // row_newbcast
+        int y = __builtin_amdgcn_update_dpp(0, both, at, 0xf, 0xf, true);
+        y = __builtin_amdgcn_update_dpp(y, both, at + 8, 0xf, 0xc, false);
+        vx[decltype(j)::value] = scale_of(__builtin_bit_cast(half2_t, y));
+      };
+      of(std::integral_constant<int, 0>());
+      of(std::integral_constant<int, 1>());
+      of(std::integral_constant<int, 2>());
+      of(std::integral_constant<int, 3>());
+    }
+    sv[w][lane] = vr;
+    load_v(step + 1);
     __syncthreads();
     int moved = 0;
 #pragma unroll
@@ -873,21 +888,21 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
         for (int n = 0; n < VD; ++n) o[r][n] *= f;
       }
     }
-#pragma unroll
-    for (int h = 0; h < VD / 4; ++h) {
+    {
+      const any_u16 *codes = reinterpret_cast<const any_u16 *>(sv[w]) + lane;
       uint32_t d[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] = __builtin_amdgcn_perm(vr[2 * j + 1], vr[2 * j], h ? 0x07060302u : 0x05040100u);
+      for (int j = 0; j < 4; ++j)
+        d[j] = __builtin_bit_cast(uint32_t, (ushort2_t){codes[128 * j], codes[128 * j + 64]});
       auto tile = [&](auto T) {
         constexpr int e = decltype(T)::value;
         const half8_t vv = __builtin_bit_cast(
             half8_t, (u32x4){value_pair<e>(d[0], vx[0], mg), value_pair<e>(d[1], vx[1], mg),
                              value_pair<e>(d[2], vx[2], mg), value_pair<e>(d[3], vx[3], mg)});
-        const int n = 4 * h + e;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+        for (int r = 0; r < RT; ++r) o[r][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][e], 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
+        for (int r = 0; r < RT; ++r) o[r][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][e], 0, 0, 0);
       };
       tile(std::integral_constant<int, 0>());
       tile(std::integral_constant<int, 1>());
@@ -895,7 +910,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       tile(std::integral_constant<int, 3>());
     }
     interleave<2 * RT * VD, 3>();
-    load_v(step + 1);
   }
 
   const bool again = __any(max(beyond[0], beyond[1]) >= kPlainScales);
