@@ -5,6 +5,7 @@
 
 #include "g4_gemv.h"
 #include "g4_internal.h"
+#include "g4_key_weights.h"
 #include "g4_kv4.h"
 
 namespace g4 {
@@ -18,7 +19,6 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t any_u16 __attribute__((may_alias));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
 // How far (log 2) a score may pass its row's reference before the outputs are scaled again.  Weights
 // are split into two FP16 values times 2^(15 - kSlack), so one is held to 2^-22 of it, or to 2^-38 of
 // its row's largest if that is more.
@@ -84,14 +84,6 @@ __device__ __forceinline__ float group_max(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-// max over aligned teams of 16 lanes
-__device__ __forceinline__ int row_max(int v) {
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
-  return max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
-}
-
 // Signed byte i of a word.
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 // Rows of q whose exponent a factor of FP32 holds with all its bits.
@@ -237,8 +229,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
-#pragma unroll
-      for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+      top = team_max<TW>(top);
       const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (r >= R) break;
       if (wd == 0) xq[r] = e - 21;  // (8 of the scales)
@@ -404,7 +395,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
           odd |= 1u << j;
           vsr[j] = u = 0;
         }
-        const int e = scale_exponent(row_max(u));
+        const int e = scale_exponent(team_max<16>(u));
         ve[j >> 2] |= (uint32_t)(e & 255) << (8 * (j & 3));
         f[j] = bf16_to_f32(vsr[j]) * pow2_8_minus(e);
       }
@@ -958,21 +949,21 @@ __device__ __forceinline__ void clear_redo(const Kv4Args &a) {
 // one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
 // under way together and before their weights are known.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
+__device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
   constexpr int U = 8, G = 256 / U, N = 8, PER = kMaxSplits / 256;
   const Scores &S = a.s;
-  const int t = threadIdx.x, u = t % U, j = t / U, row = blockIdx.x;
+  const int t = threadIdx.x, u = t % U, j = t / U;
   __shared__ float wt[kMaxSplits];
   __shared__ float wmax[4], wsum[4];
   __shared__ f32x4 sums[G][U];
-  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + blockIdx.y * U + u;
+  const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part + (size_t)row * HD) + part * U + u;
   const size_t step = (size_t)S.rows * HD / 4;
   f32x4 x[N];
   auto load = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = p[min(s0 + G * i, S.splits - 1) * step];
   };
-  if (row == 0 && blockIdx.y == 0) clear_redo(a);
+  if (row == 0 && part == 0) clear_redo(a);
   float2 ml[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) ml[i] = S.ml[(size_t)row * S.splits + min(t + 256 * i, S.splits - 1)];
@@ -1011,7 +1002,19 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) {
   const float sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] /= sum;
-  reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[blockIdx.y * U + u] = y;
+  reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[part * U + u] = y;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) { merge<HD>(a, blockIdx.x, blockIdx.y); }
+
+// Few rows whose keys' weights are asked for: both need the first kernel's sums alone, so the same
+// launch does the one and the other.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, SumArgs w) {
+  const int merges = a.s.rows * (HD / 32), b = blockIdx.x;
+  if (b < merges) merge<HD>(a, b / (HD / 32), b % (HD / 32));
+  else add_weights(w, b - merges, 0);
 }
 
 // The same for up to 16 splits of many rows: a thread per 16-byte unit.
@@ -1109,6 +1112,13 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     a.redo_rows = plan.rows;
     hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 32), splits), dim3(256), 0, stream(), a);
     G4_LAUNCH_CHECK("attn_kv4_kernel");
+  }
+  if (splits > 1 && weights && s.rows <= kGroup) {
+    const SumArgs sums{s, keylen, before, weights, nullptr};
+    hipLaunchKernelGGL(attn_kv4_merge_weights_kernel<HD>, dim3(s.rows * (HD / 32) + cdiv(keylen, 256)), dim3(256), 0,
+                       stream(), a, sums);
+    G4_LAUNCH_CHECK("attn_kv4_merge_weights_kernel");
+    return G4_OK;
   }
   if (splits > 1) {
     if (s.rows >= 64 && splits <= 16)

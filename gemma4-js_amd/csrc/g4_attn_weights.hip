@@ -4,6 +4,7 @@
 
 #include "g4_gemv.h"
 #include "g4_internal.h"
+#include "g4_key_weights.h"
 #include "g4_kv4.h"
 
 namespace g4 {
@@ -33,90 +34,11 @@ int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window) {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoScore = -3.4028235e38f;  // where a row's maximum starts
-constexpr int kGroup = 32;                  // rows that a block adds up
 constexpr int kMaxSplits = 512;
 
-struct SumArgs {
-  Scores s;
-  int keylen;
-  const float *before;
-  float *weights;
-  float *part;  // [groups][end - first], or null
-};
+__global__ __launch_bounds__(256) void weights_kernel(SumArgs a) { add_weights(a, blockIdx.x, blockIdx.y); }
 
-constexpr int kBatch = 16;  // loads of a thread that are under way together
-
-// A thread per key adds up to 32 rows; blockIdx.y counts these groups.  The first rows' scores are
-// loaded before the rows' maxima and sums are known.
-__global__ __launch_bounds__(256) void weights_kernel(SumArgs a) {
-  __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
-  const Scores &s = a.s;
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < s.n_marks; i += 256) s.marks[i] = 0;
-  const int t = threadIdx.x, r0 = blockIdx.y * kGroup, n = min(kGroup, s.rows - r0);
-  const int key = blockIdx.x * 256 + t + (a.part ? s.first : 0);
-  const bool any = key >= s.first && key < s.end;
-  const float *p = s.score + (size_t)r0 * s.stride + (any ? key - s.first : 0);
-  float x[kBatch];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) x[i] = p[(size_t)min(i0 + i, n - 1) * s.stride];
-  };
-  const float before = !a.part && a.before && key < a.keylen ? a.before[key] : 0.f;
-  if (n > 0) {
-    load(0);
-    int lanes = 4;  // per row
-    while (lanes < 64 && lanes * 2 * n <= 256) lanes *= 2;
-    const int i = t / lanes, row = r0 + min(i, n - 1);
-    const float2 *ml = s.ml + (size_t)row * s.splits;
-    float m = kNoScore, l = 0.f;
-    for (int p0 = t % lanes; p0 < s.splits; p0 += 4 * lanes) {
-      float2 y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = ml[min(p0 + e * lanes, s.splits - 1)];
-      float mn = m;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mn = fmaxf(mn, y[e].x);
-      l *= __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (p0 + e * lanes < s.splits) l = fmaf(y[e].y, __builtin_amdgcn_exp2f(y[e].x - mn), l);
-      m = mn;
-    }
-    for (int o = 1; o < lanes; o <<= 1) {
-      const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
-      const float u = l * __builtin_amdgcn_exp2f(m - mn), v = l2 * __builtin_amdgcn_exp2f(m2 - mn);
-      l = (t & o) ? v + u : u + v;
-      m = mn;
-    }
-    if (t % lanes == 0 && i < n) {
-      const int pos = s.pos0 + row / s.heads;
-      stat[i] = make_float4(m, 1.f / l, __int_as_float(pos),
-                            __int_as_float(s.window > 0 ? pos - s.window : -1));
-    }
-  }
-  __syncthreads();
-  float sum = 0.f;
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float4 st = stat[min(i0 + i, n - 1)];
-      const bool sees = i0 + i < n && key <= __float_as_int(st.z) && key > __float_as_int(st.w);
-      const float w = __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
-      if (sees) sum += w;
-    }
-    if (i0 + kBatch < n) load(i0 + kBatch);
-  }
-  if (!any) sum = 0.f;
-  if (a.part) {
-    if (any) a.part[(size_t)blockIdx.y * (s.end - s.first) + (key - s.first)] = sum;
-  } else if (key < a.keylen) {
-    a.weights[key] = before + sum;
-  }
-}
-
-// Adds the groups of a key, 8 of them under way together.
+// Adds the groups of a key, 16 of them under way together.
 __global__ __launch_bounds__(64) void weights_join_kernel(SumArgs a, int groups) {
   const int key = blockIdx.x * 64 + threadIdx.x;
   if (key >= a.keylen) return;
@@ -211,6 +133,7 @@ __device__ __forceinline__ float group_max(float v) {
 template <int HD, int DQ, int NT, int RT>
 __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   constexpr int KG = kWaves / DQ, DW = HD / DQ, KN = DW / 32, R = 16 * RT, KEYS = 16 * NT;
+  constexpr int AHEAD = NT * KN <= 4 ? KN : 2;  // a step's loads that are under way together
   __shared__ u32x4 sq[2][RT][HD / 32][64];
   __shared__ f32x4 sx[DQ > 1 ? 2 : 1][KG][DQ][DQ > 1 ? RT : 1][DQ > 1 ? NT : 1][DQ > 1 ? 64 : 1];
   __shared__ int xq[R];
@@ -227,7 +150,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   const int per = (steps + S.splits - 1) / S.splits;
   const int t0 = split * per, t1 = min(t0 + per, steps);
 
-  f32x4 kr[2][NT][2];
+  f32x4 kr[AHEAD][NT][2];
   auto load_k = [&](int step, int n, f32x4 (&x)[NT][2]) {
     const int k0 = lo + min(step, steps - 1) * KEYS, last = hi - 1 - k0;
     const char *p = reinterpret_cast<const char *>(a.k + (size_t)k0 * HD + dq * DW);
@@ -238,28 +161,40 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
       x[T][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 64);
     }
   };
-  load_k(t0 + kg, 0, kr[0]);
+#pragma unroll
+  for (int n = 0; n < (AHEAD == KN ? KN : 1); ++n) load_k(t0 + kg, n, kr[n]);
   {
     constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    constexpr int N = (R + PASS - 1) / PASS < 4 ? (R + PASS - 1) / PASS : 4;  // rows of a thread under way together
     const int wd = t % TW;
-    for (int r = t / TW; r < R; r += PASS) {
-      const int row = min(R0 + r, S.rows - 1);
-      const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 32 * (wd >> 2) + 4 * (wd & 3));
-      f32x4 x0 = p[0], x1 = p[4];
-      int top = 0;  // as bits, where NaN > infinity > numbers
+    for (int r0 = t / TW; r0 < R; r0 += PASS * N) {
+      f32x4 x[N][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        top = max(top, max(__float_as_int(x0[i]) & 0x7fffffff, __float_as_int(x1[i]) & 0x7fffffff));
+      for (int i = 0; i < N; ++i) {
+        const int row = min(R0 + min(r0 + PASS * i, R - 1), S.rows - 1);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 32 * (wd >> 2) + 4 * (wd & 3));
+        x[i][0] = p[0];
+        x[i][1] = p[4];
+      }
 #pragma unroll
-      for (int o = 1; o < TW; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
-      const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
-      if (wd == 0) xq[r] = e - 13;
+      for (int i = 0; i < N; ++i) {
+        const int r = r0 + PASS * i;
+        f32x4 x0 = x[i][0], x1 = x[i][1];
+        int top = 0;  // as bits, where NaN > infinity > numbers
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x0[i] = ldexpf(x0[i], 13 - e), x1[i] = ldexpf(x1[i], 13 - e);
-      half8_t h, l;
-      halves(x0, x1, 1.f, h, l);
-      sq[0][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, h);
-      sq[1][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, l);
+        for (int d = 0; d < 4; ++d)
+          top = max(top, max(__float_as_int(x0[d]) & 0x7fffffff, __float_as_int(x1[d]) & 0x7fffffff));
+        top = team_max<TW>(top);
+        const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
+        if (r >= R) break;
+        if (wd == 0) xq[r] = e - 13;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x0[d] = ldexpf(x0[d], 13 - e), x1[d] = ldexpf(x1[d], 13 - e);
+        half8_t h, l;
+        halves(x0, x1, 1.f, h, l);
+        sq[0][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, h);
+        sq[1][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, l);
+      }
     }
   }
   __syncthreads();
@@ -290,12 +225,12 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 #pragma unroll
         for (int T = 0; T < NT; ++T) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-      for (int n0 = 0; n0 < KN; n0 += 2)
+      for (int n0 = 0; n0 < KN; n0 += AHEAD)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < AHEAD; ++e) {
         const int n = n0 + e;
         const bool more = n + 1 < KN;
-        load_k(more ? step : step + KG, more ? n + 1 : 0, kr[1 - e]);
+        if constexpr (AHEAD < KN) load_k(more ? step : step + KG, more ? n + 1 : 0, kr[1 - e]);
         half8_t kh[NT], kl[NT];
 #pragma unroll
         for (int T = 0; T < NT; ++T) {
@@ -333,7 +268,12 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
         const int e = top[T] < INFINITY ? min(max((int)(__float_as_uint(top[T]) >> 23) - 127, -100), 127) : 0;
         up[T] = __int_as_float((127 + 8 - e) << 23);
       }
-      load_k(step, 0, kr[0]);
+      if constexpr (AHEAD < KN) load_k(step, 0, kr[0]);
+    }
+    if constexpr (AHEAD == KN) {
+      if (it + 1 < turns)
+#pragma unroll
+        for (int n = 0; n < KN; ++n) load_k(step + KG, n, kr[n]);
     }
 #pragma unroll
     for (int T = 0; T < NT; ++T) {

@@ -40,6 +40,24 @@ int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int
 // Query rows whose scores are kept at once.
 int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window);
 
+// max over aligned teams of 8, 16, 32 or 64 lanes
+template <int TEAM>
+__device__ __forceinline__ int team_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+  if constexpr (TEAM >= 16) v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+  if constexpr (TEAM >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((int)a[0], (int)a[1]);
+  }
+  if constexpr (TEAM >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max((int)a[0], (int)a[1]);
+  }
+  return v;
+}
+
 // Whether two ranges of bytes have some in common; none where one is empty.
 inline bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
