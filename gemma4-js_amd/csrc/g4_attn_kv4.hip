@@ -971,8 +971,7 @@ __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
   float M = ml[0].x;
 #pragma unroll
   for (int i = 1; i < PER; ++i) M = fmaxf(M, ml[i].x);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  M = team_max(64, M);
   if ((t & 63) == 0) wmax[t >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
@@ -983,7 +982,7 @@ __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
     wt[t + 256 * i] = z;
     e += z;
   }
-  const float L = wave_sum(e);
+  const float L = team_sum(64, e);
   if ((t & 63) == 0) wsum[t >> 6] = L;
   __syncthreads();
   f32x4 y = {0.f, 0.f, 0.f, 0.f};

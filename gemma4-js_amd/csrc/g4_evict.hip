@@ -39,11 +39,12 @@ template <int NW>
 __device__ __forceinline__ int before_me(int x, int *tmp, int &all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int s = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(s, o, 64);
-    if (lane >= o) s += y;
-  }
+  s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xf, 0xf, true);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xf, 0xf, true);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xf, 0xf, true);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xa, 0xf, false);  // rows 1 and 3: the sum before them
+  s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xc, 0xf, false);  // rows 2 and 3 likewise
   if (lane == 63) tmp[w] = s;
   __syncthreads();
   int base = 0;

@@ -21,8 +21,8 @@ struct SumArgs {
 
 constexpr int kBatch = 16;  // loads of a thread that are under way together
 
-// A thread per key adds up to 32 rows; `by` counts these groups, `bx` 256 keys each.  The first rows' scores are
-// loaded before the rows' maxima and sums are known.
+// A thread per key adds up to 32 rows; `by` counts these groups, `bx` 256 keys each.  The first rows'
+// scores are loaded before the rows' maxima and sums are known.
 __device__ __forceinline__ void add_weights(const SumArgs &a, int bx, int by) {
   __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
   const Scores &s = a.s;
@@ -58,12 +58,9 @@ __device__ __forceinline__ void add_weights(const SumArgs &a, int bx, int by) {
         if (p0 + e * lanes < s.splits) l = fmaf(y[e].y, __builtin_amdgcn_exp2f(y[e].x - mn), l);
       m = mn;
     }
-    for (int o = 1; o < lanes; o <<= 1) {
-      const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
-      const float u = l * __builtin_amdgcn_exp2f(m - mn), v = l2 * __builtin_amdgcn_exp2f(m2 - mn);
-      l = (t & o) ? v + u : u + v;
-      m = mn;
-    }
+    const float mine = m;
+    m = team_max(lanes, m);
+    l = team_sum(lanes, l * __builtin_amdgcn_exp2f(mine - m));
     if (t % lanes == 0 && i < n) {
       const int pos = s.pos0 + row / s.heads;
       stat[i] = make_float4(m, 1.f / l, __int_as_float(pos),

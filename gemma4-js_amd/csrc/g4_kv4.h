@@ -1,6 +1,8 @@
 // What the operators of long caches share.
 #pragma once
 
+#include <type_traits>
+
 #include "g4_internal.h"
 
 namespace g4 {
@@ -39,6 +41,33 @@ int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int
                    const float *before, const float *weights, const char *who);
 // Query rows whose scores are kept at once.
 int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window);
+
+// op over aligned teams of `team` lanes, 4 .. 64 and the same for all, known to each of them
+template <class Op>
+__device__ __forceinline__ float team_of(int team, float v, Op op) {
+  auto dpp = [&](auto c) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(c)::value, 0xf, 0xf, true));
+  };
+  v = op(v, dpp(std::integral_constant<int, 0xB1>()));
+  v = op(v, dpp(std::integral_constant<int, 0x4E>()));
+  if (team >= 8) v = op(v, dpp(std::integral_constant<int, 0x141>()));
+  if (team >= 16) v = op(v, dpp(std::integral_constant<int, 0x140>()));
+  if (team >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  if (team >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  return v;
+}
+__device__ __forceinline__ float team_max(int team, float v) {
+  return team_of(team, v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float team_sum(int team, float v) {
+  return team_of(team, v, [](float a, float b) { return a + b; });
+}
 
 // max over aligned teams of 8, 16, 32 or 64 lanes
 template <int TEAM>
