@@ -370,12 +370,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = lane & 15, g = lane >> 4;
-  int R0 = blockIdx.x * R, split = blockIdx.y;
-  if (S.splits % 8 == 0) {  // blocks are dealt to the 8 XCDs in turn: a split's to one, whose L2 holds its keys
-    const int b = blockIdx.y * gridDim.x + blockIdx.x, n = b / 8;
-    split = n / (int)gridDim.x * 8 + b % 8;
-    R0 = n % (int)gridDim.x * R;
-  }
+  const int R0 = blockIdx.x * R, split = blockIdx.y;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
   int lo = S.first;
   if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
@@ -628,7 +623,6 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     s.splits = plan.per_cu * cu_count() / blocks;
     if (s.splits > steps) s.splits = steps;
     if (s.splits > kMaxSplits) s.splits = kMaxSplits;
-    if (plan.again && s.splits > 8 && s.splits % 8 <= s.splits / 8) s.splits = s.splits / 8 * 8;
     if (s.splits < 1) s.splits = 1;
     const size_t scores = score_floats(s.rows, s.stride), ml = (size_t)s.splits * s.rows * 2;
     void *mem = nullptr;
