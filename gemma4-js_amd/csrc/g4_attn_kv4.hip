@@ -581,18 +581,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   }
 }
 
-// The scheduler puts `vector` vector instructions behind each of a block's `products` matrix
-// instructions: a wave's instructions issue in order, so those that stand behind a row of products
-// wait for all of them.
-template <int PRODUCTS, int VECTOR>
-__device__ __forceinline__ void interleave() {
-#pragma unroll
-  for (int i = 0; i < PRODUCTS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x2, VECTOR, 0);
-  }
-}
-
 // Many rows of a cache whose scales all are plain: a block owns 16 RT rows and a run of 32-key steps;
 // its W waves share the head dim both for the scores and for the outputs, so that each value of the
 // cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave w < RT adds
@@ -757,7 +745,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[r][n], s[r][T], 0, 0, 0);
       }
-    interleave<2 * RT * KN * NT, 2>();
     load_k(step + 1);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -900,7 +887,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
       tile(std::integral_constant<int, 2>());
       tile(std::integral_constant<int, 3>());
     }
-    interleave<2 * RT * VD, 3>();
   }
 
   const bool again = __any(max(beyond[0], beyond[1]) >= kPlainScales);
