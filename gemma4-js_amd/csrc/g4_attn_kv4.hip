@@ -1046,12 +1046,21 @@ struct Plan {
   void (*again)(Kv4Args);  // of 32 rows per block, where the first one may leave some undone
   int rows, keys, per_cu, threads;
 };
+// Many rows of 512 whose 64-row blocks would have up to 4 steps each on all CUs: blocks of 32, which
+// start and end sooner.  us, 32 / 64 rows per block: 96 rows over 2000 keys (3 steps) 29.1 / 42.2, 128
+// over 2000 and 32 over 8000 (4) 32.2 / 35.4 and 30.9 / 32.3, 160 over 2000 (5) 44.3 / 36.4, 512
+// over 4608 (36) 129 / 95.  Rows of 256 have room for three blocks of 32 on a CU, or one of 64 in
+// four waves: 512 over 4608 70.6 / 84.7 (48 rows, two blocks: 76.6), 20 over 3000 17.5 / 23.0.
 template <int HD>
-Plan plan_of(int rows) {
+Plan plan_of(int rows, int keys) {
   if (rows <= 8) return {attn_kv4_kernel<HD, 1, true, 4>, nullptr, 8, kStep * kGroups<HD, 4>, 2, 256};
   if (rows <= 16) return {attn_kv4_kernel<HD, 1, false, 4>, nullptr, 16, kStep * kGroups<HD, 4>, 2, 256};
-  if constexpr (HD == 512) return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 512};
-  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 4, 4>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 256};
+  if constexpr (HD == 512) {
+    if ((int64_t)cdiv(rows, 64) * cdiv(keys, 32) <= 4 * cu_count())
+      return {attn_kv4_rows_kernel<HD, 2, 8>, attn_kv4_kernel<HD, 2, false, 4>, 32, 32, 1, 512};
+    return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 512};
+  }
+  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 2, 4>, attn_kv4_kernel<HD, 2, false, 4>, 32, 32, 3, 256};
   else return {attn_kv4_kernel<HD, 2, false, 4>, nullptr, 32, kStep * kGroups<HD, 4>, 2, 256};
 }
 
@@ -1059,9 +1068,9 @@ Plan plan_of(int rows) {
 template <int HD>
 int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   Scores &s = a.s;
-  const Plan plan = plan_of<HD>(s.rows);
+  const int keys = s.window > 0 ? min(s.end - s.first, s.window + 64) : s.end - s.first;  // of a block
+  const Plan plan = plan_of<HD>(s.rows, keys);
   const int blocks = cdiv(s.rows, plan.rows);
-  const int keys = s.window > 0 ? min(s.end - s.first, s.window + plan.rows) : s.end - s.first;
   // A block per CU, or as many as fit where each then has several turns: the join of their outputs
   // costs more than a shorter loop gains.  One token, us: 16001 keys of 512, 251 splits of one turn
   // 14.7, 126 of two 16.4; 32003 with weights 256 of two 20.9, 512 of one 24.9; 131072 512 of

@@ -32,12 +32,14 @@ def odd_rows(rng, what, hd, qrows, keys):
     return q, k, v
 
 
-@pytest.mark.parametrize("hd", [64, 128, 256, 512])
-@pytest.mark.parametrize("window", [0, 130])
-@pytest.mark.parametrize("what", ["zero q", "tiny q", "tiny k", "large v", "one late key"])
-def test_some_rows_unlike_the_others(g4, hd, window, what):
+ODD = ["zero q", "tiny q", "tiny k", "large v", "one late key"]
+
+
+@pytest.mark.parametrize("hd,qrows,keys,window", [(hd, 45, 333, window) for hd in (64, 128, 256, 512) for window in (0, 130)] +
+                         [(512, 140, 2100, 0), (512, 200, 2100, 1500), (256, 140, 2100, 0)])
+@pytest.mark.parametrize("what", ODD)
+def test_some_rows_unlike_the_others(g4, hd, qrows, keys, window, what):
     rng = np.random.default_rng([hd, window, len(what)])
-    qrows, keys = 45, 333
     q, k, v = odd_rows(rng, what, hd, qrows, keys)
     pk, pv = ref.pack(k), ref.pack(v)
     y, w = attend(g4, cache_of(g4, pk, pv, hd), q, keys, keys - qrows, window, True)
@@ -76,7 +78,8 @@ def test_fp32_keys_unlike_the_others(g4, hd, window, what):
     assert (np.abs(got - want) <= TOL * want).all()
 
 
-@pytest.mark.parametrize("hd,qrows,keys", [(512, 45, 700), (256, 45, 700), (256, 2200, 2300)])
+@pytest.mark.parametrize("hd,qrows,keys", [(512, 45, 700), (512, 140, 2100), (512, 2100, 2200), (256, 45, 700),
+                                           (256, 2200, 2300)])
 def test_recordings_whose_rows_change_their_kernel(g4, hd, qrows, keys):
     """Replays equal eager calls to the bit, whatever the replay before needed."""
     rng = np.random.default_rng([hd, qrows])
