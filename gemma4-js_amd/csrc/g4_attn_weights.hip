@@ -558,10 +558,15 @@ struct ScorePlan {
   void (*again)(ScoreArgs);  // of 64 rows per block, where the first one may leave some undone
   int rows, keys, per_cu, threads;
 };
+// 17 to 32 rows take the kernel of few rows, two tiles of them, where it has a block per CU at most: 32
+// rows, us, in this and the other way, over 1000 / 8001 / 32000 keys of 256 10.5 / 14.3 / 21.7 and 14.8 /
+// 16.8 / 21.3 (32, 251 and 1000 blocks), of 512 12.2 / 25.3 / 33.9 and 17.3 / 22.4 / 29.7 (63, 501, 2000).
 template <int HD>
-ScorePlan score_plan(int rows) {
-  constexpr int DQ = HD >= 128 ? HD / 128 : 1;
-  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, nullptr, 16, 16 * kWaves / DQ, 2, 64 * kWaves};
+ScorePlan score_plan(int rows, int keys) {
+  constexpr int DQ = HD >= 128 ? HD / 128 : 1, FEW = 16 * kWaves / DQ;
+  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, nullptr, 16, FEW, 2, 64 * kWaves};
+  if (rows <= 32 && cdiv(keys, FEW) <= cu_count())
+    return {scores_kernel<HD, DQ, 1, 2>, nullptr, 32, FEW, 2, 64 * kWaves};
   if constexpr (HD == 512)
     return {scores_rows_kernel<HD, 4, 8>, scores_kernel<HD, 1, 2, 4>, 64, 32, 1, 512};
   else
@@ -615,11 +620,12 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
     s.end = s.pos0 + n;
     s.stride = score_stride(s.end - s.first);
-    const ScorePlan plan = head_dim == 64    ? score_plan<64>(s.rows)
-                           : head_dim == 128 ? score_plan<128>(s.rows)
-                           : head_dim == 256 ? score_plan<256>(s.rows)
-                                             : score_plan<512>(s.rows);
-    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(s.end - s.first, plan.keys);
+    const int keys = s.end - s.first;
+    const ScorePlan plan = head_dim == 64    ? score_plan<64>(s.rows, keys)
+                           : head_dim == 128 ? score_plan<128>(s.rows, keys)
+                           : head_dim == 256 ? score_plan<256>(s.rows, keys)
+                                             : score_plan<512>(s.rows, keys);
+    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(keys, plan.keys);
     s.splits = plan.per_cu * cu_count() / blocks;
     if (s.splits > steps) s.splits = steps;
     if (s.splits > kMaxSplits) s.splits = kMaxSplits;

@@ -20,7 +20,7 @@ def odd_rows(rng, what, hd, qrows, keys):
     if what == "zero q":
         q[::3] = 0
     elif what == "tiny q":
-        q[5:9] *= np.float32(2.0 ** -104)
+        q[qrows // 9:qrows // 5 + 1] *= np.float32(2.0 ** -104)
     elif what == "tiny k":
         k[100:140] *= np.float32(2.0 ** -20)  # scales below 2^-12
         k[3] *= np.float32(2.0 ** -90)
@@ -57,19 +57,20 @@ def test_some_rows_unlike_the_others(g4, hd, qrows, keys, window, what):
 @pytest.mark.parametrize("hd", [64, 256, 512])
 @pytest.mark.parametrize("window", [0, 130])
 @pytest.mark.parametrize("what", ["zero q", "tiny q", "tiny k", "large k", "large q", "large q, tiny k"])
-def test_fp32_keys_unlike_the_others(g4, hd, window, what):
+@pytest.mark.parametrize("qrows", [45, 4, 1])
+def test_fp32_keys_unlike_the_others(g4, hd, window, what, qrows):
     rng = np.random.default_rng([hd, window, len(what), 1])
-    qrows, keys = 45, 333
+    keys = 333
     q, k, _ = odd_rows(rng, what, hd, qrows, keys)
     if what == "large k":
         q[:, :, 0], k[:, 0] = 0, 0
         k[20:22, 0] = 500  # of no weight, but for the whole row's split into two values
     if what.startswith("large q"):
         q[:, :, 1], k[:, 1] = 0, 0
-        q[11:13, :, 1] = 400
+        q[qrows // 4:qrows // 4 + 2, :, 1] = 400
     if what == "large q, tiny k":
         k[60:70] *= np.float32(2.0 ** -14)
-        k[60:70, 1] = np.float32(2.0 ** -14)  # 0.024 of the score of rows 11 and 12
+        k[60:70, 1] = np.float32(2.0 ** -14)  # 0.024 of those rows' scores
     want = ref.weights(q, k, keys, keys - qrows, window).sum((0, 1))
     w = g4.Buffer.from_array(np.full(keys, np.nan, np.float32))
     g4.attention_weights(g4.Buffer.from_array(q), g4.Buffer.from_array(k), qrows, HEADS, hd, keys, keys - qrows,
