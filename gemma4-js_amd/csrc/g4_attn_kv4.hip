@@ -1142,8 +1142,13 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
     return fail(G4_E_ARG, "%s: q and y must be 16-byte aligned", who);
   const int head_dim = cache->head_dim;
   const size_t qn = (size_t)qrows * heads * head_dim * 4, wn = weights ? (size_t)keylen * 4 : 0;
+  const size_t codes = (size_t)keylen * head_dim / 2, scales = codes / 8;
+  auto in_cache = [&](const void *p, size_t n) {
+    return overlap(p, n, cache->k, codes) || overlap(p, n, cache->v, codes) || overlap(p, n, cache->k_scales, scales) ||
+           overlap(p, n, cache->v_scales, scales);
+  };
   if (overlap(q, qn, y, qn) || overlap(q, qn, weights, wn) || overlap(y, qn, weights, wn) ||
-      (before && overlap(y, qn, before, wn)))
+      (before && overlap(y, qn, before, wn)) || in_cache(y, qn) || in_cache(weights, wn))
     return fail(G4_E_ARG, "%s: y or weights overlaps another argument", who);
   G4_CHECK_INIT();
   if (keylen == 0) return ok();

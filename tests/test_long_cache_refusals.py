@@ -103,6 +103,16 @@ def test_attention_kv4_overlaps(y, w):
     refused(g4hip.lib().g4_attention_kv4(65536, cache(), 2, 8, 50, 40, 0, 0, y, y + 16, w), "overlaps")
 
 
+def test_attention_kv4_overlaps_its_cache():
+    # 50 rows of 256: 6400 bytes of codes, 800 of scales
+    planes = [1 << 20, 2 << 20, 3 << 20, 4 << 20]
+    for p, n in zip(planes, (6400, 6400, 800, 800)):
+        for x in (p, p + n - 16):
+            for y, w in ((x, 8 << 20), (8 << 20, x)):
+                refused(g4hip.lib().g4_attention_kv4(65536, cache(100, 256, *planes), 2, 8, 50, 40, 0, 0, y, None, w),
+                        "overlaps")
+
+
 @pytest.mark.parametrize("w", [65536, 65536 - 196, 65536 + 2 * 8 * 256 * 4 - 4, (1 << 20) - 4, (1 << 20) + 50 * 1024 - 4])
 def test_attention_weights_overlaps(w):
     refused(g4hip.lib().g4_attention_weights(65536, 1 << 20, 2, 8, 256, 50, 40, 0, 0, None, w), "overlaps")
