@@ -112,6 +112,15 @@ __device__ __forceinline__ float other_half(float x) {
 //                     DW / 16 dims of 8 keys
 // PAIR: 8 rows, lanes c and c + 8 both working for row c, with the hi part in the first and the lo
 // part in the second one, so that one product does both.
+// The values are used where they are unpacked, in the lanes that the matrix instructions want them:
+// nothing of k or v passes through LDS.  A row's maximum is a reference that follows the scores with
+// kSlack, so the outputs are hardly ever scaled again; a step's loads are under way during the one
+// before it.  Scales outside 2^-12 .. 8 take a slower way with exponents per row.
+// What bounds it: one token over 131072 keys of 512 (75.5 MB) 24.4 us traced, 3.1 TB/s: 4 steps per
+// wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
+// exponent, fused step) and the products between them, and as long again before and behind them
+// (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
+// 11.0 us, a chain of latencies.
 template <int HD, int RT, bool PAIR, int W>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   constexpr int DW = kDims<HD>, DQ = HD / DW, KG = kGroups<HD, W>;
@@ -581,13 +590,20 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   }
 }
 
-// Many rows of a cache whose scales all are plain: a block owns 16 RT rows and a run of 32-key steps;
-// its W waves share the head dim both for the scores and for the outputs, so that each value of the
-// cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave w < RT adds
-// those of rows 16 w .. + 15, in order, does their softmax and leaves the weights in LDS for all.
-// The next step's scores are formed before, so that one barrier per step makes both known.
+// Many rows of a cache whose scales all are plain, by the same mathematics: a block owns 16 RT rows and a
+// run of 32-key steps; its W waves share the head dim both for the scores and for the outputs, so that
+// each value of the cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave
+// w < RT adds those of rows 16 w .. + 15, in order, does their softmax and leaves the weights in LDS for
+// all.  The next step's scores are formed before, so that one barrier per step makes both known.
 // A block that meets another scale (or a q below 2^-99) says so in `redo`, and attn_kv4_kernel does
 // its rows again.
+// 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 95.8 us
+// traced, 0.76 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
+// step the matrix units are busy for 2050, of which a wave issues half while the other one of its
+// SIMD waits; the rest are vector instructions (280 per step of a wave that does softmax, 140 of the
+// others), the 64 KB of partial scores through LDS and back, and the barrier.  Tried and slower: 8
+// rows of softmax for each wave (105.7), softmax before the next step's scores (105.5), 32 rows per
+// block (129), two blocks of 4 waves per CU (alike).
 template <int HD, int RT, int W>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   constexpr int DW = HD / W, R = 16 * RT, NT = 2, KEYS = 16 * NT;
@@ -933,7 +949,7 @@ __device__ __forceinline__ void clear_redo(const Kv4Args &a) {
 
 // Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
 // one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
-// under way together and before their weights are known.
+// under way together and before their weights are known.  8 rows of 512 splits of 512: 8.4 MB in 4.2 us.
 template <int HD>
 __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
   constexpr int U = 8, G = 256 / U, N = 8, PER = kMaxSplits / 256;
@@ -994,7 +1010,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) { merge<HD>(a, blockIdx.x, blockIdx.y); }
 
 // Few rows whose keys' weights are asked for: both need the first kernel's sums alone, so the same
-// launch does the one and the other.
+// launch does the one and the other (one token of 32003 keys: 17.3 us in all, with two launches 21.3).
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, SumArgs w) {
   const int merges = a.s.rows * (HD / 32), b = blockIdx.x;
@@ -1002,7 +1018,8 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, 
   else add_weights(w, b - merges, 0);
 }
 
-// The same for up to 16 splits of many rows: a thread per 16-byte unit.
+// The same for up to 16 splits of many rows: a thread per 16-byte unit.  4096 rows of 4 splits of 512:
+// 42 MB in 10.7 us, 3.9 TB/s.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
   constexpr int MOST = 16;
