@@ -213,11 +213,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) vsr[j] = 16 * (j >> 2) + row_v + (j & 3) > last ? 0x3f80u : vsr[j];
   };
-  load_k(t0 + kg);
-  load_v(t0 + kg);
-  asm volatile("" ::: "memory");
-
-  // q: a thread takes 8 values of a row, whose largest gets the exponent 13
+  // q: a thread takes 8 values of a row, whose largest gets the exponent 13.  Its loads go first, so that
+  // it is worked on while the first k and v are under way (loads arrive in their order).
   {
     constexpr int TW = HD / 8, PASS = 64 * W / TW;
     constexpr int N = (R + PASS - 1) / PASS;
@@ -230,6 +227,10 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
       qx[i][0] = p[0];
       qx[i][1] = p[1];
     }
+    asm volatile("" ::: "memory");
+    load_k(t0 + kg);
+    load_v(t0 + kg);
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int pass = 0; pass < N; ++pass) {
       const int r = t / TW + pass * PASS;

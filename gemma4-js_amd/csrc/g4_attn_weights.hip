@@ -165,13 +165,12 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
       x[T][1] = *reinterpret_cast<const f32x4 *>(p + at + 128 * n + 64);
     }
   };
-#pragma unroll
-  for (int n = 0; n < (AHEAD == KN ? KN : 1); ++n) load_k(t0 + kg, n, kr[n]);
   {
     constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
     constexpr int N = (R + PASS - 1) / PASS < 4 ? (R + PASS - 1) / PASS : 4;  // rows of a thread under way together
     const int wd = t % TW;
-    for (int r0 = t / TW; r0 < R; r0 += PASS * N) {
+    for (int first = 0; first < R; first += PASS * N) {
+      const int r0 = first + t / TW;
       f32x4 x[N][2];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -179,6 +178,12 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
         const f32x4 *p = reinterpret_cast<const f32x4 *>(a.q + (size_t)row * HD + 32 * (wd >> 2) + 4 * (wd & 3));
         x[i][0] = p[0];
         x[i][1] = p[4];
+      }
+      if (first == 0) {  // (q's loads first: it is worked on while k's are under way)
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < (AHEAD == KN ? KN : 1); ++n) load_k(t0 + kg, n, kr[n]);
+        asm volatile("" ::: "memory");
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
