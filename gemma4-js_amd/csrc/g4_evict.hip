@@ -218,7 +218,9 @@ __global__ __launch_bounds__(256) void evict_list_kernel(EvictArgs a) {
   }
 }
 
-// ... the threshold's other bits from those, and the rows before each slice ...
+// ... the threshold's other bits from those, and the rows before each slice.  A wave takes slices w,
+// w + 16, .. and holds the first 256 of the bin's weights of two of them in registers, loaded beside
+// the bin's search ...
 __global__ __launch_bounds__(1024) void evict_threshold_kernel(EvictArgs a) {
   constexpr int NW = 16;
   __shared__ int hist[kBins];
@@ -226,6 +228,37 @@ __global__ __launch_bounds__(1024) void evict_threshold_kernel(EvictArgs a) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, set = blockIdx.x;
   const uint32_t *cand = a.cand + (size_t)set * a.slices * kSlice;
   int *count = a.count + (size_t)set * a.slices * 4;
+  constexpr int HELD = 2, PER = 4;
+  int n_held[HELD];
+  uint32_t held[HELD][PER];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) n_held[i] = wave + NW * i < a.slices ? count[4 * (wave + NW * i) + 1] : 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      held[i][j] = lane + 64 * j < n_held[i] ? cand[(size_t)(wave + NW * i) * kSlice + lane + 64 * j] : 0;
+  // f(weight) for this lane's of the wave's turn-th slice
+  auto each = [&](int turn, auto f) {
+    const int s = wave + NW * turn;
+    int i = lane, n;
+    if (turn < HELD) {
+      n = n_held[0];
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) {
+        if (h != turn) continue;
+        n = n_held[h];
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (lane + 64 * j < n) f(held[h][j]);
+      }
+      i += 64 * PER;
+    } else {
+      n = count[4 * s + 1];
+    }
+    for (; i < n; i += 64) f(cand[(size_t)s * kSlice + i]);
+  };
+  const int turns = (a.slices - wave + NW - 1) / NW;
   int want = a.keep - a.first - a.recent;
   find_bin<NW>(a.hist + set * kBins, want, tmp, found);
   for (int i = t; i < kBins; i += 1024) a.hist[set * kBins + i] = 0;  // for the next call
@@ -237,13 +270,10 @@ __global__ __launch_bounds__(1024) void evict_threshold_kernel(EvictArgs a) {
     for (int pass = 1; pass < 3; ++pass) {
       for (int i = t; i < kBins; i += 1024) hist[i] = 0;
       __syncthreads();
-      for (int s = wave; s < a.slices; s += NW) {
-        const int n = count[4 * s + 1];
-        for (int i = lane; i < n; i += 64) {
-          const uint32_t k = cand[(size_t)s * kSlice + i];
+      for (int turn = 0; turn < turns; ++turn)
+        each(turn, [&](uint32_t k) {
           if ((k & mask) == top) atomicAdd(&hist[digit(k, pass)], 1);
-        }
-      }
+        });
       __syncthreads();
       find_bin<NW>(hist, want, tmp, found);
       top |= (uint32_t)found[0] << digit_shift(pass);
@@ -253,19 +283,16 @@ __global__ __launch_bounds__(1024) void evict_threshold_kernel(EvictArgs a) {
     }
   }
   // each slice's rows above the threshold and equal to it
-  for (int s = wave; s < a.slices; s += NW) {
-    const int n = count[4 * s + 1];
+  for (int turn = 0; turn < turns; ++turn) {
+    const int s = wave + NW * turn;
     int above = 0, equal = 0;
-    for (int i = lane; i < n; i += 64) {
-      const uint32_t k = cand[(size_t)s * kSlice + i];
+    each(turn, [&](uint32_t k) {
       above += k > top ? 1 : 0;
       equal += k == top ? 1 : 0;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      above += __shfl_xor(above, o, 64);
-      equal += __shfl_xor(equal, o, 64);
-    }
+    });
+    // (whole numbers below 2^24 as floats)
+    above = (int)team_sum(64, (float)above);
+    equal = (int)team_sum(64, (float)equal);
     if (lane == 0) {
       count[4 * s + 2] = count[4 * s] + above;
       count[4 * s + 3] = equal;
