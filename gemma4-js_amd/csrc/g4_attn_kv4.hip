@@ -92,11 +92,11 @@ __device__ __forceinline__ bool usual_row(int e) { return e >= -120; }
 __device__ __forceinline__ float pow2_8_minus(int e) { return __int_as_float((135 - e) << 23); }
 __device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7) - 127, -100); }
 
-// Dims that a wave works on; the waves of a key group share the head dim.
+// Dims that a wave works on (DW); the waves of a key group share the head dim.
 template <int HD>
 constexpr int kDims = HD > 256 ? 256 : HD;
-template <int HD, int W>
-constexpr int kGroups = W / (HD / kDims<HD>);  // key groups of a block
+template <int HD, int W, int DW = kDims<HD>>
+constexpr int kGroups = W / (HD / DW);  // key groups of a block
 
 // x of lane c ^ 8 of each 16
 __device__ __forceinline__ float other_half(float x) {
@@ -121,9 +121,9 @@ __device__ __forceinline__ float other_half(float x) {
 // exponent, fused step) and the products between them, and as long again before and behind them
 // (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
 // 11.0 us, a chain of latencies.
-template <int HD, int RT, bool PAIR, int W>
+template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
-  constexpr int DW = kDims<HD>, DQ = HD / DW, KG = kGroups<HD, W>;
+  constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>;
   static_assert(!PAIR || RT == 1, "one tile");
   constexpr int KW = DW / 32;                  // words of a key per lane, and products
   constexpr int KS = DW >= 128 ? DW / 128 : 1; // scales of a key per lane
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
       u32x4 q[PAIR ? 1 : 2][RT][HD / 32][64];
       f32x4 sx[DQ > 1 ? 2 : 0][KG][DQ][RT][2][64];  // the waves' scores, two buffers
     } loop;
-    float o[KG / 2][OR][OS];
+    float o[KG > 1 ? KG / 2 : 1][OR][OS];
   };
   __shared__ Smem sm;
   __shared__ int xq[R];
@@ -252,8 +252,9 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
         hi4[i] = __builtin_bit_cast(uint32_t, h);
         lo4[i] = __builtin_bit_cast(uint32_t, l);
       }
-      const int n = HD >= 128 ? (wd >> 4) * 4 + (wd & 3) : wd & 1;
-      const int at = HD >= 128 ? (wd >> 2) & 3 : wd >> 1;
+      // the wave's lane (c, g) holds dims g DW / 4 .. of each 128, or of its 64
+      const int n = DW >= 128 ? (wd >> 4) * 4 + (wd & 3) : (wd >> 3) * 2 + (wd & 1);
+      const int at = DW >= 128 ? (wd >> 2) & 3 : (wd >> 1) & 3;
       sm.loop.q[0][r >> 4][n][(r & 15) + 16 * at] = hi4;
       sm.loop.q[PAIR ? 0 : 1][r >> 4][n][(r & 15) + 16 * at + (PAIR ? 8 : 0)] = lo4;
     }
@@ -1064,6 +1065,21 @@ struct Plan {
   void (*again)(Kv4Args);  // of 32 rows per block, where the first one may leave some undone
   int rows, keys, per_cu, threads;
 };
+// Up to 16 rows, a wave working on DW dims: whether a block per CU (of more than 8 rows, whose splits
+// cost more to join, per two) then has all keys at once.
+template <int HD, int DW>
+bool few_of(int rows, int keys, Plan &plan) {
+  constexpr int KEYS = kStep * kGroups<HD, 4, DW>;
+  if (rows <= 8) plan = {attn_kv4_kernel<HD, 1, true, 4, DW>, nullptr, 8, KEYS, 2, 256};
+  else plan = {attn_kv4_kernel<HD, 1, false, 4, DW>, nullptr, 16, KEYS, 2, 256};
+  return cdiv(keys, KEYS) <= (rows <= 8 ? cu_count() : cu_count() / 2);
+}
+
+// Few rows: less of a row per wave as long as there are CUs for the keys.  One token, us, with 64 / 128 /
+// 256 dims per wave: 4000 keys of 512 - / 9.9 / 11.3, 8000 - / 11.8 / 11.8, 30000 - / 16.2 / 15.6 (125,
+// 250 and 938 blocks of 128); 512 of 256 8.8 / 9.3 / 10.7, 4000 9.4 / 9.5 / 10.9, 16000 11.3 / 10.5 /
+// 11.7, 60000 19.7 / 15.3 / 13.9; of 128, 4000 8.7 / 9.1.  Two tokens: 4000 of 512 - / 12.3 / 12.5, 8000
+// - / 15.1 / 14.3.
 // Many rows of 512 whose 64-row blocks would have up to 4 steps each on all CUs: blocks of 32, which
 // start and end sooner.  us, 32 / 64 rows per block: 96 rows over 2000 keys (3 steps) 29.1 / 42.2, 128
 // over 2000 and 32 over 8000 (4) 32.2 / 35.4 and 30.9 / 32.3, 160 over 2000 (5) 44.3 / 36.4, 512
@@ -1071,8 +1087,18 @@ struct Plan {
 // four waves: 512 over 4608 70.6 / 84.7 (48 rows, two blocks: 76.6), 20 over 3000 17.5 / 23.0.
 template <int HD>
 Plan plan_of(int rows, int keys) {
-  if (rows <= 8) return {attn_kv4_kernel<HD, 1, true, 4>, nullptr, 8, kStep * kGroups<HD, 4>, 2, 256};
-  if (rows <= 16) return {attn_kv4_kernel<HD, 1, false, 4>, nullptr, 16, kStep * kGroups<HD, 4>, 2, 256};
+  if (rows <= 16) {
+    Plan plan;
+    if constexpr (HD == 512) {
+      if (few_of<HD, 128>(rows, keys, plan)) return plan;
+    } else if constexpr (HD == 256) {
+      if (few_of<HD, 64>(rows, keys, plan) || few_of<HD, 128>(rows, keys, plan)) return plan;
+    } else if constexpr (HD == 128) {
+      if (few_of<HD, 64>(rows, keys, plan)) return plan;
+    }
+    few_of<HD, kDims<HD>>(rows, 0, plan);
+    return plan;
+  }
   if constexpr (HD == 512) {
     if ((int64_t)cdiv(rows, 64) * cdiv(keys, 32) <= 4 * cu_count())
       return {attn_kv4_rows_kernel<HD, 2, 8>, attn_kv4_kernel<HD, 2, false, 4>, 32, 32, 1, 512};
