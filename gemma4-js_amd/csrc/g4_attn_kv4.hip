@@ -1023,11 +1023,11 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, 
 // The same for up to 16 splits of many rows: a thread per 16-byte unit.  4096 rows of 4 splits of 512:
 // 42 MB in 10.7 us, 3.9 TB/s.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
+__device__ __forceinline__ void join(const Kv4Args &a, int block) {
   constexpr int MOST = 16;
   const Scores &S = a.s;
-  const size_t unit = (size_t)blockIdx.x * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
-  if (blockIdx.x == 0) clear_redo(a);
+  const size_t unit = (size_t)block * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
+  if (block == 0) clear_redo(a);
   if (unit >= units) return;
   const float2 *ml = S.ml + unit / (HD / 4) * S.splits;
   const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part) + unit;
@@ -1051,6 +1051,16 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] /= L;
   reinterpret_cast<f32x4 *>(a.y)[unit] = y;
+}
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) { join<HD>(a, blockIdx.x); }
+
+// And with the keys' weights, as for few rows: 1624 rows over 2403 keys 49.6 us in all, with two launches 51.7.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_kv4_join_weights_kernel(Kv4Args a, SumArgs w, int joins, int tiles) {
+  const int b = blockIdx.x;
+  if (b < joins) join<HD>(a, b);
+  else add_weights(w, (b - joins) % tiles, (b - joins) / tiles);
 }
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
@@ -1158,16 +1168,26 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     G4_LAUNCH_CHECK("attn_kv4_merge_weights_kernel");
     return G4_OK;
   }
+  const int joins = (int)(((size_t)s.rows * (HD / 4) + 255) / 256);
+  const bool join = splits > 1 && s.rows >= 64 && splits <= 16;
+  float *part = a.part + n_part + n_score + n_ml;
+  if (join && weights) {
+    const SumArgs sums{s, keylen, before, weights, part};
+    const int tiles = cdiv(s.end - s.first, 256);
+    hipLaunchKernelGGL(attn_kv4_join_weights_kernel<HD>, dim3(joins + tiles * cdiv(s.rows, kGroup)), dim3(256), 0,
+                       stream(), a, sums, joins, tiles);
+    G4_LAUNCH_CHECK("attn_kv4_join_weights_kernel");
+    return launch_weights_join(s, keylen, part, before, weights);
+  }
   if (splits > 1) {
-    if (s.rows >= 64 && splits <= 16)
-      hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3((unsigned)(((size_t)s.rows * (HD / 4) + 255) / 256)), dim3(256),
-                         0, stream(), a);
+    if (join)
+      hipLaunchKernelGGL(attn_kv4_join_kernel<HD>, dim3(joins), dim3(256), 0, stream(), a);
     else
       hipLaunchKernelGGL(attn_kv4_merge_kernel<HD>, dim3(s.rows, HD / 32), dim3(256), 0, stream(), a);
     G4_LAUNCH_CHECK("attn_kv4_merge_kernel");
   }
   if (!weights) return G4_OK;
-  return launch_weights(s, keylen, a.part + n_part + n_score + n_ml, before, weights);
+  return launch_weights(s, keylen, part, before, weights);
 }
 
 }  // namespace

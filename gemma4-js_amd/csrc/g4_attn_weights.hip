@@ -71,16 +71,19 @@ size_t weight_part_floats(int rows, int keys) {
   return rows > kGroup ? (size_t)cdiv(rows, kGroup) * keys : 0;
 }
 
-int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights) {
-  SumArgs a{s, keylen, before, weights, s.rows > kGroup ? part : nullptr};
-  const int groups = s.rows > 0 ? cdiv(s.rows, kGroup) : 1;
-  hipLaunchKernelGGL(weights_kernel, dim3(cdiv(a.part ? s.end - s.first : keylen, 256), groups), dim3(256), 0,
-                     stream(), a);
-  G4_LAUNCH_CHECK("weights_kernel");
-  if (!a.part) return G4_OK;
-  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen, 64)), dim3(64), 0, stream(), a, groups);
+int launch_weights_join(const Scores &s, int keylen, float *part, const float *before, float *weights) {
+  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen, 64)), dim3(64), 0, stream(),
+                     (SumArgs{s, keylen, before, weights, part}), cdiv(s.rows, kGroup));
   G4_LAUNCH_CHECK("weights_join_kernel");
   return G4_OK;
+}
+
+int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights) {
+  const bool several = s.rows > kGroup;
+  hipLaunchKernelGGL(weights_kernel, dim3(cdiv(several ? s.end - s.first : keylen, 256), several ? cdiv(s.rows, kGroup) : 1),
+                     dim3(256), 0, stream(), (SumArgs{s, keylen, before, weights, several ? part : nullptr}));
+  G4_LAUNCH_CHECK("weights_kernel");
+  return several ? launch_weights_join(s, keylen, part, before, weights) : G4_OK;
 }
 
 namespace {

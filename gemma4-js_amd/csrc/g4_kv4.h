@@ -35,6 +35,8 @@ size_t score_floats(int rows, size_t stride);
 // `part` holds weight_part_floats(rows, end - first).
 size_t weight_part_floats(int rows, int keys);
 int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights);
+// Its second launch alone, for more than 32 rows: the sums of each 32 rows are in `part`.
+int launch_weights_join(const Scores &s, int keylen, float *part, const float *before, float *weights);
 
 // Arguments that g4_attention_kv4 and g4_attention_weights have in common.
 int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int window,
