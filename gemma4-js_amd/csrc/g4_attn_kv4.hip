@@ -116,11 +116,12 @@ __device__ __forceinline__ float other_half(float x) {
 // nothing of k or v passes through LDS.  A row's maximum is a reference that follows the scores with
 // kSlack, so the outputs are hardly ever scaled again; a step's loads are under way during the one
 // before it.  Scales outside 2^-12 .. 8 take a slower way with exponents per row.
-// What bounds it: one token over 131072 keys of 512 (75.5 MB) 24.4 us traced, 3.1 TB/s: 4 steps per
+// What bounds it: one token over 131072 keys of 512 (75.5 MB) 23.3 us traced, 3.2 TB/s: 4 steps per
 // wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
 // exponent, fused step) and the products between them, and as long again before and behind them
 // (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
-// 11.0 us, a chain of latencies.
+// 10.2 us, a chain of latencies (launch and arguments 1.2, q and the first k 1.8, the scores 1.1, softmax and
+// outputs 1.9, the groups' sums and stores 1.9).
 template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>;
@@ -599,8 +600,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 // all.  The next step's scores are formed before, so that one barrier per step makes both known.
 // A block that meets another scale (or a q below 2^-99) says so in `redo`, and attn_kv4_kernel does
 // its rows again.
-// 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 95.8 us
-// traced, 0.76 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
+// 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 94.0 us
+// traced, 0.78 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
 // step the matrix units are busy for 2050, of which a wave issues half while the other one of its
 // SIMD waits; the rest are vector instructions (280 per step of a wave that does softmax, 140 of the
 // others), the 64 KB of partial scores through LDS and back, and the barrier.  Tried and slower: 8
@@ -1012,7 +1013,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) { merge<HD>(a, blockIdx.x, blockIdx.y); }
 
 // Few rows whose keys' weights are asked for: both need the first kernel's sums alone, so the same
-// launch does the one and the other (one token of 32003 keys: 17.3 us in all, with two launches 21.3).
+// launch does the one and the other (one token of 32003 keys: 16.0 us in all; when it came in 17.3, with two launches 21.3).
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, SumArgs w) {
   const int merges = a.s.rows * (HD / 32), b = blockIdx.x;

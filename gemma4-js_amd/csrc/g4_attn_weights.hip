@@ -136,7 +136,7 @@ __device__ __forceinline__ float group_max(float v) {
 // 2^-22 of a product), q with its row's largest at the exponent 13, k times 2^8; a wave in which a
 // key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.
 // One token over 8001 keys of 512 (16.4 MB): 7.0 us traced, a step per wave whose loads are all
-// under way before q is ready; over 131072 keys 268 MB in 61 us with the sums, 4.4 TB/s: memory.
+// under way before q is ready; over 131072 keys 268 MB in 60 us with the sums, 4.5 TB/s: memory.
 template <int HD, int DQ, int NT, int RT>
 __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   constexpr int KG = kWaves / DQ, DW = HD / DQ, KN = DW / 32, R = 16 * RT, KEYS = 16 * NT;
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 // k times 2^8 in FP16 ends at 2^-24: what is lost of each is 2^-33, which 512 q below 16 make less
 // than 10^-6 of a score.  A block with a k of 128 or more, with larger q and a key that is below
 // 2^-10 throughout, or with a q below 2^-99, says so in `redo`, and scores_kernel does its rows again.
-// 256 rows over 4096 keys of 512 (8 heads, 26 GFLOP with the three products): 49 us traced.  Before
+// 256 rows over 4096 keys of 512 (8 heads, 25 GFLOP with the three products): 48 us traced.  Before
 // its first step a block needs 10 us (its 128 KB of q 3.7, their parts 1.8, the first keys and
 // products 3); a step takes 2.3: without its loads the call would take 11 us less, without two of its
 // three products 4, without a third of its vector instructions nothing.  The whole call, 57: with 32

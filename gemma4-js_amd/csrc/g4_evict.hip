@@ -159,9 +159,9 @@ __global__ __launch_bounds__(64 * NW) void evict_kernel(EvictArgs a) {
 }
 
 // Longer caches, a block of 256 threads per slice of 4096 weights (blockIdx.x), four launches: the
-// histogram of the first 11 bits ...  131072 weights: 3.4, 4.8, 7.9 and 5.1 us traced, each little more
-// than its loads' latencies; 2^20 weights 56 us.  (The bin's weights in the third kernel's registers
-// instead of read for each step: 11.2 us, as each has to find its slice.)
+// histogram of the first 11 bits ...  131072 weights: 3.5, 4.8, 7.1 and 5.3 us traced, each little more
+// than its loads' latencies; 2^20 weights 54 us in all.  (All of the bin's weights in the third kernel's
+// registers, each with its slice looked up: 11.2 us.)
 __global__ __launch_bounds__(256) void evict_count_kernel(EvictArgs a) {
   __shared__ int hist[kBins];
   const int t = threadIdx.x, set = blockIdx.y, end = a.len - a.recent;
