@@ -33,11 +33,6 @@ struct Kv4Args {
   float *y;
   float *part;  // [splits][rows][hd], each split's outputs
   Scores s;     // score null: not kept
-  // attn_kv4_rows_kernel's row blocks to do again: set by a block, and with one split also cleared;
-  // with several, all are 0 between calls, as the splits' join leaves them
-  uint32_t *redo;
-  int blocks;
-  int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
 // BF16 bits of the least plain scale, 2^-12, and how many there are, below 8.
@@ -122,38 +117,49 @@ __device__ __forceinline__ float other_half(float x) {
 // (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
 // 10.2 us, a chain of latencies (launch and arguments 1.2, q and the first k 1.8, the scores 1.1, softmax and
 // outputs 1.9, the groups' sums and stores 1.9).
-template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
-__global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
+// The keys that some of rows R0 .. R0 + n - 1 see, lo .. hi - 1, and a split's steps of them.
+struct Run {
+  int lo, hi, steps, t0, t1;
+  __device__ __forceinline__ Run(const Scores &S, int R0, int n, int split) {
+    const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + n, S.rows) - 1) / S.heads;
+    lo = S.first;
+    if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+    hi = pb + 1;
+    steps = (hi - lo + kStep - 1) / kStep;
+    const int per = (steps + S.splits - 1) / S.splits;
+    t0 = split * per;
+    t1 = min(t0 + per, steps);
+  }
+};
+
+template <int HD, int RT, bool PAIR, int W, int DW>
+struct AttendSmem {
+  static constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>, R = PAIR ? 8 : 16 * RT;
+  union {
+    struct {
+      u32x4 q[PAIR ? 1 : 2][RT][HD / 32][64];
+      f32x4 sx[DQ > 1 ? 2 : 0][KG][DQ][RT][2][64];  // the waves' scores, two buffers
+    } loop;
+    float o[KG > 1 ? KG / 2 : 1][PAIR ? 8 : 16][HD + 4];
+  };
+  int xq[R];
+  float2 wml[KG][R];
+};
+template <int HD, int RT, bool PAIR, int W, int DW>
+__device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, const Run &run, AttendSmem<HD, RT, PAIR, W, DW> &sm) {
   constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>;
   static_assert(!PAIR || RT == 1, "one tile");
   constexpr int KW = DW / 32;                  // words of a key per lane, and products
   constexpr int KS = DW >= 128 ? DW / 128 : 1; // scales of a key per lane
   constexpr int VD = DW / 16;                  // dims per lane, and output tiles
   constexpr int VW = VD >= 8 ? VD / 8 : 1;     // words of them (64: half a word)
-  constexpr int R = PAIR ? 8 : 16 * RT, OR = PAIR ? 8 : 16, OS = HD + 4;
-  union Smem {
-    struct {
-      u32x4 q[PAIR ? 1 : 2][RT][HD / 32][64];
-      f32x4 sx[DQ > 1 ? 2 : 0][KG][DQ][RT][2][64];  // the waves' scores, two buffers
-    } loop;
-    float o[KG > 1 ? KG / 2 : 1][OR][OS];
-  };
-  __shared__ Smem sm;
-  __shared__ int xq[R];
-  __shared__ float2 wml[KG][R];
+  constexpr int R = PAIR ? 8 : 16 * RT;
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
   const int cr = PAIR ? c & 7 : c;  // the lane's row of a tile
-  const int R0 = blockIdx.x * R, split = blockIdx.y;
-  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] == 0) return;
-  // the rows' positions, and the keys that some of them see
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
-  int lo = S.first;
-  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
-  const int hi = pb + 1, steps = (hi - lo + kStep - 1) / kStep;
-  const int per = (steps + S.splits - 1) / S.splits;
-  const int t0 = split * per, t1 = min(t0 + per, steps);
+  const int lo = run.lo, hi = run.hi, steps = run.steps, t0 = run.t0, t1 = run.t1;
 
   uint32_t kr[2][KW], ksr[2][KS], vr[8][VW], vsr[8];
   // Loads by an offset per lane from a step's first row; rows behind the last key give zeros, which
@@ -243,7 +249,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
       top = team_max<TW>(top);
       const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (r >= R) break;
-      if (wd == 0) xq[r] = e - 21;  // (8 of the scales)
+      if (wd == 0) sm.xq[r] = e - 21;  // (8 of the scales)
       u32x4 hi4, lo4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     pos[r] = S.pos0 + min(R0 + 16 * r + cr, S.rows - 1) / S.heads;
-    xe[r] = xq[16 * r + cr];
+    xe[r] = sm.xq[16 * r + cr];
     xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
     usual = usual && usual_row(xe[r]);
     m[r] = kNoScore;
@@ -530,7 +536,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   for (int r = 0; r < RT; ++r) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
-    if (g == 0 && dq == 0) wml[kg][16 * r + cr] = make_float2(m[r], l[r]);
+    if (g == 0 && dq == 0) sm.wml[kg][16 * r + cr] = make_float2(m[r], l[r]);
   }
   __syncthreads();
   const bool whole = S.splits == 1;
@@ -539,10 +545,10 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   for (int r = 0; r < RT; ++r) {
     float M = kNoScore, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][16 * r + cr].x);
+    for (int i = 0; i < KG; ++i) M = fmaxf(M, sm.wml[i][16 * r + cr].x);
 #pragma unroll
     for (int i = 0; i < KG; ++i)
-      L = fmaf(wml[i][16 * r + cr].y, __builtin_amdgcn_exp2f(wml[i][16 * r + cr].x - M), L);
+      L = fmaf(sm.wml[i][16 * r + cr].y, __builtin_amdgcn_exp2f(sm.wml[i][16 * r + cr].x - M), L);
     const int row = R0 + 16 * r + cr;
     if (S.ml && w == 0 && g == 0 && row < S.rows) S.ml[(size_t)row * S.splits + split] = make_float2(M, L);
     // (a split of which the row sees nothing: 0, not 0 / 0)
@@ -593,13 +599,19 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   }
 }
 
+template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
+__global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
+  __shared__ AttendSmem<HD, RT, PAIR, W, DW> sm;
+  attend<HD, RT, PAIR, W, DW>(a, blockIdx.x * sm.R, blockIdx.y, Run(a.s, blockIdx.x * sm.R, sm.R, blockIdx.y), sm);
+}
+
 // Many rows of a cache whose scales all are plain, by the same mathematics: a block owns 16 RT rows and a
 // run of 32-key steps; its W waves share the head dim both for the scores and for the outputs, so that
 // each value of the cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave
 // w < RT adds those of rows 16 w .. + 15, in order, does their softmax and leaves the weights in LDS for
 // all.  The next step's scores are formed before, so that one barrier per step makes both known.
-// A block that meets another scale (or a q below 2^-99) says so in `redo`, and attn_kv4_kernel does
-// its rows again.
+// A block that met another scale (or a q below 2^-99) does its rows again in the general way, 16 at a
+// time (a second launch for them cost all calls 2 to 3 us).
 // 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 94.0 us
 // traced, 0.78 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
 // step the matrix units are busy for 2050, of which a wave issues half while the other one of its
@@ -608,18 +620,20 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 // rows of softmax for each wave (105.7), softmax before the next step's scores (105.5), 32 rows per
 // block (129), two blocks of 4 waves per CU (alike).
 template <int HD, int RT, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(Kv4Args a) {
   constexpr int DW = HD / W, R = 16 * RT, NT = 2, KEYS = 16 * NT;
   constexpr int KN = DW / 32;         // words of a key per lane, and products
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
   static_assert(DW == 64, "32 bytes of a row per wave");
   // (two of each: what the step's readers may still look at, and the next)
+  using General = AttendSmem<HD, 1, false, W, DW>;
   union Smem {
     struct {
       f32x4 sx[2][W][RT][NT][64];
       u32x4 sp[2][RT][2][64];
     };
     float rows[R][HD + 4];  // q and the outputs, on their way from and to whole lines of memory
+    General general;
   };
   __shared__ Smem sm;
   __shared__ u32x4 sv[W][64];         // v's codes of a step
@@ -632,11 +646,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const int c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
-  int lo = S.first;
-  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
-  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
-  const int per = (steps + S.splits - 1) / S.splits;
-  const int t0 = split * per, t1 = min(t0 + per, steps);
+  const Run run(S, R0, R, split);
+  const int lo = run.lo, hi = run.hi, steps = run.steps, t0 = run.t0, t1 = run.t1;
   ushort2_t beyond = {0, 0};  // the scales' largest distance from the least plain one
 
   // A lane loads 16 bytes and a scale of a key, and of a v: lane (c, g) key 16 (g / 2) + c, bytes
@@ -908,8 +919,20 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
     }
   }
 
-  const bool again = __any(max(beyond[0], beyond[1]) >= kPlainScales);
-  if (lane == 0) stop[w][0] = again;
+  const bool odd = __any(max(beyond[0], beyond[1]) >= kPlainScales);
+  __syncthreads();
+  if (lane == 0) stop[w][0] = odd;
+  __syncthreads();
+  int again = 0;
+#pragma unroll
+  for (int d = 0; d < W; ++d) again |= stop[d][0];
+  if (__builtin_amdgcn_readfirstlane(again)) {
+    for (int r = 0; r < R && R0 + r < S.rows; r += 16) {
+      __syncthreads();
+      attend<HD, 1, false, W, DW>(a, R0 + r, split, run, sm.general);
+    }
+    return;
+  }
   const bool whole = S.splits == 1;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -918,12 +941,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 23);
   __syncthreads();  // (sf is read to the last step's end)
   if (w < RT && g == 0) sf[0][16 * w + c] = fin;
-  if (t == 0) {
-    int some = 0;
-#pragma unroll
-    for (int d = 0; d < W; ++d) some |= stop[d][0];
-    if (whole || some) a.redo[blockIdx.x] = some;
-  }
   __syncthreads();
   float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
 #pragma unroll
@@ -946,10 +963,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_rows_kernel(Kv4Args a) {
   }
 }
 
-__device__ __forceinline__ void clear_redo(const Kv4Args &a) {
-  for (int i = threadIdx.x; i < a.blocks; i += 256) a.redo[i] = 0;
-}
-
 // Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
 // one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
 // under way together and before their weights are known.  8 rows of 512 splits of 512: 8.4 MB in 4.2 us.
@@ -968,7 +981,6 @@ __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = p[min(s0 + G * i, S.splits - 1) * step];
   };
-  if (row == 0 && part == 0) clear_redo(a);
   float2 ml[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) ml[i] = S.ml[(size_t)row * S.splits + min(t + 256 * i, S.splits - 1)];
@@ -1028,7 +1040,6 @@ __device__ __forceinline__ void join(const Kv4Args &a, int block) {
   constexpr int MOST = 16;
   const Scores &S = a.s;
   const size_t unit = (size_t)block * 256 + threadIdx.x, units = (size_t)S.rows * (HD / 4);
-  if (block == 0) clear_redo(a);
   if (unit >= units) return;
   const float2 *ml = S.ml + unit / (HD / 4) * S.splits;
   const f32x4 *p = reinterpret_cast<const f32x4 *>(a.part) + unit;
@@ -1066,14 +1077,12 @@ __global__ __launch_bounds__(256) void attn_kv4_join_weights_kernel(Kv4Args a, S
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-Workspace g_kv4_ws, g_redo_ws;
-constexpr int kMostMarks = 512;  // row blocks of a call of several splits: no more than fit at once
+Workspace g_kv4_ws;
 
 // The kernel for the call's rows: its rows per block, keys per step of all its waves, blocks per
 // CU and threads.
 struct Plan {
   void (*kernel)(Kv4Args);
-  void (*again)(Kv4Args);  // of 32 rows per block, where the first one may leave some undone
   int rows, keys, per_cu, threads;
 };
 // Up to 16 rows, a wave working on DW dims: whether a block per CU (of more than 8 rows, whose splits
@@ -1081,8 +1090,8 @@ struct Plan {
 template <int HD, int DW>
 bool few_of(int rows, int keys, Plan &plan) {
   constexpr int KEYS = kStep * kGroups<HD, 4, DW>;
-  if (rows <= 8) plan = {attn_kv4_kernel<HD, 1, true, 4, DW>, nullptr, 8, KEYS, 2, 256};
-  else plan = {attn_kv4_kernel<HD, 1, false, 4, DW>, nullptr, 16, KEYS, 2, 256};
+  if (rows <= 8) plan = {attn_kv4_kernel<HD, 1, true, 4, DW>, 8, KEYS, 2, 256};
+  else plan = {attn_kv4_kernel<HD, 1, false, 4, DW>, 16, KEYS, 2, 256};
   return cdiv(keys, KEYS) <= (rows <= 8 ? cu_count() : cu_count() / 2);
 }
 
@@ -1112,11 +1121,11 @@ Plan plan_of(int rows, int keys) {
   }
   if constexpr (HD == 512) {
     if ((int64_t)cdiv(rows, 64) * cdiv(keys, 32) <= 4 * cu_count())
-      return {attn_kv4_rows_kernel<HD, 2, 8>, attn_kv4_kernel<HD, 2, false, 4>, 32, 32, 1, 512};
-    return {attn_kv4_rows_kernel<HD, 4, 8>, attn_kv4_kernel<HD, 2, false, 4>, 64, 32, 1, 512};
+      return {attn_kv4_rows_kernel<HD, 2, 8>, 32, 32, 1, 512};
+    return {attn_kv4_rows_kernel<HD, 4, 8>, 64, 32, 1, 512};
   }
-  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 2, 4>, attn_kv4_kernel<HD, 2, false, 4>, 32, 32, 3, 256};
-  else return {attn_kv4_kernel<HD, 2, false, 4>, nullptr, 32, kStep * kGroups<HD, 4>, 2, 256};
+  else if constexpr (HD == 256) return {attn_kv4_rows_kernel<HD, 2, 4>, 32, 32, 3, 256};
+  else return {attn_kv4_kernel<HD, 2, false, 4>, 32, kStep * kGroups<HD, 4>, 2, 256};
 }
 
 // The rows of a.s, all at once; `before` and `weights` of this call.
@@ -1135,7 +1144,7 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   if (turns >= 4 * plan.per_cu * splits) splits = plan.per_cu * cu_count() / blocks;
   if (splits > turns) splits = turns;
   if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits < 1 || blocks > kMostMarks) splits = 1;
+  if (splits < 1) splits = 1;
   s.splits = splits;
   const bool ml = weights || splits > 1;
   const size_t n_part = splits > 1 ? (size_t)splits * s.rows * HD : 0, n_ml = ml ? (size_t)splits * s.rows * 2 : 0;
@@ -1148,20 +1157,8 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
     s.score = weights ? a.part + n_part : nullptr;
     s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
   }
-  if (plan.again) {
-    // (the marks of calls with one split lie behind the others: they are not left 0)
-    void *mem = nullptr;
-    if (int rc = g_redo_ws.get((size_t)(kMostMarks + blocks) * 4, &mem, "g4_attention_kv4")) return rc;
-    a.redo = static_cast<uint32_t *>(mem) + (splits > 1 ? 0 : kMostMarks);
-    a.blocks = blocks;
-  }
   hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(plan.threads), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
-  if (plan.again) {
-    a.redo_rows = plan.rows;
-    hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 32), splits), dim3(256), 0, stream(), a);
-    G4_LAUNCH_CHECK("attn_kv4_kernel");
-  }
   if (splits > 1 && weights && s.rows <= kGroup) {
     const SumArgs sums{s, keylen, before, weights, nullptr};
     hipLaunchKernelGGL(attn_kv4_merge_weights_kernel<HD>, dim3(s.rows * (HD / 32) + cdiv(keylen, 256)), dim3(256), 0,
