@@ -35,8 +35,10 @@ struct Kv4Args {
   Scores s;     // score null: not kept
 };
 
-// BF16 bits of the least plain scale, 2^-12, and how many there are, below 8.
-constexpr uint16_t kLeastScale = (127 - 12) << 7, kPlainScales = 15 << 7;
+// Scales are taken times 2^kLift.  Plain ones, from 2^-18 up to 2^7, then are normal FP16 numbers, and
+// so are eight times they: BF16 bits of the least and how many there are.
+constexpr int kLift = 4;
+constexpr uint16_t kLeastScale = (127 - 14 - kLift) << 7, kPlainScales = 25 << 7;
 
 // Eight values of a cache as FP16, in pairs (0, 4) (1, 5) (2, 6) (3, 7) of the word's nibbles or of
 // two words' halves: a nibble n in the mantissa's upper four bits under the exponent of 16 is
@@ -57,12 +59,12 @@ struct Magic {
   }
 };
 // The same for two BF16 scales as they are: FP16 bits by whole numbers, and how far they lie from the
-// least plain one, kept as the largest seen (a plain scale times 2^8 is a normal FP16 number).
+// least plain one, kept as the largest seen.
 __device__ __forceinline__ Scale plain_pair(uint32_t lo, uint32_t hi, ushort2_t &beyond) {
   const ushort2_t u = __builtin_bit_cast(ushort2_t, __builtin_amdgcn_perm(hi, lo, 0x05040100u));
   const ushort2_t d = u - (ushort2_t){kLeastScale, kLeastScale};
   beyond = __builtin_elementwise_max(beyond, d);
-  constexpr uint16_t least = (kLeastScale - ((127 - 8 - 15) << 7)) << 3;
+  constexpr uint16_t least = (kLeastScale - ((127 - kLift - 15) << 7)) << 3;
   return scale_of(__builtin_bit_cast(half2_t, (ushort2_t)(d * (ushort2_t){8, 8} + (ushort2_t){least, least})));
 }
 template <int T>
@@ -110,28 +112,13 @@ __device__ __forceinline__ float other_half(float x) {
 // The values are used where they are unpacked, in the lanes that the matrix instructions want them:
 // nothing of k or v passes through LDS.  A row's maximum is a reference that follows the scores with
 // kSlack, so the outputs are hardly ever scaled again; a step's loads are under way during the one
-// before it.  Scales outside 2^-12 .. 8 take a slower way with exponents per row.
+// before it.  Scales that are not plain take a slower way with exponents per row.
 // What bounds it: one token over 131072 keys of 512 (75.5 MB) 23.3 us traced, 3.2 TB/s: 4 steps per
 // wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
 // exponent, fused step) and the products between them, and as long again before and behind them
 // (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
 // 10.2 us, a chain of latencies (launch and arguments 1.2, q and the first k 1.8, the scores 1.1, softmax and
 // outputs 1.9, the groups' sums and stores 1.9).
-// The keys that some of rows R0 .. R0 + n - 1 see, lo .. hi - 1, and a split's steps of them.
-struct Run {
-  int lo, hi, steps, t0, t1;
-  __device__ __forceinline__ Run(const Scores &S, int R0, int n, int split) {
-    const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + n, S.rows) - 1) / S.heads;
-    lo = S.first;
-    if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
-    hi = pb + 1;
-    steps = (hi - lo + kStep - 1) / kStep;
-    const int per = (steps + S.splits - 1) / S.splits;
-    t0 = split * per;
-    t1 = min(t0 + per, steps);
-  }
-};
-
 template <int HD, int RT, bool PAIR, int W, int DW>
 struct AttendSmem {
   static constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>, R = PAIR ? 8 : 16 * RT;
@@ -249,7 +236,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
       top = team_max<TW>(top);
       const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
       if (r >= R) break;
-      if (wd == 0) sm.xq[r] = e - 21;  // (8 of the scales)
+      if (wd == 0) sm.xq[r] = e - 13 - kLift;
       u32x4 hi4, lo4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -280,7 +267,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     usual = usual && usual_row(xe[r]);
     m[r] = kNoScore;
     l[r] = 0.f;
-    E[r] = -1000.f;  // outputs are held times 2^(23 - E)
+    E[r] = -1000.f;  // outputs are held times 2^(15 + kLift - E)
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
@@ -319,7 +306,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
             x[T][J] = scale_pair(f, f);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e, 4 * g + i, 64) & 255) << (8 * i);
+          for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e - 8 + kLift, 4 * g + i, 64) & 255) << (8 * i);
         }
       }
     }
@@ -414,7 +401,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
           vsr[j] = u = 0;
         }
         const int e = scale_exponent(team_max<16>(u));
-        ve[j >> 2] |= (uint32_t)(e & 255) << (8 * (j & 3));
+        ve[j >> 2] |= (uint32_t)((e - 8 + kLift) & 255) << (8 * (j & 3));
         f[j] = bf16_to_f32(vsr[j]) * pow2_8_minus(e);
       }
 #pragma unroll
@@ -554,7 +541,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     // (a split of which the row sees nothing: 0, not 0 / 0)
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
     if (!whole && L == 0.f) f = 0.f;
-    f = ldexpf(f, (int)E[r] - 23);
+    f = ldexpf(f, (int)E[r] - 15 - kLift);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
@@ -602,7 +589,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
 template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   __shared__ AttendSmem<HD, RT, PAIR, W, DW> sm;
-  attend<HD, RT, PAIR, W, DW>(a, blockIdx.x * sm.R, blockIdx.y, Run(a.s, blockIdx.x * sm.R, sm.R, blockIdx.y), sm);
+  attend<HD, RT, PAIR, W, DW>(a, blockIdx.x * sm.R, blockIdx.y, Run(a.s, blockIdx.x * sm.R, sm.R, blockIdx.y, kStep), sm);
 }
 
 // Many rows of a cache whose scales all are plain, by the same mathematics: a block owns 16 RT rows and a
@@ -610,7 +597,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 // each value of the cache is unpacked once for all rows.  The waves' partial scores go through LDS; wave
 // w < RT adds those of rows 16 w .. + 15, in order, does their softmax and leaves the weights in LDS for
 // all.  The next step's scores are formed before, so that one barrier per step makes both known.
-// A block that met another scale (or a q below 2^-99) does its rows again in the general way, 16 at a
+// A block that met another scale (or a row of q below 2^-103) does its rows again in the general way, 16 at a
 // time (a second launch for them cost all calls 2 to 3 us).
 // 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 94.0 us
 // traced, 0.78 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
@@ -626,7 +613,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
   static_assert(DW == 64, "32 bytes of a row per wave");
   // (two of each: what the step's readers may still look at, and the next)
-  using General = AttendSmem<HD, 1, false, W, DW>;
+  using General = AttendSmem<HD, 1, false, W, DW>;  // (of 32 rows: spills that all calls feel, 102.7 us for 94)
   union Smem {
     struct {
       f32x4 sx[2][W][RT][NT][64];
@@ -646,7 +633,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   const int c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
-  const Run run(S, R0, R, split);
+  const Run run(S, R0, R, split, KEYS);
   const int lo = run.lo, hi = run.hi, steps = run.steps, t0 = run.t0, t1 = run.t1;
   ushort2_t beyond = {0, 0};  // the scales' largest distance from the least plain one
 
@@ -721,8 +708,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
 #pragma unroll
       for (int d = 0; d < W; ++d) top = max(top, stop[d][16 * r + c]);
       const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
-      if (w == 0 && g == 0) sxq[16 * r + c] = e - 21;  // (8 of the scales)
-      if (!usual_row(e - 21)) beyond = (ushort2_t){0xffff, 0xffff};
+      if (w == 0 && g == 0) sxq[16 * r + c] = e - 13 - kLift;
+      if (!usual_row(e - 13 - kLift)) beyond = (ushort2_t){0xffff, 0xffff};
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
         u32x4 h4, l4;
@@ -784,7 +771,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
 
   constexpr float kWeight = 1 << (15 - (int)kSlack);
   float m = kNoScore, l = 0.f;  // of row 16 w + c
-  f32x4 o[RT][VD];              // outputs times 2^(23 - kSlack)
+  f32x4 o[RT][VD];              // outputs times 2^(15 + kLift - kSlack)
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -938,7 +925,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   l += __shfl_xor(l, 32, 64);
   if (S.ml && w < RT && g == 0 && my_row < S.rows) S.ml[(size_t)my_row * S.splits + split] = make_float2(m, l);
   // (a split of which the row sees nothing: 0, not 0 / 0)
-  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 23);
+  const float fin = !whole && l == 0.f ? 0.f : ldexpf(1.f / l, (int)kSlack - 15 - kLift);
   __syncthreads();  // (sf is read to the last step's end)
   if (w < RT && g == 0) sf[0][16 * w + c] = fin;
   __syncthreads();

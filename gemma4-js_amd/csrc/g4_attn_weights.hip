@@ -97,9 +97,6 @@ constexpr int kWaves = 4;
 struct ScoreArgs {
   const float *q, *k;
   Scores s;
-  // scores_rows_kernel's row blocks to do again; all 0 between calls, as weights_kernel leaves them
-  uint32_t *redo;
-  int redo_rows;  // > 0: only rows of such blocks, of this many
 };
 
 // Eight FP32 values, times `up`, as sums of two FP16 values.
@@ -137,25 +134,24 @@ __device__ __forceinline__ float group_max(float v) {
 // key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.
 // One token over 8001 keys of 512 (16.4 MB): 7.0 us traced, a step per wave whose loads are all
 // under way before q is ready; over 131072 keys 268 MB in 60 us with the sums, 4.5 TB/s: memory.
-template <int HD, int DQ, int NT, int RT>
-__global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
-  constexpr int KG = kWaves / DQ, DW = HD / DQ, KN = DW / 32, R = 16 * RT, KEYS = 16 * NT;
+template <int HD, int DQ, int NT, int RT, int W>
+struct ScoreSmem {
+  static constexpr int KG = W / DQ, R = 16 * RT;
+  u32x4 q[2][RT][HD / 32][64];
+  f32x4 sx[DQ > 1 ? 2 : 1][KG][DQ][DQ > 1 ? RT : 1][DQ > 1 ? NT : 1][DQ > 1 ? 64 : 1];
+  int xq[R];
+  float2 wml[KG][R];
+};
+template <int HD, int DQ, int NT, int RT, int W>
+__device__ __forceinline__ void few_scores(const ScoreArgs &a, int R0, int split, const Run &run,
+                                           ScoreSmem<HD, DQ, NT, RT, W> &sm) {
+  constexpr int KG = W / DQ, DW = HD / DQ, KN = DW / 32, R = 16 * RT, KEYS = 16 * NT;
   constexpr int AHEAD = NT * KN <= 4 ? KN : 2;  // a step's loads that are under way together
-  __shared__ u32x4 sq[2][RT][HD / 32][64];
-  __shared__ f32x4 sx[DQ > 1 ? 2 : 1][KG][DQ][DQ > 1 ? RT : 1][DQ > 1 ? NT : 1][DQ > 1 ? 64 : 1];
-  __shared__ int xq[R];
-  __shared__ float2 wml[KG][R];
   const Scores &S = a.s;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / DQ, dq = w % DQ, c = lane & 15, g = lane >> 4;
-  const int R0 = blockIdx.x * R, split = blockIdx.y;
-  if (a.redo_rows > 0 && a.redo[R0 / a.redo_rows] == 0) return;
   const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
-  int lo = S.first;
-  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
-  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
-  const int per = (steps + S.splits - 1) / S.splits;
-  const int t0 = split * per, t1 = min(t0 + per, steps);
+  const int lo = run.lo, hi = run.hi, steps = run.steps, t0 = run.t0, t1 = run.t1;
 
   f32x4 kr[AHEAD][NT][2];
   auto load_k = [&](int step, int n, f32x4 (&x)[NT][2]) {
@@ -169,7 +165,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
     }
   };
   {
-    constexpr int TW = HD / 8, PASS = 64 * kWaves / TW;
+    constexpr int TW = HD / 8, PASS = 64 * W / TW;
     constexpr int N = (R + PASS - 1) / PASS < 4 ? (R + PASS - 1) / PASS : 4;  // rows of a thread under way together
     const int wd = t % TW;
     for (int first = 0; first < R; first += PASS * N) {
@@ -199,13 +195,13 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
         top = team_max<TW>(top);
         const int e = top == 0 || top >= 0x7f800000 ? 0 : max((top >> 23) - 127, -126);
         if (r >= R) break;
-        if (wd == 0) xq[r] = e - 13;
+        if (wd == 0) sm.xq[r] = e - 13;
 #pragma unroll
         for (int d = 0; d < 4; ++d) x0[d] = ldexpf(x0[d], 13 - e), x1[d] = ldexpf(x1[d], 13 - e);
         half8_t h, l;
         halves(x0, x1, 1.f, h, l);
-        sq[0][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, h);
-        sq[1][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, l);
+        sm.q[0][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, h);
+        sm.q[1][r >> 4][wd >> 2][(r & 15) + 16 * (wd & 3)] = __builtin_bit_cast(u32x4, l);
       }
     }
   }
@@ -216,7 +212,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     pos[r] = S.pos0 + min(R0 + 16 * r + c, S.rows - 1) / S.heads;
-    xe[r] = xq[16 * r + c];
+    xe[r] = sm.xq[16 * r + c];
     m[r] = kNoScore;
     l[r] = 0.f;
   }
@@ -251,8 +247,8 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const half8_t qh = __builtin_bit_cast(half8_t, sq[0][r][dq * KN + n][lane]);
-          const half8_t ql = __builtin_bit_cast(half8_t, sq[1][r][dq * KN + n][lane]);
+          const half8_t qh = __builtin_bit_cast(half8_t, sm.q[0][r][dq * KN + n][lane]);
+          const half8_t ql = __builtin_bit_cast(half8_t, sm.q[1][r][dq * KN + n][lane]);
 #pragma unroll
           for (int T = 0; T < NT; ++T)
             s[r][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[T], ql, s[r][T], 0, 0, 0);
@@ -303,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int T = 0; T < NT; ++T) sx[it & 1][kg][dq][r][T][lane] = s[r][T];
+        for (int T = 0; T < NT; ++T) sm.sx[it & 1][kg][dq][r][T][lane] = s[r][T];
       __syncthreads();
       if (dq > 0) continue;
 #pragma unroll
@@ -311,7 +307,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 #pragma unroll
         for (int T = 0; T < NT; ++T)
 #pragma unroll
-          for (int d = 1; d < DQ; ++d) s[r][T] += sx[it & 1][kg][d][r][T][lane];
+          for (int d = 1; d < DQ; ++d) s[r][T] += sm.sx[it & 1][kg][d][r][T][lane];
     }
     if (!mine) continue;
     const bool inner = key0 + KEYS - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
@@ -348,16 +344,23 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
   for (int r = 0; r < RT; ++r) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
-    if (g == 0 && dq == 0) wml[kg][16 * r + c] = make_float2(m[r], l[r]);
+    if (g == 0 && dq == 0) sm.wml[kg][16 * r + c] = make_float2(m[r], l[r]);
   }
   __syncthreads();
-  for (int r = t; r < R; r += 64 * kWaves) {
+  for (int r = t; r < R; r += 64 * W) {
     if (R0 + r >= S.rows) break;
     float M = kNoScore, L = 0.f;
-    for (int i = 0; i < KG; ++i) M = fmaxf(M, wml[i][r].x);
-    for (int i = 0; i < KG; ++i) L = fmaf(wml[i][r].y, __builtin_amdgcn_exp2f(wml[i][r].x - M), L);
+    for (int i = 0; i < KG; ++i) M = fmaxf(M, sm.wml[i][r].x);
+    for (int i = 0; i < KG; ++i) L = fmaf(sm.wml[i][r].y, __builtin_amdgcn_exp2f(sm.wml[i][r].x - M), L);
     S.ml[(size_t)(R0 + r) * S.splits + split] = make_float2(M, L);
   }
+}
+
+template <int HD, int DQ, int NT, int RT>
+__global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
+  __shared__ ScoreSmem<HD, DQ, NT, RT, kWaves> sm;
+  const int R0 = blockIdx.x * sm.R;
+  few_scores<HD, DQ, NT, RT, kWaves>(a, R0, blockIdx.y, Run(a.s, R0, sm.R, blockIdx.y, 16 * NT), sm);
 }
 
 // Many rows: a block owns 16 RT rows and a run of 32-key steps; its W waves share the head dim, so that
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 // in order and keeps the running maximum and sum of its own.
 // k times 2^8 in FP16 ends at 2^-24: what is lost of each is 2^-33, which 512 q below 16 make less
 // than 10^-6 of a score.  A block with a k of 128 or more, with larger q and a key that is below
-// 2^-10 throughout, or with a q below 2^-99, says so in `redo`, and scores_kernel does its rows again.
+// 2^-10 throughout, or with a q below 2^-99, does its rows again, as scores_kernel does.
 // 256 rows over 4096 keys of 512 (8 heads, 25 GFLOP with the three products): 48 us traced.  Before
 // its first step a block needs 10 us (its 128 KB of q 3.7, their parts 1.8, the first keys and
 // products 3); a step takes 2.3: without its loads the call would take 11 us less, without two of its
@@ -379,6 +382,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   union Smem {
     f32x4 sx[2][W][RT][NT][64];
     float rows[R][HD + 4];  // q, on its way from whole lines of memory
+    ScoreSmem<HD, 1, NT, RT, W> general;
   };
   __shared__ Smem sm;
   __shared__ float stop[2][W][KEYS];  // the keys' largest values
@@ -388,12 +392,8 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int R0 = blockIdx.x * R, split = blockIdx.y;
-  const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + R, S.rows) - 1) / S.heads;
-  int lo = S.first;
-  if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
-  const int hi = pb + 1, steps = (hi - lo + KEYS - 1) / KEYS;
-  const int per = (steps + S.splits - 1) / S.splits;
-  const int t0 = split * per, t1 = min(t0 + per, steps);
+  const Run run(S, R0, R, split, KEYS);
+  const int lo = run.lo, hi = run.hi, steps = run.steps, t0 = run.t0, t1 = run.t1;
   bool fits = true, large = false;  // large: some q of 16 or more, for which small k matter
 
   struct Keys {
@@ -553,7 +553,17 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     turn(step, kb, ka);
     if (step + 1 < t1) turn(step + 1, ka, kb);
   }
-  if (!__all(fits) && lane == 0) a.redo[R0 / R] = 1;
+  const bool odd = !__all(fits);
+  __syncthreads();
+  if (lane == 0) sq[w][0] = odd;
+  __syncthreads();
+  int again = 0;
+#pragma unroll
+  for (int d = 0; d < W; ++d) again |= sq[d][0];
+  if (__builtin_amdgcn_readfirstlane(again)) {
+    few_scores<HD, 1, NT, RT, W>(a, R0, split, run, sm.general);
+    return;
+  }
   const float M = group_max(m);
   l *= __builtin_amdgcn_exp2f(m - M);
   l += __shfl_xor(l, 16, 64);
@@ -572,7 +582,6 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
 // and threads.
 struct ScorePlan {
   void (*kernel)(ScoreArgs);
-  void (*again)(ScoreArgs);  // of 64 rows per block, where the first one may leave some undone
   int rows, keys, per_cu, threads;
 };
 // 17 to 32 rows take the kernel of few rows, two tiles of them, where it has a block per CU at most: 32
@@ -581,16 +590,16 @@ struct ScorePlan {
 template <int HD>
 ScorePlan score_plan(int rows, int keys) {
   constexpr int DQ = HD >= 128 ? HD / 128 : 1, FEW = 16 * kWaves / DQ;
-  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, nullptr, 16, FEW, 2, 64 * kWaves};
+  if (rows <= 16) return {scores_kernel<HD, DQ, 1, 1>, 16, FEW, 2, 64 * kWaves};
   if (rows <= 32 && cdiv(keys, FEW) <= cu_count())
-    return {scores_kernel<HD, DQ, 1, 2>, nullptr, 32, FEW, 2, 64 * kWaves};
+    return {scores_kernel<HD, DQ, 1, 2>, 32, FEW, 2, 64 * kWaves};
   if constexpr (HD == 512)
-    return {scores_rows_kernel<HD, 4, 8>, scores_kernel<HD, 1, 2, 4>, 64, 32, 1, 512};
+    return {scores_rows_kernel<HD, 4, 8>, 64, 32, 1, 512};
   else
-    return {scores_kernel<HD, 1, 2, 4>, nullptr, 64, 32 * kWaves, 2, 64 * kWaves};
+    return {scores_kernel<HD, 1, 2, 4>, 64, 32 * kWaves, 2, 64 * kWaves};
 }
 
-Workspace g_weights_ws, g_score_redo_ws;
+Workspace g_weights_ws;
 
 }  // namespace
 }  // namespace g4
@@ -653,20 +662,8 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
       return rc;
     s.score = static_cast<float *>(mem);
     s.ml = reinterpret_cast<float2 *>(s.score + scores);
-    if (plan.again) {
-      void *redo = nullptr;
-      if ((rc = g_score_redo_ws.get((size_t)blocks * 4, &redo, who))) return rc;
-      a.redo = static_cast<uint32_t *>(redo);
-      s.marks = a.redo;
-      s.n_marks = blocks;
-    }
     hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(plan.threads), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");
-    if (plan.again) {
-      a.redo_rows = plan.rows;
-      hipLaunchKernelGGL(plan.again, dim3(cdiv(s.rows, 64), s.splits), dim3(64 * kWaves), 0, stream(), a);
-      G4_LAUNCH_CHECK("scores_kernel");
-    }
     rc = launch_weights(s, keylen, s.score + scores + ml, r0 ? weights : before, weights);
     if (rc) return rc;
   }

@@ -27,8 +27,6 @@ constexpr int kBatch = 16;  // loads of a thread that are under way together
 __device__ __forceinline__ void add_weights(const SumArgs &a, int bx, int by) {
   __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
   const Scores &s = a.s;
-  if (bx == 0 && by == 0)
-    for (int i = threadIdx.x; i < s.n_marks; i += 256) s.marks[i] = 0;
   const int t = threadIdx.x, r0 = by * kGroup, n = min(kGroup, s.rows - r0);
   const int key = bx * 256 + t + (a.part ? s.first : 0);
   const bool any = key >= s.first && key < s.end;

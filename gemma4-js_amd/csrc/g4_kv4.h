@@ -24,8 +24,22 @@ struct Scores {
   size_t stride;
   int rows, heads, splits;
   int first, end, pos0, window;  // keys first .. end - 1 are seen by some row
-  uint32_t *marks;               // that weights_kernel clears
-  int n_marks;
+};
+
+// The keys that some of rows R0 .. R0 + n - 1 see, lo .. hi - 1, and a split's steps of
+// `keys` of them.
+struct Run {
+  int lo, hi, steps, t0, t1;
+  __device__ __forceinline__ Run(const Scores &S, int R0, int n, int split, int keys) {
+    const int pa = S.pos0 + R0 / S.heads, pb = S.pos0 + (min(R0 + n, S.rows) - 1) / S.heads;
+    lo = S.first;
+    if (S.window > 0) lo += max(0, pa - S.window + 1 - S.first) & ~3;
+    hi = pb + 1;
+    steps = (hi - lo + keys - 1) / keys;
+    const int per = (steps + S.splits - 1) / S.splits;
+    t0 = split * per;
+    t1 = min(t0 + per, steps);
+  }
 };
 
 size_t score_stride(int keys);

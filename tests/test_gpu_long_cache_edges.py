@@ -22,13 +22,13 @@ def odd_rows(rng, what, hd, qrows, keys):
     elif what == "tiny q":
         q[qrows // 9:qrows // 5 + 1] *= np.float32(2.0 ** -104)
     elif what == "tiny k":
-        k[100:140] *= np.float32(2.0 ** -20)  # scales below 2^-12
+        k[100:140] *= np.float32(2.0 ** -20)  # scales below 2^-18
         k[3] *= np.float32(2.0 ** -90)
     elif what == "large v":
-        v[50:60] *= 32  # scales above 8
+        v[50:60] *= 1024  # scales above 2^7
         v[7, :64] = 0   # scales of 1
     elif what == "one late key":
-        v[-1] *= 64     # seen by the last row alone
+        v[-1] *= 2048     # seen by the last row alone
     return q, k, v
 
 
