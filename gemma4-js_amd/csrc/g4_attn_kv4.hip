@@ -1012,7 +1012,8 @@ template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(Kv4Args a) { merge<HD>(a, blockIdx.x, blockIdx.y); }
 
 // Few rows whose keys' weights are asked for: both need the first kernel's sums alone, so the same
-// launch does the one and the other (one token of 32003 keys: 16.0 us in all; when it came in 17.3, with two launches 21.3).
+// launch does the one and the other (one token of 32003 keys, when it came in: 17.3 us in all, with two
+// launches 21.3).
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_merge_weights_kernel(Kv4Args a, SumArgs w) {
   const int merges = a.s.rows * (HD / 32), b = blockIdx.x;
@@ -1054,7 +1055,8 @@ __device__ __forceinline__ void join(const Kv4Args &a, int block) {
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) { join<HD>(a, blockIdx.x); }
 
-// And with the keys' weights, as for few rows: 1624 rows over 2403 keys 49.6 us in all, with two launches 51.7.
+// And with the keys' weights, as for few rows: 1624 rows over 2403 keys, when it came
+// in, 49.6 us in all, with two launches 51.7.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_kv4_join_weights_kernel(Kv4Args a, SumArgs w, int joins, int tiles) {
   const int b = blockIdx.x;

@@ -132,7 +132,7 @@ __device__ __forceinline__ float group_max(float v) {
 // q and k enter the FP16 matrix cores as two values each (hi hi, hi lo and lo hi; lo lo is below
 // 2^-22 of a product), q with its row's largest at the exponent 13, k times 2^8; a wave in which a
 // key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.
-// One token over 8001 keys of 512 (16.4 MB): 7.0 us traced, a step per wave whose loads are all
+// One token over 8001 keys of 512 (16.4 MB): 6.6 us traced, a step per wave whose loads are all
 // under way before q is ready; over 131072 keys 268 MB in 60 us with the sums, 4.5 TB/s: memory.
 template <int HD, int DQ, int NT, int RT, int W>
 struct ScoreSmem {
