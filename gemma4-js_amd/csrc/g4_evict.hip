@@ -7,9 +7,10 @@ namespace {
 
 constexpr int kMaxSets = 256;
 constexpr int kBins = 2048;
-constexpr int kPerThread = 16;                  // weights
-constexpr int kSlice = 256 * kPerThread;        // weights of a block of 256 threads
-constexpr int kOneBlock = 1024 * kPerThread;    // the most that one block takes
+constexpr int kOneBlock = 1024 * 8;             // the most that one block takes (15 sets of 16000: 21.4 us, 17.2 by several)
+constexpr int kThreads = 1024;                  // of a block of several
+constexpr int kPerThread = 4;                   // weights
+constexpr int kSlice = kThreads * kPerThread;   // a block's weights
 
 struct EvictArgs {
   const float *w;
@@ -87,14 +88,14 @@ __device__ __forceinline__ uint32_t digit(uint32_t key, int pass) {
 
 // Selection by digits: 11 bits of the order at a time, the histogram of those that agree so far gives the
 // next; no sort, and the rows come out in their order by a scan.
-// A block per set of up to 16 weights per thread, which stay in registers: histograms of the
+// A block per set of up to P weights per thread, which stay in registers: histograms of the
 // weights that agree with the bits found before, then one scan that counts the rows above the
 // threshold (the first and last ones among them) and, in the upper half, those equal to it.  2112
-// weights: 7.9 us traced, three histograms and four scans one after the other (9.1 with the scans by
-// LDS permutes, not DPP).
-template <int NW>
-__global__ __launch_bounds__(64 * NW) void evict_kernel(EvictArgs a) {
-  constexpr int P = kPerThread;
+// weights: 5.7 us traced, three histograms and four scans one after the other, each short of
+// nothing but instructions to fetch: 256 threads of 16 weights each, four times the code, take 7.9.
+template <int P>
+__global__ __launch_bounds__(1024) void evict_kernel(EvictArgs a) {
+  constexpr int NW = 16;
   __shared__ int hist[3][kBins];
   __shared__ int tmp[NW];
   __shared__ int found[2];
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(64 * NW) void evict_kernel(EvictArgs a) {
   uint32_t top = want > 0 ? 0 : 0xfffffffeu;  // the threshold (which no weight has)
   __syncthreads();
   if (want > 0) {
-#pragma unroll
+#pragma unroll 1  // (less code to fetch: 2112 weights, unrolled, 8.9 us for 8.35)
     for (int pass = 0; pass < 3; ++pass) {
 #pragma unroll
       for (int j = 0; j < P; ++j)
@@ -158,56 +159,57 @@ __global__ __launch_bounds__(64 * NW) void evict_kernel(EvictArgs a) {
     for (int i = a.keep + t; i < a.len; i += 64 * NW) kept[i] = 0.f;
 }
 
-// Longer caches, a block of 256 threads per slice of 4096 weights (blockIdx.x), four launches: the
-// histogram of the first 11 bits ...  131072 weights: 3.5, 4.8, 7.1 and 5.3 us traced, each little more
-// than its loads' latencies; 2^20 weights 54 us in all.  (All of the bin's weights in the third kernel's
+// Longer caches, a block per slice of 4096 weights (blockIdx.x), four launches: the
+// histogram of the first 11 bits ...  131072 weights: 2.6, 3.6, 7.2 and 3.3 us traced (with 256
+// threads of 16 weights each 3.5, 4.8, 7.1 and 5.3), each little more than its loads' latencies; 2^20
+// weights 50 us in all.  (All of the bin's weights in the third kernel's
 // registers, each with its slice looked up: 11.2 us.)
-__global__ __launch_bounds__(256) void evict_count_kernel(EvictArgs a) {
+__global__ __launch_bounds__(kThreads) void evict_count_kernel(EvictArgs a) {
   __shared__ int hist[kBins];
   const int t = threadIdx.x, set = blockIdx.y, end = a.len - a.recent;
   const float *w = a.w + (size_t)set * a.stride;
-  for (int i = t; i < kBins; i += 256) hist[i] = 0;
+  for (int i = t; i < kBins; i += kThreads) hist[i] = 0;
   __syncthreads();
   float x[kPerThread];
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) x[j] = w[min((int)blockIdx.x * kSlice + 256 * j + t, a.len - 1)];
+  for (int j = 0; j < kPerThread; ++j) x[j] = w[min((int)blockIdx.x * kSlice + kThreads * j + t, a.len - 1)];
 #pragma unroll
   for (int j = 0; j < kPerThread; ++j) {
-    const int i = blockIdx.x * kSlice + 256 * j + t;
+    const int i = blockIdx.x * kSlice + kThreads * j + t;
     if (i >= a.first && i < end) atomicAdd(&hist[digit(order_of(x[j]), 0)], 1);
   }
   __syncthreads();
-  for (int i = t; i < kBins; i += 256)
+  for (int i = t; i < kBins; i += kThreads)
     if (hist[i]) atomicAdd(&a.hist[set * kBins + i], hist[i]);
 }
 
 // ... each slice's weights in the bin of the threshold, and how many lie above it ...
-__global__ __launch_bounds__(256) void evict_list_kernel(EvictArgs a) {
-  __shared__ int tmp[4], found[2];
+__global__ __launch_bounds__(kThreads) void evict_list_kernel(EvictArgs a) {
+  __shared__ int tmp[kThreads / 64], found[2];
   const int t = threadIdx.x, set = blockIdx.y, slice = blockIdx.x, end = a.len - a.recent;
   const float *w = a.w + (size_t)set * a.stride;
   float x[kPerThread];
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) x[j] = w[min(slice * kSlice + 256 * j + t, a.len - 1)];
+  for (int j = 0; j < kPerThread; ++j) x[j] = w[min(slice * kSlice + kThreads * j + t, a.len - 1)];
   const int want = a.keep - a.first - a.recent;
-  find_bin<4>(a.hist + set * kBins, want, tmp, found);
+  find_bin<kThreads / 64>(a.hist + set * kBins, want, tmp, found);
   const uint32_t bin = want > 0 ? (uint32_t)found[0] : (uint32_t)kBins;  // (none)
   const size_t base = ((size_t)set * a.slices + slice) * kSlice;
   int mine = 0, above = 0, all;
 #pragma unroll
   for (int j = 0; j < kPerThread; ++j) {
-    const int i = slice * kSlice + 256 * j + t;
-    if (a.copy && i < a.len) a.copy[base + 256 * j + t] = x[j];
+    const int i = slice * kSlice + kThreads * j + t;
+    if (a.copy && i < a.len) a.copy[base + kThreads * j + t] = x[j];
     const uint32_t d = digit(order_of(x[j]), 0);
     const bool mid = i >= a.first && i < end;
     // the first and last rows count as above
     if (i < a.len && (!mid || d > bin)) ++above;
     if (mid && d == bin) ++mine;
   }
-  int at = before_me<4>(mine | above << 16, tmp, all) & 0xffff;
+  int at = before_me<kThreads / 64>(mine | above << 16, tmp, all) & 0xffff;
 #pragma unroll
   for (int j = 0; j < kPerThread; ++j) {
-    const int i = slice * kSlice + 256 * j + t;
+    const int i = slice * kSlice + kThreads * j + t;
     const uint32_t k = order_of(x[j]);
     if (i >= a.first && i < end && digit(k, 0) == bin) a.cand[base + at++] = k;
   }
@@ -321,22 +323,22 @@ __global__ __launch_bounds__(1024) void evict_threshold_kernel(EvictArgs a) {
 }
 
 // ... and the rows.
-__global__ __launch_bounds__(256) void evict_rows_kernel(EvictArgs a) {
+__global__ __launch_bounds__(kThreads) void evict_rows_kernel(EvictArgs a) {
   constexpr int P = kPerThread;
-  __shared__ int tmp[4];
+  __shared__ int tmp[kThreads / 64];
   __shared__ float sw[kSlice];
   const int t = threadIdx.x, set = blockIdx.y, slice = blockIdx.x, end = a.len - a.recent;
   const size_t base = ((size_t)set * a.slices + slice) * kSlice;
   const float *w = a.copy ? a.copy + base : a.w + (size_t)set * a.stride + (size_t)slice * kSlice;
   const int n = min(kSlice, a.len - slice * kSlice);
 #pragma unroll
-  for (int j = 0; j < P; ++j) sw[256 * j + t] = w[min(256 * j + t, n - 1)];
+  for (int j = 0; j < P; ++j) sw[kThreads * j + t] = w[min(kThreads * j + t, n - 1)];
   const uint32_t top = a.top[2 * set];
   const int want = (int)a.top[2 * set + 1];
   const int *c = a.count + ((size_t)set * a.slices + slice) * 4;
   const int rows_before = c[2], equal_before = c[3];
   __syncthreads();
-  // thread t has weights 16 t .. of the slice
+  // thread t has weights P t .. of the slice
   float x[P];
   uint32_t key[P];
   int mine = 0, all;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(EvictArgs a) {
     key[j] = i >= a.first && i < end ? order_of(x[j]) : 0xffffffffu;
     if (P * t + j < n) mine += key[j] > top ? 1 : key[j] == top ? 1 << 16 : 0;
   }
-  const int before = before_me<4>(mine, tmp, all);
+  const int before = before_me<kThreads / 64>(mine, tmp, all);
   int above = before & 0xffff, equal = equal_before + (before >> 16);
   const int base_equal = min(equal_before, want);
   int *rows = a.rows + (size_t)set * a.keep;
@@ -366,7 +368,7 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(EvictArgs a) {
     equal += same ? 1 : 0;
   }
   if (!kept) return;
-  for (int j = t; j < n; j += 256)
+  for (int j = t; j < n; j += kThreads)
     if (slice * kSlice + j >= a.keep) kept[slice * kSlice + j] = 0.f;
 }
 
@@ -410,8 +412,8 @@ G4_API int g4_cache_evict(const float *weights, size_t stride, int sets, int len
   a.first = first;
   a.recent = recent;
   if (len <= kOneBlock) {
-    hipLaunchKernelGGL(len <= kSlice ? evict_kernel<4> : evict_kernel<16>, dim3(sets),
-                       dim3(len <= kSlice ? 256 : 1024), 0, stream(), a);
+    hipLaunchKernelGGL(len <= 4096 ? evict_kernel<4> : evict_kernel<8>, dim3(sets),
+                       dim3(1024), 0, stream(), a);
     G4_LAUNCH_CHECK("evict_kernel");
     return ok();
   }
@@ -427,13 +429,13 @@ G4_API int g4_cache_evict(const float *weights, size_t stride, int sets, int len
   a.top = reinterpret_cast<uint32_t *>(a.count + all * 4);
   a.cand = a.top + (size_t)sets * 2;
   a.copy = n_copy ? reinterpret_cast<float *>(a.cand + all * kSlice) : nullptr;
-  hipLaunchKernelGGL(evict_count_kernel, dim3(a.slices, sets), dim3(256), 0, stream(), a);
+  hipLaunchKernelGGL(evict_count_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
   G4_LAUNCH_CHECK("evict_count_kernel");
-  hipLaunchKernelGGL(evict_list_kernel, dim3(a.slices, sets), dim3(256), 0, stream(), a);
+  hipLaunchKernelGGL(evict_list_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
   G4_LAUNCH_CHECK("evict_list_kernel");
   hipLaunchKernelGGL(evict_threshold_kernel, dim3(sets), dim3(1024), 0, stream(), a);
   G4_LAUNCH_CHECK("evict_threshold_kernel");
-  hipLaunchKernelGGL(evict_rows_kernel, dim3(a.slices, sets), dim3(256), 0, stream(), a);
+  hipLaunchKernelGGL(evict_rows_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
   G4_LAUNCH_CHECK("evict_rows_kernel");
   return ok();
 }

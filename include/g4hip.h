@@ -453,7 +453,7 @@ int g4_cache_rows(float *const *dst, const float *const *src, const int *widths,
  * Rows keep the RoPE of their own positions; qpos0 counts cache rows.
  * Arguments are checked before anything else, so a refusal needs no device.  What is
  * written overlaps no other argument, unless it says so.  All can be recorded:
- * g4_attention_kv4, g4_attention_weights and g4_cache_evict of more than 16384 rows
+ * g4_attention_kv4, g4_attention_weights and g4_cache_evict of more than 8192 rows
  * after one call outside a recorder of the same sizes, for their scratch. */
 
 /* One layer's k and v rows in 4 bits, in the caller's device memory (no handle: the

@@ -44,8 +44,8 @@ def weights(rng, sets, n):
 @pytest.mark.parametrize("sets,n,keep,first,recent", [
     (1, 1, 1, 0, 0), (1, 1, 0, 0, 0), (1, 2, 1, 0, 0), (1, 2, 1, 1, 0), (1, 2, 1, 0, 1), (2, 63, 20, 4, 8),
     (1, 64, 64, 0, 0), (3, 65, 12, 4, 8), (1, 1000, 999, 0, 0), (1, 1023, 500, 4, 128), (2, 1024, 1000, 0, 0),
-    (15, 1025, 600, 3, 64), (1, 2112, 2048, 4, 128), (3, 2112, 2048, 4, 128), (5, 4097, 1, 0, 0),
-    (1, 16384, 4096, 4, 512), (2, 16385, 16000, 4, 512), (1, 40000, 39999, 0, 0), (1, 32768, 0, 0, 0),
+    (15, 1025, 600, 3, 64), (1, 2112, 2048, 4, 128), (3, 2112, 2048, 4, 128), (5, 4097, 1, 0, 0), (3, 4096, 100, 1, 1), (2, 8192, 5000, 4, 30),
+    (2, 8193, 5000, 4, 30),    (1, 16384, 4096, 4, 512), (2, 16385, 16000, 4, 512), (1, 40000, 39999, 0, 0), (1, 32768, 0, 0, 0),
     (3, 33000, 8000, 16, 300), (1, 131072, 32768, 4, 512), (2, 100003, 50001, 0, 1), (7, 20000, 19000, 9000, 9000)])
 def test_shapes(g4, sets, n, keep, first, recent, place):
     check(g4, weights(np.random.default_rng([sets, n, keep]), sets, n), keep, first, recent, place=place)
