@@ -950,6 +950,10 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   }
 }
 
+// The power of two that takes a sum of weights to 1 .. 2: outputs added under it stay in FP32's range
+// wherever their mean does, and no bit of them changes otherwise.
+__device__ __forceinline__ float to_one(float sum) { return ldexpf(1.f, 127 - (int)(__float_as_uint(sum) >> 23)); }
+
 // Adds the key splits of a row: y = sum_s w_s y_s / sum_s w_s, w_s = 2^(m_s - M) l_s.  A block is
 // one row's 32 dims; thread (j, u) adds splits j, j + 32, .. of 16-byte unit u in order, 8 of them
 // under way together and before their weights are known.  8 rows of 512 splits of 512: 8.4 MB in 4.2 us.
@@ -989,11 +993,12 @@ __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
   const float L = team_sum(64, e);
   if ((t & 63) == 0) wsum[t >> 6] = L;
   __syncthreads();
+  const float sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), one = to_one(sum);
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = j; s0 < S.splits; s0 += G * N) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (s0 + G * i < S.splits) y += wt[s0 + G * i] * x[i];
+      if (s0 + G * i < S.splits) y += wt[s0 + G * i] * one * x[i];
     if (s0 + G * N < S.splits) load(s0 + G * N);
   }
   sums[j][u] = y;
@@ -1002,9 +1007,8 @@ __device__ __forceinline__ void merge(const Kv4Args &a, int row, int part) {
   y = sums[0][u];
 #pragma unroll
   for (int i = 1; i < G; ++i) y += sums[i][u];
-  const float sum = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] /= sum;
+  for (int i = 0; i < 4; ++i) y[i] /= sum * one;
   reinterpret_cast<f32x4 *>(a.y + (size_t)row * HD)[part * U + u] = y;
 }
 
@@ -1045,11 +1049,12 @@ __device__ __forceinline__ void join(const Kv4Args &a, int block) {
     e[i] = i < S.splits ? z.y * __builtin_amdgcn_exp2f(z.x - M) : 0.f;
     L += e[i];
   }
+  const float one = to_one(L);
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < MOST; ++i) y += e[i] * x[i];
+  for (int i = 0; i < MOST; ++i) y += e[i] * one * x[i];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] /= L;
+  for (int i = 0; i < 4; ++i) y[i] /= L * one;
   reinterpret_cast<f32x4 *>(a.y)[unit] = y;
 }
 template <int HD>
