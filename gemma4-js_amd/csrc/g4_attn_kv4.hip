@@ -23,6 +23,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // are split into two FP16 values times 2^(15 - kSlack), so one is held to 2^-22 of it, or to 2^-38 of
 // its row's largest if that is more.
 constexpr float kSlack = 2.f;
+constexpr float kWeight = 1 << (15 - (int)kSlack);
 constexpr int kStep = 32;                   // keys of a wave's step
 constexpr int kMaxSplits = 512;
 
@@ -34,6 +35,10 @@ struct Kv4Args {
   float *part;  // [splits][rows][hd], each split's outputs
   Scores s;     // score null: not kept
 };
+
+// v's scales that are not plain: how many octaves of them one product takes, and how far (log 2) a
+// key's largest contribution may pass the outputs' own exponent.
+constexpr int kBand = 12, kRoom = 64;
 
 // Scales are taken times 2^kLift.  Plain ones, from 2^-18 up to 2^7, then are normal FP16 numbers, and
 // so are eight times they: BF16 bits of the least and how many there are.
@@ -95,6 +100,23 @@ constexpr int kDims = HD > 256 ? 256 : HD;
 template <int HD, int W, int DW = kDims<HD>>
 constexpr int kGroups = W / (HD / DW);  // key groups of a block
 
+// Eight weights times `up` as sums of two FP16 values.  PAIR: the lo part alone for lanes 8 .. 15 of each
+// 16.
+template <bool PAIR>
+__device__ __forceinline__ void weight_parts(const float (&p)[8], float up, half8_t &h, half8_t &l) {
+  u32x4 h4, l4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f32x2_t z = {p[2 * j] * up, p[2 * j + 1] * up};
+    const half2_t y = __builtin_convertvector(z, half2_t);
+    h4[j] = __builtin_bit_cast(uint32_t, y);
+    l4[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(z - __builtin_convertvector(y, f32x2_t), half2_t));
+    if (PAIR && (threadIdx.x & 8)) h4[j] = l4[j];
+  }
+  h = __builtin_bit_cast(half8_t, h4);
+  l = __builtin_bit_cast(half8_t, l4);
+}
+
 // x of lane c ^ 8 of each 16
 __device__ __forceinline__ float other_half(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));  // row_ror:8
@@ -112,7 +134,13 @@ __device__ __forceinline__ float other_half(float x) {
 // The values are used where they are unpacked, in the lanes that the matrix instructions want them:
 // nothing of k or v passes through LDS.  A row's maximum is a reference that follows the scores with
 // kSlack, so the outputs are hardly ever scaled again; a step's loads are under way during the one
-// before it.  Scales that are not plain take a slower way with exponents per row.
+// before it.
+// A block that met a scale that is not plain (or a row of q below 2^-103) does its rows again in the
+// general way, without PLAIN: k with an exponent per key, which the score takes back; v in as many
+// products as the step has bands of kBand octaves of scales, each with the weights of the keys in it
+// scaled for their largest and with its exponent put back in FP32.  (With one exponent per row, a single
+// large value took the bits of all other keys' weights, in all dims.)  One token over 16001 keys of
+// 512, all scales plain / none: 13.3 / 18.8 us; both ways in one loop, 188 bytes of spills per lane.
 // What bounds it: one token over 131072 keys of 512 (75.5 MB) 23.3 us traced, 3.2 TB/s: 4 steps per
 // wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
 // exponent, fused step) and the products between them, and as long again before and behind them
@@ -131,8 +159,9 @@ struct AttendSmem {
   };
   int xq[R];
   float2 wml[KG][R];
+  int other[W];
 };
-template <int HD, int RT, bool PAIR, int W, int DW>
+template <int HD, int RT, bool PAIR, int W, int DW, bool PLAIN>
 __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, const Run &run, AttendSmem<HD, RT, PAIR, W, DW> &sm) {
   constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>;
   static_assert(!PAIR || RT == 1, "one tile");
@@ -221,10 +250,12 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
       qx[i][0] = p[0];
       qx[i][1] = p[1];
     }
-    asm volatile("" ::: "memory");
-    load_k(t0 + kg);
-    load_v(t0 + kg);
-    asm volatile("" ::: "memory");
+    if constexpr (PLAIN) {
+      asm volatile("" ::: "memory");
+      load_k(t0 + kg);
+      load_v(t0 + kg);
+      asm volatile("" ::: "memory");
+    }
 #pragma unroll
     for (int pass = 0; pass < N; ++pass) {
       const int r = t / TW + pass * PASS;
@@ -256,58 +287,57 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
   __syncthreads();
 
   int pos[RT], xe[RT];
-  float xf[RT], m[RT], l[RT], E[RT];
-  bool usual = true;
+  int E[RT];  // outputs are held times 2^(15 + kLift - E)
+  float xf[RT], m[RT], l[RT];
+  ushort2_t beyond = {0, 0};  // the scales' largest distance from the least plain one
   f32x4 o[RT][VD];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     pos[r] = S.pos0 + min(R0 + 16 * r + cr, S.rows - 1) / S.heads;
     xe[r] = sm.xq[16 * r + cr];
     xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
-    usual = usual && usual_row(xe[r]);
+    if (!usual_row(xe[r])) beyond = (ushort2_t){0xffff, 0xffff};
     m[r] = kNoScore;
     l[r] = 0.f;
-    E[r] = -1000.f;  // outputs are held times 2^(15 + kLift - E)
+    E[r] = (int)kSlack;
 #pragma unroll
     for (int n = 0; n < VD; ++n) o[r][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
   uint32_t none = 0;  // bit 4 r + v: register v of row tile r holds no numbers
   const Magic mg;
   const int turns = (t1 - t0 + KG - 1) / KG;
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the waits in the loop then count its own loads
+  if constexpr (PLAIN) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the waits in the loop then count its own loads
   for (int it = 0; it < turns; ++it) {
     const int step = t0 + kg + it * KG, key0 = lo + step * kStep;
     const bool mine = step < t1;
     const int last = hi - 1 - (lo + min(step, steps - 1) * kStep);  // row of the step
+    if constexpr (!PLAIN) load_k(step);
     if (last < kStep - 1) look_k(last);
-    // the keys' exponents, where a scale needs them
-    uint32_t ke[2] = {0, 0};  // a byte each
+    uint32_t ke[2] = {0, 0};  // the keys' exponents, a byte each
     Scale x[2][KS];
-    bool kplain;
-    {
-      ushort2_t beyond = {0, 0};
+    if constexpr (PLAIN) {
+      ushort2_t far = {0, 0};
 #pragma unroll
       for (int T = 0; T < 2; ++T)
 #pragma unroll
-        for (int J = 0; J < KS; ++J) x[T][J] = plain_pair(ksr[T][J], ksr[T][J], beyond);
-      kplain = __all(usual && beyond[0] < kPlainScales);
-      if (!kplain) {
+        for (int J = 0; J < KS; ++J) x[T][J] = plain_pair(ksr[T][J], ksr[T][J], far);
+      if (mine) beyond = __builtin_elementwise_max(beyond, far);
+    } else {
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          int top = 0;
+      for (int T = 0; T < 2; ++T) {
+        int top = 0;
 #pragma unroll
-          for (int J = 0; J < KS; ++J) top = max(top, (int)(ksr[T][J] & 0x7fffu));
-          top = max(top, __shfl_xor(top, 16, 64));
-          top = max(top, __shfl_xor(top, 32, 64));
-          const int e = min(scale_exponent(top), 127);
+        for (int J = 0; J < KS; ++J) top = max(top, (int)(ksr[T][J] & 0x7fffu));
+        top = max(top, __shfl_xor(top, 16, 64));
+        top = max(top, __shfl_xor(top, 32, 64));
+        const int e = min(scale_exponent(top), 127);
 #pragma unroll
-          for (int J = 0; J < KS; ++J) {
-            const float f = bf16_to_f32(ksr[T][J]) * pow2_8_minus(e);
-            x[T][J] = scale_pair(f, f);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e - 8 + kLift, 4 * g + i, 64) & 255) << (8 * i);
+        for (int J = 0; J < KS; ++J) {
+          const float f = bf16_to_f32(ksr[T][J]) * pow2_8_minus(e);
+          x[T][J] = scale_pair(f, f);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e - 8 + kLift, 4 * g + i, 64) & 255) << (8 * i);
       }
     }
     f32x4 s[RT][2];
@@ -352,7 +382,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             s[r][T][i] = (sh[r][T][i] + (PAIR ? other_half(sh[r][T][i]) : sl[r][T][i])) * xf[r];
-      if (!kplain) {
+      if constexpr (!PLAIN) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -362,7 +392,8 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
               s[r][T][i] = ldexpf(s[r][T][i], (usual_row(xe[r]) ? 0 : xe[r]) + byte_of(ke[T], i));
       }
     }
-    load_k(step + KG);
+    if constexpr (PLAIN) load_k(step + KG);
+    else load_v(step);
     if constexpr (DQ > 1) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -379,33 +410,22 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
         }
     }
 
-    // v's exponents: keys 4 g + i of each half, as the weights are held
+    // v: keys 4 g + i of each half, as the weights are held
     if (last < kStep - 1) look_v(last);
-    uint32_t ve[2] = {0, 0};
     Scale vx[4];
     uint32_t odd = 0;  // keys of which this lane's dims are no numbers
-    bool vplain;
-    {
-      ushort2_t beyond = {0, 0};
+    if constexpr (PLAIN) {
+      ushort2_t far = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vx[j] = plain_pair(vsr[2 * j], vsr[2 * j + 1], beyond);
-      vplain = __all(max(beyond[0], beyond[1]) < kPlainScales);
-    }
-    if (!vplain) {
-      float f[8];
+      for (int j = 0; j < 4; ++j) vx[j] = plain_pair(vsr[2 * j], vsr[2 * j + 1], far);
+      if (mine) beyond = __builtin_elementwise_max(beyond, far);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        int u = vsr[j] & 0x7fff;
-        if (u >= 0x7f80) {
+      for (int j = 0; j < 8; ++j)
+        if ((vsr[j] & 0x7fff) >= 0x7f80) {
           odd |= 1u << j;
-          vsr[j] = u = 0;
+          vsr[j] = 0;
         }
-        const int e = scale_exponent(team_max<16>(u));
-        ve[j >> 2] |= (uint32_t)((e - 8 + kLift) & 255) << (8 * (j & 3));
-        f[j] = bf16_to_f32(vsr[j]) * pow2_8_minus(e);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vx[j] = scale_pair(f[2 * j], f[2 * j + 1]);
     }
     // whether every row sees every key of the step
     const bool inner = mine && key0 + kStep - 1 <= pa && (S.window == 0 || key0 > pb - S.window);
@@ -440,45 +460,23 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
       tm = group_max(tm);
       const float mn = tm > m[r] + kSlack ? tm : m[r];
       const float corr = __builtin_amdgcn_exp2f(m[r] - mn);
-      float E2 = E[r] + fmaxf(ceilf(m[r] - mn), -1000.f);
-      float bound = kSlack;
-      if (!vplain) {
-        bound = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bound = fmaxf(bound, (float)byte_of(ve[j >> 2], j & 3) + ceilf(x[j] - mn));
-        bound = group_max(bound);
-      }
-      E2 = fmaxf(fmaxf(E2, bound), -1000.f);
       float p[8], sum = 0.f;
-      const int up = 15 - (int)E2;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         p[j] = __builtin_amdgcn_exp2f(x[j] - mn);
         sum += p[j];
+        s[r][j >> 2][j & 3] = x[j] - mn;
       }
       l[r] = fmaf(l[r], corr, sum);
-      u32x4 h4, l4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x2_t z = {ldexpf(p[2 * j], up + byte_of(ve[j >> 1], 2 * j & 3)),
-                             ldexpf(p[2 * j + 1], up + byte_of(ve[j >> 1], 2 * j + 1 & 3))};
-        const half2_t h = __builtin_convertvector(z, half2_t);
-        h4[j] = __builtin_bit_cast(uint32_t, h);
-        l4[j] = __builtin_bit_cast(
-            uint32_t, __builtin_convertvector(z - __builtin_convertvector(h, f32x2_t), half2_t));
-        if (PAIR && c >= 8) h4[j] = l4[j];
-      }
-      ph[r] = __builtin_bit_cast(half8_t, h4);
-      pl[r] = __builtin_bit_cast(half8_t, l4);
-      const float f = ldexpf(corr, (int)(E[r] - E2));
+      if constexpr (PLAIN) weight_parts<PAIR>(p, kWeight, ph[r], pl[r]);
       m[r] = mn;
-      E[r] = E2;
-      if (__any(f != 1.f)) {
+      if (__any(corr != 1.f)) {
 #pragma unroll
-        for (int n = 0; n < VD; ++n) o[r][n] *= f;
+        for (int n = 0; n < VD; ++n) o[r][n] *= corr;
       }
     }
-    {
+    // O^T += V^T . P^T with the values' scales vs, or a factor of the products
+    auto outputs = [&](const Scale (&vs)[4], const half8_t (&wh)[RT], const half8_t (&wl)[RT], auto scaled, const float (&factor)[RT]) {
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
 #pragma unroll
@@ -490,13 +488,15 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
           auto tile = [&](auto T) {
             constexpr int e = decltype(T)::value;
             const half8_t vv = __builtin_bit_cast(
-                half8_t, (u32x4){value_pair<e>(d[0], vx[0], mg), value_pair<e>(d[1], vx[1], mg), value_pair<e>(d[2], vx[2], mg),
-                                 value_pair<e>(d[3], vx[3], mg)});
+                half8_t, (u32x4){value_pair<e>(d[0], vs[0], mg), value_pair<e>(d[1], vs[1], mg), value_pair<e>(d[2], vs[2], mg),
+                                 value_pair<e>(d[3], vs[3], mg)});
             const int n = 8 * i + 4 * h + e;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-              o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[r], o[r][n], 0, 0, 0);
-              if constexpr (!PAIR) o[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[r], o[r][n], 0, 0, 0);
+              f32x4 y = scaled ? (f32x4){0.f, 0.f, 0.f, 0.f} : o[r][n];
+              y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, wh[r], y, 0, 0, 0);
+              if constexpr (!PAIR) y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, wl[r], y, 0, 0, 0);
+              o[r][n] = scaled ? o[r][n] + y * factor[r] : y;
             }
           };
           tile(std::integral_constant<int, 0>());
@@ -506,8 +506,68 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+    };
+    float factor[RT] = {};
+    if constexpr (PLAIN) {
+      outputs(vx, ph, pl, std::false_type(), factor);
+    } else {
+      uint32_t left = 0;  // keys of which this lane's dims have yet to be added
+#pragma unroll
+      for (int j = 0; j < 8; ++j) left |= (vsr[j] & 0x7fff ? 1u : 0u) << j;
+      auto exponent = [&](int j) { return max((int)(vsr[j] >> 7 & 255), 1); };
+      for (;;) {  // 22 times at most: each takes kBand of 254 exponents, and some key
+        int top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (left >> j & 1) top = max(top, exponent(j));
+        top = __builtin_amdgcn_readfirstlane(team_max<64>(top));
+        if (top == 0) break;
+        // (each time anew: unpacked before the loop, the codes alone would fill the registers)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) asm volatile("" : "+v"(vr[j][i]));
+        float f[8];  // from 2^(6 - kBand) up to 2^6, or 0
+        uint32_t take = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = (left >> j & 1) && exponent(j) > top - kBand;
+          take |= (in ? 1u : 0u) << j;
+          f[j] = in ? ldexpf(bf16_to_f32(vsr[j]), 132 - top) : 0.f;
+        }
+        left &= ~take;
+        Scale vs[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[j] = scale_pair(f[2 * j], f[2 * j + 1]);
+        uint32_t here = take;  // of any dims
+#pragma unroll
+        for (int i = 1; i < 16; i *= 2) here |= (uint32_t)__shfl_xor((int)here, i, 64);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          // these keys' weights times 2^(15 - F)
+          float F = -1000.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (here >> j & 1) F = fmaxf(F, s[r][j >> 2][j & 3]);
+          F = ceilf(group_max(F));
+          float z[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            z[j] = here >> j & 1 ? __builtin_amdgcn_exp2f(s[r][j >> 2][j & 3] - F) : 0.f;
+          weight_parts<PAIR>(z, 32768.f, ph[r], pl[r]);
+          const int E2 = max(E[r], (int)F + top - 123 - kRoom);
+          if (__any(E2 != E[r])) {
+            const float down = ldexpf(1.f, E[r] - E2);
+#pragma unroll
+            for (int n = 0; n < VD; ++n) o[r][n] *= down;
+          }
+          E[r] = E2;
+          factor[r] = ldexpf(1.f, (int)F + top - 132 + kLift - E2);
+        }
+        outputs(vs, ph, pl, std::true_type(), factor);
+      }
     }
-    if (!vplain && __any(odd != 0)) {  // rows that see such a key: NaN in its dims
+    if (!PLAIN && __any(odd != 0)) {  // rows that see such a key: NaN in its dims
 #pragma unroll
       for (int r = 0; r < RT; ++r)
         for (int i = 0; i < 16; ++i) {  // keys of lanes (., i / 4), dims of register i % 4
@@ -515,7 +575,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
           if (bad & (uint32_t)__shfl((int)seen[r], 16 * (i >> 2) + c, 64)) none |= 1u << (4 * r + (i & 3));
         }
     }
-    load_v(step + KG);
+    if constexpr (PLAIN) load_v(step + KG);
   }
 
   // the key groups' sums through LDS, the upper half of the groups to the lower one
@@ -525,7 +585,21 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     l[r] += __shfl_xor(l[r], 32, 64);
     if (g == 0 && dq == 0) sm.wml[kg][16 * r + cr] = make_float2(m[r], l[r]);
   }
+  if constexpr (PLAIN) {
+    const bool other = __any(max(beyond[0], beyond[1]) >= kPlainScales);
+    if (lane == 0) sm.other[w] = other;
+  }
   __syncthreads();
+  if constexpr (PLAIN) {
+    int again = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) again |= sm.other[i];
+    if (__builtin_amdgcn_readfirstlane(again)) {
+      __syncthreads();
+      attend<HD, RT, PAIR, W, DW, false>(a, R0, split, run, sm);
+      return;
+    }
+  }
   const bool whole = S.splits == 1;
   float *out = whole ? a.y : a.part + (size_t)split * S.rows * HD;
 #pragma unroll
@@ -541,7 +615,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     // (a split of which the row sees nothing: 0, not 0 / 0)
     float f = __builtin_amdgcn_exp2f(m[r] - M) / L;
     if (!whole && L == 0.f) f = 0.f;
-    f = ldexpf(f, (int)E[r] - 15 - kLift);
+    f = ldexpf(f, E[r] - 15 - kLift);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float fv = none >> (4 * r + v) & 1 ? __int_as_float(0x7fc00000) : f;
@@ -589,7 +663,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
 template <int HD, int RT, bool PAIR, int W, int DW = kDims<HD>>
 __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
   __shared__ AttendSmem<HD, RT, PAIR, W, DW> sm;
-  attend<HD, RT, PAIR, W, DW>(a, blockIdx.x * sm.R, blockIdx.y, Run(a.s, blockIdx.x * sm.R, sm.R, blockIdx.y, kStep), sm);
+  attend<HD, RT, PAIR, W, DW, true>(a, blockIdx.x * sm.R, blockIdx.y, Run(a.s, blockIdx.x * sm.R, sm.R, blockIdx.y, kStep), sm);
 }
 
 // Many rows of a cache whose scales all are plain, by the same mathematics: a block owns 16 RT rows and a
@@ -769,7 +843,6 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
       for (int T = 0; T < NT; ++T) sm.sx[(step - t0) & 1][w][r][T][lane] = s[r][T];
   };
 
-  constexpr float kWeight = 1 << (15 - (int)kSlack);
   float m = kNoScore, l = 0.f;  // of row 16 w + c
   f32x4 o[RT][VD];              // outputs times 2^(15 + kLift - kSlack)
 #pragma unroll
@@ -916,7 +989,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   if (__builtin_amdgcn_readfirstlane(again)) {
     for (int r = 0; r < R && R0 + r < S.rows; r += 16) {
       __syncthreads();
-      attend<HD, 1, false, W, DW>(a, R0 + r, split, run, sm.general);
+      attend<HD, 1, false, W, DW, false>(a, R0 + r, split, run, sm.general);
     }
     return;
   }

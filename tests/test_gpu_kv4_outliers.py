@@ -35,3 +35,49 @@ def test_all_values_near_the_largest_number(g4, hd, qrows, keys, exp):
     q[::2] = 0
     v = (np.clip(np.abs(v), 0, 4) * np.float32(2.0 ** exp)).astype(np.float32)
     check_groups(g4, q, ref.pack(k), ref.pack(v), keys, keys - qrows, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("qrows", [1, 2, 12, 45])
+@pytest.mark.parametrize("b", [12, 28, 40, 50, 90, -40, -90])
+def test_one_group_of_one_row(g4, hd, qrows, b):
+    rng = np.random.default_rng([hd, qrows, b + 100])
+    keys = 320
+    q, k, v = inputs(rng, qrows, 8, hd, keys)
+    group = rng.integers(0, hd // 32)
+    v[77, 32 * group:32 * group + 32] *= np.float32(2.0 ** b)
+    check_groups(g4, q, ref.pack(k), ref.pack(v), keys, keys - qrows, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("qrows", [1, 12, 45])
+@pytest.mark.parametrize("window", [0, 130])
+def test_groups_of_any_size(g4, hd, qrows, window):
+    # every group of every row 2^-45 to 2^45 times the usual
+    rng = np.random.default_rng([hd, qrows, window])
+    keys = 333
+    q, k, v = inputs(rng, qrows, 8, hd, keys)
+    e = np.repeat(rng.integers(-45, 46, (keys, hd // 32)), 32, axis=1)
+    check_groups(g4, q, ref.pack(k), ref.pack((v * np.exp2(e)).astype(np.float32)), keys, keys - qrows, window)
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("qrows", [1, 40])
+def test_the_largest_values_beside_small_ones(g4, hd, qrows):
+    # 2^122 and 2^-70 in different dims, the large ones in the first, a middle and the last row
+    rng = np.random.default_rng([hd, qrows, 5])
+    keys = 300
+    q, k, v = inputs(rng, qrows, 8, hd, keys)
+    v[:, 32:64] *= np.float32(2.0 ** -70)
+    v[0, :32] *= np.float32(2.0 ** 122)
+    v[150, :32] *= np.float32(2.0 ** 115)
+    v[keys - 1, :32] *= np.float32(2.0 ** 122)
+    check_groups(g4, q, ref.pack(k), ref.pack(v), keys, keys - qrows, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 512])
+@pytest.mark.parametrize("exp", [-124, -118])
+def test_all_values_near_the_smallest_number(g4, hd, exp):
+    rng = np.random.default_rng([hd, exp + 200])
+    q, k, v = inputs(rng, 3, 8, hd, 2000)
+    check_groups(g4, q, ref.pack(k), ref.pack((v * np.float32(2.0 ** exp)).astype(np.float32)), 2000, 1997, 0)
