@@ -36,8 +36,8 @@ struct Kv4Args {
   Scores s;     // score null: not kept
 };
 
-// v's scales that are not plain: how many octaves of them one product takes, and how far (log 2) a
-// key's largest contribution may pass the outputs' own exponent.
+// Scales that are not plain: how many octaves of them one product takes, and how far (log 2) a key's
+// largest contribution may pass the outputs' own exponent.
 constexpr int kBand = 12, kRoom = 64;
 
 // Scales are taken times 2^kLift.  Plain ones, from 2^-18 up to 2^7, then are normal FP16 numbers, and
@@ -86,13 +86,20 @@ __device__ __forceinline__ float group_max(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-// Signed byte i of a word.
-__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 // Rows of q whose exponent a factor of FP32 holds with all its bits.
 __device__ __forceinline__ bool usual_row(int e) { return e >= -120; }
-// 2^(8 - e) for -100 <= e <= 127
-__device__ __forceinline__ float pow2_8_minus(int e) { return __int_as_float((135 - e) << 23); }
-__device__ __forceinline__ int scale_exponent(int bits) { return max((bits >> 7) - 127, -100); }
+// A BF16 scale's exponent, 127 more: 1 .. 254, 255 if it is no number; 0 for a scale of 0.  And the scale
+// under another one: from 2^(6 - kBand) up to 2^6 if that is within kBand above it.
+__device__ __forceinline__ int scale_exponent(uint32_t bits) { return bits & 0x7fffu ? max((int)(bits >> 7 & 255u), 1) : 0; }
+__device__ __forceinline__ float scale_under(uint32_t bits, int top) { return ldexpf(bf16_to_f32(bits), 132 - top); }
+
+// The kernel's arguments once more from memory, for the general way behind its loop: held in registers
+// through it, they cost 4000 rows of 256 with a window of 512 66.3 us for 63.6.
+__device__ __forceinline__ const Kv4Args &args_again() {
+  uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const Kv4Args *)reinterpret_cast<const __attribute__((address_space(4))) Kv4Args *>(p);
+}
 
 // Dims that a wave works on (DW); the waves of a key group share the head dim.
 template <int HD>
@@ -136,11 +143,12 @@ __device__ __forceinline__ float other_half(float x) {
 // kSlack, so the outputs are hardly ever scaled again; a step's loads are under way during the one
 // before it.
 // A block that met a scale that is not plain (or a row of q below 2^-103) does its rows again in the
-// general way, without PLAIN: k with an exponent per key, which the score takes back; v in as many
-// products as the step has bands of kBand octaves of scales, each with the weights of the keys in it
-// scaled for their largest and with its exponent put back in FP32.  (With one exponent per row, a single
-// large value took the bits of all other keys' weights, in all dims.)  One token over 16001 keys of
-// 512, all scales plain / none: 13.3 / 18.8 us; both ways in one loop, 188 bytes of spills per lane.
+// general way, without PLAIN, in as many products as the step has bands of kBand octaves of scales: k's
+// counted from each key's largest, v's from the step's, these with the weights of the keys in a band
+// scaled for their largest; exponents are put back in FP32.  (With one exponent per row of the cache and
+// of the outputs, a large value takes the bits of the row's small ones and of all other keys' weights,
+// in all dims.)  One token over 16001 keys of 512, all scales plain / none: 13.4 / 19.5 us; both ways in
+// one loop, 188 bytes of spills per lane.
 // What bounds it: one token over 131072 keys of 512 (75.5 MB) 23.3 us traced, 3.2 TB/s: 4 steps per
 // wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
 // exponent, fused step) and the products between them, and as long again before and behind them
@@ -295,7 +303,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
   for (int r = 0; r < RT; ++r) {
     pos[r] = S.pos0 + min(R0 + 16 * r + cr, S.rows - 1) / S.heads;
     xe[r] = sm.xq[16 * r + cr];
-    xf[r] = ldexpf(kLog2e, usual_row(xe[r]) ? xe[r] : 0);
+    xf[r] = PLAIN ? ldexpf(kLog2e, xe[r]) : kLog2e;
     if (!usual_row(xe[r])) beyond = (ushort2_t){0xffff, 0xffff};
     m[r] = kNoScore;
     l[r] = 0.f;
@@ -313,35 +321,8 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     const int last = hi - 1 - (lo + min(step, steps - 1) * kStep);  // row of the step
     if constexpr (!PLAIN) load_k(step);
     if (last < kStep - 1) look_k(last);
-    uint32_t ke[2] = {0, 0};  // the keys' exponents, a byte each
-    Scale x[2][KS];
-    if constexpr (PLAIN) {
-      ushort2_t far = {0, 0};
-#pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int J = 0; J < KS; ++J) x[T][J] = plain_pair(ksr[T][J], ksr[T][J], far);
-      if (mine) beyond = __builtin_elementwise_max(beyond, far);
-    } else {
-#pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        int top = 0;
-#pragma unroll
-        for (int J = 0; J < KS; ++J) top = max(top, (int)(ksr[T][J] & 0x7fffu));
-        top = max(top, __shfl_xor(top, 16, 64));
-        top = max(top, __shfl_xor(top, 32, 64));
-        const int e = min(scale_exponent(top), 127);
-#pragma unroll
-        for (int J = 0; J < KS; ++J) {
-          const float f = bf16_to_f32(ksr[T][J]) * pow2_8_minus(e);
-          x[T][J] = scale_pair(f, f);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ke[T] |= (uint32_t)(__shfl(e - 8 + kLift, 4 * g + i, 64) & 255) << (8 * i);
-      }
-    }
-    f32x4 s[RT][2];
-    {
+    // S^T = K . Q^T with the values' scales x
+    auto scores = [&](const Scale (&x)[2][KS], f32x4 (&y)[RT][2]) {
       f32x4 sh[RT][2], sl[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -380,16 +361,61 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
 #pragma unroll
         for (int T = 0; T < 2; ++T)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[r][T][i] = (sh[r][T][i] + (PAIR ? other_half(sh[r][T][i]) : sl[r][T][i])) * xf[r];
-      if constexpr (!PLAIN) {
+          for (int i = 0; i < 4; ++i) y[r][T][i] = (sh[r][T][i] + (PAIR ? other_half(sh[r][T][i]) : sl[r][T][i])) * xf[r];
+    };
+    f32x4 s[RT][2];
+    Scale x[2][KS];
+    if constexpr (PLAIN) {
+      ushort2_t far = {0, 0};
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+      for (int T = 0; T < 2; ++T)
 #pragma unroll
-          for (int T = 0; T < 2; ++T)
+        for (int J = 0; J < KS; ++J) x[T][J] = plain_pair(ksr[T][J], ksr[T][J], far);
+      if (mine) beyond = __builtin_elementwise_max(beyond, far);
+      scores(x, s);
+    } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[r][T][i] = ldexpf(s[r][T][i], (usual_row(xe[r]) ? 0 : xe[r]) + byte_of(ke[T], i));
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) s[r][T] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      uint32_t left = ~0u;  // scales of this lane that have yet to be taken
+      for (;;) {  // 22 times at most: each takes kBand of 255 exponents of every key, and some scale
+        int top[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          top[T] = 0;
+#pragma unroll
+          for (int J = 0; J < KS; ++J)
+            if (left >> (T * KS + J) & 1) top[T] = max(top[T], scale_exponent(ksr[T][J]));
+          top[T] = max(top[T], __shfl_xor(top[T], 16, 64));
+          top[T] = max(top[T], __shfl_xor(top[T], 32, 64));
+        }
+        if (!__any(max(top[0], top[1]) > 0)) break;
+        // (each time anew, as v below)
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int i = 0; i < KW; ++i) asm volatile("" : "+v"(kr[T][i]));
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int J = 0; J < KS; ++J) {
+            const bool in = (left >> (T * KS + J) & 1) && scale_exponent(ksr[T][J]) > max(top[T] - kBand, 0);
+            if (in) left &= ~(1u << (T * KS + J));
+            const float f = in ? scale_under(ksr[T][J], top[T]) : 0.f;
+            x[T][J] = scale_pair(f, f);
+          }
+        f32x4 y[RT][2];
+        scores(x, y);
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = __shfl(top[T], 4 * g + i, 64) - 132 + kLift;
+            // (q's exponent and the key's at once: either alone may overflow)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r][T][i] += ldexpf(y[r][T][i], xe[r] + e);
+          }
       }
     }
     if constexpr (PLAIN) load_k(step + KG);
@@ -514,12 +540,11 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
       uint32_t left = 0;  // keys of which this lane's dims have yet to be added
 #pragma unroll
       for (int j = 0; j < 8; ++j) left |= (vsr[j] & 0x7fff ? 1u : 0u) << j;
-      auto exponent = [&](int j) { return max((int)(vsr[j] >> 7 & 255), 1); };
       for (;;) {  // 22 times at most: each takes kBand of 254 exponents, and some key
         int top = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (left >> j & 1) top = max(top, exponent(j));
+          if (left >> j & 1) top = max(top, scale_exponent(vsr[j]));
         top = __builtin_amdgcn_readfirstlane(team_max<64>(top));
         if (top == 0) break;
         // (each time anew: unpacked before the loop, the codes alone would fill the registers)
@@ -527,13 +552,13 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
         for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int i = 0; i < VW; ++i) asm volatile("" : "+v"(vr[j][i]));
-        float f[8];  // from 2^(6 - kBand) up to 2^6, or 0
+        float f[8];
         uint32_t take = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool in = (left >> j & 1) && exponent(j) > top - kBand;
+          const bool in = (left >> j & 1) && scale_exponent(vsr[j]) > top - kBand;
           take |= (in ? 1u : 0u) << j;
-          f[j] = in ? ldexpf(bf16_to_f32(vsr[j]), 132 - top) : 0.f;
+          f[j] = in ? scale_under(vsr[j], top) : 0.f;
         }
         left &= ~take;
         Scale vs[4];
@@ -596,7 +621,8 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
     for (int i = 0; i < W; ++i) again |= sm.other[i];
     if (__builtin_amdgcn_readfirstlane(again)) {
       __syncthreads();
-      attend<HD, RT, PAIR, W, DW, false>(a, R0, split, run, sm);
+      const Kv4Args &b = args_again();
+      attend<HD, RT, PAIR, W, DW, false>(b, R0, split, Run(b.s, R0, R, split, kStep), sm);
       return;
     }
   }
@@ -987,9 +1013,11 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
 #pragma unroll
   for (int d = 0; d < W; ++d) again |= stop[d][0];
   if (__builtin_amdgcn_readfirstlane(again)) {
-    for (int r = 0; r < R && R0 + r < S.rows; r += 16) {
+    const Kv4Args &b = args_again();
+    const Run all(b.s, R0, R, split, KEYS);
+    for (int r = 0; r < R && R0 + r < b.s.rows; r += 16) {
       __syncthreads();
-      attend<HD, 1, false, W, DW, false>(a, R0 + r, split, run, sm.general);
+      attend<HD, 1, false, W, DW, false>(b, R0 + r, split, all, sm.general);
     }
     return;
   }

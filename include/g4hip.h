@@ -487,8 +487,7 @@ int g4_kv4_read(const g4_kv4 *cache, int at, int n, float *k, float *v);
  * Rows that a query row does not see have no influence on it, whatever they hold.
  * heads <= 8; qrows <= 2^20; keylen <= 2^28; q and y 16-byte aligned.
  * Products are of FP16 pairs with sums in FP32: a q and a weight are held to 2^-22 of
- * them, or to 2^-38 of their row's largest if that is more; v as it is, and k but for
- * values whose scale is less than 2^-25 of their row's largest, which lose bits.  A q or k
+ * them, or to 2^-38 of their row's largest if that is more; k and v as they are.  A q or k
  * without a number gives the row NaN, a v whose scale is none (an infinite one too) its
  * 32 dims. */
 int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int heads, int keylen,

@@ -81,3 +81,39 @@ def test_all_values_near_the_smallest_number(g4, hd, exp):
     rng = np.random.default_rng([hd, exp + 200])
     q, k, v = inputs(rng, 3, 8, hd, 2000)
     check_groups(g4, q, ref.pack(k), ref.pack((v * np.float32(2.0 ** exp)).astype(np.float32)), 2000, 1997, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("qrows", [1, 12, 40])
+def test_the_largest_q_and_small_k(g4, hd, qrows):
+    # scores of up to 2^27, 2^25 and more apart: each row's weight is on one key
+    keys = 300
+    rng = np.random.default_rng([hd, qrows, 6])
+    q, k, v = inputs(rng, qrows, 8, hd, keys)
+    q[:], k[:] = 0, 0
+    q[:, :, 0] = np.float32(2.0 ** 124)
+    k[:, 0], k[:, 1] = np.float32(2.0 ** -100), np.float32(7 * 2.0 ** -100)  # (the second one for the scale)
+    k[37, 0] = np.float32(5 * 2.0 ** -100)
+    k[keys - 1, 0] = np.float32(7 * 2.0 ** -100)
+    check_groups(g4, q, ref.pack(k), ref.pack(v), keys, keys - qrows, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("qrows", [1, 12, 45])
+@pytest.mark.parametrize("what", ["zeros", "large", "any"])
+def test_small_k_beside_large_ones(g4, hd, qrows, what):
+    # the scores come from one group of k, 2^-40 times the usual; the others hold zeros, whose scale is 1,
+    # values 2^30 times the usual that q does not look at, or ones of any size in each key
+    keys = 320
+    rng = np.random.default_rng([hd, qrows, len(what)])
+    q, k, v = inputs(rng, qrows, 8, hd, keys)
+    group = rng.integers(0, hd // 32)
+    mine = np.arange(hd) // 32 == group
+    q[:, :, ~mine] = 0
+    q[:, :, mine] *= np.float32(2.0 ** 40)
+    k[:, mine] *= np.float32(2.0 ** -40)
+    if what == "any":
+        k[:, ~mine] *= np.repeat(np.exp2(rng.integers(-60, 61, (keys, hd // 32 - 1))), 32, axis=1).astype(np.float32)
+    else:
+        k[:, ~mine] *= np.float32(0 if what == "zeros" else 2.0 ** 30)
+    check_groups(g4, q, ref.pack(k), ref.pack(v), keys, keys - qrows, 0)
