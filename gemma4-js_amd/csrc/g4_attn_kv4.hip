@@ -473,7 +473,7 @@ __device__ __forceinline__ void attend(const Kv4Args &a, int R0, int split, cons
           }
         }
       }
-      const int row = R0 + 16 * r + cr;
+      const int row = min(R0 + 16 * r + cr, S.rows - 1);
       if (S.score && mine && dq == 0) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
@@ -913,7 +913,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
       if (S.score) {
 #pragma unroll
         for (int T = 0; T < NT; ++T)
-          *reinterpret_cast<f32x4 *>(S.score + (size_t)my_row * S.stride + (key0 + 16 * T + 4 * g - S.first)) =
+          *reinterpret_cast<f32x4 *>(S.score + (size_t)min(my_row, S.rows - 1) * S.stride + (key0 + 16 * T + 4 * g - S.first)) =
               (f32x4){x[T][0], x[T][1], x[T][2], x[T][3]};
       }
       float tm = kNoScore;
@@ -1223,36 +1223,50 @@ Plan plan_of(int rows, int keys) {
   else return {attn_kv4_kernel<HD, 2, false, 4>, 32, kStep * kGroups<HD, 4>, 2, 256};
 }
 
-// The rows of a.s, all at once; `before` and `weights` of this call.
+// What the rows of s, all at once, take.
+struct Needs {
+  Plan plan;
+  int blocks, splits;
+  size_t part, score, ml, sum;  // floats
+  size_t bytes() const { return (part + score + ml + sum) * 4; }
+};
 template <int HD>
-int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
-  Scores &s = a.s;
+Needs needs_of(const Scores &s, bool weights) {
   const int keys = s.window > 0 ? min(s.end - s.first, s.window + 64) : s.end - s.first;  // of a block
-  const Plan plan = plan_of<HD>(s.rows, keys);
-  const int blocks = cdiv(s.rows, plan.rows);
+  Needs n;
+  n.plan = plan_of<HD>(s.rows, keys);
+  n.blocks = cdiv(s.rows, n.plan.rows);
   // A block per CU, or as many as fit where each then has several turns: the join of their outputs
   // costs more than a shorter loop gains.  One token, us: 16001 keys of 512, 251 splits of one turn
   // 14.7, 126 of two 16.4; 32003 with weights 256 of two 20.9, 512 of one 24.9; 131072 512 of
   // four 29.1, 256 of eight 30.7.
-  const int turns = cdiv(keys, plan.keys);
-  int splits = cu_count() / blocks;
-  if (turns >= 4 * plan.per_cu * splits) splits = plan.per_cu * cu_count() / blocks;
-  if (splits > turns) splits = turns;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits < 1) splits = 1;
-  s.splits = splits;
-  const bool ml = weights || splits > 1;
-  const size_t n_part = splits > 1 ? (size_t)splits * s.rows * HD : 0, n_ml = ml ? (size_t)splits * s.rows * 2 : 0;
-  const size_t n_score = weights ? score_floats(s.rows, s.stride) : 0;
-  const size_t n_sum = weights ? weight_part_floats(s.rows, s.end - s.first) : 0;
-  if (n_part + n_ml + n_score + n_sum) {
-    void *mem = nullptr;
-    if (int rc = g_kv4_ws.get((n_part + n_ml + n_score + n_sum) * 4, &mem, "g4_attention_kv4")) return rc;
+  const int turns = cdiv(keys, n.plan.keys);
+  n.splits = cu_count() / n.blocks;
+  if (turns >= 4 * n.plan.per_cu * n.splits) n.splits = n.plan.per_cu * cu_count() / n.blocks;
+  if (n.splits > turns) n.splits = turns;
+  if (n.splits > kMaxSplits) n.splits = kMaxSplits;
+  if (n.splits < 1) n.splits = 1;
+  n.part = n.splits > 1 ? (size_t)n.splits * s.rows * HD : 0;
+  n.ml = weights || n.splits > 1 ? (size_t)n.splits * s.rows * 2 : 0;
+  n.score = weights ? s.rows * s.stride : 0;
+  n.sum = weights ? weight_part_floats(s.rows, s.end - s.first) : 0;
+  return n;
+}
+
+// The rows of a.s, all at once; `before` and `weights` of this call.
+template <int HD>
+int launch_rows(Kv4Args a, void *mem, int keylen, const float *before, float *weights) {
+  Scores &s = a.s;
+  const Needs n = needs_of<HD>(s, weights != nullptr);
+  const int splits = s.splits = n.splits;
+  float *part = nullptr;
+  if (n.bytes()) {
     a.part = static_cast<float *>(mem);
-    s.score = weights ? a.part + n_part : nullptr;
-    s.ml = reinterpret_cast<float2 *>(a.part + n_part + n_score);
+    s.score = weights ? a.part + n.part : nullptr;
+    s.ml = reinterpret_cast<float2 *>(a.part + n.part + n.score);
+    part = a.part + n.part + n.score + n.ml;
   }
-  hipLaunchKernelGGL(plan.kernel, dim3(blocks, splits), dim3(plan.threads), 0, stream(), a);
+  hipLaunchKernelGGL(n.plan.kernel, dim3(n.blocks, splits), dim3(n.plan.threads), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
   if (splits > 1 && weights && s.rows <= kGroup) {
     const SumArgs sums{s, keylen, before, weights, nullptr};
@@ -1263,7 +1277,6 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   }
   const int joins = (int)(((size_t)s.rows * (HD / 4) + 255) / 256);
   const bool join = splits > 1 && s.rows >= 64 && splits <= 16;
-  float *part = a.part + n_part + n_score + n_ml;
   if (join && weights) {
     const SumArgs sums{s, keylen, before, weights, part};
     const int tiles = cdiv(s.end - s.first, 256);
@@ -1281,6 +1294,30 @@ int launch_rows(Kv4Args a, int keylen, const float *before, float *weights) {
   }
   if (!weights) return G4_OK;
   return launch_weights(s, keylen, part, before, weights);
+}
+
+// All rows of a call, in chunks whose scores are kept at once.
+template <int HD>
+int launch_chunks(const Kv4Args &call, int qrows, int heads, int keylen, int qpos0, int win, const float *before,
+                  float *weights) {
+  const int most = weights ? weighted_rows(qrows, heads, keylen, qpos0, win) : qrows;
+  auto scores_at = [&](int r0) { return scores_of(qrows - r0 < most ? qrows - r0 : most, heads, qpos0 + r0, win); };
+  size_t need = 0;  // of the chunk that takes most, before the first one
+  for (int r0 = 0; r0 < qrows; r0 += most) {
+    const size_t n = needs_of<HD>(scores_at(r0), weights != nullptr).bytes();
+    if (n > need) need = n;
+  }
+  void *mem = nullptr;
+  if (need)
+    if (int rc = growing_scratch(g_kv4_ws, need, &mem, "g4_attention_kv4")) return rc;
+  for (int r0 = 0; r0 < qrows; r0 += most) {
+    Kv4Args a = call;
+    a.q += (size_t)r0 * heads * HD;
+    a.y += (size_t)r0 * heads * HD;
+    a.s = scores_at(r0);
+    if (int rc = launch_rows<HD>(a, mem, keylen, r0 ? weights : before, weights)) return rc;
+  }
+  return G4_OK;
 }
 
 }  // namespace
@@ -1322,32 +1359,18 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
     if (weights) rc = launch_weights(s, keylen, nullptr, before, weights);
     return rc ? rc : ok();
   }
-  const int most = weights ? weighted_rows(qrows, heads, keylen, qpos0, win) : qrows;
-  for (int r0 = 0; r0 < qrows; r0 += most) {
-    const int n = qrows - r0 < most ? qrows - r0 : most;
-    Kv4Args a{};
-    a.q = q + (size_t)r0 * heads * head_dim;
-    a.y = y + (size_t)r0 * heads * head_dim;
-    a.k = cache->k;
-    a.v = cache->v;
-    a.ks = cache->k_scales;
-    a.vs = cache->v_scales;
-    Scores &s = a.s;
-    s.rows = n * heads;
-    s.heads = heads;
-    s.pos0 = qpos0 + r0;
-    s.window = win;
-    s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
-    s.end = s.pos0 + n;
-    s.stride = score_stride(s.end - s.first);
-    const float *b = r0 ? weights : before;
-    switch (head_dim) {
-      case 64: rc = launch_rows<64>(a, keylen, b, weights); break;
-      case 128: rc = launch_rows<128>(a, keylen, b, weights); break;
-      case 256: rc = launch_rows<256>(a, keylen, b, weights); break;
-      default: rc = launch_rows<512>(a, keylen, b, weights); break;
-    }
-    if (rc) return rc;
+  Kv4Args a{};
+  a.q = q;
+  a.y = y;
+  a.k = cache->k;
+  a.v = cache->v;
+  a.ks = cache->k_scales;
+  a.vs = cache->v_scales;
+  switch (head_dim) {
+    case 64: rc = launch_chunks<64>(a, qrows, heads, keylen, qpos0, win, before, weights); break;
+    case 128: rc = launch_chunks<128>(a, qrows, heads, keylen, qpos0, win, before, weights); break;
+    case 256: rc = launch_chunks<256>(a, qrows, heads, keylen, qpos0, win, before, weights); break;
+    default: rc = launch_chunks<512>(a, qrows, heads, keylen, qpos0, win, before, weights); break;
   }
-  return ok();
+  return rc ? rc : ok();
 }

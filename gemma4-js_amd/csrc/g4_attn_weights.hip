@@ -66,7 +66,25 @@ int cdiv(int a, int b) { return (a + b - 1) / b; }
 }  // namespace
 
 size_t score_stride(int keys) { return (size_t)((keys + 3) & ~3) + 32; }
-size_t score_floats(int rows, size_t stride) { return (size_t)((rows + 63) & ~63) * stride; }
+Scores scores_of(int qrows, int heads, int pos0, int window) {
+  Scores s{};
+  s.rows = qrows * heads;
+  s.heads = heads;
+  s.pos0 = pos0;
+  s.window = window;
+  s.first = window > 0 && pos0 >= window ? pos0 - window + 1 : 0;
+  s.end = pos0 + qrows;
+  s.stride = score_stride(s.end - s.first);
+  return s;
+}
+int growing_scratch(Workspace &ws, size_t need, void **p, const char *who) {
+  const size_t ahead = ws.bytes + ws.bytes / 2;
+  if (need > ws.bytes && need < ahead && !encoding()) {
+    const int rc = ws.get(ahead, p, who);
+    if (rc != G4_E_NOMEM) return rc;
+  }
+  return ws.get(need, p, who);
+}
 size_t weight_part_floats(int rows, int keys) {
   return rows > kGroup ? (size_t)cdiv(rows, kGroup) * keys : 0;
 }
@@ -322,7 +340,7 @@ __device__ __forceinline__ void few_scores(const ScoreArgs &a, int R0, int split
             if (key > pos[r] || (S.window > 0 && key <= pos[r] - S.window)) s[r][T][i] = -INFINITY;
           }
       }
-      const int row = R0 + 16 * r + c;
+      const int row = min(R0 + 16 * r + c, S.rows - 1);
       float tm = kNoScore;
 #pragma unroll
       for (int T = 0; T < NT; ++T) {
@@ -511,7 +529,7 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
 
   // this wave's rows and keys
   const int mr = w % RT, mt = w / RT;
-  const int my_row = R0 + 16 * mr + c, my_pos = S.pos0 + min(my_row, S.rows - 1) / S.heads;
+  const int my_row = min(R0 + 16 * mr + c, S.rows - 1), my_pos = S.pos0 + my_row / S.heads;
   float m = kNoScore, l = 0.f;
   if (t0 < t1) scores(t0, ka, kb);
   asm volatile("" ::: "memory");  // (else loads move into the loop, with an address of 64 bits each)
@@ -599,6 +617,32 @@ ScorePlan score_plan(int rows, int keys) {
     return {scores_kernel<HD, 1, 2, 4>, 64, 32 * kWaves, 2, 64 * kWaves};
 }
 
+// What one launch over s takes.
+struct ScoreNeeds {
+  ScorePlan plan;
+  int blocks, splits;
+  size_t score, ml, sum;  // floats
+  size_t bytes() const { return (score + ml + sum) * 4; }
+};
+ScoreNeeds needs_of(const Scores &s, int head_dim) {
+  const int keys = s.end - s.first;
+  ScoreNeeds n;
+  n.plan = head_dim == 64    ? score_plan<64>(s.rows, keys)
+           : head_dim == 128 ? score_plan<128>(s.rows, keys)
+           : head_dim == 256 ? score_plan<256>(s.rows, keys)
+                             : score_plan<512>(s.rows, keys);
+  const int steps = cdiv(keys, n.plan.keys);
+  n.blocks = cdiv(s.rows, n.plan.rows);
+  n.splits = n.plan.per_cu * cu_count() / n.blocks;
+  if (n.splits > steps) n.splits = steps;
+  if (n.splits > kMaxSplits) n.splits = kMaxSplits;
+  if (n.splits < 1) n.splits = 1;
+  n.score = s.rows * s.stride;
+  n.ml = (size_t)n.splits * s.rows * 2;
+  n.sum = weight_part_floats(s.rows, keys);
+  return n;
+}
+
 Workspace g_weights_ws;
 
 }  // namespace
@@ -633,38 +677,26 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     return rc ? rc : ok();
   }
   const int most = weighted_rows(qrows, heads, keylen, qpos0, win);
+  auto scores_at = [&](int r0) { return scores_of(qrows - r0 < most ? qrows - r0 : most, heads, qpos0 + r0, win); };
+  size_t need = 0;  // of the chunk that takes most, before the first one
   for (int r0 = 0; r0 < qrows; r0 += most) {
-    const int n = qrows - r0 < most ? qrows - r0 : most;
+    const size_t n = needs_of(scores_at(r0), head_dim).bytes();
+    if (n > need) need = n;
+  }
+  void *mem = nullptr;
+  if ((rc = growing_scratch(g_weights_ws, need, &mem, who))) return rc;
+  for (int r0 = 0; r0 < qrows; r0 += most) {
     ScoreArgs a{};
     a.q = q + (size_t)r0 * heads * head_dim;
     a.k = k;
-    Scores &s = a.s;
-    s.rows = n * heads;
-    s.heads = heads;
-    s.pos0 = qpos0 + r0;
-    s.window = win;
-    s.first = win > 0 && s.pos0 >= win ? s.pos0 - win + 1 : 0;
-    s.end = s.pos0 + n;
-    s.stride = score_stride(s.end - s.first);
-    const int keys = s.end - s.first;
-    const ScorePlan plan = head_dim == 64    ? score_plan<64>(s.rows, keys)
-                           : head_dim == 128 ? score_plan<128>(s.rows, keys)
-                           : head_dim == 256 ? score_plan<256>(s.rows, keys)
-                                             : score_plan<512>(s.rows, keys);
-    const int blocks = cdiv(s.rows, plan.rows), steps = cdiv(keys, plan.keys);
-    s.splits = plan.per_cu * cu_count() / blocks;
-    if (s.splits > steps) s.splits = steps;
-    if (s.splits > kMaxSplits) s.splits = kMaxSplits;
-    if (s.splits < 1) s.splits = 1;
-    const size_t scores = score_floats(s.rows, s.stride), ml = (size_t)s.splits * s.rows * 2;
-    void *mem = nullptr;
-    if ((rc = g_weights_ws.get((scores + ml + weight_part_floats(s.rows, s.end - s.first)) * 4, &mem, who)))
-      return rc;
+    Scores &s = a.s = scores_at(r0);
+    const ScoreNeeds n = needs_of(s, head_dim);
+    s.splits = n.splits;
     s.score = static_cast<float *>(mem);
-    s.ml = reinterpret_cast<float2 *>(s.score + scores);
-    hipLaunchKernelGGL(plan.kernel, dim3(blocks, s.splits), dim3(plan.threads), 0, stream(), a);
+    s.ml = reinterpret_cast<float2 *>(s.score + n.score);
+    hipLaunchKernelGGL(n.plan.kernel, dim3(n.blocks, n.splits), dim3(n.plan.threads), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");
-    rc = launch_weights(s, keylen, s.score + scores + ml, r0 ? weights : before, weights);
+    rc = launch_weights(s, keylen, s.score + n.score + n.ml, r0 ? weights : before, weights);
     if (rc) return rc;
   }
   return ok();

@@ -16,8 +16,8 @@ int check_kv4_memory(const g4_kv4 *c, size_t rows, bool k, bool v, const char *w
 // units of log 2, and (maximum, sum of 2^(score - maximum)) of each row and key split.  Query row
 // i sits at position pos0 + i; a key is seen at positions key .. key + window - 1 (window 0: all
 // from key on).
-// Kernels of up to 64 rows and 32 keys per step store whole blocks: what score_stride and
-// score_floats add to the rows and keys is theirs.
+// Kernels store whole steps of up to 32 keys: what score_stride adds to the keys is theirs.  Rows that
+// pad a block are the last row again, scores and address.
 struct Scores {
   float *score;
   float2 *ml;  // [rows][splits]
@@ -42,8 +42,14 @@ struct Run {
   }
 };
 
+// Query rows at positions pos0 .. without their memory.
+Scores scores_of(int qrows, int heads, int pos0, int window);
 size_t score_stride(int keys);
-size_t score_floats(int rows, size_t stride);
+
+// Scratch whose need follows a cache's length: a little more than there is asks for half as much again,
+// so that a chat whose every token needs a few rows more allocates (and clears) it now and then, not
+// at each of them.
+int growing_scratch(Workspace &ws, size_t need, void **p, const char *who);
 
 // weights[key] = before[key] + sum over the rows of 2^(score - max) / sum, for all keys < keylen;
 // `part` holds weight_part_floats(rows, end - first).
