@@ -1253,9 +1253,9 @@ Needs needs_of(const Scores &s, bool weights) {
   return n;
 }
 
-// The rows of a.s, all at once; `before` and `weights` of this call.
+// The rows of a.s, all at once; `before` and `weights` of keys key0 .. keylen - 1.
 template <int HD>
-int launch_rows(Kv4Args a, void *mem, int keylen, const float *before, float *weights) {
+int launch_rows(Kv4Args a, void *mem, int key0, int keylen, const float *before, float *weights) {
   Scores &s = a.s;
   const Needs n = needs_of<HD>(s, weights != nullptr);
   const int splits = s.splits = n.splits;
@@ -1269,8 +1269,8 @@ int launch_rows(Kv4Args a, void *mem, int keylen, const float *before, float *we
   hipLaunchKernelGGL(n.plan.kernel, dim3(n.blocks, splits), dim3(n.plan.threads), 0, stream(), a);
   G4_LAUNCH_CHECK("attn_kv4_kernel");
   if (splits > 1 && weights && s.rows <= kGroup) {
-    const SumArgs sums{s, keylen, before, weights, nullptr};
-    hipLaunchKernelGGL(attn_kv4_merge_weights_kernel<HD>, dim3(s.rows * (HD / 32) + cdiv(keylen, 256)), dim3(256), 0,
+    const SumArgs sums{s, key0, keylen, before, weights, nullptr};
+    hipLaunchKernelGGL(attn_kv4_merge_weights_kernel<HD>, dim3(s.rows * (HD / 32) + cdiv(keylen - key0, 256)), dim3(256), 0,
                        stream(), a, sums);
     G4_LAUNCH_CHECK("attn_kv4_merge_weights_kernel");
     return G4_OK;
@@ -1278,12 +1278,12 @@ int launch_rows(Kv4Args a, void *mem, int keylen, const float *before, float *we
   const int joins = (int)(((size_t)s.rows * (HD / 4) + 255) / 256);
   const bool join = splits > 1 && s.rows >= 64 && splits <= 16;
   if (join && weights) {
-    const SumArgs sums{s, keylen, before, weights, part};
+    const SumArgs sums{s, key0, keylen, before, weights, part};
     const int tiles = cdiv(s.end - s.first, 256);
     hipLaunchKernelGGL(attn_kv4_join_weights_kernel<HD>, dim3(joins + tiles * cdiv(s.rows, kGroup)), dim3(256), 0,
                        stream(), a, sums, joins, tiles);
     G4_LAUNCH_CHECK("attn_kv4_join_weights_kernel");
-    return launch_weights_join(s, keylen, part, before, weights);
+    return launch_weights_join(s, key0, keylen, part, before, weights);
   }
   if (splits > 1) {
     if (join)
@@ -1293,14 +1293,14 @@ int launch_rows(Kv4Args a, void *mem, int keylen, const float *before, float *we
     G4_LAUNCH_CHECK("attn_kv4_merge_kernel");
   }
   if (!weights) return G4_OK;
-  return launch_weights(s, keylen, part, before, weights);
+  return launch_weights(s, key0, keylen, part, before, weights);
 }
 
 // All rows of a call, in chunks whose scores are kept at once.
 template <int HD>
 int launch_chunks(const Kv4Args &call, int qrows, int heads, int keylen, int qpos0, int win, const float *before,
                   float *weights) {
-  const int most = weights ? weighted_rows(qrows, heads, keylen, qpos0, win) : qrows;
+  const int most = weights ? weighted_rows(qrows, heads, qpos0, win) : qrows;
   auto scores_at = [&](int r0) { return scores_of(qrows - r0 < most ? qrows - r0 : most, heads, qpos0 + r0, win); };
   size_t need = 0;  // of the chunk that takes most, before the first one
   for (int r0 = 0; r0 < qrows; r0 += most) {
@@ -1315,7 +1315,10 @@ int launch_chunks(const Kv4Args &call, int qrows, int heads, int keylen, int qpo
     a.q += (size_t)r0 * heads * HD;
     a.y += (size_t)r0 * heads * HD;
     a.s = scores_at(r0);
-    if (int rc = launch_rows<HD>(a, mem, keylen, r0 ? weights : before, weights)) return rc;
+    // (later chunks add to the keys that they see)
+    const int rc = r0 ? launch_rows<HD>(a, mem, a.s.first, a.s.end, weights, weights)
+                      : launch_rows<HD>(a, mem, 0, keylen, before, weights);
+    if (rc) return rc;
   }
   return G4_OK;
 }
@@ -1356,7 +1359,7 @@ G4_API int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int 
   if (qrows == 0) {
     Scores s{};
     s.heads = 1;
-    if (weights) rc = launch_weights(s, keylen, nullptr, before, weights);
+    if (weights) rc = launch_weights(s, 0, keylen, nullptr, before, weights);
     return rc ? rc : ok();
   }
   Kv4Args a{};

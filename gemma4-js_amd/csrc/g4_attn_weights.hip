@@ -24,11 +24,13 @@ int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int
   return G4_OK;
 }
 
-int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window) {
-  const size_t keys = window > 0 && window + qrows < keylen ? window + qrows : keylen;
-  size_t rows = kScoreFloats / (keys * heads);
-  if (rows < 8) rows = 8;
-  return rows < (size_t)qrows ? (int)rows : qrows;
+// The most rows r with r * heads * keys <= kScoreFloats, where they see no more than the call's keys, or
+// than window + r of them.
+int weighted_rows(int qrows, int heads, int qpos0, int window) {
+  const double most = (double)(kScoreFloats / heads), w = window;
+  double rows = most / (qpos0 + qrows);
+  if (window > 0) rows = fmax(rows, (sqrt(w * w + 4 * most) - w) / 2);
+  return rows >= qrows ? qrows : rows < 8 ? 8 : (int)rows;
 }
 
 namespace {
@@ -42,7 +44,7 @@ __global__ __launch_bounds__(256) void weights_kernel(SumArgs a) { add_weights(a
 // 8.1 and 3.9: 2048 rows over 4096 keys.)
 // Adds the groups of a key, 16 of them under way together.
 __global__ __launch_bounds__(64) void weights_join_kernel(SumArgs a, int groups) {
-  const int key = blockIdx.x * 64 + threadIdx.x;
+  const int key = a.key0 + blockIdx.x * 64 + threadIdx.x;
   if (key >= a.keylen) return;
   const float before = a.before ? a.before[key] : 0.f;
   float sum = 0.f;
@@ -89,19 +91,19 @@ size_t weight_part_floats(int rows, int keys) {
   return rows > kGroup ? (size_t)cdiv(rows, kGroup) * keys : 0;
 }
 
-int launch_weights_join(const Scores &s, int keylen, float *part, const float *before, float *weights) {
-  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen, 64)), dim3(64), 0, stream(),
-                     (SumArgs{s, keylen, before, weights, part}), cdiv(s.rows, kGroup));
+int launch_weights_join(const Scores &s, int key0, int keylen, float *part, const float *before, float *weights) {
+  hipLaunchKernelGGL(weights_join_kernel, dim3(cdiv(keylen - key0, 64)), dim3(64), 0, stream(),
+                     (SumArgs{s, key0, keylen, before, weights, part}), cdiv(s.rows, kGroup));
   G4_LAUNCH_CHECK("weights_join_kernel");
   return G4_OK;
 }
 
-int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights) {
+int launch_weights(const Scores &s, int key0, int keylen, float *part, const float *before, float *weights) {
   const bool several = s.rows > kGroup;
-  hipLaunchKernelGGL(weights_kernel, dim3(cdiv(several ? s.end - s.first : keylen, 256), several ? cdiv(s.rows, kGroup) : 1),
-                     dim3(256), 0, stream(), (SumArgs{s, keylen, before, weights, several ? part : nullptr}));
+  hipLaunchKernelGGL(weights_kernel, dim3(cdiv(several ? s.end - s.first : keylen - key0, 256), several ? cdiv(s.rows, kGroup) : 1),
+                     dim3(256), 0, stream(), (SumArgs{s, key0, keylen, before, weights, several ? part : nullptr}));
   G4_LAUNCH_CHECK("weights_kernel");
-  return several ? launch_weights_join(s, keylen, part, before, weights) : G4_OK;
+  return several ? launch_weights_join(s, key0, keylen, part, before, weights) : G4_OK;
 }
 
 namespace {
@@ -673,10 +675,10 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
   if (qrows == 0) {
     Scores s{};
     s.heads = 1;
-    rc = launch_weights(s, keylen, nullptr, before, weights);
+    rc = launch_weights(s, 0, keylen, nullptr, before, weights);
     return rc ? rc : ok();
   }
-  const int most = weighted_rows(qrows, heads, keylen, qpos0, win);
+  const int most = weighted_rows(qrows, heads, qpos0, win);
   auto scores_at = [&](int r0) { return scores_of(qrows - r0 < most ? qrows - r0 : most, heads, qpos0 + r0, win); };
   size_t need = 0;  // of the chunk that takes most, before the first one
   for (int r0 = 0; r0 < qrows; r0 += most) {
@@ -696,7 +698,10 @@ G4_API int g4_attention_weights(const float *q, const float *k, int qrows, int h
     s.ml = reinterpret_cast<float2 *>(s.score + n.score);
     hipLaunchKernelGGL(n.plan.kernel, dim3(n.blocks, n.splits), dim3(n.plan.threads), 0, stream(), a);
     G4_LAUNCH_CHECK("scores_kernel");
-    rc = launch_weights(s, keylen, s.score + n.score + n.ml, r0 ? weights : before, weights);
+    // (later chunks add to the keys that they see)
+    float *part = s.score + n.score + n.ml;
+    rc = r0 ? launch_weights(s, s.first, s.end, part, weights, weights)
+            : launch_weights(s, 0, keylen, part, before, weights);
     if (rc) return rc;
   }
   return ok();

@@ -13,7 +13,7 @@ constexpr int kGroup = 32;                  // rows that a block adds up
 
 struct SumArgs {
   Scores s;
-  int keylen;
+  int key0, keylen;  // weights of keys key0 .. keylen - 1 are written
   const float *before;
   float *weights;
   float *part;  // [groups][end - first], or null
@@ -28,7 +28,7 @@ __device__ __forceinline__ void add_weights(const SumArgs &a, int bx, int by) {
   __shared__ float4 stat[kGroup];  // maximum, 1 / sum, last and (window) first key as bits
   const Scores &s = a.s;
   const int t = threadIdx.x, r0 = by * kGroup, n = min(kGroup, s.rows - r0);
-  const int key = bx * 256 + t + (a.part ? s.first : 0);
+  const int key = bx * 256 + t + (a.part ? s.first : a.key0);
   const bool any = key >= s.first && key < s.end;
   const float *p = s.score + (size_t)r0 * s.stride + (any ? key - s.first : 0);
   float x[kBatch];

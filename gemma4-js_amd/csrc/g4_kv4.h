@@ -51,18 +51,18 @@ size_t score_stride(int keys);
 // at each of them.
 int growing_scratch(Workspace &ws, size_t need, void **p, const char *who);
 
-// weights[key] = before[key] + sum over the rows of 2^(score - max) / sum, for all keys < keylen;
+// weights[key] = before[key] + sum over the rows of 2^(score - max) / sum, for keys key0 .. keylen - 1;
 // `part` holds weight_part_floats(rows, end - first).
 size_t weight_part_floats(int rows, int keys);
-int launch_weights(const Scores &s, int keylen, float *part, const float *before, float *weights);
+int launch_weights(const Scores &s, int key0, int keylen, float *part, const float *before, float *weights);
 // Its second launch alone, for more than 32 rows: the sums of each 32 rows are in `part`.
-int launch_weights_join(const Scores &s, int keylen, float *part, const float *before, float *weights);
+int launch_weights_join(const Scores &s, int key0, int keylen, float *part, const float *before, float *weights);
 
 // Arguments that g4_attention_kv4 and g4_attention_weights have in common.
 int check_weighted(int qrows, int heads, int keylen, int qpos0, int sliding, int window,
                    const float *before, const float *weights, const char *who);
-// Query rows whose scores are kept at once.
-int weighted_rows(int qrows, int heads, int keylen, int qpos0, int window);
+// Query rows of a call whose scores are kept at once.
+int weighted_rows(int qrows, int heads, int qpos0, int window);
 
 // op over aligned teams of `team` lanes, 4 .. 64 and the same for all, known to each of them
 template <class Op>
