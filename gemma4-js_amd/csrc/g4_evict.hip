@@ -361,8 +361,10 @@ __global__ __launch_bounds__(kThreads) void evict_rows_kernel(EvictArgs a) {
     const bool same = key[j] == top;
     if (key[j] > top || (same && equal < want)) {
       const int at = rows_before + above + min(equal, want) - base_equal;
-      rows[at] = i;
-      if (kept) kept[at] = x[j];
+      if ((unsigned)at < (unsigned)a.keep) {  // (always, unless another stream changes the weights meanwhile)
+        rows[at] = i;
+        if (kept) kept[at] = x[j];
+      }
     }
     above += key[j] > top ? 1 : 0;
     equal += same ? 1 : 0;
@@ -372,8 +374,24 @@ __global__ __launch_bounds__(kThreads) void evict_rows_kernel(EvictArgs a) {
     if (slice * kSlice + j >= a.keep) kept[slice * kSlice + j] = 0.f;
 }
 
+__global__ __launch_bounds__(kThreads) void evict_clear_kernel(int *hist) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) hist[blockIdx.x * kBins + i] = 0;
+}
+
 // The histograms, which each call leaves zero as it found them, and the rest.
 Workspace g_hist_ws, g_evict_ws;
+
+int launch_slices(const EvictArgs &a, int sets) {
+  hipLaunchKernelGGL(evict_count_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
+  G4_LAUNCH_CHECK("evict_count_kernel");
+  hipLaunchKernelGGL(evict_list_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
+  G4_LAUNCH_CHECK("evict_list_kernel");
+  hipLaunchKernelGGL(evict_threshold_kernel, dim3(sets), dim3(1024), 0, stream(), a);
+  G4_LAUNCH_CHECK("evict_threshold_kernel");
+  hipLaunchKernelGGL(evict_rows_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
+  G4_LAUNCH_CHECK("evict_rows_kernel");
+  return G4_OK;
+}
 
 }  // namespace
 }  // namespace g4
@@ -429,13 +447,12 @@ G4_API int g4_cache_evict(const float *weights, size_t stride, int sets, int len
   a.top = reinterpret_cast<uint32_t *>(a.count + all * 4);
   a.cand = a.top + (size_t)sets * 2;
   a.copy = n_copy ? reinterpret_cast<float *>(a.cand + all * kSlice) : nullptr;
-  hipLaunchKernelGGL(evict_count_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
-  G4_LAUNCH_CHECK("evict_count_kernel");
-  hipLaunchKernelGGL(evict_list_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
-  G4_LAUNCH_CHECK("evict_list_kernel");
-  hipLaunchKernelGGL(evict_threshold_kernel, dim3(sets), dim3(1024), 0, stream(), a);
-  G4_LAUNCH_CHECK("evict_threshold_kernel");
-  hipLaunchKernelGGL(evict_rows_kernel, dim3(a.slices, sets), dim3(kThreads), 0, stream(), a);
-  G4_LAUNCH_CHECK("evict_rows_kernel");
-  return ok();
+  rc = launch_slices(a, sets);
+  if (rc) {
+    // The third kernel, which clears the histograms, may be missing behind the first one, which adds to
+    // them: counts of this call would give later ones rows that do not exist.
+    hipLaunchKernelGGL(evict_clear_kernel, dim3(sets), dim3(kThreads), 0, stream(), a.hist);
+    if (hipGetLastError() != hipSuccess) g_hist_ws = Workspace();  // (the next call makes others)
+  }
+  return rc ? rc : ok();
 }
