@@ -44,6 +44,16 @@ bool overlaps_cache(const g4_kv4 *c, int at, int n, const float *k, const float 
   return false;
 }
 
+// The planes' first n rows against one another.
+bool planes_overlap(const g4_kv4 *c, size_t n) {
+  const void *p[] = {c->k, c->v, c->k_scales, c->v_scales};
+  const size_t codes = n * c->head_dim / 2, bytes[] = {codes, codes, codes / 8, codes / 8};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (overlap(p[i], bytes[i], p[j], bytes[j])) return true;
+  return false;
+}
+
 constexpr long kMaxBlocks = 1 << 23;  // of a launch, which has less than 2^32 threads
 
 struct Rows4 {
@@ -140,6 +150,7 @@ G4_API int g4_kv4_append(const g4_kv4 *c, const float *k, const float *v, int n,
   if (unaligned(k) || unaligned(v))
     return fail(G4_E_ARG, "g4_kv4_append: k and v must be 16-byte aligned");
   if (overlaps_cache(c, at, n, k, v)) return fail(G4_E_ARG, "g4_kv4_append: k or v overlaps the cache");
+  if (n > 0 && planes_overlap(c, (size_t)at + n)) return fail(G4_E_ARG, "g4_kv4_append: the cache's planes overlap");
   G4_CHECK_INIT();
   if (n == 0) return ok();
   const size_t bytes = (size_t)n * c->head_dim * 4;

@@ -471,7 +471,8 @@ typedef struct {
 /* cache rows at .. at + n - 1 = the n FP32 rows k and v [n, head_dim], with the PLE
  * builder's steps: scale = bf16_rne(max |x| / 7), 1 where that is 0, and codes
  * rint(x / scale) within 7, halves to even.  32 values of which one is not finite get a
- * NaN scale: all of them read as NaN.  k and v 16-byte aligned. */
+ * NaN scale: all of them read as NaN.  k and v 16-byte aligned.  The planes' rows up to
+ * the last one written overlap no other plane. */
 int g4_kv4_append(const g4_kv4 *cache, const float *k, const float *v, int n, int at);
 
 /* The values of cache rows at .. at + n - 1 as FP32 rows [n, head_dim] (exact); k or v
