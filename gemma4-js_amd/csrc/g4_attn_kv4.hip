@@ -21,7 +21,10 @@ typedef uint16_t any_u16 __attribute__((may_alias));
 constexpr float kLog2e = 1.4426950408889634f;
 // How far (log 2) a score may pass its row's reference before the outputs are scaled again.  Weights
 // are split into two FP16 values times 2^(15 - kSlack), so one is held to 2^-22 of it, or to 2^-38 of
-// its row's largest if that is more.
+// its row's largest if that is more.  (The attention over FP32 caches takes three BF16 parts of all four
+// operands, 24 bits.  Here k and v are exact in one FP16 value and would not be in one of BF16, 11 bits of
+// a nibble times a scale, so q and the weights are FP16 too: two values each, two products instead
+// of six, and the error that is left is far below what 4 bits of k and v make.)
 constexpr float kSlack = 2.f;
 constexpr float kWeight = 1 << (15 - (int)kSlack);
 constexpr int kStep = 32;                   // keys of a wave's step
@@ -713,7 +716,9 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void attn_kv4_rows_kernel(K
   constexpr int VD = DW / 16;         // dims per lane, and output tiles
   static_assert(DW == 64, "32 bytes of a row per wave");
   // (two of each: what the step's readers may still look at, and the next)
-  using General = AttendSmem<HD, 1, false, W, DW>;  // (of 32 rows: spills that all calls feel, 102.7 us for 94)
+  // (of 32 rows: spills that all calls feel, 102.7 us for 94.  So, HD 256 at three blocks per CU spills 9
+  // registers, HD 512 of 64 rows one: outside the loop, but for one where a reference moves.)
+  using General = AttendSmem<HD, 1, false, W, DW>;
   union Smem {
     struct {
       f32x4 sx[2][W][RT][NT][64];

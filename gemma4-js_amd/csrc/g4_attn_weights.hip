@@ -151,7 +151,10 @@ __device__ __forceinline__ float group_max(float v) {
 // turn; the DQ waves of a group share the head dim and add their scores through LDS, in order.
 // q and k enter the FP16 matrix cores as two values each (hi hi, hi lo and lo hi; lo lo is below
 // 2^-22 of a product), q with its row's largest at the exponent 13, k times 2^8; a wave in which a
-// key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.
+// key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.  (The
+// attention over FP32 caches takes three BF16 parts of each, all 24 bits, in six products.  What these sums
+// decide is which rows are heavier; with three products they are nearer to 64 bits than sums of FP32
+// products on usual rows, and small values beside large ones keep what the header says.)
 // One token over 8001 keys of 512 (16.4 MB): 6.6 us traced, a step per wave whose loads are all
 // under way before q is ready; over 131072 keys 268 MB in 60 us with the sums, 4.5 TB/s: memory.
 template <int HD, int DQ, int NT, int RT, int W>
@@ -543,7 +546,8 @@ __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
     f32x4 y[W];  // (loaded before the next step's products)
 #pragma unroll
     for (int d = 0; d < W; ++d) y[d] = sm.sx[at][d][mr][mt][lane];
-    scores(step + 1, kr, next);  // (behind the last one: its keys once more, looked at by nobody)
+    // (behind the last one: keys of no score of this block, which may send it the general way all the same)
+    scores(step + 1, kr, next);
     f32x4 x = y[0];
 #pragma unroll
     for (int d = 1; d < W; ++d) x += y[d];

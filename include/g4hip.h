@@ -485,7 +485,10 @@ int g4_kv4_read(const g4_kv4 *cache, int at, int n, float *k, float *v);
  * With `weights` (FP32 [keylen], may be NULL) in addition
  *   weights[key] = before[key] + the weight of that key, summed over rows and heads,
  * before NULL counting as zeros; it may be weights itself, but not overlap it otherwise.
- * Rows that a query row does not see have no influence on it, whatever they hold.
+ * Rows that a query row does not see have no part in its results, whatever they hold.
+ * Those that other query rows of the call see may change their last bits, within the
+ * bounds below, and the call's time: scales outside 2^-18 .. 2^7 take blocks of rows
+ * another, slower way.
  * heads <= 8; qrows <= 2^20; keylen <= 2^28; q and y 16-byte aligned.
  * Products are of FP16 pairs with sums in FP32: a q and a weight are held to 2^-22 of
  * them, or to 2^-38 of their row's largest if that is more; k and v as they are.  A q or k
@@ -497,8 +500,11 @@ int g4_attention_kv4(const float *q, const g4_kv4 *cache, int qrows, int heads, 
 
 /* Those weights over FP32 keys: k [keylen, head_dim], rows and masks as g4_attention's,
  * before and weights as above, q held as it is there, k to 2^-22 of it or 2^-23 of its
- * row's largest; a k that is no number gives the rows that see it NaN.  head_dim 64,
- * 128, 256 or 512; heads, qrows and keylen as above; q and k 16-byte aligned. */
+ * row's largest, or to 2^-33 where that is more and all q nearby are below 16 (a score is
+ * then off by less than 10^-6); a k that is no number gives the rows that see it NaN, and
+ * keys that a row does not see have no part in its weights, but for last bits as above.
+ * head_dim 64, 128, 256 or 512; heads, qrows and keylen as above; q and k 16-byte
+ * aligned. */
 int g4_attention_weights(const float *q, const float *k, int qrows, int heads, int head_dim,
                          int keylen, int qpos0, int sliding, int window, const float *before,
                          float *weights);
