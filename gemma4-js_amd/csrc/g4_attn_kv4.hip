@@ -152,12 +152,13 @@ __device__ __forceinline__ float other_half(float x) {
 // of the outputs, a large value takes the bits of the row's small ones and of all other keys' weights,
 // in all dims.)  One token over 16001 keys of 512, all scales plain / none: 13.4 / 19.5 us; both ways in
 // one loop, 188 bytes of spills per lane.
-// What bounds it: one token over 131072 keys of 512 (75.5 MB) 23.3 us traced, 3.2 TB/s: 4 steps per
-// wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
+// What bounds it: one token over 131072 keys of 512 (75.5 MB) 22.0 us without its join, 3.4 TB/s: 4 steps
+// per wave, each about 600 vector instructions (three per pair of values unpacked: shift, mask and
 // exponent, fused step) and the products between them, and as long again before and behind them
 // (launch, q, the groups' sums, 8.4 MB of partial outputs).  Over 16001 keys a wave has one step:
-// 10.2 us, a chain of latencies (launch and arguments 1.2, q and the first k 1.8, the scores 1.1, softmax and
-// outputs 1.9, the groups' sums and stores 1.9).
+// 9.1 us, a chain of latencies (by the clock in a block, as it came in: launch and arguments 1.2, q and the
+// first k 1.8, the scores 1.1, softmax and outputs 1.9, the groups' sums and stores 1.9; what is left
+// lies between two launches).
 template <int HD, int RT, bool PAIR, int W, int DW>
 struct AttendSmem {
   static constexpr int DQ = HD / DW, KG = kGroups<HD, W, DW>, R = PAIR ? 8 : 16 * RT;
@@ -702,11 +703,12 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_kernel(Kv4Args a) {
 // all.  The next step's scores are formed before, so that one barrier per step makes both known.
 // A block that met another scale (or a row of q below 2^-103) does its rows again in the general way, 16 at a
 // time (a second launch for them cost all calls 2 to 3 us).
-// 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 94.0 us
-// traced, 0.78 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08.  Of about 4500 cycles per
-// step the matrix units are busy for 2050, of which a wave issues half while the other one of its
-// SIMD waits; the rest are vector instructions (280 per step of a wave that does softmax, 140 of the
-// others), the 64 KB of partial scores through LDS and back, and the barrier.  Tried and slower: 8
+// 512 rows over 4608 keys of 512 (8 heads, 73 GFLOP with both parts of q and of the weights): 83.0 us
+// without the join, 0.88 PFLOP/s, where a product of 8192^3 FP16 values runs at 1.08 (traced 92, until its
+// 33.5 MB of partial outputs are in memory).  The matrix units are busy for 40% of the cycles, and a
+// wave issues half of theirs while the other one of its SIMD waits; the rest are vector instructions (280
+// per step of a wave that does softmax, 140 of the others), the 64 KB of partial scores through
+// LDS and back, and the barrier.  Tried and slower, by passes of the whole call at the time: 8
 // rows of softmax for each wave (105.7), softmax before the next step's scores (105.5), 32 rows per
 // block (129), two blocks of 4 waves per CU (alike).
 template <int HD, int RT, int W>

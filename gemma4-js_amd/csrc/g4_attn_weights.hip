@@ -153,10 +153,11 @@ __device__ __forceinline__ float group_max(float v) {
 // 2^-22 of a product), q with its row's largest at the exponent 13, k times 2^8; a wave in which a
 // key's largest then is outside 2^-2 .. 2^15 does its step again with these keys' exponents.  (The
 // attention over FP32 caches takes three BF16 parts of each, all 24 bits, in six products.  What these sums
-// decide is which rows are heavier; with three products they are nearer to 64 bits than sums of FP32
-// products on usual rows, and small values beside large ones keep what the header says.)
-// One token over 8001 keys of 512 (16.4 MB): 6.6 us traced, a step per wave whose loads are all
-// under way before q is ready; over 131072 keys 268 MB in 60 us with the sums, 4.5 TB/s: memory.
+// decide is which rows are heavier; with three products they are about as near to 64 bits as sums of FP32
+// products, 5.1e-7 for 5.2e-7 and 4.2e-8 for 1.0e-7 of one and of 256 rows, and small values beside large
+// ones keep what the header says.)
+// One token over 8001 keys of 512 (16.4 MB): 6.1 us without the sums, a step per wave whose loads are all
+// under way before q is ready; over 131072 keys 268 MB in 56 us with the sums, 4.8 TB/s: memory.
 template <int HD, int DQ, int NT, int RT, int W>
 struct ScoreSmem {
   static constexpr int KG = W / DQ, R = 16 * RT;
@@ -393,11 +394,11 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoreArgs a) {
 // k times 2^8 in FP16 ends at 2^-24: what is lost of each is 2^-33, which 512 q below 16 make less
 // than 10^-6 of a score.  A block with a k of 128 or more, with larger q and a key that is below
 // 2^-10 throughout, or with a q below 2^-99, does its rows again, as scores_kernel does.
-// 256 rows over 4096 keys of 512 (8 heads, 25 GFLOP with the three products): 48 us traced.  Before
-// its first step a block needs 10 us (its 128 KB of q 3.7, their parts 1.8, the first keys and
+// 256 rows over 4096 keys of 512 (8 heads, 25 GFLOP with the three products): 45.9 us without the sums.
+// Before its first step a block needs 10 us (its 128 KB of q 3.7, their parts 1.8, the first keys and
 // products 3); a step takes 2.3: without its loads the call would take 11 us less, without two of its
-// three products 4, without a third of its vector instructions nothing.  The whole call, 57: with 32
-// rows per block 85; with blocks of 4 waves, two per CU, alike.
+// three products 4, without a third of its vector instructions nothing.  The whole call, 55, when it took
+// 57: with 32 rows per block 85; with blocks of 4 waves, two per CU, alike.
 template <int HD, int RT, int W>
 __global__ __launch_bounds__(64 * W, 2) void scores_rows_kernel(ScoreArgs a) {
   constexpr int DW = HD / W, KN = DW / 32, R = 16 * RT, NT = W / RT, KEYS = 16 * NT;
